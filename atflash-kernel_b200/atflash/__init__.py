@@ -9,7 +9,10 @@
                    windowed paged-KV GQA decode (split-KV + LSE merge)
     rope_pack      fused RoPE + pair-order pack (pre-RoPE HF q/k -> kernel layout)
     append_paged_kv_cache
-                   write new K/V tokens into a paged cache (RoPE + pack on K)
+                   write new K/V tokens into a paged cache (RoPE + pack on K); bf16
+                   pages, or e4m3 pages with a scale for each page and kv head
+    build_page_tables
+                   page tables and slot maps of a step from the requests' lengths
     dist           zig-zag sharded prefill and KV-sharded decode over torch.distributed
     hf             transformers AttentionInterface function (import atflash.hf)
 
@@ -23,6 +26,7 @@ from .append import append_paged_kv_cache, get_batch_indices_positions
 from .decode import BatchDecodeWithPagedKVCacheWrapper, lse_merge
 from .prefill import _flash_attn_fwd, flash_attn_func, prefill_fwd
 from .rope import cos_sin_table, inv_freq, rope_pack
+from .tables import PageTables, build_page_tables
 from .window_table import WindowTable
 from . import dist
 
@@ -41,4 +45,4 @@ _fail_loudly_without_library()
 __all__ = ["window_table", "WindowTable", "flash_attn_func", "prefill_fwd", "_flash_attn_fwd",
            "BatchDecodeWithPagedKVCacheWrapper", "lse_merge", "rope_pack", "cos_sin_table",
            "inv_freq", "check_device_errors", "dist", "AtfError", "append_paged_kv_cache",
-           "get_batch_indices_positions"]
+           "get_batch_indices_positions", "build_page_tables", "PageTables"]

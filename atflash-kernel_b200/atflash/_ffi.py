@@ -18,13 +18,15 @@ ATF_KV_NHD, ATF_KV_HND = 0, 1
 ATF_WINDOW_OFF, ATF_WINDOW_SNAP16, ATF_WINDOW_VEC8 = 0, 1, 2
 ATF_DTYPE_BF16, ATF_DTYPE_F32 = 0, 1
 ATF_NOALLOC_MAX_PARTIAL_ROWS = 16384
+ATF_TABLES_MAX_BATCH = 8192
 
 EXPORTED = ("atf_window_widths", "atf_window_zhi16", "atf_window_zhi8", "atf_window_deff",
             "atf_prefill_fwd", "atf_decode_plan", "atf_decode_run", "atf_decode_run_noalloc", "atf_lse_merge",
             "atf_rope_pack", "atf_paged_kv_append", "atf_status_string", "atf_version",
             "atf_read_error_flag", "atf_selftest_wait_timeout", "atf_params_size",
             "atf_exchange_region_bytes", "atf_state_push", "atf_state_merge", "atf_decode_run_exchange",
-            "atf_ipc_export", "atf_ipc_import", "atf_ipc_release")
+            "atf_ipc_export", "atf_ipc_import", "atf_ipc_release",
+            "atf_build_page_tables", "atf_paged_kv_append_e4m3")
 ATF_IPC_HANDLE_BYTES = 64
 
 _i64, _i32, _f32, _vp = ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p
@@ -108,6 +110,19 @@ class AtfExchangeParams(ctypes.Structure):
                 ("lse_out", _vp), ("error_flag", _vp)]
 
 
+class AtfPageTablesParams(ctypes.Structure):
+    _fields_ = [("kv_lens", _vp), ("append_lens", _vp), ("batch", _i32), ("page_size", _i32),
+                ("req_pages", _vp), ("req_stride", _i64), ("num_rows", _i32), ("max_req_pages", _i32),
+                ("req_rows", _vp), ("free_pages", _vp), ("free_head", _vp), ("free_head_out", _vp),
+                ("num_free", _i32), ("max_pages", _i32), ("max_tokens", _i32), ("indptr", _vp), ("indices", _vp),
+                ("last_page_len", _vp), ("append_indptr", _vp), ("batch_indices", _vp), ("positions", _vp),
+                ("slot_mapping", _vp), ("error_flag", _vp)]
+
+
+class AtfKvScales(ctypes.Structure):
+    _fields_ = [("k_scale", _vp), ("v_scale", _vp), ("stride_page", _i64), ("stride_head", _i64)]
+
+
 class AtfError(RuntimeError):
     """A non-zero status from the C ABI."""
 
@@ -155,6 +170,8 @@ def load() -> ctypes.CDLL:
             lib.atf_ipc_export.argtypes = [_vp, _vp, P(_i64)]
             lib.atf_ipc_import.argtypes = [_vp, _i64, P(_vp), P(_vp)]
             lib.atf_ipc_release.argtypes = [_vp]
+            lib.atf_build_page_tables.argtypes = [P(AtfPageTablesParams), _vp]
+            lib.atf_paged_kv_append_e4m3.argtypes = [P(AtfAppendParams), P(AtfKvScales), _vp]
             for name in EXPORTED:
                 if name not in ("atf_status_string", "atf_params_size", "atf_exchange_region_bytes"):
                     getattr(lib, name).restype = ctypes.c_int

@@ -29,11 +29,39 @@ def get_batch_indices_positions(append_indptr: torch.Tensor, seq_lens: torch.Ten
     return batch.to(torch.int32), pos.to(torch.int32)
 
 
+def _check_e4m3_cache(kc: torch.Tensor, vc: torch.Tensor, kv_scales, kv_layout: str) -> None:
+    """Pages and scales of an e4m3 cache: the append's and the decode's checks."""
+    if kc.dtype != torch.float8_e4m3fn or vc.dtype != torch.float8_e4m3fn:
+        raise ValueError("with kv_scales the cache pages must be float8_e4m3fn")
+    if kc.dim() != 4 or kc.shape != vc.shape or kc.stride() != vc.stride():
+        raise ValueError("k and v pages must have the same 4-d shape and strides")
+    if kc.shape[-1] != 128 or kc.stride(-1) != 1:
+        raise ValueError("the cache pages must have a contiguous head_dim of 128")
+    if not isinstance(kv_scales, (tuple, list)) or len(kv_scales) != 2:
+        raise ValueError("kv_scales is (k_scales, v_scales)")
+    ks, vs = kv_scales
+    want = (kc.shape[0], kc.shape[1 if kv_layout == "HND" else 2])
+    for t in (ks, vs):
+        if not t.is_cuda or t.device != kc.device or t.dtype != torch.float32 or tuple(t.shape) != want:
+            raise ValueError(f"k_scales and v_scales must be float32 {want} tensors (pages, kv heads) on {kc.device}")
+    if ks.stride() != vs.stride():
+        raise ValueError("k_scales and v_scales must have the same strides")
+
+
+def e4m3_scales(kv_scales) -> _ffi.AtfKvScales:
+    ks, vs = kv_scales
+    sc = _ffi.AtfKvScales()
+    sc.k_scale, sc.v_scale = ks.data_ptr(), vs.data_ptr()
+    sc.stride_page, sc.stride_head = ks.stride(0), ks.stride(1)
+    return sc
+
+
 def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, batch_indices: torch.Tensor,
                           positions: torch.Tensor, paged_kv_cache, kv_indices: torch.Tensor,
                           kv_indptr: torch.Tensor, kv_last_page_len: Optional[torch.Tensor] = None,
                           kv_layout: str = "NHD", *, rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
-                          rope_positions: Optional[torch.Tensor] = None, out_layout: str = "sorted_pair") -> None:
+                          rope_positions: Optional[torch.Tensor] = None, out_layout: str = "sorted_pair",
+                          kv_scales: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> None:
     """append_key / append_value (nnz, Hkv, 128) bf16; token i goes to request
     batch_indices[i] at KV position positions[i]. paged_kv_cache = (k_pages,
     v_pages) or one tensor with a k/v axis at dim 1; kv_layout "NHD" or "HND".
@@ -41,14 +69,27 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
     and is rotated at rope_positions[i] (default positions[i]) and written in
     out_layout order. Out-of-range page indices are skipped and reported by
     ``atflash.check_device_errors()`` (code 2). kv_last_page_len is accepted for
-    call compatibility; positions fully determine the slots."""
+    call compatibility; positions fully determine the slots.
+
+    kv_scales = (k_scales, v_scales), fp32 (num_pages, Hkv): the cache pages are
+    float8_e4m3fn (not level-major) and each (page, kv head) has one scale, which
+    the call sets for pages it begins and raises for pages it goes on filling
+    (``atf_paged_kv_append_e4m3``). The tokens of a request are then adjacent and in
+    position order, as ``build_page_tables`` and ``get_batch_indices_positions`` list
+    them; a batch index of -1 is padding."""
     if isinstance(paged_kv_cache, (tuple, list)):
         kc, vc = paged_kv_cache
     else:
         kc, vc = paged_kv_cache[:, 0], paged_kv_cache[:, 1]
     dev = _runtime.require_cuda(append_key, append_value, kc, vc)
+    e4m3 = kv_scales is not None
+    if not e4m3 and torch.float8_e4m3fn in (kc.dtype, vc.dtype):
+        raise ValueError("float8_e4m3fn pages need kv_scales")
+    if e4m3:
+        _check_e4m3_cache(kc, vc, kv_scales, kv_layout)
     k_level_major = kc.dim() == 5
-    for t in (append_key, append_value, vc) + (() if k_level_major else (kc,)):
+    bf16 = (append_key, append_value) if e4m3 else (append_key, append_value, vc) + (() if k_level_major else (kc,))
+    for t in bf16:
         if t.dtype != torch.bfloat16 or t.stride(-1) != 1 or t.shape[-1] != 128:
             raise ValueError("keys, values and cache pages must be bf16 with a contiguous head_dim of 128")
     if append_key.shape != append_value.shape or append_key.stride() != append_value.stride():
@@ -79,6 +120,8 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
     ix = kv_indices.to(device=dev, dtype=torch.int32).contiguous()
     if bi.numel() != nnz or ps.numel() != nnz:
         raise ValueError("batch_indices and positions need one entry per appended token")
+    if e4m3 and nnz == 0:
+        return
     p = _ffi.AtfAppendParams()
     p.append_k, p.append_v, p.nnz = append_key.data_ptr(), append_value.data_ptr(), nnz
     p.a_stride_n, p.a_stride_h = append_key.stride(0), append_key.stride(1)
@@ -90,11 +133,15 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
     keep = [bi, ps, ip, ix]
     if rope is not None:
         cos, sin = rope
-        if cos.dtype != torch.float32 or cos.shape != sin.shape or cos.stride() != sin.stride() or cos.stride(1) != 1:
+        if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() != 2
+                or cos.shape[1] < 64 or cos.stride() != sin.stride() or cos.stride(1) != 1 or cos.device != dev
+                or sin.device != dev):
             raise ValueError("cos/sin must be matching fp32 (n_pos, >=64) tables")
         p.cos, p.sin, p.cs_stride_pos, p.n_pos = cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0]
         if rope_positions is not None:
             rp = rope_positions.to(device=dev, dtype=torch.int64).contiguous()
+            if rp.numel() != nnz:
+                raise ValueError("rope_positions needs one entry per appended token")
             keep.append(rp)
             p.rope_positions = rp.data_ptr()
     p.out_layout = _LAYOUTS[out_layout]
@@ -104,6 +151,12 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
             raise ValueError("level-major k pages do not match the v pages")
         p.k_level_major = 1
         p.k_stride_page, p.k_stride_head, p.k_stride_level = kc.stride(0), kc.stride(1), kc.stride(2)
+    if e4m3:
+        sc = e4m3_scales(kv_scales)
+        with torch.cuda.device(dev):
+            rc = _ffi.load().atf_paged_kv_append_e4m3(ctypes.byref(p), ctypes.byref(sc), _runtime.stream_handle(dev))
+        _ffi.check("atf_paged_kv_append_e4m3", rc)
+        return
     with torch.cuda.device(dev):
         rc = _ffi.load().atf_paged_kv_append(ctypes.byref(p), _runtime.stream_handle(dev))
     _ffi.check("atf_paged_kv_append", rc)

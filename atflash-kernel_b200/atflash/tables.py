@@ -1,0 +1,106 @@
+"""Page tables and slot maps of a serving step, built on the GPU from the
+requests' lengths (``atf_build_page_tables``): what the decode's plan, the paged
+append and the packed prefill take, without a host round trip.
+
+The reference decodes one request over a contiguous cache
+(e2e_pipeline/atflash_e2e_fafi.py:219-223) and has no counterpart."""
+import ctypes
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _ffi, _runtime
+
+
+@dataclass
+class PageTables:
+    """indptr (B+1) / indices / last_page_len (B): the CSR page table;
+    append_indptr (B+1), batch_indices, positions, slot_mapping (int64): request,
+    position and cache slot (page * page_size + slot) of each new token. Entries
+    past the end are -1. free_head (1): the next free list position, or None."""
+    indptr: torch.Tensor
+    indices: torch.Tensor
+    last_page_len: torch.Tensor
+    append_indptr: torch.Tensor
+    batch_indices: torch.Tensor
+    positions: torch.Tensor
+    slot_mapping: torch.Tensor
+    free_head: Optional[torch.Tensor]
+
+
+def _i32(t: torch.Tensor, name: str, n: Optional[int] = None) -> torch.Tensor:
+    if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or (n is not None and t.numel() != n):
+        raise ValueError(f"{name} must be a 1-d integer tensor" + (f" of {n} entries" if n is not None else ""))
+    return t.to(torch.int32).contiguous()
+
+
+def build_page_tables(kv_lens: torch.Tensor, append_lens: torch.Tensor, req_pages: torch.Tensor, page_size: int, *,
+                      num_tokens: int, max_pages: int, req_rows: Optional[torch.Tensor] = None,
+                      free_pages: Optional[torch.Tensor] = None,
+                      free_head: Optional[torch.Tensor] = None) -> PageTables:
+    """Build a step's tables in one launch.
+
+    kv_lens (B): tokens of each request after the step; append_lens (B): how many
+    of them are new. req_pages int32 (rows, pages): the engine's table of page ids,
+    row req_rows[b] (default b) for request b. With free_pages (int32, 1-d) and
+    free_head (int32, 1 entry) the pages that a request lacks are taken from
+    free_pages[free_head:] in request order and written into req_pages, in place;
+    the next head is in the result (free_head itself stays). Without them req_pages
+    holds every page already.
+
+    num_tokens and max_pages are the sizes of the token outputs and of indices: the
+    step's totals, or capacities (a fixed shape for a CUDA graph): entries past the
+    end are -1. Bad lengths or rows, an exhausted free list and exceeded
+    capacities are reported by ``atflash.check_device_errors()`` (code 2)."""
+    dev = _runtime.require_cuda(kv_lens, append_lens, req_pages)
+    B = kv_lens.numel()
+    if B < 1 or B > _ffi.ATF_TABLES_MAX_BATCH:
+        raise ValueError(f"between 1 and {_ffi.ATF_TABLES_MAX_BATCH} requests")
+    kv_lens, append_lens = _i32(kv_lens, "kv_lens"), _i32(append_lens, "append_lens", B)
+    if req_pages.dim() != 2 or req_pages.dtype != torch.int32 or (req_pages.shape[1] > 1 and req_pages.stride(1) != 1):
+        raise ValueError("req_pages must be an int32 (rows, pages) tensor with contiguous rows")
+    if req_pages.shape[0] < 1 or (req_rows is None and req_pages.shape[0] < B):
+        raise ValueError("req_pages needs a row for each request")
+    if req_pages.shape[0] > 1 and req_pages.stride(0) < req_pages.shape[1]:
+        raise ValueError("the rows of req_pages must not overlap")
+    if page_size < 1 or num_tokens < 0 or max_pages < 0:
+        raise ValueError("page_size must be positive, num_tokens and max_pages not negative")
+    if max(num_tokens, max_pages) > 0x7fffffff:
+        raise ValueError("num_tokens and max_pages must fit 32 bits")
+    if (free_pages is None) != (free_head is None):
+        raise ValueError("free_pages and free_head go together")
+    keep = [kv_lens, append_lens]
+    p = _ffi.AtfPageTablesParams()
+    p.kv_lens, p.append_lens, p.batch, p.page_size = kv_lens.data_ptr(), append_lens.data_ptr(), B, int(page_size)
+    p.req_pages = req_pages.data_ptr() or kv_lens.data_ptr()  # no columns: never read
+    p.req_stride = req_pages.stride(0) if req_pages.shape[0] > 1 else max(1, req_pages.shape[1])
+    p.num_rows, p.max_req_pages = req_pages.shape
+    if req_rows is not None:
+        _runtime.require_cuda(kv_lens, req_rows)
+        rows = _i32(req_rows, "req_rows", B)
+        keep.append(rows)
+        p.req_rows = rows.data_ptr()
+    head_out = None
+    if free_pages is not None:
+        _runtime.require_cuda(kv_lens, free_pages, free_head)
+        free_pages = _i32(free_pages, "free_pages")
+        free_head = _i32(free_head, "free_head", 1)
+        keep += [free_pages, free_head]
+        head_out = torch.empty(1, dtype=torch.int32, device=dev)
+        # an empty list still has a head: any valid address will do for its pages
+        p.free_pages = free_pages.data_ptr() or free_head.data_ptr()
+        p.free_head, p.free_head_out, p.num_free = free_head.data_ptr(), head_out.data_ptr(), free_pages.numel()
+    # one allocation for the 32-bit outputs
+    sizes = (B + 1, max_pages, B, B + 1, num_tokens, num_tokens)
+    parts = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes)
+    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    p.max_pages, p.max_tokens = int(max_pages), int(num_tokens)
+    p.indptr, p.indices, p.last_page_len, p.append_indptr, p.batch_indices, p.positions = \
+        (t.data_ptr() for t in parts)
+    p.slot_mapping = slots.data_ptr()
+    p.error_flag = _runtime.error_flag(dev).data_ptr()
+    with torch.cuda.device(dev):
+        rc = _ffi.load().atf_build_page_tables(ctypes.byref(p), _runtime.stream_handle(dev))
+    _ffi.check("atf_build_page_tables", rc)
+    return PageTables(*parts, slots, head_out)

@@ -81,6 +81,8 @@ extern "C" int64_t atf_params_size(const char* name) {
       {"AtfRopeParams", static_cast<int64_t>(sizeof(AtfRopeParams))},
       {"AtfAppendParams", static_cast<int64_t>(sizeof(AtfAppendParams))},
       {"AtfExchangeParams", static_cast<int64_t>(sizeof(AtfExchangeParams))},
+      {"AtfPageTablesParams", static_cast<int64_t>(sizeof(AtfPageTablesParams))},
+      {"AtfKvScales", static_cast<int64_t>(sizeof(AtfKvScales))},
   };
   for (const Entry& e : kSizes)
     if (std::strcmp(e.n, name) == 0) return e.size;

@@ -395,13 +395,74 @@ typedef struct {
  * decode (e2e_pipeline/atflash_e2e_fafi.py:219-223). */
 int atf_paged_kv_append(const AtfAppendParams* p, atf_stream_t stream);
 
+/* ------------------------------------------------------------------ page tables */
+
+typedef struct {
+  const int32_t* kv_lens;     /* device [batch]: tokens of each request after the step */
+  const int32_t* append_lens; /* device [batch]: tokens that the step adds (0..kv_lens[b]) */
+  int32_t batch, page_size;
+  int32_t* req_pages;         /* device [num_rows, >= max_req_pages]: page ids of each request, in order */
+  int64_t req_stride;         /* elements between rows */
+  int32_t num_rows, max_req_pages;
+  const int32_t* req_rows;    /* optional device [batch]: row of each request (default b) */
+  /* Pages for requests that outgrow theirs (optional): the step takes
+   * free_pages[*free_head ..] in request order, writes them into req_pages and
+   * the next head into *free_head_out (another word than free_head). Without
+   * them req_pages holds every page already. */
+  const int32_t* free_pages;  /* device [num_free] */
+  const int32_t* free_head;   /* device [1] */
+  int32_t* free_head_out;     /* device [1] */
+  int32_t num_free;
+  int32_t max_pages, max_tokens; /* capacities of indices and of the token outputs */
+  int32_t* indptr;            /* device [batch + 1] */
+  int32_t* indices;           /* device [max_pages]: page ids, -1 past the end */
+  int32_t* last_page_len;     /* device [batch], 0 for an empty request */
+  int32_t* append_indptr;     /* device [batch + 1] */
+  int32_t* batch_indices;     /* device [max_tokens], -1 past the end */
+  int32_t* positions;         /* device [max_tokens], -1 past the end */
+  int64_t* slot_mapping;      /* device [max_tokens]: page * page_size + slot, -1 past the end */
+  int* error_flag;            /* optional: set to 2, see below */
+} AtfPageTablesParams;
+
+#define ATF_TABLES_MAX_BATCH 8192
+
+/* Page table (CSR) and slot map of one step from the requests' lengths, in one
+ * launch without a host synchronisation. A request with a negative length, more
+ * new tokens than tokens, more than max_req_pages pages or a row out of range
+ * counts as empty; a page that the free list cannot give is -1, as are its slots;
+ * pages and tokens past a capacity are cut off. Each of these sets *error_flag
+ * to 2. Requests of one call use different rows. */
+int atf_build_page_tables(const AtfPageTablesParams* p, atf_stream_t stream);
+
+/* ------------------------------------------------------------------ e4m3 paged cache */
+
+/* An e4m3 cache keeps one fp32 scale for each (page, kv head) of K and of V: an
+ * element stands for its e4m3 value times its page's scale. */
+typedef struct {
+  float* k_scale; /* device [num_pages, num_kv_heads] through the strides (elements) */
+  float* v_scale;
+  int64_t stride_page, stride_head; /* same for both */
+} AtfKvScales;
+
+/* atf_paged_kv_append into an e4m3 cache: k_cache / v_cache hold e4m3 bytes
+ * (strides in bytes, multiples of 16; no level-major pages). Tokens of one
+ * request are adjacent and in position order, so that its new rows in a page are
+ * one run; batch_indices[i] = -1 marks padding, which is skipped. Per (page, kv
+ * head), with amax over the run's finite-or-infinite elements: want = the
+ * smallest power of two s in [2^-126, 2^120] with amax <= 448 s; a run that begins
+ * at slot 0 sets the scale to want, any other to max(scale, want), and where that
+ * is more than the scale was, the rows before the run are rounded again under
+ * the new one. Rows are rounded to nearest even, saturating at 448 s. */
+int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvScales* s, atf_stream_t stream);
+
 /* ------------------------------------------------------------------ misc */
 
 const char* atf_status_string(int status);
 int atf_version(void);
 /* sizeof of the named params struct ("AtfPrefillParams", "AtfDecodePlanParams",
  * "AtfDecodePlan", "AtfDecodeParams", "AtfMergeParams", "AtfRopeParams",
- * "AtfAppendParams", "AtfExchangeParams"), or -1: lets an FFI binding check its struct mirrors. */
+ * "AtfAppendParams", "AtfExchangeParams", "AtfPageTablesParams", "AtfKvScales"),
+ * or -1: lets an FFI binding check its struct mirrors. */
 int64_t atf_params_size(const char* name);
 /* Synchronises the current device, copies *error_flag to *out and clears it. */
 int atf_read_error_flag(int* error_flag_device, int* out);
