@@ -26,7 +26,7 @@ EXPORTED = ("atf_window_widths", "atf_window_zhi16", "atf_window_zhi8", "atf_win
             "atf_read_error_flag", "atf_selftest_wait_timeout", "atf_params_size",
             "atf_exchange_region_bytes", "atf_state_push", "atf_state_merge", "atf_decode_run_exchange",
             "atf_ipc_export", "atf_ipc_import", "atf_ipc_release",
-            "atf_build_page_tables", "atf_paged_kv_append_e4m3")
+            "atf_build_page_tables", "atf_paged_kv_append_e4m3", "atf_decode_run_e4m3")
 ATF_IPC_HANDLE_BYTES = 64
 
 _i64, _i32, _f32, _vp = ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p
@@ -171,6 +171,7 @@ def load() -> ctypes.CDLL:
             lib.atf_ipc_import.argtypes = [_vp, _i64, P(_vp), P(_vp)]
             lib.atf_ipc_release.argtypes = [_vp]
             lib.atf_build_page_tables.argtypes = [P(AtfPageTablesParams), _vp]
+            lib.atf_decode_run_e4m3.argtypes = [P(AtfDecodeParams), P(AtfKvScales), _vp]
             lib.atf_paged_kv_append_e4m3.argtypes = [P(AtfAppendParams), P(AtfKvScales), _vp]
             for name in EXPORTED:
                 if name not in ("atf_status_string", "atf_params_size", "atf_exchange_region_bytes"):

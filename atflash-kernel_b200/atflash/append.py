@@ -29,7 +29,7 @@ def get_batch_indices_positions(append_indptr: torch.Tensor, seq_lens: torch.Ten
     return batch.to(torch.int32), pos.to(torch.int32)
 
 
-def _check_e4m3_cache(kc: torch.Tensor, vc: torch.Tensor, kv_scales, kv_layout: str) -> None:
+def check_e4m3_cache(kc: torch.Tensor, vc: torch.Tensor, kv_scales, kv_layout: str) -> None:
     """Pages and scales of an e4m3 cache: the append's and the decode's checks."""
     if kc.dtype != torch.float8_e4m3fn or vc.dtype != torch.float8_e4m3fn:
         raise ValueError("with kv_scales the cache pages must be float8_e4m3fn")
@@ -86,7 +86,7 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
     if not e4m3 and torch.float8_e4m3fn in (kc.dtype, vc.dtype):
         raise ValueError("float8_e4m3fn pages need kv_scales")
     if e4m3:
-        _check_e4m3_cache(kc, vc, kv_scales, kv_layout)
+        check_e4m3_cache(kc, vc, kv_scales, kv_layout)
     k_level_major = kc.dim() == 5
     bf16 = (append_key, append_value) if e4m3 else (append_key, append_value, vc) + (() if k_level_major else (kc,))
     for t in bf16:

@@ -18,6 +18,7 @@ import numpy as np
 import torch
 
 from . import _ffi, _runtime
+from .append import check_e4m3_cache, e4m3_scales
 from .window_table import KERNEL_CAP, WindowTable, zhi_slice_vec8
 
 _LAYOUTS = {"sorted_pair": _ffi.ATF_LAYOUT_SORTED_PAIR, "rotate_half": _ffi.ATF_LAYOUT_ROTATE_HALF}
@@ -205,7 +206,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
             out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
             return_lse: bool = False, enable_pdl=None, window_left=None,
             q_pos: Optional[torch.Tensor] = None, kv_pos0: Optional[torch.Tensor] = None,
-            out_dtype: Optional[torch.dtype] = None, exchange=None):
+            out_dtype: Optional[torch.dtype] = None, exchange=None,
+            kv_scales: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
         """q (B, Hq, 128) bf16; paged_kv_cache = (k_pages, v_pages) or one tensor with
         a k/v axis at dim 1. Returns out (B, Hq, 128) [, lse (B, Hq), natural log].
 
@@ -219,19 +221,35 @@ class BatchDecodeWithPagedKVCacheWrapper:
         With `exchange` (an atflash.dist.StateExchange whose ranks run on
         different GPUs) this is one KV-sharded step: the decode's split merge also
         exchanges the ranks' states (atf_decode_run_exchange), and out / lse are
-        the merge over every rank of the exchange."""
+        the merge over every rank of the exchange.
+
+        kv_scales = (k_scales, v_scales), fp32 (num_pages, Hkv): the pages are
+        float8_e4m3fn and an element stands for its value times its page's scale
+        (``append_paged_kv_cache(kv_scales=...)`` writes such a cache). Page sizes 16
+        to 256 (powers of two); no window, or a snap16 window over sorted pairs."""
         if self._plan is None:
             raise RuntimeError("plan() must be called before run()")
         if q_scale is not None or k_scale is not None or v_scale is not None:
-            raise NotImplementedError("fp8 scales are not supported")
+            raise NotImplementedError("per-tensor scales are not supported (kv_scales: one per page and kv head)")
         P = self._plan
         if isinstance(paged_kv_cache, (tuple, list)):
             kc, vc = paged_kv_cache
         else:
             kc, vc = paged_kv_cache[:, 0], paged_kv_cache[:, 1]
         dev = _runtime.require_cuda(q, kc, vc)
-        if kc.dtype != torch.bfloat16 or vc.dtype != torch.bfloat16 or q.dtype != torch.bfloat16:
-            raise TypeError("q and the KV cache must be bfloat16")
+        if kv_scales is not None:
+            if q.dtype != torch.bfloat16:
+                raise TypeError("q must be bfloat16")
+            check_e4m3_cache(kc, vc, kv_scales, self._kv_layout)
+            if exchange is not None:
+                raise NotImplementedError("the KV-sharded exchange reads bfloat16 caches")
+            if P["page_size"] not in (16, 32, 64, 128, 256):
+                raise NotImplementedError("an e4m3 cache has pages of 16, 32, 64, 128 or 256 tokens")
+            if P["window"] == _ffi.ATF_WINDOW_VEC8 or (P["window"] != _ffi.ATF_WINDOW_OFF
+                                                       and P["layout"] != _ffi.ATF_LAYOUT_SORTED_PAIR):
+                raise NotImplementedError("an e4m3 cache takes snap16 windows over sorted pairs")
+        elif kc.dtype != torch.bfloat16 or vc.dtype != torch.bfloat16 or q.dtype != torch.bfloat16:
+            raise TypeError("q and the KV cache must be bfloat16 (float8_e4m3fn pages need kv_scales)")
         # K pages are either laid out like V (4-d, NHD / HND) or level-major:
         # (P, Hkv, 8 levels, page, 16) in sorted-pair order, so that a page's
         # in-window levels are one contiguous run
@@ -301,6 +319,12 @@ class BatchDecodeWithPagedKVCacheWrapper:
                 rc = _ffi.load().atf_decode_run_exchange(ctypes.byref(a), ctypes.byref(x),
                                                          _runtime.stream_handle(dev))
             _ffi.check("atf_decode_run_exchange", rc)
+            return (out, lse) if return_lse else out
+        if kv_scales is not None:
+            sc = e4m3_scales(kv_scales)
+            with torch.cuda.device(dev):
+                rc = _ffi.load().atf_decode_run_e4m3(ctypes.byref(a), ctypes.byref(sc), _runtime.stream_handle(dev))
+            _ffi.check("atf_decode_run_e4m3", rc)
             return (out, lse) if return_lse else out
         with torch.cuda.device(dev):
             rc = _ffi.load().atf_decode_run(ctypes.byref(a), _runtime.stream_handle(dev))

@@ -18,9 +18,9 @@ EncodeTiledFn g_encode = nullptr;
 std::once_flag g_encode_once;
 }  // namespace
 
-int encode_tiled_bf16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
-                      const uint64_t* strides_bytes, const uint32_t* box,
-                      CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+static int encode_tiled(CUtensorMapDataType type, CUtensorMap* map, const void* base, int rank,
+                        const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+                        CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -41,11 +41,24 @@ int encode_tiled_bf16(CUtensorMap* map, const void* base, int rank, const uint64
       if ((s[i - 1] & 15u) != 0 || s[i - 1] == 0) return ATF_ERR_ALIGNMENT;
     }
   }
-  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank),
+  CUresult r = g_encode(map, type, static_cast<cuuint32_t>(rank),
                         const_cast<void*>(base), d, s, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle, promotion,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? ATF_OK : ATF_ERR_CUDA;
+}
+
+int encode_tiled_bf16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                      const uint64_t* strides_bytes, const uint32_t* box,
+                      CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+  return encode_tiled(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, map, base, rank, dims, strides_bytes, box, swizzle,
+                      promotion);
+}
+
+int encode_tiled_u8(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                    const uint64_t* strides_bytes, const uint32_t* box,
+                    CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+  return encode_tiled(CU_TENSOR_MAP_DATA_TYPE_UINT8, map, base, rank, dims, strides_bytes, box, swizzle, promotion);
 }
 
 int check_device(int* device_out) {

@@ -21,6 +21,11 @@ int encode_tiled_bf16(CUtensorMap* map, const void* base, int rank, const uint64
                       CUtensorMapSwizzle swizzle,
                       CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 
+// The same over bytes (e4m3 caches).
+int encode_tiled_u8(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                    const uint64_t* strides_bytes, const uint32_t* box,
+                    CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion);
+
 // True when the current device is an sm_100 part.
 int check_device(int* device_out);
 

@@ -30,6 +30,7 @@
 
 #include "atf_internal.h"
 #include "atf_ptx.cuh"
+#include "decode_common.cuh"
 #include "merge.cuh"
 
 namespace atf {
@@ -72,16 +73,6 @@ __device__ __forceinline__ int level_of_chunk(int layout, int c) {
   return layout == ATF_LAYOUT_SORTED_PAIR ? (c >> 1) : 7 - (c & 7);
 }
 
-// The window as limits on local key indices, computed once per CTA and kept in
-// registers: a key of local index n is at distance z = zb - n (zb = q_pos -
-// kv_pos0) and reads a level or chunk whose zhi is >= z, i.e. when n >= zb - zhi.
-// Per-key level counts are then 32-bit compares against registers; evaluating
-// 64-bit distances against the table in the kernel parameters for every key
-// group took most of a consumer warp's time per stage.
-__device__ __forceinline__ int key_limit(long long zb, long long zhi) {
-  const long long v = zb - zhi;
-  return static_cast<int>(v < INT_MIN ? INT_MIN : (v > INT_MAX ? INT_MAX : v));
-}
 // level i (0..7): snap16, L(z) = max(1, #{i : zhi16[i] >= z}) (zhi16 is
 // non-increasing, so level 0 always and level i when zhi16[i] >= z); vec8, a
 // level when its first (wider) slice is read; every level when the window is off
@@ -100,14 +91,6 @@ __device__ __forceinline__ int chunk_limit(const Args& a, long long zb, int c) {
   }
   return key_limit(zb, a.zhi8[c]);
 }
-// levels read by local key n
-__device__ __forceinline__ int levels_of(const int (&lim)[ATF_MAX_LEVELS], int n) {
-  int L = 0;
-#pragma unroll
-  for (int i = 0; i < ATF_MAX_LEVELS; ++i) L += n >= lim[i] ? 1 : 0;
-  return L;
-}
-
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool pred) {
   const int n = pred ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
@@ -121,25 +104,6 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
-                                        uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
-                                          uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-// Transpose of an 8x8 b16 matrix held one row pair per thread (the mma
-// fragment layout): lane (g, t4) gets elements (2 t4, g) and (2 t4 + 1, g).
-__device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {
-  uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
-  return d;
-}
 // D = A(16x16 bf16, row) * B(16x8 bf16, col) + D, fp32 accumulate.
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
@@ -162,12 +126,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Byte offset of (key row, logical 16-B chunk) inside a 64-row stage buffer;
 // the chunk index is XOR-swizzled with the row so that ldmatrix reads of 8
 // consecutive rows hit 8 distinct bank groups.
@@ -1093,26 +1051,6 @@ extern "C" int atf_decode_plan(const AtfDecodePlanParams* p, int32_t* items_host
   out->partial_o_floats = static_cast<int64_t>(n) * p->num_qo_heads * ATF_HEAD_DIM;
   out->partial_lse_floats = static_cast<int64_t>(n) * p->num_qo_heads;
   return ATF_OK;
-}
-
-// A kernel launch, with programmatic stream serialization when `pdl`: the grid
-// may then start while the previous kernel on the stream is still running; the
-// decode kernels read only the plan and the page table before their
-// griddepcontrol.wait.
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, int threads, uint32_t smem, cudaStream_t st,
-                              bool pdl, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
 // Validates an atf_decode_run call and launches its split-KV kernel (none when

@@ -455,6 +455,15 @@ typedef struct {
  * the new one. Rows are rounded to nearest even, saturating at 448 s. */
 int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvScales* s, atf_stream_t stream);
 
+/* atf_decode_run over an e4m3 cache: k_cache / v_cache hold e4m3 bytes (strides
+ * in bytes, multiples of 16). Plans, workspaces, outputs and enable_pdl are
+ * atf_decode_run's (the scales may be written by the kernel just before). Page
+ * sizes 16, 32, 64, 128 and 256; window off (either pair order) or 16-snap over
+ * sorted pairs; no level-major K: anything else is ATF_ERR_UNSUPPORTED. A scale
+ * may be any non-negative number. A page id outside the cache is not read and sets
+ * *error_flag to 2 (the call's outputs are not valid then). */
+int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* s, atf_stream_t stream);
+
 /* ------------------------------------------------------------------ misc */
 
 const char* atf_status_string(int status);
