@@ -5,6 +5,8 @@
                    with the reference's atflash/window_table.py
     flash_attn_func / prefill_fwd / _flash_attn_fwd
                    windowed causal prefill on the tcgen05/TMEM kernel
+    BatchPrefillWithRaggedKVCacheWrapper / flash_attn_varlen_func
+                   the prefill over packed sequences of different lengths
     BatchDecodeWithPagedKVCacheWrapper
                    windowed paged-KV GQA decode (split-KV + LSE merge)
     rope_pack      fused RoPE + pair-order pack (pre-RoPE HF q/k -> kernel layout)
@@ -25,6 +27,7 @@ from ._runtime import check_device_errors
 from .append import append_paged_kv_cache, get_batch_indices_positions
 from .decode import BatchDecodeWithPagedKVCacheWrapper, lse_merge
 from .prefill import _flash_attn_fwd, flash_attn_func, prefill_fwd
+from .ragged import BatchPrefillWithRaggedKVCacheWrapper, flash_attn_varlen_func
 from .rope import cos_sin_table, inv_freq, rope_pack
 from .tables import PageTables, build_page_tables
 from .window_table import WindowTable
@@ -45,4 +48,5 @@ _fail_loudly_without_library()
 __all__ = ["window_table", "WindowTable", "flash_attn_func", "prefill_fwd", "_flash_attn_fwd",
            "BatchDecodeWithPagedKVCacheWrapper", "lse_merge", "rope_pack", "cos_sin_table",
            "inv_freq", "check_device_errors", "dist", "AtfError", "append_paged_kv_cache",
-           "get_batch_indices_positions", "build_page_tables", "PageTables"]
+           "get_batch_indices_positions", "build_page_tables", "PageTables",
+           "BatchPrefillWithRaggedKVCacheWrapper", "flash_attn_varlen_func"]

@@ -26,7 +26,8 @@ EXPORTED = ("atf_window_widths", "atf_window_zhi16", "atf_window_zhi8", "atf_win
             "atf_read_error_flag", "atf_selftest_wait_timeout", "atf_params_size",
             "atf_exchange_region_bytes", "atf_state_push", "atf_state_merge", "atf_decode_run_exchange",
             "atf_ipc_export", "atf_ipc_import", "atf_ipc_release",
-            "atf_build_page_tables", "atf_paged_kv_append_e4m3", "atf_decode_run_e4m3")
+            "atf_build_page_tables", "atf_paged_kv_append_e4m3", "atf_decode_run_e4m3",
+            "atf_prefill_ragged_plan", "atf_prefill_ragged_fwd")
 ATF_IPC_HANDLE_BYTES = 64
 
 _i64, _i32, _f32, _vp = ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p
@@ -123,6 +124,19 @@ class AtfKvScales(ctypes.Structure):
     _fields_ = [("k_scale", _vp), ("v_scale", _vp), ("stride_page", _i64), ("stride_head", _i64)]
 
 
+class AtfPrefillRaggedPlanParams(ctypes.Structure):
+    _fields_ = [("batch_size", _i32), ("qo_indptr_host", _vp), ("kv_indptr_host", _vp), ("causal", ctypes.c_int)]
+
+
+class AtfPrefillRaggedParams(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("lse", _vp), ("total_q", _i64), ("total_k", _i64),
+                ("num_heads_q", _i64), ("num_heads_kv", _i64), ("head_dim", _i64), ("q_stride_s", _i64),
+                ("q_stride_h", _i64), ("k_stride_s", _i64), ("k_stride_h", _i64), ("v_stride_s", _i64),
+                ("v_stride_h", _i64), ("o_stride_s", _i64), ("o_stride_h", _i64), ("items", _vp),
+                ("num_items", _i32), ("softmax_scale", _f32), ("causal", ctypes.c_int), ("qk_layout", ctypes.c_int),
+                ("window", ctypes.c_int), ("zhi", _i32 * 8), ("error_flag", _vp)]
+
+
 class AtfError(RuntimeError):
     """A non-zero status from the C ABI."""
 
@@ -171,6 +185,8 @@ def load() -> ctypes.CDLL:
             lib.atf_ipc_import.argtypes = [_vp, _i64, P(_vp), P(_vp)]
             lib.atf_ipc_release.argtypes = [_vp]
             lib.atf_build_page_tables.argtypes = [P(AtfPageTablesParams), _vp]
+            lib.atf_prefill_ragged_plan.argtypes = [P(AtfPrefillRaggedPlanParams), P(_i32), _i32, P(_i32)]
+            lib.atf_prefill_ragged_fwd.argtypes = [P(AtfPrefillRaggedParams), _vp]
             lib.atf_decode_run_e4m3.argtypes = [P(AtfDecodeParams), P(AtfKvScales), _vp]
             lib.atf_paged_kv_append_e4m3.argtypes = [P(AtfAppendParams), P(AtfKvScales), _vp]
             for name in EXPORTED:

@@ -96,6 +96,8 @@ extern "C" int64_t atf_params_size(const char* name) {
       {"AtfExchangeParams", static_cast<int64_t>(sizeof(AtfExchangeParams))},
       {"AtfPageTablesParams", static_cast<int64_t>(sizeof(AtfPageTablesParams))},
       {"AtfKvScales", static_cast<int64_t>(sizeof(AtfKvScales))},
+      {"AtfPrefillRaggedPlanParams", static_cast<int64_t>(sizeof(AtfPrefillRaggedPlanParams))},
+      {"AtfPrefillRaggedParams", static_cast<int64_t>(sizeof(AtfPrefillRaggedParams))},
   };
   for (const Entry& e : kSizes)
     if (std::strcmp(e.n, name) == 0) return e.size;

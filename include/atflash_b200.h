@@ -139,6 +139,47 @@ typedef struct {
  * microbench/b1_correctness.py:113-135 for q, fused into the kernel). */
 int atf_prefill_fwd(const AtfPrefillParams* p, atf_stream_t stream);
 
+/* Packed (ragged) prefill: the rows of all sequences lie one after another in
+ * q [total_q, Hq, 128] and k, v [total_k, Hkv, 128]; sequence b holds the query
+ * rows [qo_indptr[b], qo_indptr[b+1]) and the keys [kv_indptr[b], kv_indptr[b+1]).
+ * Its queries are the last of its keys (causal: row i sees the keys up to
+ * nk - nq + i); a row that sees no key gets 0 and an LSE of -inf. The reference
+ * runs one sequence at a time. */
+typedef struct {
+  int32_t batch_size;
+  const int32_t* qo_indptr_host; /* [batch+1] (host) */
+  const int32_t* kv_indptr_host; /* [batch+1] (host) */
+  int causal;
+} AtfPrefillRaggedPlanParams;
+
+/* The work items of a packed batch: 8 int32 each, blocks of 256 query rows, the
+ * ones with the most key tiles first. items_host NULL: only *num_items is set. */
+int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int32_t* items_host,
+                            int32_t items_capacity, int32_t* num_items);
+
+typedef struct {
+  const void* q; /* bf16 [total_q, Hq, 128] */
+  const void* k; /* bf16 [total_k, Hkv, 128] */
+  const void* v;
+  void* out;     /* bf16 [total_q, Hq, 128] */
+  float* lse;    /* optional fp32 [total_q, Hq], natural log */
+  int64_t total_q, total_k, num_heads_q, num_heads_kv, head_dim;
+  int64_t q_stride_s, q_stride_h, k_stride_s, k_stride_h, v_stride_s, v_stride_h, o_stride_s, o_stride_h;
+  const int32_t* items; /* device, from atf_prefill_ragged_plan; 16-byte aligned */
+  int32_t num_items;
+  float softmax_scale;
+  int causal;           /* as planned */
+  int qk_layout;        /* ATF_LAYOUT_* */
+  int window;           /* ATF_WINDOW_OFF or ATF_WINDOW_SNAP16 */
+  int32_t zhi[ATF_MAX_LEVELS]; /* level 0 is always read */
+  int* error_flag;      /* optional; 2: an item outside the packed rows was skipped */
+} AtfPrefillRaggedParams;
+
+/* atf_prefill_fwd over packed sequences; the window is quantised per (query tile,
+ * key tile) of each sequence, so that a sequence's rows are those of a run of its
+ * own. */
+int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_stream_t stream);
+
 /* ------------------------------------------------------------------ decode */
 
 typedef struct {
@@ -470,7 +511,8 @@ const char* atf_status_string(int status);
 int atf_version(void);
 /* sizeof of the named params struct ("AtfPrefillParams", "AtfDecodePlanParams",
  * "AtfDecodePlan", "AtfDecodeParams", "AtfMergeParams", "AtfRopeParams",
- * "AtfAppendParams", "AtfExchangeParams", "AtfPageTablesParams", "AtfKvScales"),
+ * "AtfAppendParams", "AtfExchangeParams", "AtfPageTablesParams", "AtfKvScales",
+ * "AtfPrefillRaggedPlanParams", "AtfPrefillRaggedParams"),
  * or -1: lets an FFI binding check its struct mirrors. */
 int64_t atf_params_size(const char* name);
 /* Synchronises the current device, copies *error_flag to *out and clears it. */
