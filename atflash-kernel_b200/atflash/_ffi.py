@@ -52,7 +52,7 @@ class AtfDecodePlanParams(ctypes.Structure):
                 ("head_dim", _i32), ("page_size", _i32), ("indptr_host", _vp),
                 ("last_page_len_host", _vp), ("num_sms", _i32), ("min_chunk_keys", _i32),
                 ("max_chunk_keys", _i32), ("window", ctypes.c_int), ("zhi16", _i32 * 8),
-                ("q_pos_host", _vp), ("kv_pos0_host", _vp)]
+                ("q_pos_host", _vp), ("kv_pos0_host", _vp), ("units", _i32)]
 
 
 class AtfDecodePlan(ctypes.Structure):

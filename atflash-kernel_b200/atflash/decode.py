@@ -76,6 +76,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
         q_pos / kv_pos0: the positions run() will be given (per request; defaults
         kv_len - 1 and 0). Under a snap16 window the work items are cut to equal
         bytes read at these distances; they steer the balance only, never the result.
+        kv_data_type: torch.float8_e4m3fn lays the schedule out for an e4m3 cache (any
+        plan runs with either cache, this one keeps ragged batches balanced).
         """
         if pos_encoding_mode != "NONE":
             raise NotImplementedError("RoPE is applied before the cache (pos_encoding_mode NONE)")
@@ -106,6 +108,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
         pp.last_page_len_host = lpl_h.ctypes.data
         pp.num_sms = torch.cuda.get_device_properties(dev).multi_processor_count
         pp.min_chunk_keys, pp.max_chunk_keys = int(min_chunk_keys), int(max_chunk_keys)
+        pp.units = 1 if kv_data_type in (torch.float8_e4m3fn, "float8_e4m3fn") else 0
         # window tables
         zhi16 = [KERNEL_CAP] * 8
         zhi8 = [2 ** 31 - 1] * 16

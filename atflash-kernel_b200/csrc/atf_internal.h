@@ -35,4 +35,10 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // (decode.cu); atf_decode_run and atf_decode_run_exchange add their merges.
 int decode_launch_split(const AtfDecodeParams* p, cudaStream_t st);
 
+namespace decode8 {
+// atf_decode_plan's cut into units, on checked parameters (decode_e4m3.cu).
+int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_host, int32_t items_capacity,
+               int32_t* item_indptr_host, AtfDecodePlan* out);
+}  // namespace decode8
+
 }  // namespace atf

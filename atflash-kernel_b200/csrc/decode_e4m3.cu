@@ -29,13 +29,18 @@
 // where the bf16 decode keeps 8). m and M move only when a score exceeds them by
 // more than 8, so most stages need no maximum over lanes and no pass over O.
 //
-// CTA = (work item of atf_decode_plan, kv head): one producer warp with TMA boxes
-// per page slice (K as 32-byte slabs of two window levels each, only those in the
-// window; V rows of 128 bytes), 8 consumer warps with 16 keys each of a 128-key
-// stage. Two CTAs per SM.
+// CTA = (unit of atf_decode_plan, kv head): one producer warp with TMA boxes per
+// page slice (V rows of 128 bytes, and K's; under a window K as 32-byte slabs of
+// two levels, only those in the window), and 8 consumer warps in two quads that
+// take 64-key stages in turn, 16 keys per warp. Two CTAs per SM. A unit holds
+// pieces of several requests, cut so that all units cost the same: one wave of
+// CTAs, equally long, whatever the requests' lengths; the producer runs through
+// the pieces without a stop while the consumers write each piece's state.
 #include <cuda_fp16.h>
 #include <limits.h>
 #include <math.h>
+
+#include <vector>
 
 #include "atf_internal.h"
 #include "atf_ptx.cuh"
@@ -52,25 +57,35 @@ using decode::ldsm_x4_t;
 using decode::levels_of;
 using decode::movmatrix_t;
 
-constexpr int STAGE_KEYS = 128;
-constexpr int CONSUMERS = 8;
+constexpr int STAGE_KEYS = 64;
+constexpr int CONSUMERS = 8;                          // two quads of 4 warps, alternate stages
 constexpr int THREADS = (CONSUMERS + 1) * 32;
-constexpr int NSTAGE_MAX = 4;
+// Even, so that a slot of the ring is always the same quad's: its waits then see
+// every phase of the slot's barrier (a parity wait one phase early returns at once).
+constexpr int NSTAGE = 4;
+static_assert(NSTAGE % 2 == 0, "a slot belongs to one quad");
 constexpr int SLABS = 4;                              // 32-byte slabs of a K row
 constexpr uint32_t SLAB_BYTES = STAGE_KEYS * 32;
+constexpr uint32_t K_BYTES = SLABS * SLAB_BYTES;
 constexpr uint32_t V_BYTES = STAGE_KEYS * 128;
-constexpr uint32_t RING_BYTES = 3 * (SLABS * SLAB_BYTES + V_BYTES);  // 96 KB
-constexpr int MAX_ITEM_KEYS = 16384;  // atf_decode_plan never makes longer items
-constexpr int MAX_ITEM_PAGES = MAX_ITEM_KEYS / 16 + 2;
-constexpr uint32_t OFF_BAR = RING_BYTES;
-constexpr uint32_t OFF_ABORT = OFF_BAR + 8 * 2 * NSTAGE_MAX;
-constexpr uint32_t OFF_ZB = OFF_ABORT + 8;
-constexpr uint32_t OFF_PAGES = OFF_BAR + 128;
-constexpr uint32_t OFF_SCALES = OFF_PAGES + 4 * MAX_ITEM_PAGES;
-constexpr uint32_t SMEM_BYTES = OFF_SCALES + 8 * MAX_ITEM_PAGES + 1024;
+constexpr uint32_t STAGE_BYTES = K_BYTES + V_BYTES;   // 16 KB
+constexpr uint32_t RING_BYTES = NSTAGE * STAGE_BYTES; // 64 KB
+constexpr uint32_t MERGE_BYTES = 16384;
+constexpr int MAX_UNIT_PAGES = ATF_DECODE_UNIT_PAGES;
+constexpr int MAX_UNIT_ITEMS = ATF_DECODE_UNIT_ITEMS;
+constexpr uint32_t OFF_MERGE = RING_BYTES;
+constexpr uint32_t OFF_STATS = OFF_MERGE + MERGE_BYTES;            // 3 x [CONSUMERS][16] floats
+constexpr uint32_t OFF_META = OFF_STATS + 3 * CONSUMERS * 16 * 4;  // Meta[MAX_UNIT_ITEMS]
+constexpr uint32_t OFF_SCALES = OFF_META + 32 * MAX_UNIT_ITEMS;    // float2[MAX_UNIT_PAGES]
+constexpr uint32_t OFF_PAGES = OFF_SCALES + 8 * MAX_UNIT_PAGES;    // int[MAX_UNIT_PAGES]
+constexpr uint32_t OFF_BAR = OFF_PAGES + 4 * MAX_UNIT_PAGES;
+constexpr uint32_t OFF_ABORT = OFF_BAR + 8 * 2 * NSTAGE;
+constexpr uint32_t SMEM_BYTES = OFF_ABORT + 16 + 1024;
 constexpr uint32_t FULLMASK = 0xffffffffu;
-constexpr float LAZY = 8.f;  // P <= 2^8: exact enough in f16, far from its largest value
-static_assert(OFF_ZB + 8 <= OFF_PAGES && (OFF_SCALES & 7) == 0, "shared memory layout");
+constexpr float LAZY = 8.f;      // P <= 2^8: exact enough in f16, far from its largest value
+constexpr float LOWEST = -1e30f; // a running maximum before any key
+static_assert((OFF_META & 15) == 0 && (OFF_SCALES & 7) == 0 && (OFF_BAR & 7) == 0, "shared memory layout");
+static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
 
 struct Args {
   const __nv_bfloat16* q;
@@ -79,6 +94,7 @@ struct Args {
   const int* indices;
   const int* last_page_len;
   const int* items;
+  int num_items;
   const int64_t* q_pos;
   const int64_t* kv_pos0;
   const float* ks;
@@ -87,18 +103,27 @@ struct Args {
   long long num_pages;
   int Hq, G, page_size, page_shift, rows;
   float scale_log2;
-  int window;
   int zhi16[ATF_MAX_LEVELS];
   float* part_o;
   float* part_lse;
   int* err;
 };
 
-// K tensor maps over (32 bytes of a slab, token, slab, kv head, page); map n-1
-// has the box {32, rows, n, 1, 1}
+// K tensor maps. Under a window: over (32 bytes of a slab, token, slab, kv head,
+// page), map n-1 with the box {32, rows, n, 1, 1}. Without: n[0] alone, as V's.
 struct KMaps {
   CUtensorMap n[SLABS];
 };
+
+// an item of the unit, as staged in shared memory
+struct Meta {
+  int b, k_beg, k_end;
+  int page0;     // first of its pages in the unit's list
+  int list0;     // where those begin in `indices`
+  int first;     // its first page within the request
+  long long zb;  // q_pos - kv_pos0
+};
+static_assert(sizeof(Meta) == 32, "two 16-byte words");
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
@@ -120,9 +145,12 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
+__device__ __forceinline__ void consumers_sync() {
+  __barrier_sync_count(1, CONSUMERS * 32);
+}
 
-// NT: tiles of 8 query heads (the group's size is at most 8 NT)
-template <int NT>
+// NT: tiles of 8 query heads (the group's size is at most 8 NT). WIN: a window.
+template <int NT, bool WIN>
 __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     decode_e4m3_kernel(const __grid_constant__ KMaps tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
   extern __shared__ uint8_t smem_raw[];
@@ -133,135 +161,201 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   const uint32_t sb = (raw + 1023u) & ~1023u;
   uint8_t* sp = smem_raw + (sb - raw);
   auto full_bar = [&](int s) { return sb + OFF_BAR + 8u * s; };
-  auto empty_bar = [&](int s) { return sb + OFF_BAR + 8u * (NSTAGE_MAX + s); };
+  auto empty_bar = [&](int s) { return sb + OFF_BAR + 8u * (NSTAGE + s); };
   volatile int* s_abort = reinterpret_cast<volatile int*>(sp + OFF_ABORT);
-  volatile long long* s_zb = reinterpret_cast<volatile long long*>(sp + OFF_ZB);
+  int* s_total = reinterpret_cast<int*>(sp + OFF_ABORT + 4);  // pages of the unit, -1: refused
+  Meta* s_meta = reinterpret_cast<Meta*>(sp + OFF_META);
   int* s_pages = reinterpret_cast<int*>(sp + OFF_PAGES);
-  float2* s_scale = reinterpret_cast<float2*>(sp + OFF_SCALES);  // (ks, log2 vs) of the item's pages
+  float2* s_scale = reinterpret_cast<float2*>(sp + OFF_SCALES);  // (ks, log2 vs) of the unit's pages
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int item = blockIdx.x, hk = blockIdx.y;
+  const int hk = blockIdx.y;
+  // The unit's items: row x of the plan names its first item (1-based; 0: the
+  // row is a unit of its own, negative: no unit).
+  const int x = blockIdx.x;
+  const int tag = a.items[4 * x + 3];
+  const int next = x + 1 < a.num_items ? a.items[4 * x + 7] : 0;
+  if (tag < 0) return;
+  const int it0 = tag > 0 ? tag - 1 : x;
+  const int n_items = (tag > 0 ? (next > 0 ? next - 1 : a.num_items) : x + 1) - it0;
   // Prologue, part 1: only the plan and the page table, which no kernel of this
   // step writes (it runs before the previous kernel's end under programmatic
-  // dependent launch).
-  const int b = a.items[4 * item + 0];
-  const int k_beg = a.items[4 * item + 1];
-  const int k_end = a.items[4 * item + 2];
-  const int pg0 = a.indptr[b];
-  const int npages = a.indptr[b + 1] - pg0;
-  const long long kv_len =
-      npages > 0 ? static_cast<long long>(npages - 1) * a.page_size + a.last_page_len[b] : 0;
-  // an item starts on a 64-key boundary, lies inside its request and holds at
-  // most MAX_ITEM_KEYS keys; any other is reported and skipped
-  if (k_beg < 0 || k_end < k_beg || (k_beg & 63) || k_end > kv_len || k_end - k_beg > MAX_ITEM_KEYS) {
-    if (tid == 0 && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
-    return;
-  }
-  const int G = a.G, hq0 = hk * G;
-  const int nst = (k_end - k_beg + STAGE_KEYS - 1) / STAGE_KEYS;
-  if (tid == 0) {
-    *s_abort = (a.err != nullptr && *reinterpret_cast<volatile int*>(a.err) != 0) ? 1 : 0;
-    for (int s = 0; s < NSTAGE_MAX; ++s) {
-      mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), CONSUMERS);
+  // dependent launch). An item starts on a 64-key boundary and lies inside its
+  // request; the unit's pages fit the list. Else it is reported and skipped.
+  if (warp == 0) {
+    int total = 0;
+    bool bad = n_items < 1 || n_items > MAX_UNIT_ITEMS || it0 < 0 || it0 + n_items > a.num_items;
+    for (int i0 = 0; !bad && i0 < n_items; i0 += 32) {
+      const int i = i0 + lane;
+      int n = 0;
+      Meta m;
+      bool wrong = false;
+      if (i < n_items) {
+        const int4 row = reinterpret_cast<const int4*>(a.items)[it0 + i];
+        m.b = row.x;
+        m.k_beg = row.y;
+        m.k_end = row.z;
+        const int pg0 = a.indptr[m.b], npages = a.indptr[m.b + 1] - pg0;
+        const long long len =
+            npages > 0 ? static_cast<long long>(npages - 1) * a.page_size + a.last_page_len[m.b] : 0;
+        wrong = m.k_beg < 0 || m.k_end <= m.k_beg || (m.k_beg & 63) || m.k_end > len;
+        m.first = m.k_beg >> a.page_shift;
+        m.list0 = pg0 + m.first;
+        m.zb = len - 1;
+        n = wrong ? 0 : ((m.k_end - 1) >> a.page_shift) - m.first + 1;
+      }
+      int sum = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(FULLMASK, sum, off);
+        if (lane >= off) sum += y;
+      }
+      m.page0 = total + sum - n;
+      if (i < n_items) s_meta[i] = m;
+      // (a page list past MAX_UNIT_PAGES cannot wrap: the sum is checked per 32 items)
+      total += __shfl_sync(FULLMASK, sum, 31);
+      bad = __any_sync(FULLMASK, wrong || n > MAX_UNIT_PAGES) || total > MAX_UNIT_PAGES;
     }
-    fence_mbar_init();
-  }
-  const int first_page = k_beg >> a.page_shift;
-  const int n_item_pages = k_end > k_beg ? ((k_end - 1) >> a.page_shift) - first_page + 1 : 0;
-  if (warp == CONSUMERS) {
-    if (lane < SLABS) tma_prefetch_desc(&tmK.n[lane]);
+    if (lane == 0) {
+      *s_total = bad ? -1 : total;
+      *s_abort = (a.err != nullptr && *reinterpret_cast<volatile int*>(a.err) != 0) ? 1 : 0;
+      if (bad && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
+      for (int s = 0; s < NSTAGE; ++s) {
+        mbar_init(full_bar(s), 1);
+        mbar_init(empty_bar(s), CONSUMERS / 2);
+      }
+      fence_mbar_init();
+    }
+  } else if (warp == CONSUMERS) {
+    if (WIN ? lane < SLABS : lane == 0) tma_prefetch_desc(&tmK.n[lane]);
     if (lane == SLABS) tma_prefetch_desc(&tmV);
   }
-  for (int i = tid; i < n_item_pages; i += THREADS) s_pages[i] = a.indices[pg0 + first_page + i];
+  __syncthreads();
+  const int total_pages = *s_total;
+  if (total_pages < 0) return;
+  // page j of the unit is page j - page0 of the last item with page0 <= j
+  auto item_of_page = [&](int j) {
+    int lo = 0, hi = n_items;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_meta[mid].page0 <= j) lo = mid; else hi = mid;
+    }
+    return lo;
+  };
+  for (int j = tid; j < total_pages; j += THREADS) {
+    const Meta& m = s_meta[item_of_page(j)];
+    s_pages[j] = a.indices[m.list0 + j - m.page0];
+  }
   // Part 2: what a preceding kernel may have written (positions, query, pages,
   // scales) is read from here on.
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (tid == 0) {
-    const long long q_pos = a.q_pos != nullptr ? a.q_pos[b] : kv_len - 1;
-    const long long pos0 = a.kv_pos0 != nullptr ? a.kv_pos0[b] : 0;
-    *s_zb = q_pos - pos0;
+  if (WIN && tid < n_items) {
+    const int b = s_meta[tid].b;
+    const long long q_pos = a.q_pos != nullptr ? a.q_pos[b] : s_meta[tid].zb;
+    s_meta[tid].zb = q_pos - (a.kv_pos0 != nullptr ? a.kv_pos0[b] : 0);
   }
   __syncthreads();
-  const long long zb = *s_zb;
-  int lim[ATF_MAX_LEVELS];  // level i is read by local keys n >= lim[i]
-#pragma unroll
-  for (int i = 0; i < ATF_MAX_LEVELS; ++i)
-    lim[i] = (!a.window || i == 0) ? INT_MIN : key_limit(zb, a.zhi16[i]);
-  // ring geometry of this item: the slabs that its newest key reads
-  const int Sc = k_end > k_beg ? (levels_of(lim, k_end - 1) + 1) >> 1 : SLABS;
-  const uint32_t K_BYTES = static_cast<uint32_t>(Sc) * SLAB_BYTES;
-  const uint32_t STAGE_BYTES = K_BYTES + V_BYTES;
-  const int NSTAGE = min(NSTAGE_MAX, static_cast<int>(RING_BYTES / STAGE_BYTES));
   const AbortCtl ab{s_abort, a.err};
-  const bool start_ok = (*s_abort == 0);
-  const int g = lane >> 2, t4 = lane & 3;
+  if (*s_abort != 0) return;
+  // the window of an item as limits on its local keys: level i is read from lim[i] on
+  auto limit = [&](const Meta& m, int l) { return l == 0 ? INT_MIN : key_limit(m.zb, a.zhi16[l]); };
 
-  // this thread's heads: 8 nt + 2 t4 + {0, 1}
-  float m_s[NT][2], m_u[NT][2], l_run[NT][2], o[NT][8][4];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m_s[nt][0] = m_s[nt][1] = m_u[nt][0] = m_u[nt][1] = -INFINITY;
-    l_run[nt][0] = l_run[nt][1] = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
-  }
-
-  if (start_ok && warp == CONSUMERS) {
+  if (warp == CONSUMERS) {
     // ------------------------------------------------------------ producer
     const int R = a.rows;
     const int slice = lane >> 1, is_v = lane & 1;  // one lane per box
     const int r0 = slice * R;
-    int issued = 0;
-    for (int s = 0; s < nst; ++s) {
-      const int buf = s % NSTAGE;
-      if (!__all_sync(FULLMASK, mbar_wait(empty_bar(buf), ((s / NSTAGE) & 1) ^ 1, ab, kDevErrTimeout))) break;
-      const int k0 = k_beg + s * STAGE_KEYS;
-      const int nkeys = min(STAGE_KEYS, k_end - k0);
-      const bool live = r0 < nkeys && r0 < STAGE_KEYS;
-      int n_slab = 0;
-      if (live) n_slab = (levels_of(lim, min(k0 + r0 + R, k_end) - 1) + 1) >> 1;
-      uint32_t bytes = live ? static_cast<uint32_t>(R) * (is_v ? 128u : 32u * n_slab) : 0u;
-      const uint32_t mine = bytes;
+    int buf = 0, ph = 1, issued = 0;
+    bool ok = true;
+    for (int i = 0; ok && i < n_items; ++i) {
+      const Meta m = s_meta[i];
+      int lim[ATF_MAX_LEVELS];
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) bytes += __shfl_xor_sync(FULLMASK, bytes, off);
-      mbar_arrive_expect_tx_elect(full_bar(buf), bytes);
-      __syncwarp();
-      if (mine != 0) {
-        const int n = k0 + r0;
-        const int page = s_pages[(n >> a.page_shift) - first_page];
-        const int tok = n & (a.page_size - 1);
-        const uint32_t st = sb + buf * STAGE_BYTES;
-        if (is_v)
-          tma_load_4d(st + K_BYTES + static_cast<uint32_t>(r0) * 128u, &tmV, full_bar(buf), 0, tok, hk, page);
-        else
-          tma_load_5d(st + static_cast<uint32_t>(r0 * Sc) * 32u, &tmK.n[n_slab - 1], full_bar(buf), 0, tok, 0, hk,
-                      page);
+      for (int l = 0; l < ATF_MAX_LEVELS; ++l) lim[l] = WIN ? limit(m, l) : INT_MIN;
+      for (int k0 = m.k_beg; k0 < m.k_end; k0 += STAGE_KEYS) {
+        ok = __all_sync(FULLMASK, mbar_wait(empty_bar(buf), ph, ab, kDevErrTimeout));
+        if (!ok) break;
+        const bool live = r0 < STAGE_KEYS && k0 + r0 < m.k_end;
+        int n_slab = SLABS;
+        if (WIN && live) n_slab = (levels_of(lim, min(k0 + r0 + R, m.k_end) - 1) + 1) >> 1;
+        uint32_t bytes = live ? static_cast<uint32_t>(R) * (is_v ? 128u : 32u * n_slab) : 0u;
+#pragma unroll
+        for (int off = 4; off > 0; off >>= 1) bytes += __shfl_xor_sync(FULLMASK, bytes, off);  // lanes 0..7
+        if (lane == 0) mbar_arrive_expect_tx(full_bar(buf), bytes);
+        __syncwarp();
+        if (live) {
+          const int n = k0 + r0;
+          const int page = s_pages[m.page0 + (n >> a.page_shift) - m.first];
+          const int tok = n & (a.page_size - 1);
+          const uint32_t st = sb + buf * STAGE_BYTES;
+          if (is_v)
+            tma_load_4d(st + K_BYTES + static_cast<uint32_t>(r0) * 128u, &tmV, full_bar(buf), 0, tok, hk, page);
+          else if (WIN)
+            tma_load_5d(st + static_cast<uint32_t>(r0) * 128u, &tmK.n[n_slab - 1], full_bar(buf), 0, tok, 0, hk,
+                        page);
+          else
+            tma_load_4d(st + static_cast<uint32_t>(r0) * 128u, &tmK.n[0], full_bar(buf), 0, tok, hk, page);
+        }
+        __syncwarp();
+        ++issued;
+        if (++buf == NSTAGE) {
+          buf = 0;
+          ph ^= 1;
+        }
       }
-      __syncwarp();
-      issued = s + 1;
     }
-    // every copy in flight lands before shared memory is used again
-    for (int s = issued - NSTAGE; s < issued; ++s)
-      if (s >= 0) {
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(full_bar(s % NSTAGE), (s / NSTAGE) & 1))
-          if (globaltimer_ns() - t0 > kWaitLimitNs) break;
-      }
-  } else if (start_ok) {
-    // ------------------------------------------------------------ consumers
-    // the item's scales, once, while the first pages are on their way
-    for (int i = tid; i < n_item_pages; i += CONSUMERS * 32) {
-      const int page = s_pages[i];
-      float2 v = make_float2(0.f, -INFINITY);
-      if (page >= 0 && page < a.num_pages) {
-        const long long at = page * a.ss_page + hk * a.ss_head;
-        v = make_float2(a.ks[at], log2f(a.vs[at]));
-      } else if (a.err != nullptr) {
-        atomicCAS(a.err, 0, kDevErrIndex);
-      }
-      s_scale[i] = v;
+    // every copy in flight lands before the CTA ends
+    for (int s = issued > NSTAGE ? issued - NSTAGE : 0; s < issued; ++s) {
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(full_bar(s % NSTAGE), (s / NSTAGE) & 1))
+        if (globaltimer_ns() - t0 > kWaitLimitNs) break;
     }
+    return;
+  }
+
+  // -------------------------------------------------------------- consumers
+  // the unit's scales, once, while the first pages are on their way
+  for (int j = tid; j < total_pages; j += CONSUMERS * 32) {
+    const int page = s_pages[j];
+    float2 v = make_float2(0.f, -INFINITY);
+    if (page >= 0 && page < a.num_pages) {
+      const long long at = page * a.ss_page + hk * a.ss_head;
+      v = make_float2(a.ks[at], log2f(a.vs[at]));
+    } else if (a.err != nullptr) {
+      atomicCAS(a.err, 0, kDevErrIndex);
+    }
+    s_scale[j] = v;
+  }
+  consumers_sync();
+
+  const int g = lane >> 2, t4 = lane & 3;
+  const int G = a.G, hq0 = hk * G;
+  const int quad = warp >> 2, wq = warp & 3;  // this warp: keys 16 wq .. of every second stage
+  const uint32_t R = static_cast<uint32_t>(a.rows);
+  const int mi = lane >> 3, mr = lane & 7;
+  // ldmatrix rows of the warp's 16 keys, matrices (keys 0-7, chunk c), (keys 8-15, c),
+  // (0-7, c + 1), (8-15, c + 1). Rows of 128 bytes: 16-byte chunks XORed with the row.
+  const uint32_t row = static_cast<uint32_t>(16 * wq) + ((mi & 1) << 3) + mr;
+  uint32_t off[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) off[p] = row * 128u + 16u * ((2u * p + static_cast<uint32_t>(mi >> 1)) ^ (row & 7u));
+  // K under a window: slabs of 32-byte rows per slice, 16-byte halves swapped by bit
+  // 2 of the row
+  const uint32_t in_slice = row % R;
+  const uint32_t koff = (row - in_slice) * 128u + in_slice * 32u +
+                        16u * (static_cast<uint32_t>(mi >> 1) ^ ((in_slice >> 2) & 1u));
+  const uint32_t slab_stride = 32u * R;
+
+  int cur = quad, buf = quad, ph = 0;  // this quad's next stage, its slot and parity
+  int end = 0;                         // stages of the items so far
+  bool ok = true;
+  // (after a wait that ran out the items pass without their stages, through the
+  // same barriers)
+  for (int i = 0; i < n_items; ++i) {
+    const Meta m = s_meta[i];
+    // levels that every key of the last group read, and where the next one begins
+    // (keys come in rising order, their distance falls)
+    int Lmin = 0, next_lim = INT_MIN;
     // q as the B operand, heads as columns: in the MMA of level i, k-rows 2 t4,
     // 2 t4 + 1 are dims 16 i + 4 t4 + {0, 1} and k-rows 2 t4 + {8, 9} dims + {2, 3}
     uint32_t qb[NT][8][2];
@@ -271,14 +365,14 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
       const int h = 8 * nt + g;
       const bool v0 = h < G;
       const __nv_bfloat16* qrow =
-          a.q + static_cast<long long>(b) * a.q_sb + static_cast<long long>(hq0 + (v0 ? h : 0)) * a.q_sh;
+          a.q + static_cast<long long>(m.b) * a.q_sb + static_cast<long long>(hq0 + (v0 ? h : 0)) * a.q_sh;
       float mx = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int l = 0; l < 8; ++l)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t w = v0 ? *reinterpret_cast<const uint32_t*>(qrow + 16 * i + 4 * t4 + 2 * e) : 0u;
-          qb[nt][i][e] = w;
+          const uint32_t w = v0 ? *reinterpret_cast<const uint32_t*>(qrow + 16 * l + 4 * t4 + 2 * e) : 0u;
+          qb[nt][l][e] = w;
           mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))));
         }
       mx = fmaxf(mx, __shfl_xor_sync(FULLMASK, mx, 1));
@@ -288,97 +382,112 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
       const int sh = (mx > 0.f && ex < 255) ? min(14 + 127 - ex, 126) : 0;
       const float up = __uint_as_float(static_cast<uint32_t>(sh + 127) << 23);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int l = 0; l < 8; ++l)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t w = qb[nt][i][e];
-          qb[nt][i][e] = pack_f16(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
+          const uint32_t w = qb[nt][l][e];
+          qb[nt][l][e] = pack_f16(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
         }
       // log2-domain factor of this lane's column head, then of this thread's heads
       const float f = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
       qsl[nt][0] = __shfl_sync(FULLMASK, f, 8 * t4);
       qsl[nt][1] = __shfl_sync(FULLMASK, f, 8 * t4 + 4);
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");  // s_scale is complete
-
-    // this warp's 16 keys of a stage lie in slice 16 warp / R
-    const uint32_t R = static_cast<uint32_t>(a.rows);
-    const uint32_t slice = static_cast<uint32_t>(warp * 16) / R, in_slice = static_cast<uint32_t>(warp * 16) % R;
-    const int mi = lane >> 3, mr = lane & 7;
-    // ldmatrix rows. K: matrices (keys 0-7, level 2p), (keys 8-15, 2p), (0-7, 2p+1),
-    // (8-15, 2p+1) in 32-byte rows, 16-byte halves swapped by bit 2 of the row
-    const uint32_t krow = in_slice + ((mi & 1) << 3) + mr;
-    const uint32_t k_off = slice * R * 32u * static_cast<uint32_t>(Sc) + krow * 32u +
-                           16u * (static_cast<uint32_t>(mi >> 1) ^ ((krow >> 2) & 1u));
-    const uint32_t slab_stride = 32u * R;
-    // V: matrices (keys 0-7, 16 dims), (8-15, same), (0-7, next 16 dims), (8-15, next)
-    // in 128-byte rows whose 16-byte chunks are XORed with the row
-    const uint32_t vrow = static_cast<uint32_t>(warp * 16) + ((mi & 1) << 3) + mr;
-    const uint32_t v_off = vrow * 128u;
-    const uint32_t vx = vrow & 7u;
-
-    for (int s = 0; s < nst; ++s) {
-      const int buf = s % NSTAGE;
-      if (!__all_sync(FULLMASK, mbar_wait(full_bar(buf), (s / NSTAGE) & 1, ab, kDevErrTimeout))) break;
-      const uint32_t kb = sb + buf * STAGE_BYTES + k_off;
-      const uint32_t vb = sb + buf * STAGE_BYTES + K_BYTES + v_off;
-      const int key0 = k_beg + s * STAGE_KEYS + warp * 16;
-      if (key0 < k_end) {
-        const int last = min(key0 + 15, k_end - 1);
-        const int Lmax = levels_of(lim, last), Lmin = levels_of(lim, key0);
-        const float2 sc = s_scale[(key0 >> a.page_shift) - first_page];
+    // this thread's heads: 8 nt + 2 t4 + {0, 1}
+    float m_s[NT][2], m_u[NT][2], l_run[NT][2], o[NT][8][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m_s[nt][0] = m_s[nt][1] = m_u[nt][0] = m_u[nt][1] = LOWEST;
+      l_run[nt][0] = l_run[nt][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+    }
+    const int begin = end;
+    end += (m.k_end - m.k_beg + STAGE_KEYS - 1) / STAGE_KEYS;
+    while (cur < end) {
+      ok = ok && __all_sync(FULLMASK, mbar_wait(full_bar(buf), ph, ab, kDevErrTimeout));
+      if (!ok) break;
+      const uint32_t kb = sb + buf * STAGE_BYTES;
+      const uint32_t vb = kb + K_BYTES;
+      const int key0 = m.k_beg + (cur - begin) * STAGE_KEYS + 16 * wq;
+      if (key0 < m.k_end) {
+        const int last = min(key0 + 15, m.k_end - 1);
+        const bool whole = last == key0 + 15;
+        const float2 sc = s_scale[m.page0 + (key0 >> a.page_shift) - m.first];
         // this thread's keys: key0 + g (c[0], c[1]) and key0 + g + 8 (c[2], c[3])
-        const int key_a = key0 + g, key_b = key0 + g + 8;
-        float c[NT][4];
+        float c[NT][4], c2[NT][4];  // two sums, so that the MMAs wait less for each other
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int p = 0; p < SLABS; ++p) {
-          if (2 * p < Lmax) {
-            uint32_t r[4];
-            ldsm_x4(kb + p * slab_stride, r[0], r[1], r[2], r[3]);
+          for (int e = 0; e < 4; ++e) c[nt][e] = c2[nt][e] = 0.f;
+        if constexpr (!WIN) {
 #pragma unroll
-            for (int hl = 0; hl < 2; ++hl) {
-              const int i = 2 * p + hl;
-              uint32_t a0, a1, a2, a3;
-              e4m3x4_to_f16(r[2 * hl], a0, a2);
-              e4m3x4_to_f16(r[2 * hl + 1], a1, a3);
-              if (i < Lmin) {
+          for (int p = 0; p < SLABS; ++p) {
+            uint32_t r[4], a0, a1, a2, a3;
+            ldsm_x4(kb + off[p], r[0], r[1], r[2], r[3]);
+            e4m3x4_to_f16(r[0], a0, a2);
+            e4m3x4_to_f16(r[1], a1, a3);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_f16(c[nt], a0, a1, a2, a3, qb[nt][i][0], qb[nt][i][1]);
-              } else if (i < Lmax) {
-                // a level that only the newer keys of the group read
-                const bool in_a = key_a >= lim[i], in_b = key_b >= lim[i];
+            for (int nt = 0; nt < NT; ++nt) mma_f16(c[nt], a0, a1, a2, a3, qb[nt][2 * p][0], qb[nt][2 * p][1]);
+            e4m3x4_to_f16(r[2], a0, a2);
+            e4m3x4_to_f16(r[3], a1, a3);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  float t[4] = {0.f, 0.f, 0.f, 0.f};
-                  mma_f16(t, a0, a1, a2, a3, qb[nt][i][0], qb[nt][i][1]);
-                  if (in_a) {
-                    c[nt][0] += t[0];
-                    c[nt][1] += t[1];
-                  }
-                  if (in_b) {
-                    c[nt][2] += t[2];
-                    c[nt][3] += t[3];
+            for (int nt = 0; nt < NT; ++nt)
+              mma_f16(c2[nt], a0, a1, a2, a3, qb[nt][2 * p + 1][0], qb[nt][2 * p + 1][1]);
+          }
+        } else {
+          int Lmax = Lmin;
+          if (last >= next_lim) {  // the keys have come to another level
+            while (Lmin < ATF_MAX_LEVELS && key0 >= limit(m, Lmin)) ++Lmin;
+            next_lim = Lmin < ATF_MAX_LEVELS ? limit(m, Lmin) : INT_MAX;
+            Lmax = Lmin;
+            while (Lmax < ATF_MAX_LEVELS && last >= limit(m, Lmax)) ++Lmax;
+          }
+#pragma unroll
+          for (int p = 0; p < SLABS; ++p) {
+            if (2 * p < Lmax) {
+              uint32_t r[4];
+              ldsm_x4(kb + koff + p * slab_stride, r[0], r[1], r[2], r[3]);
+#pragma unroll
+              for (int hl = 0; hl < 2; ++hl) {
+                const int l = 2 * p + hl;
+                uint32_t a0, a1, a2, a3;
+                e4m3x4_to_f16(r[2 * hl], a0, a2);
+                e4m3x4_to_f16(r[2 * hl + 1], a1, a3);
+                if (l < Lmin) {
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+                    mma_f16(hl ? c2[nt] : c[nt], a0, a1, a2, a3, qb[nt][l][0], qb[nt][l][1]);
+                } else if (l < Lmax) {
+                  // a level that only the newer keys of the group read
+                  const int from = limit(m, l);
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt) {
+                    float t[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_f16(t, a0, a1, a2, a3, qb[nt][l][0], qb[nt][l][1]);
+                    c[nt][0] += key0 + g >= from ? t[0] : 0.f;
+                    c[nt][1] += key0 + g >= from ? t[1] : 0.f;
+                    c[nt][2] += key0 + g + 8 >= from ? t[2] : 0.f;
+                    c[nt][3] += key0 + g + 8 >= from ? t[3] : 0.f;
                   }
                 }
               }
             }
           }
         }
-        const bool ok_a = key_a <= last, ok_b = key_b <= last;
         bool need = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float f0 = qsl[nt][0] * sc.x, f1 = qsl[nt][1] * sc.x;
-          c[nt][0] = ok_a ? c[nt][0] * f0 : -INFINITY;
-          c[nt][1] = ok_a ? c[nt][1] * f1 : -INFINITY;
-          c[nt][2] = ok_b ? c[nt][2] * f0 : -INFINITY;
-          c[nt][3] = ok_b ? c[nt][3] * f1 : -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[nt][e] = (c[nt][e] + c2[nt][e]) * (qsl[nt][e & 1] * sc.x);
+          if (!whole) {
+            if (key0 + g > last) c[nt][0] = c[nt][1] = -INFINITY;
+            if (key0 + g + 8 > last) c[nt][2] = c[nt][3] = -INFINITY;
+          }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float mx = fmaxf(c[nt][e], c[nt][e + 2]);
-            need |= mx > m_s[nt][e] + LAZY || mx + sc.y > m_u[nt][e] + LAZY;
+            const float mx = fmaxf(c[nt][e], c[nt][e + 2]) - LAZY;
+            need |= mx > m_s[nt][e] || mx + sc.y > m_u[nt][e];
           }
         }
         if (__any_sync(FULLMASK, need)) {
@@ -388,10 +497,10 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
             for (int e = 0; e < 2; ++e) {
               float mh = fmaxf(c[nt][e], c[nt][e + 2]);  // over the group's 16 keys
 #pragma unroll
-              for (int off = 4; off < 32; off <<= 1) mh = fmaxf(mh, __shfl_xor_sync(FULLMASK, mh, off));
+              for (int of = 4; of < 32; of <<= 1) mh = fmaxf(mh, __shfl_xor_sync(FULLMASK, mh, of));
               const float ns = fmaxf(m_s[nt][e], mh), nu = fmaxf(m_u[nt][e], mh + sc.y);
-              l_run[nt][e] *= m_s[nt][e] == -INFINITY ? 0.f : ex2f(m_s[nt][e] - ns);
-              const float al = m_u[nt][e] == -INFINITY ? 0.f : ex2f(m_u[nt][e] - nu);
+              l_run[nt][e] *= ex2f(m_s[nt][e] - ns);
+              const float al = ex2f(m_u[nt][e] - nu);
               m_s[nt][e] = ns;
               m_u[nt][e] = nu;
 #pragma unroll
@@ -407,9 +516,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
           float w[4];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float ms = m_s[nt][e] == -INFINITY ? 0.f : m_s[nt][e];
-            const float mu = sc.y - (m_u[nt][e] == -INFINITY ? 0.f : m_u[nt][e]);
-            l_run[nt][e] += ex2f(c[nt][e] - ms) + ex2f(c[nt][e + 2] - ms);
+            const float mu = sc.y - m_u[nt][e];
+            l_run[nt][e] += ex2f(c[nt][e] - m_s[nt][e]) + ex2f(c[nt][e + 2] - m_s[nt][e]);
             w[e] = ex2f(c[nt][e] + mu);
             w[e + 2] = ex2f(c[nt][e + 2] + mu);
           }
@@ -417,93 +525,221 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
           pb[nt][0] = movmatrix_t(pack_f16(w[0], w[1]));
           pb[nt][1] = movmatrix_t(pack_f16(w[2], w[3]));
         }
-        // rows past the item's end may hold anything: their P is 0, so that their V
-        // must be a number (this thread's V elements are keys 2 t4, 2 t4 + 1 of each 8)
-        uint32_t keep0 = FULLMASK, keep1 = FULLMASK;
-        if (last < key0 + 15) {
-          const int k = key0 + 2 * t4;
-          keep0 = (k <= last ? 0x00ff00ffu : 0u) | (k + 1 <= last ? 0xff00ff00u : 0u);
-          keep1 = (k + 8 <= last ? 0x00ff00ffu : 0u) | (k + 9 <= last ? 0xff00ff00u : 0u);
-        }
+        // V: bytes (key, dim 2g), (key, dim 2g + 1), (next key, 2g), (next key, 2g + 1)
+        // are sorted by dim; MMA rows g and g + 8 are dims 2g and 2g + 1 of the chunk
+        auto pv = [&](uint32_t keep0, uint32_t keep1) {
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-          uint32_t r[4];
-          ldsm_x4_t(vb + 16u * ((2u * jj + static_cast<uint32_t>(mi >> 1)) ^ vx), r[0], r[1], r[2], r[3]);
+          for (int jj = 0; jj < 4; ++jj) {
+            uint32_t r[4];
+            ldsm_x4_t(vb + off[jj], r[0], r[1], r[2], r[3]);
 #pragma unroll
-          for (int hl = 0; hl < 2; ++hl) {
-            // bytes (key, dim 2g), (key, dim 2g + 1), (next key, 2g), (next key, 2g + 1):
-            // sort by dim; MMA rows g and g + 8 are dims 2g and 2g + 1 of the chunk
-            uint32_t a0, a1, a2, a3;
-            e4m3x4_to_f16(__byte_perm(r[2 * hl], 0, 0x3120) & keep0, a0, a1);
-            e4m3x4_to_f16(__byte_perm(r[2 * hl + 1], 0, 0x3120) & keep1, a2, a3);
+            for (int hl = 0; hl < 2; ++hl) {
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_f16(__byte_perm(r[2 * hl], 0, 0x3120) & keep0, a0, a1);
+              e4m3x4_to_f16(__byte_perm(r[2 * hl + 1], 0, 0x3120) & keep1, a2, a3);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_f16(o[nt][2 * jj + hl], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+              for (int nt = 0; nt < NT; ++nt)
+                mma_f16(o[nt][2 * jj + hl], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+            }
           }
+        };
+        if (whole) {
+          pv(FULLMASK, FULLMASK);
+        } else {
+          // rows past the item's end may hold anything: their P is 0, so that their V
+          // must be a number (this thread's V elements are keys 2 t4, 2 t4 + 1 of each 8)
+          const int k = key0 + 2 * t4;
+          pv((k <= last ? 0x00ff00ffu : 0u) | (k + 1 <= last ? 0xff00ff00u : 0u),
+             (k + 8 <= last ? 0x00ff00ffu : 0u) | (k + 9 <= last ? 0xff00ff00u : 0u));
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty_bar(buf));
+      cur += 2;
+      buf += 2;
+      if (buf >= NSTAGE) {
+        buf -= NSTAGE;
+        ph ^= 1;
+      }
     }
-  }
-  __syncthreads();
-
-  // merge the consumer warps' states (the ring is free now)
-  constexpr int ROWS = 8 * NT;
-  float* sm_o = reinterpret_cast<float*>(sp);        // [CONSUMERS][ROWS][128]
-  float* sm_s = sm_o + CONSUMERS * ROWS * 128;       // [CONSUMERS][ROWS] each
-  float* sm_u = sm_s + CONSUMERS * ROWS;
-  float* sm_l = sm_u + CONSUMERS * ROWS;
-  if (warp < CONSUMERS) {
+    // ---------------------------------------------------------- the item's state
+    // The 8 warps' states are merged through shared memory of their own, in 2 NT
+    // passes over the dims, while the producer goes on with the next item.
+    constexpr int ROWS = 8 * NT, PASSES = 2 * NT, DP = 128 / PASSES, JP = 8 / PASSES;
+    float* sm_o = reinterpret_cast<float*>(sp + OFF_MERGE);  // [CONSUMERS][ROWS][DP]
+    float* sm_s = reinterpret_cast<float*>(sp + OFF_STATS);  // [CONSUMERS][ROWS] each
+    float* sm_u = sm_s + CONSUMERS * ROWS;
+    float* sm_l = sm_u + CONSUMERS * ROWS;
+    static_assert(CONSUMERS * ROWS * DP * 4 <= MERGE_BYTES, "merge buffer");
+    float l_sum[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         // the sums are per thread (its two keys of each group): add the 8 key rows
-        float l = l_run[nt][e];
+        l_sum[nt][e] = l_run[nt][e];
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(FULLMASK, l, off);
-        const int row = warp * ROWS + 8 * nt + 2 * t4 + e;
-        float2* dst = reinterpret_cast<float2*>(sm_o + row * 128);
+        for (int of = 4; of < 32; of <<= 1) l_sum[nt][e] += __shfl_xor_sync(FULLMASK, l_sum[nt][e], of);
+      }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dst[8 * j + g] = make_float2(o[nt][j][e], o[nt][j][e + 2]);
-        if (g == 0) {
-          sm_s[row] = m_s[nt][e];
-          sm_u[row] = m_u[nt][e];
-          sm_l[row] = l;
+    for (int pass = 0; pass < PASSES; ++pass) {
+      consumers_sync();  // the buffer has been read
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int rw = warp * ROWS + 8 * nt + 2 * t4 + e;
+          float2* dst = reinterpret_cast<float2*>(sm_o + rw * DP);
+#pragma unroll
+          for (int j = 0; j < JP; ++j)
+            dst[8 * j + g] = make_float2(o[nt][JP * pass + j][e], o[nt][JP * pass + j][e + 2]);
+          if (pass == 0 && g == 0) {
+            sm_s[rw] = m_s[nt][e];
+            sm_u[rw] = m_u[nt][e];
+            sm_l[rw] = l_sum[nt][e];
+          }
         }
-      }
-  }
-  __syncthreads();
-  if (!start_ok || *s_abort) return;
-  for (int e = tid; e < G * 32; e += THREADS) {
-    const int row = e >> 5, d = 4 * (e & 31);
-    float ms = -INFINITY, mu = -INFINITY;
+      consumers_sync();
+      for (int e = tid; e < G * (DP / 4); e += CONSUMERS * 32) {
+        const int rw = e / (DP / 4), d = 4 * (e % (DP / 4));
+        float ms = LOWEST, mu = LOWEST;
 #pragma unroll
-    for (int w = 0; w < CONSUMERS; ++w) {
-      ms = fmaxf(ms, sm_s[w * ROWS + row]);
-      mu = fmaxf(mu, sm_u[w * ROWS + row]);
-    }
-    float L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < CONSUMERS; ++w) {
+          ms = fmaxf(ms, sm_s[w * ROWS + rw]);
+          mu = fmaxf(mu, sm_u[w * ROWS + rw]);
+        }
+        float L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < CONSUMERS; ++w) {
-      const float s = sm_s[w * ROWS + row], u = sm_u[w * ROWS + row];
-      L += s == -INFINITY ? 0.f : ex2f(s - ms) * sm_l[w * ROWS + row];
-      if (u != -INFINITY) {
-        const float f = ex2f(u - mu);
-        const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * ROWS + row) * 128 + d);
-        acc.x += f * x.x;
-        acc.y += f * x.y;
-        acc.z += f * x.z;
-        acc.w += f * x.w;
+        for (int w = 0; w < CONSUMERS; ++w) {
+          L += ex2f(sm_s[w * ROWS + rw] - ms) * sm_l[w * ROWS + rw];
+          const float f = ex2f(sm_u[w * ROWS + rw] - mu);
+          const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * ROWS + rw) * DP + d);
+          acc.x += f * v.x;
+          acc.y += f * v.y;
+          acc.z += f * v.z;
+          acc.w += f * v.w;
+        }
+        // every V scale 0: mu is still the lowest, and so is f
+        const float f = L > 0.f ? ex2f(mu - ms) / L : 0.f;
+        const long long at = static_cast<long long>(it0 + i) * a.Hq + hq0 + rw;
+        *reinterpret_cast<float4*>(a.part_o + at * 128 + pass * DP + d) =
+            make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+        if (pass == 0 && d == 0) a.part_lse[at] = L > 0.f ? ms + log2f(L) : -INFINITY;
       }
     }
-    const float f = (L > 0.f && mu != -INFINITY) ? ex2f(mu - ms) / L : 0.f;
-    const long long at = static_cast<long long>(item) * a.Hq + hq0 + row;
-    *reinterpret_cast<float4*>(a.part_o + at * 128 + d) = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
-    if (d == 0) a.part_lse[at] = L > 0.f ? ms + log2f(L) : -INFINITY;
   }
+}
+
+// Units: the requests' 64-key blocks lie on one line, each with the cost of the
+// bytes a CTA reads for it (in 32-byte units: 4 for a V row, 1/2 per in-window level
+// of a K row) and each request's piece with a fixed cost for its state; unit u is
+// the part of the line up to (u + 1) / U of the whole. U fills the slots (two
+// resident CTAs per SM, over the kv heads) in as few waves as the units' limits
+// allow, with at least min_chunk_keys (64) keys per unit.
+int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_host, int32_t items_capacity,
+               int32_t* item_indptr_host, AtfDecodePlan* out) {
+  const int B = p->batch_size, ps = p->page_size;
+  long long cap = static_cast<long long>(MAX_UNIT_PAGES) * ps;  // keys of an item
+  if (cap > 16384) cap = 16384;
+  if (p->max_chunk_keys > 0 && p->max_chunk_keys < cap) cap = p->max_chunk_keys;
+  cap = cap / 64 * 64;
+  if (cap < 64) cap = 64;
+  const long long min_keys = p->min_chunk_keys > 64 ? p->min_chunk_keys : 64;
+  const bool by_bytes = p->window == ATF_WINDOW_SNAP16;
+  constexpr long long ITEM_COST = 64 * 16;  // an item's state: about the time of 64 keys
+  struct Req {
+    long long len, lim[ATF_MAX_LEVELS];
+  };
+  std::vector<Req> reqs(static_cast<size_t>(B));
+  // cost of the keys [n0, n1) of a request, in 16-byte units
+  auto cost = [](const Req& r, long long n0, long long n1) {
+    long long c = 8 * (n1 - n0);
+    for (int i = 0; i < ATF_MAX_LEVELS; ++i) {
+      const long long lo = n0 > r.lim[i] ? n0 : r.lim[i];
+      if (n1 > lo) c += n1 - lo;
+    }
+    return c;
+  };
+  long long whole = 0, keys = 0;
+  for (int b = 0; b < B; ++b) {
+    Req& r = reqs[static_cast<size_t>(b)];
+    const int np = p->indptr_host[b + 1] - p->indptr_host[b];
+    r.len = np > 0 ? static_cast<long long>(np - 1) * ps + p->last_page_len_host[b] : 0;
+    const long long q_pos = p->q_pos_host != nullptr ? p->q_pos_host[b] : r.len - 1;
+    const long long pos0 = p->kv_pos0_host != nullptr ? p->kv_pos0_host[b] : 0;
+    for (int i = 0; i < ATF_MAX_LEVELS; ++i)
+      r.lim[i] = (!by_bytes || i == 0) ? LLONG_MIN / 4 : q_pos - pos0 - static_cast<long long>(p->zhi16[i]);
+    if (r.len > 0) whole += cost(r, 0, r.len) + ITEM_COST;
+    keys += r.len;
+  }
+  long long per_wave = slots / p->num_kv_heads;
+  if (per_wave < 1) per_wave = 1;
+  const long long unit_cap = MAX_UNIT_PAGES * static_cast<long long>(ps) < 16384 ? MAX_UNIT_PAGES * static_cast<long long>(ps) : 16384;
+  long long waves = (keys + per_wave * unit_cap - 1) / (per_wave * unit_cap);
+  long long U = per_wave * (waves < 1 ? 1 : waves);
+  if (U > (keys + min_keys - 1) / min_keys) U = (keys + min_keys - 1) / min_keys;
+  if (U < 1) U = 1;
+  int n = 0, units = 0;
+  long long longest = 0, done = 0;       // cost of everything cut so far
+  long long unit_pages = 0, unit_items = 0;
+  bool open = false;
+  for (int b = 0; b < B; ++b) {
+    const Req& r = reqs[static_cast<size_t>(b)];
+    if (item_indptr_host != nullptr) item_indptr_host[b] = n;
+    long long n0 = 0;
+    while (n0 < r.len) {
+      // the unit in progress is full: by cost, by items or by pages
+      if (!open || done * U >= whole * units || unit_items >= MAX_UNIT_ITEMS || unit_pages >= MAX_UNIT_PAGES) {
+        if (items_host != nullptr) {
+          if (units >= items_capacity) return ATF_ERR_WORKSPACE;
+          items_host[4 * units + 3] = n + 1;
+        }
+        ++units;
+        unit_pages = unit_items = 0;
+        open = true;
+      }
+      done += n0 == 0 ? ITEM_COST : 0;
+      // the first 64-key boundary at which the unit has its share, or the end
+      long long room = (MAX_UNIT_PAGES - unit_pages) * static_cast<long long>(ps);
+      // (an item begins at a multiple of 64, so inside a page of 128 or 256)
+      room -= n0 % ps;
+      if (room > cap) room = cap;
+      room = room / 64 * 64;
+      long long ulo = n0 / 64 + 1, uhi = (r.len + 63) / 64;
+      while (ulo < uhi) {
+        const long long mid = ulo + (uhi - ulo) / 2;
+        if ((done + cost(r, n0, mid * 64 < r.len ? mid * 64 : r.len)) * U >= whole * units) uhi = mid; else ulo = mid + 1;
+      }
+      long long n1 = ulo * 64 < r.len ? ulo * 64 : r.len;
+      if (room < 64) {  // no room for a block: the next unit takes it
+        unit_pages = MAX_UNIT_PAGES;
+        done -= n0 == 0 ? ITEM_COST : 0;
+        continue;
+      }
+      if (n1 - n0 > room) n1 = n0 + room;
+      if (items_host != nullptr) {
+        if (n >= items_capacity) return ATF_ERR_WORKSPACE;
+        items_host[4 * n + 0] = b;
+        items_host[4 * n + 1] = static_cast<int32_t>(n0);
+        items_host[4 * n + 2] = static_cast<int32_t>(n1);
+      }
+      unit_pages += (n1 - 1) / ps - n0 / ps + 1;
+      ++unit_items;
+      done += cost(r, n0, n1);
+      longest = n1 - n0 > longest ? n1 - n0 : longest;
+      n0 = n1;
+      ++n;
+    }
+  }
+  if (items_host != nullptr)
+    for (int i = units; i < n; ++i) items_host[4 * i + 3] = -1;
+  if (item_indptr_host != nullptr) item_indptr_host[B] = n;
+  out->num_items = n;
+  out->chunk_keys = static_cast<int32_t>(longest);
+  out->partial_o_floats = static_cast<int64_t>(n) * p->num_qo_heads * ATF_HEAD_DIM;
+  out->partial_lse_floats = static_cast<int64_t>(n) * p->num_qo_heads;
+  return ATF_OK;
 }
 
 }  // namespace decode8
@@ -554,6 +790,7 @@ extern "C" int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* 
     a.indices = p->indices;
     a.last_page_len = p->last_page_len;
     a.items = p->items;
+    a.num_items = p->num_items;
     a.q_pos = p->q_pos;
     a.kv_pos0 = p->kv_pos0;
     a.ks = sc->k_scale;
@@ -568,7 +805,7 @@ extern "C" int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* 
     while ((1 << a.page_shift) < ps) ++a.page_shift;
     a.rows = ps < 64 ? ps : 64;
     a.scale_log2 = p->sm_scale * 1.4426950408889634f;
-    a.window = p->window == ATF_WINDOW_SNAP16 ? 1 : 0;
+    const bool win = p->window == ATF_WINDOW_SNAP16;
     for (int i = 0; i < ATF_MAX_LEVELS; ++i) a.zhi16[i] = p->zhi16[i];
     a.part_o = p->partial_o;
     a.part_lse = p->partial_lse;
@@ -579,25 +816,30 @@ extern "C" int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* 
     const uint32_t rows = static_cast<uint32_t>(a.rows);
     const uint64_t s_tok = static_cast<uint64_t>(p->kv_stride_token), s_head = stride_b(hkv, p->kv_stride_head),
                    s_page = stride_b(npg, p->kv_stride_page);
-    const uint64_t kdims[5] = {32, static_cast<uint64_t>(ps), decode8::SLABS, hkv, npg};
-    const uint64_t kstr[4] = {s_tok, 32, s_head, s_page};
     const uint64_t vdims[4] = {128, static_cast<uint64_t>(ps), hkv, npg};
     const uint64_t vstr[3] = {s_tok, s_head, s_page};
+    const uint32_t vbox[4] = {128, rows, 1, 1};
     decode8::KMaps tk;
     CUtensorMap tv;
-    for (uint32_t n = 1; n <= decode8::SLABS; ++n) {
-      const uint32_t box[5] = {32, rows, n, 1, 1};
-      // under a window no promotion: the slabs out of the window are not fetched
-      if ((rc = encode_tiled_u8(&tk.n[n - 1], p->k_cache, 5, kdims, kstr, box, CU_TENSOR_MAP_SWIZZLE_32B,
-                                a.window ? CU_TENSOR_MAP_L2_PROMOTION_NONE : CU_TENSOR_MAP_L2_PROMOTION_L2_128B)) !=
-          ATF_OK)
-        return rc;
+    if (win) {
+      const uint64_t kdims[5] = {32, static_cast<uint64_t>(ps), decode8::SLABS, hkv, npg};
+      const uint64_t kstr[4] = {s_tok, 32, s_head, s_page};
+      for (uint32_t n = 1; n <= decode8::SLABS; ++n) {
+        const uint32_t box[5] = {32, rows, n, 1, 1};
+        // no promotion: the slabs out of the window are not fetched
+        if ((rc = encode_tiled_u8(&tk.n[n - 1], p->k_cache, 5, kdims, kstr, box, CU_TENSOR_MAP_SWIZZLE_32B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_NONE)) != ATF_OK)
+          return rc;
+      }
+    } else if ((rc = encode_tiled_u8(&tk.n[0], p->k_cache, 4, vdims, vstr, vbox, CU_TENSOR_MAP_SWIZZLE_128B,
+                                     CU_TENSOR_MAP_L2_PROMOTION_L2_128B)) != ATF_OK) {
+      return rc;
     }
-    const uint32_t vbox[4] = {128, rows, 1, 1};
     if ((rc = encode_tiled_u8(&tv, p->v_cache, 4, vdims, vstr, vbox, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B)) != ATF_OK)
       return rc;
-    auto kern = G > 8 ? decode8::decode_e4m3_kernel<2> : decode8::decode_e4m3_kernel<1>;
+    auto kern = G > 8 ? (win ? decode8::decode_e4m3_kernel<2, true> : decode8::decode_e4m3_kernel<2, false>)
+                      : (win ? decode8::decode_e4m3_kernel<1, true> : decode8::decode_e4m3_kernel<1, false>);
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, decode8::SMEM_BYTES) != cudaSuccess)
       return ATF_ERR_CUDA;
     const dim3 grid(static_cast<unsigned>(p->num_items), static_cast<unsigned>(p->num_kv_heads));

@@ -199,7 +199,16 @@ typedef struct {
   int32_t zhi16[ATF_MAX_LEVELS];
   const int64_t* q_pos_host;
   const int64_t* kv_pos0_host;
+  /* 1: a plan for atf_decode_run_e4m3, whose CTAs each work through a unit of
+   * several items: the requests' keys, one after another, are cut into units of
+   * equal cost (at most ATF_DECODE_UNIT_ITEMS items and ATF_DECODE_UNIT_PAGES
+   * pages each), so that requests of different lengths keep the SMs equally busy.
+   * 0: one item per CTA. Both plans run with both kinds of cache. */
+  int32_t units;
 } AtfDecodePlanParams;
+
+#define ATF_DECODE_UNIT_ITEMS 64
+#define ATF_DECODE_UNIT_PAGES 1024
 
 typedef struct {
   int32_t num_items;       /* work items (request, key range) */
@@ -209,8 +218,9 @@ typedef struct {
 } AtfDecodePlan;
 
 /* Build the split-KV schedule on the host. items_host receives num_items rows
- * of int32[4] = {request, key_begin, key_end, 0}; item_indptr_host receives
- * batch+1 offsets. Pass NULL buffers to query sizes only. Items start on
+ * of int32[4] = {request, key_begin, key_end, unit}, with unit 0, or in a plan
+ * with units, in row u, 1 + the first item of unit u (-1 in the rows past the
+ * last unit); item_indptr_host receives batch+1 offsets. Pass NULL buffers to query sizes only. Items start on
  * multiples of 64 keys and hold at most 16384 keys (atf_decode_run's kernels
  * report longer or unaligned items through error_flag and skip them). */
 int atf_decode_plan(const AtfDecodePlanParams* p, int32_t* items_host, int32_t items_capacity,

@@ -200,7 +200,7 @@ def test_decode_e4m3_strides_stream_pdl_and_graph():
     qw[:, 2:10, :128] = q.to(DEV)
     ws = torch.empty(64 << 20, dtype=torch.uint8, device=DEV)
     w = atflash.BatchDecodeWithPagedKVCacheWrapper(ws, "NHD", use_cuda_graph=True)
-    w.plan(indptr, indices, last, 8, 2, 128, 16)
+    w.plan(indptr, indices, last, 8, 2, 128, 16, kv_data_type=torch.float8_e4m3fn)
     st = torch.cuda.Stream()
     st.wait_stream(torch.cuda.current_stream())
     out = torch.empty((3, 8, 128), dtype=torch.bfloat16, device=DEV)
@@ -278,6 +278,42 @@ def test_decode_e4m3_after_append_equals_the_written_values():
         assert torch.all((rows - x).abs() <= torch.maximum(x.abs() * 2.0 ** -4, s * 2.0 ** -10))
         at += n
     assert atflash.check_device_errors() == 0
+
+
+@pytest.mark.parametrize("window", [None, Z16])
+def test_decode_e4m3_with_either_plan(window):
+    """A plan of one item per CTA, and one of units that run through many requests."""
+    lens = [1, 0, 90, 64, 5, 700, 33, 128, 2, 2, 2, 1300, 65] * 9
+    cache, q, indptr, indices, last = _setup(lens, 32, 8, 2, "HND", 26)
+    want = _exact(cache, q, indptr, indices, lens, "HND", zhi=window)
+    import atflash
+    d = [t.to(DEV) for t in cache]
+    for dtype in ("bfloat16", torch.float8_e4m3fn):
+        w = atflash.BatchDecodeWithPagedKVCacheWrapper(torch.empty(64 << 20, dtype=torch.uint8, device=DEV), "HND")
+        w.plan(indptr, indices, last, 16, 8, 128, 32, kv_data_type=dtype, window_table=window)
+        _close(w.run(q.to(DEV), (d[0], d[2]), kv_scales=(d[1], d[3]), return_lse=True, out_dtype=torch.float32), want)
+    # and the plan of units with a bf16 cache
+    bf = [(d[i].float() * d[i + 1][:, :, None, None]).bfloat16() for i in (0, 2)]
+    a = w.run(q.to(DEV), tuple(bf), out_dtype=torch.float32)
+    w.plan(indptr, indices, last, 16, 8, 128, 32, window_table=window)
+    b = w.run(q.to(DEV), tuple(bf), out_dtype=torch.float32)
+    assert torch.all((a - b).abs() <= 2.0 ** -8 * torch.from_numpy(want[1]).to(DEV) + 1e-30)
+    assert atflash.check_device_errors() == 0
+
+
+@pytest.mark.parametrize("page,layout", [(16, "NHD"), (64, "HND")])
+@pytest.mark.parametrize("window", [None, Z16])
+def test_decode_e4m3_long_units(page, layout, window):
+    """Units of over a hundred stages, so that the ring turns many times, and the same
+    answer from every run."""
+    lens = [9000, 13011, 77, 4032]
+    cache, q, indptr, indices, last = _setup(lens, page, 2, 2, layout, 27)
+    want = _exact(cache, q, indptr, indices, lens, layout, zhi=window)
+    first = _run(cache, q, indptr, indices, last, page, 2, layout, window_table=window, min_chunk_keys=8192)
+    _close(first, want)
+    for _ in range(5):
+        got = _run(cache, q, indptr, indices, last, page, 2, layout, window_table=window, min_chunk_keys=8192)
+        assert torch.equal(got[0], first[0]) and torch.equal(got[1], first[1])
 
 
 def test_decode_e4m3_bad_pages_are_reported():
