@@ -116,6 +116,36 @@ __device__ __forceinline__ void qk_group_asm(uint32_t d_tmem, uint64_t qd, uint6
       ::"r"(d_tmem), "l"(qd), "l"(kd), "r"(idesc), "r"(L), "r"(bar_addr)
       : "memory");
 }
+// The same with Q as two boxes of 64 dims in 128-byte rows (128-byte swizzle, 16
+// KB each): level i advances A by 32 bytes inside a row, and to the next box after
+// four levels.
+__device__ __forceinline__ void qk_group_rows_asm(uint32_t d_tmem, uint64_t qd, uint64_t kd, uint32_t idesc, int L,
+                                                  uint32_t bar_addr) {
+  asm volatile(
+      "{\n\t.reg .pred pe, p1, p2, p3, p4, p5, p6, p7;\n\t.reg .b64 a, b;\n\t"
+      "elect.sync _|pe, 0xffffffff;\n\t"
+      "setp.gt.and.s32 p1, %4, 1, pe;\n\tsetp.gt.and.s32 p2, %4, 2, pe;\n\tsetp.gt.and.s32 p3, %4, 3, pe;\n\t"
+      "setp.gt.and.s32 p4, %4, 4, pe;\n\tsetp.gt.and.s32 p5, %4, 5, pe;\n\tsetp.gt.and.s32 p6, %4, 6, pe;\n\t"
+      "setp.gt.and.s32 p7, %4, 7, pe;\n\t"
+      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, 0;\n\t"
+      "add.u64 a, %1, 2;\n\tadd.u64 b, %2, 256;\n\t"
+      "@p1 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+      "add.u64 a, a, 2;\n\tadd.u64 b, b, 256;\n\t"
+      "@p2 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+      "add.u64 a, a, 2;\n\tadd.u64 b, b, 256;\n\t"
+      "@p3 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+      "add.u64 a, a, 1018;\n\tadd.u64 b, b, 256;\n\t"
+      "@p4 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+      "add.u64 a, a, 2;\n\tadd.u64 b, b, 256;\n\t"
+      "@p5 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+      "add.u64 a, a, 2;\n\tadd.u64 b, b, 256;\n\t"
+      "@p6 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+      "add.u64 a, a, 2;\n\tadd.u64 b, b, 256;\n\t"
+      "@p7 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+      "@pe tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
+      ::"r"(d_tmem), "l"(qd), "l"(kd), "r"(idesc), "r"(L), "r"(bar_addr)
+      : "memory");
+}
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -411,6 +441,13 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
           if (nk[t] == 0) continue;
+          if (RAGGED && a.layout == ATF_LAYOUT_SORTED_PAIR) {
+            // two boxes of 128-byte rows: a sixteenth of the 8-dim boxes' row pieces
+            tma_load_4d_elect(sb + OFF_Q + t * QTILE_BYTES, &tmQ, bar(B_Q), 0, q_tok + row0[t], h, bi);
+            tma_load_4d_elect(sb + OFF_Q + t * QTILE_BYTES + QTILE_BYTES / 2, &tmQ, bar(B_Q), 64, q_tok + row0[t], h,
+                              bi);
+            continue;
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -469,6 +506,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // the start-address field (all offsets stay inside the 14-bit field).
       const uint32_t tm = __shfl_sync(FULL, tmem, 0);
       const uint64_t qdesc0 = make_sdesc(sb + OFF_Q, QHALF_BYTES, 128, kLayoutNone);
+      const uint64_t qrows0 = make_sdesc(sb + OFF_Q, 16, 1024, kLayoutSw128);
       const uint64_t kdesc0 = make_sdesc(sb + OFF_K, KHALF_BYTES, 128, kLayoutNone);
       // sorted-pair K level slabs: 128 keys x 32 B, 32-byte swizzle (SBO = 8 rows)
       const uint64_t kdesc32 = make_sdesc(sb + OFF_K, 16, 256, kLayoutSw32);
@@ -481,7 +519,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t d_tmem = tm + static_cast<uint32_t>(t * 128);
         const uint64_t qd = qdesc0 + ((t * QTILE_BYTES) >> 4);
         const uint64_t kd = (sorted ? kdesc32 : kdesc0) + (((j % KST) * KSTAGE_BYTES) >> 4);
-        qk_group_asm(d_tmem, qd, kd, IDESC_QK, L, bar(B_SFULL + t));
+        if (RAGGED && sorted)
+          qk_group_rows_asm(d_tmem, qrows0 + ((t * QTILE_BYTES) >> 4), kd, IDESC_QK, L, bar(B_SFULL + t));
+        else
+          qk_group_asm(d_tmem, qd, kd, IDESC_QK, L, bar(B_SFULL + t));
       };
       // O_t += P_t(j) V_j; P_t sits in columns 64..127 of the other tile's S
       auto issue_PV = [&](int t, int j) {
@@ -1018,16 +1059,19 @@ extern "C" int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_strea
   auto sane = [](int64_t stride, int64_t size) -> uint64_t {
     return static_cast<uint64_t>(size == 1 ? 16 : stride * 2);
   };
+  const bool sorted = p->qk_layout == ATF_LAYOUT_SORTED_PAIR;
   const uint64_t nq = static_cast<uint64_t>(p->total_q), nk = static_cast<uint64_t>(p->total_k);
   const uint64_t hq = static_cast<uint64_t>(p->num_heads_q), hkv = static_cast<uint64_t>(p->num_heads_kv);
   {
     const uint64_t dims[4] = {128, nq, hq, 1};
     const uint64_t str[3] = {sane(p->q_stride_s, p->total_q), sane(p->q_stride_h, p->num_heads_q), 16};
-    const uint32_t box[4] = {8, static_cast<uint32_t>(BM), 1, 1};
-    if ((rc = encode_tiled_bf16(&tq, p->q, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_NONE)) != ATF_OK) return rc;
+    const uint32_t box[4] = {sorted ? 64u : 8u, static_cast<uint32_t>(BM), 1, 1};
+    if ((rc = encode_tiled_bf16(&tq, p->q, 4, dims, str, box,
+                                sorted ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE)) != ATF_OK)
+      return rc;
   }
   const uint64_t ks = sane(p->k_stride_s, p->total_k), kh = sane(p->k_stride_h, p->num_heads_kv);
-  if (p->qk_layout == ATF_LAYOUT_ROTATE_HALF) {
+  if (!sorted) {
     const uint64_t dims[4] = {128, nk, hkv, 1};
     const uint64_t str[3] = {ks, kh, 16};
     const uint32_t box[4] = {8, static_cast<uint32_t>(BN), 1, 1};
