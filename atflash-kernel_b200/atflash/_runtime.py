@@ -39,6 +39,20 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def launch(name: str, fn, device: torch.device, *args) -> None:
+    """fn(*args, current stream) with `device` current; raises on a non-zero status.
+    (The device guard and a Stream object cost more than the call itself: both are
+    left out where `device` is current already.)"""
+    idx = device.index
+    if idx == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if rc:
+        _ffi.check(name, rc)
+
+
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
     dev = None
     for t in tensors:

@@ -153,9 +153,8 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
         p.k_stride_page, p.k_stride_head, p.k_stride_level = kc.stride(0), kc.stride(1), kc.stride(2)
     if e4m3:
         sc = e4m3_scales(kv_scales)
-        with torch.cuda.device(dev):
-            rc = _ffi.load().atf_paged_kv_append_e4m3(ctypes.byref(p), ctypes.byref(sc), _runtime.stream_handle(dev))
-        _ffi.check("atf_paged_kv_append_e4m3", rc)
+        _runtime.launch("atf_paged_kv_append_e4m3", _ffi.load().atf_paged_kv_append_e4m3, dev, ctypes.byref(p),
+                        ctypes.byref(sc))
         return
     with torch.cuda.device(dev):
         rc = _ffi.load().atf_paged_kv_append(ctypes.byref(p), _runtime.stream_handle(dev))

@@ -325,9 +325,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
             return (out, lse) if return_lse else out
         if kv_scales is not None:
             sc = e4m3_scales(kv_scales)
-            with torch.cuda.device(dev):
-                rc = _ffi.load().atf_decode_run_e4m3(ctypes.byref(a), ctypes.byref(sc), _runtime.stream_handle(dev))
-            _ffi.check("atf_decode_run_e4m3", rc)
+            _runtime.launch("atf_decode_run_e4m3", _ffi.load().atf_decode_run_e4m3, dev, ctypes.byref(a),
+                            ctypes.byref(sc))
             return (out, lse) if return_lse else out
         with torch.cuda.device(dev):
             rc = _ffi.load().atf_decode_run(ctypes.byref(a), _runtime.stream_handle(dev))

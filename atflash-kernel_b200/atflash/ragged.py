@@ -121,9 +121,7 @@ class BatchPrefillWithRaggedKVCacheWrapper:
             p.k_stride_s, p.k_stride_h, _ = k.stride()
             p.v_stride_s, p.v_stride_h, _ = v.stride()
             p.o_stride_s, p.o_stride_h, _ = out.stride()
-            with torch.cuda.device(dev):
-                rc = _ffi.load().atf_prefill_ragged_fwd(ctypes.byref(p), _runtime.stream_handle(dev))
-            _ffi.check("atf_prefill_ragged_fwd", rc)
+            _runtime.launch("atf_prefill_ragged_fwd", _ffi.load().atf_prefill_ragged_fwd, dev, ctypes.byref(p))
         return (out, lse) if return_lse else out
 
     forward = run

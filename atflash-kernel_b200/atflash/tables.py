@@ -32,7 +32,9 @@ class PageTables:
 def _i32(t: torch.Tensor, name: str, n: Optional[int] = None) -> torch.Tensor:
     if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or (n is not None and t.numel() != n):
         raise ValueError(f"{name} must be a 1-d integer tensor" + (f" of {n} entries" if n is not None else ""))
-    return t.to(torch.int32).contiguous()
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        t = t.to(torch.int32).contiguous()
+    return t
 
 
 def build_page_tables(kv_lens: torch.Tensor, append_lens: torch.Tensor, req_pages: torch.Tensor, page_size: int, *,
@@ -93,14 +95,17 @@ def build_page_tables(kv_lens: torch.Tensor, append_lens: torch.Tensor, req_page
         p.free_head, p.free_head_out, p.num_free = free_head.data_ptr(), head_out.data_ptr(), free_pages.numel()
     # one allocation for the 32-bit outputs
     sizes = (B + 1, max_pages, B, B + 1, num_tokens, num_tokens)
-    parts = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes)
+    buf = torch.empty(sum(sizes), dtype=torch.int32, device=dev)
     slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
     p.max_pages, p.max_tokens = int(max_pages), int(num_tokens)
-    p.indptr, p.indices, p.last_page_len, p.append_indptr, p.batch_indices, p.positions = \
-        (t.data_ptr() for t in parts)
+    at = buf.data_ptr()
+    p.indptr = at
+    p.indices = at + 4 * (B + 1)
+    p.last_page_len = p.indices + 4 * max_pages
+    p.append_indptr = p.last_page_len + 4 * B
+    p.batch_indices = p.append_indptr + 4 * (B + 1)
+    p.positions = p.batch_indices + 4 * num_tokens
     p.slot_mapping = slots.data_ptr()
     p.error_flag = _runtime.error_flag(dev).data_ptr()
-    with torch.cuda.device(dev):
-        rc = _ffi.load().atf_build_page_tables(ctypes.byref(p), _runtime.stream_handle(dev))
-    _ffi.check("atf_build_page_tables", rc)
-    return PageTables(*parts, slots, head_out)
+    _runtime.launch("atf_build_page_tables", _ffi.load().atf_build_page_tables, dev, ctypes.byref(p))
+    return PageTables(*buf.split_with_sizes(sizes), slots, head_out)

@@ -7,18 +7,23 @@
 // loses bits only where it falls below e4m3's normal range. A run that begins
 // inside a page keeps the page's scale unless its own amax needs a larger one.
 //
-// One warp owns a (run, kv head), K and V, so the scale's read, its update and
-// the rows under it need no atomics and the result has one value. 8 lanes hold a
-// row (16 elements each), so a warp reads 4 rows of 256 bytes at once and writes
-// 16 bytes per lane. Runs of up to 16 rows stay in registers between the maximum
-// and the rounding; longer ones (pages over 16) are read a second time, from L2.
+// A task is (run, kv head, K or V). Up to 8 warps share a task, 16 rows each, so
+// that runs of large pages are as parallel as those of small ones; they exchange
+// their maxima through shared memory, and the scale's read, its update and the rows
+// under it need no atomics: the result has one value. 8 lanes hold a row (16
+// elements each), so a warp reads 4 rows of 256 bytes at once and writes 16 bytes
+// per lane. Rows stay in registers between the maximum and the rounding (a run over
+// 128 rows, in pages of 256, is read a second time, from L2).
 //
 // What bounds it: HBM for prompts (2 x 256 bytes read and 2 x 128 written per
 // token and head); for one token per request the chain of dependent loads (token
-// -> page list -> scale -> row). A CTA covers a window of tokens and hands its
-// (run, head) pairs to 8 warps; the window shrinks with the token count so that a
-// decode step's tokens spread over the SMs.
+// -> page list -> row). A CTA covers a window of tokens: its first warp finds the
+// runs that begin there, their pages and lengths once, and all warps then go
+// through the tasks. The window shrinks with the token count so that a decode
+// step's tokens spread over the SMs.
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "atf_internal.h"
 #include "rope_math.cuh"
@@ -29,7 +34,7 @@ namespace append8 {
 constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
 constexpr int MAX_WINDOW = 32;
-constexpr int REG_ROWS = 16;  // rows of a run kept in registers: 4 steps of 4
+constexpr int WARP_ROWS = 16;  // rows of a run that a warp keeps in registers: 4 steps of 4
 
 struct Args {
   const __nv_bfloat16* ak;
@@ -40,7 +45,7 @@ struct Args {
   uint8_t* kc;
   uint8_t* vc;
   long long num_pages, s_page, s_tok, s_head;
-  int H, page_size, B, window;
+  int H, page_size, B, window, share, heads;  // share: warps of a task (1, 2, 4 or 8)
   const int32_t* kv_indptr;
   const int32_t* kv_indices;
   float* ks;
@@ -50,7 +55,7 @@ struct Args {
   const float* sn;
   long long cs_stride, n_pos;
   const int64_t* rope_pos;
-  int rope, sorted;
+  int sorted;
   int* err;
 };
 
@@ -99,200 +104,283 @@ __device__ __forceinline__ float mul_odd(float x, float r) {
   return __fmaf_rn(x, r, -q) != 0.f ? __uint_as_float(__float_as_uint(q) | 1u) : q;
 }
 
-// the 16 elements under scale s: the product with 1/s is exact for a power of two
-// (what this kernel writes); a scale set by another program is divided by
+// the 16 elements under a scale that is no power of two (another program's), divided
+// by it; out of line, since this kernel writes powers of two only
+__device__ __noinline__ uint4 divide_words(uint4 lo, uint4 hi, float s) {
+  const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  uint32_t o[4];
+  for (int i = 0; i < 4; ++i) {
+    float f[4];
+    for (int j = 0; j < 2; ++j) {
+      f[2 * j] = div_odd(ropemath::bf2f(w[2 * i + j] & 0xffffu), s);
+      f[2 * j + 1] = div_odd(__uint_as_float(w[2 * i + j] & 0xffff0000u), s);
+    }
+    o[i] = e4m3x2(f[0], f[1]) | (e4m3x2(f[2], f[3]) << 16);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+// the 16 elements under scale s: for a power of two the product with 1/s is exact
 __device__ __forceinline__ void round_words(const Words& x, float s, uint32_t (&o)[4]) {
-  const bool pow2 = (__float_as_uint(s) & 0x7fffffu) == 0;
-  const float inv = __fdiv_rn(1.f, s);
+  if ((__float_as_uint(s) & 0x7fffffu) != 0) {
+    const uint4 v = divide_words(make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]),
+                                 make_uint4(x.w[4], x.w[5], x.w[6], x.w[7]), s);
+    o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+    return;
+  }
+  const float inv = __uint_as_float(0x7f000000u - __float_as_uint(s));  // 2^-e of 2^e, |e| <= 126
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float f[4];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      f[2 * j] = ropemath::bf2f(x.w[2 * i + j] & 0xffffu);
-      f[2 * j + 1] = __uint_as_float(x.w[2 * i + j] & 0xffff0000u);
+      f[2 * j] = __uint_as_float(x.w[2 * i + j] << 16) * inv;
+      f[2 * j + 1] = __uint_as_float(x.w[2 * i + j] & 0xffff0000u) * inv;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = pow2 ? f[j] * inv : div_odd(f[j], s);
     o[i] = e4m3x2(f[0], f[1]) | (e4m3x2(f[2], f[3]) << 16);
   }
 }
 
 // this lane's 16 elements of a row: contiguous (16c..), or for RoPE the 8 pairs
-// (8c.., 64 + 8c..) rotated, as the pairs' words in the order they are written
-__device__ __forceinline__ Words load_plain(const __nv_bfloat16* row, int c) {
+// (8c.., 64 + 8c..)
+__device__ __forceinline__ Words load_row(const __nv_bfloat16* row, int c, bool pairs) {
   Words x;
-  const uint4 a = *reinterpret_cast<const uint4*>(row + 16 * c);
-  const uint4 b = *reinterpret_cast<const uint4*>(row + 16 * c + 8);
+  const uint4 a = *reinterpret_cast<const uint4*>(row + (pairs ? 8 * c : 16 * c));
+  const uint4 b = *reinterpret_cast<const uint4*>(row + (pairs ? 64 + 8 * c : 16 * c + 8));
   x.w[0] = a.x; x.w[1] = a.y; x.w[2] = a.z; x.w[3] = a.w;
   x.w[4] = b.x; x.w[5] = b.y; x.w[6] = b.z; x.w[7] = b.w;
   return x;
 }
-__device__ __forceinline__ Words load_rope(const Args& a, const __nv_bfloat16* row, long long i, int pos, int c) {
-  long long rp = a.rope_pos != nullptr ? a.rope_pos[i] : pos;
-  rp = rp < 0 ? 0 : (rp >= a.n_pos ? a.n_pos - 1 : rp);
-  const float* cr = a.cs + rp * a.cs_stride;
-  const float* sr = a.sn + rp * a.cs_stride;
-  Words x;
-  ropemath::rotate_chunk_sorted_words(row, cr, sr, c, x.w);
-  if (!a.sorted) {
-    // sorted word jl packs (x1, x2) of pair 8c + 7 - jl: back to the halves' order
-    Words y;
+// the 8 pairs rotated as in rope_math.cuh (separately rounded products, then bf16),
+// as words in the order they are written; cr and sr: the position's table rows
+__device__ __forceinline__ Words rotate(const Words& in, const float* cr, const float* sr, int c, bool sorted) {
+  float cv[8], sv[8];
 #pragma unroll
-    for (int i2 = 0; i2 < 4; ++i2) {
-      const uint32_t p0 = x.w[7 - 2 * i2], p1 = x.w[6 - 2 * i2];
-      y.w[i2] = (p0 & 0xffffu) | (p1 << 16);
-      y.w[4 + i2] = (p0 >> 16) | (p1 & 0xffff0000u);
+  for (int q = 0; q < 2; ++q) {
+    const float4 c4 = *reinterpret_cast<const float4*>(cr + 8 * c + 4 * q);
+    const float4 s4 = *reinterpret_cast<const float4*>(sr + 8 * c + 4 * q);
+    cv[4 * q] = c4.x; cv[4 * q + 1] = c4.y; cv[4 * q + 2] = c4.z; cv[4 * q + 3] = c4.w;
+    sv[4 * q] = s4.x; sv[4 * q + 1] = s4.y; sv[4 * q + 2] = s4.z; sv[4 * q + 3] = s4.w;
+  }
+  float r1[8], r2[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t l2 = in.w[e >> 1], h2 = in.w[4 + (e >> 1)];
+    const float x1 = (e & 1) ? __uint_as_float(l2 & 0xffff0000u) : __uint_as_float(l2 << 16);
+    const float x2 = (e & 1) ? __uint_as_float(h2 & 0xffff0000u) : __uint_as_float(h2 << 16);
+    r1[e] = __fsub_rn(__fmul_rn(x1, cv[e]), __fmul_rn(x2, sv[e]));
+    r2[e] = __fadd_rn(__fmul_rn(x2, cv[e]), __fmul_rn(x1, sv[e]));
+  }
+  Words x;
+  if (sorted) {  // pairs in falling order, (x1, x2) adjacent
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x.w[7 - e] = ropemath::pack_rn(r1[e], r2[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x.w[e] = ropemath::pack_rn(r1[2 * e], r1[2 * e + 1]);
+      x.w[4 + e] = ropemath::pack_rn(r2[2 * e], r2[2 * e + 1]);
     }
-    return y;
   }
   return x;
 }
 
-template <bool ROPE>
-__device__ __forceinline__ Words load_k(const Args& a, const __nv_bfloat16* row, long long i, int pos, int c) {
-  if constexpr (ROPE) return load_rope(a, row, i, pos, c);
-  else return load_plain(row, c);
-}
-template <bool ROPE>
-__device__ __forceinline__ void store_k(const Args& a, uint8_t* row, int c, const uint32_t (&o)[4]) {
-  if (ROPE && !a.sorted) {
-    *reinterpret_cast<uint2*>(row + 8 * c) = make_uint2(o[0], o[1]);
-    *reinterpret_cast<uint2*>(row + 64 + 8 * c) = make_uint2(o[2], o[3]);
-  } else {
-    *reinterpret_cast<uint4*>(row + 16 * (ROPE ? 7 - c : c)) = make_uint4(o[0], o[1], o[2], o[3]);
-  }
-}
-
 // rows [0, n) of a page under the scale s_new instead of s_old; s_new is a power of
 // two here (a scale only grows to one), so the ratio is exact
-__device__ __forceinline__ void round_again(uint8_t* page_row0, long long s_tok, int n, float s_old, float s_new,
-                                            int lane) {
+__device__ __forceinline__ void round_again(uint8_t* page_row0, long long s_tok, int first, int step, int n,
+                                            float s_old, float s_new, int c) {
   const float ratio = __fdiv_rn(s_old, s_new);
-  for (int r = lane >> 3; r < n; r += 4) {
-    uint4* at = reinterpret_cast<uint4*>(page_row0 + r * s_tok + 16 * (lane & 7));
+  for (int r = first; r < n; r += step) {
+    uint4* at = reinterpret_cast<uint4*>(page_row0 + r * s_tok + 16 * c);
     const uint4 v = *at;
     const uint32_t in[4] = {v.x, v.y, v.z, v.w};
     uint32_t out[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 a = e4m3x2_to_f32(in[i] & 0xffffu), b = e4m3x2_to_f32(in[i] >> 16);
-      out[i] = e4m3x2(mul_odd(a.x, ratio), mul_odd(a.y, ratio)) | (e4m3x2(mul_odd(b.x, ratio), mul_odd(b.y, ratio)) << 16);
+      out[i] = e4m3x2(mul_odd(a.x, ratio), mul_odd(a.y, ratio)) |
+               (e4m3x2(mul_odd(b.x, ratio), mul_odd(b.y, ratio)) << 16);
     }
     *at = make_uint4(out[0], out[1], out[2], out[3]);
   }
 }
 
-template <bool ROPE>
-__global__ void __launch_bounds__(THREADS) append_e4m3_kernel(const Args a) {
-  __shared__ int s_lead[MAX_WINDOW];
-  __shared__ int s_n;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long i0 = static_cast<long long>(blockIdx.x) * a.window;
-  // the runs that begin in this window: a token begins one unless the token before
-  // it is its predecessor in the same page
-  if (warp == 0) {
-    const long long i = i0 + lane;
-    bool lead = false;
-    if (lane < a.window && i < a.nnz) {
-      const int b = a.batch_indices[i], pos = a.positions[i];
-      lead = b >= 0;
-      if (lead && i > 0 && pos > 0 && pos % a.page_size != 0)
-        lead = !(a.batch_indices[i - 1] == b && a.positions[i - 1] == pos - 1);
-    }
-    const unsigned m = __ballot_sync(0xffffffffu, lead);
-    if (lead) s_lead[__popc(m & ((1u << lane) - 1u))] = lane;
-    if (lane == 0) s_n = __popc(m);
+// A run: the tokens i .. i + n - 1 of the window, from slot `slot` of page `page` on
+struct Run {
+  long long page;
+  int i, n, slot, pos;
+};
+
+// The runs that begin in the CTA's window of tokens, by its first warp. A token
+// begins one unless the token before it is its predecessor in the same page; a run
+// ends before the next one, a padding token or the page's end. Runs with a page
+// that is not the request's or the cache's are reported and left out.
+__device__ __forceinline__ int find_runs(const Args& a, long long i0, Run* runs, int lane) {
+  const long long i = i0 + lane;
+  const bool in = lane < a.window && i < a.nnz;
+  int b = -1, pos = 0;
+  if (in) {
+    b = a.batch_indices[i];
+    pos = a.positions[i];
   }
-  __syncthreads();
-  const int tasks = s_n * a.H;
-  for (int task = warp; task < tasks; task += WARPS) {
-    const long long i = i0 + s_lead[task / a.H];
-    const int h = task % a.H;
-    const int b = a.batch_indices[i], pos = a.positions[i];
-    bool bad = b >= a.B || pos < 0;
-    long long page = -1;
-    if (!bad) {
-      const long long pidx = static_cast<long long>(a.kv_indptr[b]) + pos / a.page_size;
-      bad = pidx >= a.kv_indptr[b + 1];
-      if (!bad) {
-        page = a.kv_indices[pidx];
-        bad = page < 0 || page >= a.num_pages;
-      }
+  bool lead = in && b >= 0;
+  if (lead && i > 0 && pos > 0 && pos % a.page_size != 0)
+    lead = !(a.batch_indices[i - 1] == b && a.positions[i - 1] == pos - 1);
+  const unsigned leads = __ballot_sync(0xffffffffu, lead);
+  const unsigned stops = __ballot_sync(0xffffffffu, lead || (in && b < 0));
+  bool good = lead && b < a.B && pos >= 0;
+  long long page = -1;
+  if (good) {
+    const long long pidx = static_cast<long long>(a.kv_indptr[b]) + pos / a.page_size;
+    good = pidx < a.kv_indptr[b + 1];
+    if (good) {
+      page = a.kv_indices[pidx];
+      good = page >= 0 && page < a.num_pages;
     }
-    if (bad) {  // the run is skipped
-      if (a.err != nullptr && lane == 0) atomicCAS(a.err, 0, kDevErrIndex);
-      continue;
-    }
-    const int slot = pos % a.page_size;
-    // length of the run
-    int n = 0;
-    const int most = static_cast<int>(min(static_cast<long long>(a.page_size - slot), a.nnz - i));
-    while (n < most) {
-      const int j = n + lane;
-      const bool in = j < most && a.batch_indices[i + j] == b && a.positions[i + j] == pos + j;
-      const unsigned out = ~__ballot_sync(0xffffffffu, in);
+  }
+  if (lead && !good && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
+  const int tokens = static_cast<int>(min(static_cast<long long>(a.window), a.nnz - i0));
+  // inside the window a run ends at the next stop
+  const unsigned later = lane < 31 ? stops >> (lane + 1) : 0u;
+  int n = later != 0 ? __ffs(later) : tokens - lane;
+  // the last run may go on past the window
+  const unsigned open = __ballot_sync(0xffffffffu, lead && later == 0);
+  if (open != 0) {
+    const int l = __ffs(open) - 1;
+    const int ob = __shfl_sync(0xffffffffu, b, l), opos = __shfl_sync(0xffffffffu, pos, l);
+    const int most = a.page_size - (opos >= 0 ? opos % a.page_size : 0);
+    int on = tokens - l;
+    while (on < most) {
+      const long long j = i0 + l + on + lane;
+      const bool same = on + lane < most && j < a.nnz && a.batch_indices[j] == ob && a.positions[j] == opos + on + lane;
+      const unsigned out = ~__ballot_sync(0xffffffffu, same);
       if (out != 0) {
-        n += __ffs(out) - 1;
+        on += __ffs(out) - 1;
         break;
       }
-      n += 32;
+      on += 32;
     }
-    const long long src0 = i * a.as_n + static_cast<long long>(h) * a.as_h;
-    const long long dst0 = page * a.s_page + static_cast<long long>(h) * a.s_head;
-    const long long sc = page * a.ss_page + static_cast<long long>(h) * a.ss_head;
-    const float ks_old = slot > 0 ? a.ks[sc] : 0.f, vs_old = slot > 0 ? a.vs[sc] : 0.f;
-    const int c = lane & 7, r0 = lane >> 3;
-    const bool in_regs = n <= REG_ROWS;
-    Words kw[REG_ROWS / 4], vw[REG_ROWS / 4];
-    float km = 0.f, vm = 0.f;
-    for (int base = 0; base < n; base += REG_ROWS) {
+    if (lane == l) n = on;
+  }
+  const unsigned goods = __ballot_sync(0xffffffffu, good);
+  if (good) {
+    Run r;
+    r.page = page;
+    r.i = lane;
+    r.slot = pos % a.page_size;
+    r.n = min(n, a.page_size - r.slot);
+    r.pos = pos;
+    runs[__popc(goods & ((1u << lane) - 1u))] = r;
+  }
+  return __popc(goods);
+}
+
+template <bool ROPE>
+__global__ void __launch_bounds__(THREADS, 3) append_e4m3_kernel(const Args a) {
+  __shared__ Run s_run[MAX_WINDOW];
+  __shared__ int s_n;
+  __shared__ float s_max[2][WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const long long i0 = static_cast<long long>(blockIdx.x) * a.window;
+  if (warp == 0) {
+    const int n = find_runs(a, i0, s_run, lane);
+    if (lane == 0) s_n = n;
+  }
+  __syncthreads();
+  // this CTA's heads: a block's y takes `heads` of them
+  const int h0 = static_cast<int>(blockIdx.y) * a.heads, nh = min(a.heads, a.H - h0);
+  const int tasks = s_n * nh * 2;
+  const int W = a.share, wi = warp & (W - 1), slots = WARPS / W;
+  const int c = lane & 7, r0 = wi * WARP_ROWS + (lane >> 3), step = W * WARP_ROWS;
+  int turn = 0;
+  for (int base = 0; base < tasks; base += slots, turn ^= 1) {
+    const int task = base + warp / W;
+    const bool live = task < tasks;
+    // K and V of a (run, head) are neighbouring tasks; idle warps repeat the last
+    const int t = live ? task : tasks - 1;
+    const bool is_v = t & 1;
+    const int h = h0 + (t >> 1) % nh;
+    const Run run = s_run[(t >> 1) / nh];
+    const int n = live ? run.n : 0;
+    const __nv_bfloat16* src = (is_v ? a.av : a.ak) + (i0 + run.i) * a.as_n + static_cast<long long>(h) * a.as_h;
+    uint8_t* page0 = (is_v ? a.vc : a.kc) + run.page * a.s_page + static_cast<long long>(h) * a.s_head;
+    float* scale = (is_v ? a.vs : a.ks) + run.page * a.ss_page + static_cast<long long>(h) * a.ss_head;
+    const bool rot = ROPE && !is_v;
+    const float s_old = run.slot > 0 && live ? *scale : 0.f;
+    Words w[WARP_ROWS / 4];
+    // Rows b0 + r0 + 4 u: all loads are issued before the first is used, without a
+    // branch between them; rows past the run's end read its last row again, which
+    // changes no maximum, and are not written.
+    auto load = [&](int b0, auto steps) {
+      constexpr int U = decltype(steps)::value;
+      int r[U];
 #pragma unroll
-      for (int u = 0; u < REG_ROWS / 4; ++u) {
-        const int r = base + 4 * u + r0;
-        if (r < n) {
-          kw[u] = load_k<ROPE>(a, a.ak + src0 + r * a.as_n, i + r, pos + r, c);
-          vw[u] = load_plain(a.av + src0 + r * a.as_n, c);
+      for (int u = 0; u < U; ++u) {
+        r[u] = min(b0 + r0 + 4 * u, n - 1);
+        w[u] = load_row(src + r[u] * a.as_n, c, rot);
+      }
+      if (rot) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          long long rp = a.rope_pos != nullptr ? a.rope_pos[i0 + run.i + r[u]] : run.pos + r[u];
+          rp = rp < 0 ? 0 : (rp >= a.n_pos ? a.n_pos - 1 : rp);
+          w[u] = rotate(w[u], a.cs + rp * a.cs_stride, a.sn + rp * a.cs_stride, c, a.sorted != 0);
         }
       }
+    };
+    const std::integral_constant<int, 1> one{};
+    const std::integral_constant<int, WARP_ROWS / 4> all{};
+    const bool few = n <= 4 && W == 1;  // a step of a decode: one row of the four
+    float m = 0.f;
+    if (few) {
+      if (n > 0) {
+        load(0, one);
+        m = abs_max(w[0], m);
+      }
+    } else {
+      for (int b0 = 0; b0 < n; b0 += step) {
+        load(b0, all);
 #pragma unroll
-      for (int u = 0; u < REG_ROWS / 4; ++u)
-        if (base + 4 * u + r0 < n) {
-          km = abs_max(kw[u], km);
-          vm = abs_max(vw[u], vm);
-        }
+        for (int u = 0; u < WARP_ROWS / 4; ++u) m = abs_max(w[u], m);
+      }
     }
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, off));
-      vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, off));
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    if (W > 1) {
+      if (lane == 0) s_max[turn][warp] = m;
+      __syncthreads();  // also: every warp of the task has read the old scale
+      for (int k = 0; k < W; ++k) m = fmaxf(m, s_max[turn][(warp & ~(W - 1)) + k]);
     }
-    const float ks_new = slot > 0 ? fmaxf(ks_old, scale_for(km)) : scale_for(km);
-    const float vs_new = slot > 0 ? fmaxf(vs_old, scale_for(vm)) : scale_for(vm);
-    if (slot > 0 && ks_new != ks_old) round_again(a.kc + dst0, a.s_tok, slot, ks_old, ks_new, lane);
-    if (slot > 0 && vs_new != vs_old) round_again(a.vc + dst0, a.s_tok, slot, vs_old, vs_new, lane);
-    for (int base = 0; base < n; base += REG_ROWS) {
+    const float s_new = run.slot > 0 ? fmaxf(s_old, scale_for(m)) : scale_for(m);
+    if (!live) continue;
+    if (run.slot > 0 && s_new != s_old)
+      round_again(page0, a.s_tok, wi * 4 + (lane >> 3), 4 * W, run.slot, s_old, s_new, c);
+    auto store = [&](int b0, auto steps) {
+      constexpr int U = decltype(steps)::value;
 #pragma unroll
-      for (int u = 0; u < REG_ROWS / 4; ++u) {
-        const int r = base + 4 * u + r0;
+      for (int u = 0; u < U; ++u) {
+        const int r = b0 + r0 + 4 * u;
+        uint32_t o[4];
+        round_words(w[u], s_new, o);
         if (r < n) {
-          if (!in_regs) {
-            kw[u] = load_k<ROPE>(a, a.ak + src0 + r * a.as_n, i + r, pos + r, c);
-            vw[u] = load_plain(a.av + src0 + r * a.as_n, c);
+          uint8_t* dst = page0 + static_cast<long long>(run.slot + r) * a.s_tok;
+          if (rot && !a.sorted) {
+            *reinterpret_cast<uint2*>(dst + 8 * c) = make_uint2(o[0], o[1]);
+            *reinterpret_cast<uint2*>(dst + 64 + 8 * c) = make_uint2(o[2], o[3]);
+          } else {
+            *reinterpret_cast<uint4*>(dst + 16 * (rot ? 7 - c : c)) = make_uint4(o[0], o[1], o[2], o[3]);
           }
-          const long long dst = dst0 + static_cast<long long>(slot + r) * a.s_tok;
-          uint32_t o[4];
-          round_words(kw[u], ks_new, o);
-          store_k<ROPE>(a, a.kc + dst, c, o);
-          round_words(vw[u], vs_new, o);
-          *reinterpret_cast<uint4*>(a.vc + dst + 16 * c) = make_uint4(o[0], o[1], o[2], o[3]);
         }
       }
+    };
+    if (few) {
+      store(0, one);
+    } else {
+      for (int b0 = 0; b0 < n; b0 += step) {
+        if (n > step) load(b0, all);
+        store(b0, all);
+      }
     }
-    if (lane == 0) {
-      a.ks[sc] = ks_new;
-      a.vs[sc] = vs_new;
-    }
+    if (lane == 0 && wi == 0) *scale = s_new;
   }
 }
 
@@ -314,6 +402,7 @@ extern "C" int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvSca
   if (rope && (p->n_pos < 1 || p->cs_stride_pos < 64)) return ATF_ERR_INVALID_ARG;
   if (p->out_layout != ATF_LAYOUT_SORTED_PAIR && p->out_layout != ATF_LAYOUT_ROTATE_HALF)
     return ATF_ERR_INVALID_ARG;
+  if (rope && (!aligned16(p->cos) || !aligned16(p->sin) || (p->cs_stride_pos & 3))) return ATF_ERR_ALIGNMENT;
   if (!aligned16(p->append_k) || !aligned16(p->append_v) || !aligned16(p->k_cache) || !aligned16(p->v_cache) ||
       (p->a_stride_n & 7) || (p->a_stride_h & 7) || (p->kv_stride_page & 15) || (p->kv_stride_token & 15) ||
       (p->kv_stride_head & 15))
@@ -350,18 +439,27 @@ extern "C" int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvSca
   a.cs_stride = p->cs_stride_pos;
   a.n_pos = p->n_pos;
   a.rope_pos = p->rope_positions;
-  a.rope = rope ? 1 : 0;
   a.sorted = p->out_layout == ATF_LAYOUT_SORTED_PAIR ? 1 : 0;
   a.err = p->error_flag;
-  // tokens per CTA: about four CTAs per SM, between 1 and 32 tokens
+  // warps per task: a page's rows, 16 each
+  a.share = 1;
+  while (a.share < append8::WARPS && a.share * append8::WARP_ROWS < a.page_size) a.share <<= 1;
+  // tokens per CTA: the most, up to 32, that give every SM a CTA
   a.window = append8::MAX_WINDOW;
-  while (a.window > 1 && (a.nnz + a.window - 1) / a.window < 4 * 148) a.window >>= 1;
+  while (a.window > 1 && (a.nnz + a.window - 1) / a.window < 148) a.window >>= 1;
   const long long blocks = (a.nnz + a.window - 1) / a.window;
   if (blocks > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  // few CTAs with more tasks than warps: the heads go to several
+  const long long runs = a.window / p->page_size + 1;  // that a window may begin, for one request
+  const long long at_once = append8::WARPS / a.share;
+  int split = 1;
+  while (split < a.H && blocks * split < 2 * 148 && runs * ((a.H + split - 1) / split) * 2 > at_once) split <<= 1;
+  a.heads = (a.H + split - 1) / split;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((a.H + a.heads - 1) / a.heads));
   if (rope)
-    append8::append_e4m3_kernel<true><<<static_cast<unsigned>(blocks), append8::THREADS, 0, st>>>(a);
+    append8::append_e4m3_kernel<true><<<grid, append8::THREADS, 0, st>>>(a);
   else
-    append8::append_e4m3_kernel<false><<<static_cast<unsigned>(blocks), append8::THREADS, 0, st>>>(a);
+    append8::append_e4m3_kernel<false><<<grid, append8::THREADS, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
 }

@@ -21,7 +21,8 @@ namespace tables {
 
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
-constexpr int ENTRIES_PER_CTA = THREADS * 4;
+constexpr int PER_LANE = 4;  // entries of a lane in one step
+constexpr int CHUNK = 32 * PER_LANE;
 
 struct Args {
   const int32_t* kv_lens;
@@ -83,18 +84,27 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool first_cta = blockIdx.x == 0;
 
-  // each thread sums a run of requests; the runs' sums are scanned over the CTA.
-  // 64-bit sums: the offsets are cut at the capacities, the sums need not fit.
+  // The requests, read side by side into shared memory (n, new tokens, owned
+  // pages), then summed run by run: each thread a run of `per`, the runs' sums
+  // scanned over the CTA. 64-bit sums: the offsets are cut at the capacities, the
+  // sums need not fit.
+  bool bad = false;
+  for (int b = tid; b < a.B; b += THREADS) {
+    const Req r = load_req(a, b);
+    bad |= r.bad;
+    s_page[b] = r.n;
+    s_tok[b] = r.app;
+    s_have[b] = r.have;
+    if (first_cta) a.last[b] = r.n > 0 ? r.len - (r.n - 1) * a.page : 0;
+  }
+  __syncthreads();
   const int per = (a.B + THREADS - 1) / THREADS;
   const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
   long long sum[3] = {0, 0, 0};
-  bool bad = false;
   for (int b = b0; b < b1; ++b) {
-    const Req r = load_req(a, b);
-    bad |= r.bad;
-    sum[0] += r.n;
-    sum[1] += r.app;
-    sum[2] += r.n - r.have;
+    sum[0] += s_page[b];
+    sum[1] += s_tok[b];
+    sum[2] += s_page[b] - s_have[b];
   }
   long long incl[3];
 #pragma unroll
@@ -121,23 +131,15 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
     incl[k] += before - sum[k];  // exclusive
     total[k] = all;
   }
-  for (int b = b0; b < b1; ++b) {
-    const Req r = load_req(a, b);
-    const int p = static_cast<int>(min(incl[0], static_cast<long long>(a.cap_pages)));
-    const int t = static_cast<int>(min(incl[1], static_cast<long long>(a.cap_tokens)));
-    s_page[b] = p;
-    s_tok[b] = t;
+  for (int b = b0; b < b1; ++b) {  // each thread turns its own run into offsets
+    const int n = s_page[b], app = s_tok[b];
+    s_page[b] = static_cast<int>(min(incl[0], static_cast<long long>(a.cap_pages)));
+    s_tok[b] = static_cast<int>(min(incl[1], static_cast<long long>(a.cap_tokens)));
     // past the free list's end every index is refused, so a cut keeps its meaning
     s_new[b] = static_cast<int>(min(incl[2], static_cast<long long>(0x3fffffff)));
-    s_have[b] = r.have;
-    if (first_cta) {
-      a.indptr[b] = p;
-      a.aptr[b] = t;
-      a.last[b] = r.n > 0 ? r.len - (r.n - 1) * a.page : 0;
-    }
-    incl[0] += r.n;
-    incl[1] += r.app;
-    incl[2] += r.n - r.have;
+    incl[0] += n;
+    incl[1] += app;
+    incl[2] += n - s_have[b];
   }
   const int n_pages = static_cast<int>(min(total[0], static_cast<long long>(a.cap_pages)));
   const int n_tok = static_cast<int>(min(total[1], static_cast<long long>(a.cap_tokens)));
@@ -154,44 +156,82 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
     }
     if (bad && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
   }
+  if (tid == 0) {  // the ends, for the walk below
+    s_page[a.B] = 0x7fffffff;
+    s_tok[a.B] = 0x7fffffff;
+  }
   __syncthreads();
+  if (first_cta)
+    for (int b = tid; b < a.B; b += THREADS) {
+      a.indptr[b] = s_page[b];
+      a.aptr[b] = s_tok[b];
+    }
 
   // page j of request b: its table's, or a new one
   auto new_page = [&](int b, int j) -> int {
     const long long at = head + s_new[b] + (j - s_have[b]);
     return at >= 0 && head >= 0 && at < a.F ? a.free_pages[at] : -1;
   };
-  const long long stride = static_cast<long long>(gridDim.x) * THREADS;
-  for (long long e = static_cast<long long>(blockIdx.x) * THREADS + tid; e < a.cap_pages; e += stride) {
-    int id = -1;
-    if (e < n_pages) {
-      const int b = bracket(s_page, a.B, static_cast<int>(e));
-      const int j = static_cast<int>(e) - s_page[b];
-      const long long row = a.req_rows != nullptr ? a.req_rows[b] : b;
-      int32_t* at = a.req_pages + row * a.req_stride + j;
-      if (j < s_have[b]) {
-        id = *at;
-      } else {
-        id = new_page(b, j);
-        *at = id;
+  // A warp takes chunks of 128 entries: one search for the chunk's first entry, and
+  // from there each lane walks to the requests of its four (a chunk meets few).
+  const int gw = static_cast<int>(blockIdx.x) * WARPS + warp, nw = static_cast<int>(gridDim.x) * WARPS;
+  for (long long e0 = static_cast<long long>(gw) * CHUNK; e0 < a.cap_pages; e0 += static_cast<long long>(nw) * CHUNK) {
+    int b = e0 < n_pages ? bracket(s_page, a.B, static_cast<int>(e0)) : 0;
+    int id[PER_LANE];
+    int32_t* put[PER_LANE];
+#pragma unroll
+    for (int k = 0; k < PER_LANE; ++k) {
+      const long long e = e0 + 32 * k + lane;
+      id[k] = -1;
+      put[k] = nullptr;
+      if (e < n_pages) {
+        while (s_page[b + 1] <= e) ++b;
+        const int j = static_cast<int>(e) - s_page[b];
+        const long long row = a.req_rows != nullptr ? a.req_rows[b] : b;
+        int32_t* at = a.req_pages + row * a.req_stride + j;
+        if (j < s_have[b]) {
+          id[k] = *at;
+        } else {
+          id[k] = new_page(b, j);
+          put[k] = at;
+        }
       }
     }
-    a.indices[e] = id;
-  }
-  for (long long t = static_cast<long long>(blockIdx.x) * THREADS + tid; t < a.cap_tokens; t += stride) {
-    int b = -1, pos = -1;
-    int64_t slot = -1;
-    if (t < n_tok) {
-      b = bracket(s_tok, a.B, static_cast<int>(t));
-      pos = a.kv_lens[b] - a.append_lens[b] + (static_cast<int>(t) - s_tok[b]);
-      const int j = pos / a.page;
-      const long long row = a.req_rows != nullptr ? a.req_rows[b] : b;
-      const int id = j < s_have[b] ? a.req_pages[row * a.req_stride + j] : new_page(b, j);
-      if (id >= 0) slot = static_cast<int64_t>(id) * a.page + pos % a.page;
+#pragma unroll
+    for (int k = 0; k < PER_LANE; ++k) {
+      const long long e = e0 + 32 * k + lane;
+      if (put[k] != nullptr) *put[k] = id[k];
+      if (e < a.cap_pages) a.indices[e] = id[k];
     }
-    a.bidx[t] = b;
-    a.pos[t] = pos;
-    a.slots[t] = slot;
+  }
+  for (long long t0 = static_cast<long long>(gw) * CHUNK; t0 < a.cap_tokens; t0 += static_cast<long long>(nw) * CHUNK) {
+    int b = t0 < n_tok ? bracket(s_tok, a.B, static_cast<int>(t0)) : 0;
+    int bi[PER_LANE], pos[PER_LANE];
+    int64_t slot[PER_LANE];
+#pragma unroll
+    for (int k = 0; k < PER_LANE; ++k) {
+      const long long t = t0 + 32 * k + lane;
+      bi[k] = pos[k] = -1;
+      slot[k] = -1;
+      if (t < n_tok) {
+        while (s_tok[b + 1] <= t) ++b;
+        bi[k] = b;
+        pos[k] = a.kv_lens[b] - a.append_lens[b] + (static_cast<int>(t) - s_tok[b]);
+        const int j = pos[k] / a.page;
+        const long long row = a.req_rows != nullptr ? a.req_rows[b] : b;
+        const int id = j < s_have[b] ? a.req_pages[row * a.req_stride + j] : new_page(b, j);
+        if (id >= 0) slot[k] = static_cast<int64_t>(id) * a.page + pos[k] % a.page;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < PER_LANE; ++k) {
+      const long long t = t0 + 32 * k + lane;
+      if (t < a.cap_tokens) {
+        a.bidx[t] = bi[k];
+        a.pos[t] = pos[k];
+        a.slots[t] = slot[k];
+      }
+    }
   }
 }
 
@@ -246,7 +286,7 @@ extern "C" int atf_build_page_tables(const AtfPageTablesParams* p, atf_stream_t 
                                                static_cast<int>(smem)) != cudaSuccess)
     return ATF_ERR_CUDA;
   const long long most = a.cap_pages > a.cap_tokens ? a.cap_pages : a.cap_tokens;
-  long long grid = (most + tables::ENTRIES_PER_CTA - 1) / tables::ENTRIES_PER_CTA;
+  long long grid = (most + tables::WARPS * tables::CHUNK - 1) / (tables::WARPS * tables::CHUNK);
   if (grid < 1) grid = 1;
   if (grid > 148) grid = 148;
   tables::tables_kernel<<<static_cast<unsigned>(grid), tables::THREADS, smem,
