@@ -68,8 +68,8 @@ def build_page_tables(kv_lens: torch.Tensor, append_lens: torch.Tensor, req_page
         raise ValueError("the rows of req_pages must not overlap")
     if page_size < 1 or num_tokens < 0 or max_pages < 0:
         raise ValueError("page_size must be positive, num_tokens and max_pages not negative")
-    if max(num_tokens, max_pages) > 0x7fffffff:
-        raise ValueError("num_tokens and max_pages must fit 32 bits")
+    if max(num_tokens, max_pages) >= 1 << 30:
+        raise ValueError("num_tokens and max_pages must be under 2^30")
     if (free_pages is None) != (free_head is None):
         raise ValueError("free_pages and free_head go together")
     keep = [kv_lens, append_lens]

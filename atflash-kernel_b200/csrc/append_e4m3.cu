@@ -394,7 +394,7 @@ extern "C" int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvSca
       p->batch_indices == nullptr || p->positions == nullptr || p->k_cache == nullptr || p->v_cache == nullptr ||
       p->kv_indptr == nullptr || p->kv_indices == nullptr || s->k_scale == nullptr || s->v_scale == nullptr)
     return ATF_ERR_INVALID_ARG;
-  if (p->head_dim != ATF_HEAD_DIM || p->k_level_major) return ATF_ERR_UNSUPPORTED;
+  if (p->head_dim != ATF_HEAD_DIM || p->k_level_major || p->num_kv_heads > 65535) return ATF_ERR_UNSUPPORTED;
   if (p->nnz < 0 || p->num_kv_heads < 1 || p->page_size < 1 || p->batch_size < 1 || p->num_pages < 1)
     return ATF_ERR_INVALID_ARG;
   const bool rope = p->cos != nullptr;

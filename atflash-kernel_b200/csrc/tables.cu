@@ -24,10 +24,16 @@ constexpr int WARPS = THREADS / 32;
 constexpr int PER_LANE = 4;  // entries of a lane in one step
 constexpr int CHUNK = 32 * PER_LANE;
 
+constexpr int LIMIT = 1 << 30;
+// sum of a sum and a count, at most LIMIT
+__device__ __forceinline__ int add(int sum, int n) {
+  return static_cast<int>(min(static_cast<unsigned>(sum) + static_cast<unsigned>(n), static_cast<unsigned>(LIMIT)));
+}
+
 struct Args {
   const int32_t* kv_lens;
   const int32_t* append_lens;
-  int B, page;
+  int B, page, shift;  // shift: log2(page), or -1
   int32_t* req_pages;
   long long req_stride;
   int R, M;
@@ -41,9 +47,12 @@ struct Args {
   int* err;
 };
 
-__device__ __forceinline__ int pages_of(int len, int page) {
-  return static_cast<int>((static_cast<unsigned>(len) + static_cast<unsigned>(page) - 1u) /
-                          static_cast<unsigned>(page));
+// x / page, by a shift where the page size is a power of two
+__device__ __forceinline__ int over_page(const Args& a, unsigned x) {
+  return static_cast<int>(a.shift >= 0 ? x >> a.shift : x / static_cast<unsigned>(a.page));
+}
+__device__ __forceinline__ int pages_of(const Args& a, int len) {
+  return over_page(a, static_cast<unsigned>(len) + static_cast<unsigned>(a.page) - 1u);
 }
 
 struct Req {
@@ -52,20 +61,19 @@ struct Req {
 };
 __device__ __forceinline__ Req load_req(const Args& a, int b) {
   Req r;
-  r.len = a.kv_lens[b];
-  r.app = a.append_lens[b];
-  const int row = a.req_rows != nullptr ? a.req_rows[b] : b;
-  r.bad = r.len < 0 || r.app < 0 || r.app > r.len || row < 0 || row >= a.R || pages_of(max(r.len, 0), a.page) > a.M;
+  r.len = __ldg(a.kv_lens + b);
+  r.app = __ldg(a.append_lens + b);
+  const int row = a.req_rows != nullptr ? __ldg(a.req_rows + b) : b;
+  r.bad = r.len < 0 || r.app < 0 || r.app > r.len || row < 0 || row >= a.R || pages_of(a, max(r.len, 0)) > a.M;
   if (r.bad) r.len = r.app = 0;
-  r.n = pages_of(r.len, a.page);
+  r.n = pages_of(a, r.len);
   // without a free list every page is in the table already
-  r.have = a.free_pages != nullptr ? pages_of(r.len - r.app, a.page) : r.n;
+  r.have = a.free_pages != nullptr ? pages_of(a, r.len - r.app) : r.n;
   return r;
 }
 
-// largest i in [0, n) with off[i] <= x (off[0] = 0, non-decreasing)
-__device__ __forceinline__ int bracket(const int* off, int n, int x) {
-  int lo = 0, hi = n;
+// largest i in [lo, hi) with off[i] <= x (off[lo] <= x, non-decreasing)
+__device__ __forceinline__ int bracket(const int* off, int lo, int hi, int x) {
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (off[mid] <= x) lo = mid; else hi = mid;
@@ -80,15 +88,15 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
   int* s_tok = s_page + a.B + 1;
   int* s_new = s_tok + a.B + 1;
   int* s_have = s_new + a.B + 1;
-  __shared__ long long w_sum[3][WARPS];
+  __shared__ __align__(16) int w_sum[3][WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool first_cta = blockIdx.x == 0;
 
   // The requests, read side by side into shared memory (n, new tokens, owned
   // pages), then summed run by run: each thread a run of `per`, the runs' sums
-  // scanned over the CTA. 64-bit sums: the offsets are cut at the capacities, the
-  // sums need not fit.
+  // scanned over the CTA. Sums stop at LIMIT, over every capacity.
   bool bad = false;
+#pragma unroll 4
   for (int b = tid; b < a.B; b += THREADS) {
     const Req r = load_req(a, b);
     bad |= r.bad;
@@ -97,68 +105,65 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
     s_have[b] = r.have;
     if (first_cta) a.last[b] = r.n > 0 ? r.len - (r.n - 1) * a.page : 0;
   }
+  const int head = a.free_pages != nullptr ? __ldg(a.free_head) : 0;
   __syncthreads();
-  const int per = (a.B + THREADS - 1) / THREADS;
+  // (an odd run length: neighbouring threads' runs begin in different banks)
+  const int per = ((a.B + THREADS - 1) / THREADS) | 1;
   const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
-  long long sum[3] = {0, 0, 0};
+  int sum[3] = {0, 0, 0};
   for (int b = b0; b < b1; ++b) {
-    sum[0] += s_page[b];
-    sum[1] += s_tok[b];
-    sum[2] += s_page[b] - s_have[b];
+    sum[0] = add(sum[0], s_page[b]);
+    sum[1] = add(sum[1], s_tok[b]);
+    sum[2] = add(sum[2], s_page[b] - s_have[b]);
   }
-  long long incl[3];
+  int before[3], total[3];
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
-    long long x = sum[k];
+    int x = sum[k];
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, off);
-      if (lane >= off) x += y;
+      const int y = __shfl_up_sync(0xffffffffu, x, off);
+      if (lane >= off) x = add(x, y);
     }
-    incl[k] = x;
+    before[k] = __shfl_up_sync(0xffffffffu, x, 1);
+    if (lane == 0) before[k] = 0;
     if (lane == 31) w_sum[k][warp] = x;
   }
   __syncthreads();
-  long long total[3];
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
-    long long before = 0, all = 0;
+    total[k] = 0;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) before += w_sum[k][w];
-      all += w_sum[k][w];
+    for (int w4 = 0; w4 < WARPS; w4 += 4) {
+      const int4 v = *reinterpret_cast<const int4*>(&w_sum[k][w4]);
+      const int e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (w4 + q == warp) before[k] = add(before[k], total[k]);
+        total[k] = add(total[k], e[q]);
+      }
     }
-    incl[k] += before - sum[k];  // exclusive
-    total[k] = all;
   }
   for (int b = b0; b < b1; ++b) {  // each thread turns its own run into offsets
     const int n = s_page[b], app = s_tok[b];
-    s_page[b] = static_cast<int>(min(incl[0], static_cast<long long>(a.cap_pages)));
-    s_tok[b] = static_cast<int>(min(incl[1], static_cast<long long>(a.cap_tokens)));
-    // past the free list's end every index is refused, so a cut keeps its meaning
-    s_new[b] = static_cast<int>(min(incl[2], static_cast<long long>(0x3fffffff)));
-    incl[0] += n;
-    incl[1] += app;
-    incl[2] += n - s_have[b];
+    s_page[b] = min(before[0], a.cap_pages);
+    s_tok[b] = min(before[1], a.cap_tokens);
+    s_new[b] = before[2];
+    before[0] = add(before[0], n);
+    before[1] = add(before[1], app);
+    before[2] = add(before[2], n - s_have[b]);
   }
-  const int n_pages = static_cast<int>(min(total[0], static_cast<long long>(a.cap_pages)));
-  const int n_tok = static_cast<int>(min(total[1], static_cast<long long>(a.cap_tokens)));
-  const long long head = a.free_pages != nullptr ? *a.free_head : 0;
+  const int n_pages = min(total[0], a.cap_pages), n_tok = min(total[1], a.cap_tokens);
   if (first_cta) {
     if (tid == 0) {
       a.indptr[a.B] = n_pages;
       a.aptr[a.B] = n_tok;
-      const bool short_of = a.free_pages != nullptr && (head < 0 || head + total[2] > a.F);
-      if (a.free_pages != nullptr)
-        *a.free_head_out = static_cast<int>(min(max(head, 0ll) + total[2], max(static_cast<long long>(a.F), head)));
+      const bool short_of = a.free_pages != nullptr && (head < 0 || total[2] > a.F - head);
+      if (a.free_pages != nullptr) *a.free_head_out = short_of ? max(a.F, head) : head + total[2];
       if (a.err != nullptr && (short_of || total[0] > a.cap_pages || total[1] > a.cap_tokens))
         atomicCAS(a.err, 0, kDevErrIndex);
     }
     if (bad && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
-  }
-  if (tid == 0) {  // the ends, for the walk below
-    s_page[a.B] = 0x7fffffff;
-    s_tok[a.B] = 0x7fffffff;
   }
   __syncthreads();
   if (first_cta)
@@ -169,14 +174,20 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
 
   // page j of request b: its table's, or a new one
   auto new_page = [&](int b, int j) -> int {
-    const long long at = head + s_new[b] + (j - s_have[b]);
-    return at >= 0 && head >= 0 && at < a.F ? a.free_pages[at] : -1;
+    const long long at = static_cast<long long>(head) + s_new[b] + (j - s_have[b]);
+    return head >= 0 && at < a.F ? __ldg(a.free_pages + at) : -1;
   };
-  // A warp takes chunks of 128 entries: one search for the chunk's first entry, and
-  // from there each lane walks to the requests of its four (a chunk meets few).
+  // A warp takes chunks of 128 entries, four per lane, whose loads are issued
+  // together: searches for the chunk's ends, and from them short ones per entry.
   const int gw = static_cast<int>(blockIdx.x) * WARPS + warp, nw = static_cast<int>(gridDim.x) * WARPS;
-  for (long long e0 = static_cast<long long>(gw) * CHUNK; e0 < a.cap_pages; e0 += static_cast<long long>(nw) * CHUNK) {
-    int b = e0 < n_pages ? bracket(s_page, a.B, static_cast<int>(e0)) : 0;
+  const int page_chunks = (a.cap_pages + CHUNK - 1) / CHUNK, tok_chunks = (a.cap_tokens + CHUNK - 1) / CHUNK;
+  for (int ch = gw; ch < page_chunks; ch += nw) {
+    const long long e0 = static_cast<long long>(ch) * CHUNK;
+    int lo = 0, hi = 0;
+    if (e0 < n_pages) {
+      lo = bracket(s_page, 0, a.B, static_cast<int>(e0));
+      hi = bracket(s_page, lo, a.B, static_cast<int>(min(e0 + CHUNK, static_cast<long long>(n_pages)) - 1)) + 1;
+    }
     int id[PER_LANE];
     int32_t* put[PER_LANE];
 #pragma unroll
@@ -185,9 +196,9 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
       id[k] = -1;
       put[k] = nullptr;
       if (e < n_pages) {
-        while (s_page[b + 1] <= e) ++b;
+        const int b = bracket(s_page, lo, hi, static_cast<int>(e));
         const int j = static_cast<int>(e) - s_page[b];
-        const long long row = a.req_rows != nullptr ? a.req_rows[b] : b;
+        const long long row = a.req_rows != nullptr ? __ldg(a.req_rows + b) : b;
         int32_t* at = a.req_pages + row * a.req_stride + j;
         if (j < s_have[b]) {
           id[k] = *at;
@@ -204,8 +215,14 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
       if (e < a.cap_pages) a.indices[e] = id[k];
     }
   }
-  for (long long t0 = static_cast<long long>(gw) * CHUNK; t0 < a.cap_tokens; t0 += static_cast<long long>(nw) * CHUNK) {
-    int b = t0 < n_tok ? bracket(s_tok, a.B, static_cast<int>(t0)) : 0;
+  // (tokens go to the last warps first, which have the fewest chunks of pages)
+  for (int ch = nw - 1 - gw; ch < tok_chunks; ch += nw) {
+    const long long t0 = static_cast<long long>(ch) * CHUNK;
+    int lo = 0, hi = 0;
+    if (t0 < n_tok) {
+      lo = bracket(s_tok, 0, a.B, static_cast<int>(t0));
+      hi = bracket(s_tok, lo, a.B, static_cast<int>(min(t0 + CHUNK, static_cast<long long>(n_tok)) - 1)) + 1;
+    }
     int bi[PER_LANE], pos[PER_LANE];
     int64_t slot[PER_LANE];
 #pragma unroll
@@ -214,13 +231,13 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
       bi[k] = pos[k] = -1;
       slot[k] = -1;
       if (t < n_tok) {
-        while (s_tok[b + 1] <= t) ++b;
+        const int b = bracket(s_tok, lo, hi, static_cast<int>(t));
         bi[k] = b;
-        pos[k] = a.kv_lens[b] - a.append_lens[b] + (static_cast<int>(t) - s_tok[b]);
-        const int j = pos[k] / a.page;
-        const long long row = a.req_rows != nullptr ? a.req_rows[b] : b;
+        pos[k] = __ldg(a.kv_lens + b) - __ldg(a.append_lens + b) + (static_cast<int>(t) - s_tok[b]);
+        const int j = over_page(a, static_cast<unsigned>(pos[k]));
+        const long long row = a.req_rows != nullptr ? __ldg(a.req_rows + b) : b;
         const int id = j < s_have[b] ? a.req_pages[row * a.req_stride + j] : new_page(b, j);
-        if (id >= 0) slot[k] = static_cast<int64_t>(id) * a.page + pos[k] % a.page;
+        if (id >= 0) slot[k] = static_cast<int64_t>(id) * a.page + (pos[k] - j * a.page);
       }
     }
 #pragma unroll
@@ -253,7 +270,9 @@ extern "C" int atf_build_page_tables(const AtfPageTablesParams* p, atf_stream_t 
   if (p->free_pages != nullptr &&
       (p->free_head == nullptr || p->free_head_out == nullptr || p->free_head == p->free_head_out))
     return ATF_ERR_INVALID_ARG;
-  if (p->batch > ATF_TABLES_MAX_BATCH) return ATF_ERR_UNSUPPORTED;
+  if (p->batch > ATF_TABLES_MAX_BATCH || p->max_pages >= tables::LIMIT || p->max_tokens >= tables::LIMIT ||
+      p->num_free >= tables::LIMIT)
+    return ATF_ERR_UNSUPPORTED;
   int dev = 0;
   int rc = check_device(&dev);
   if (rc != ATF_OK) return rc;
@@ -262,6 +281,9 @@ extern "C" int atf_build_page_tables(const AtfPageTablesParams* p, atf_stream_t 
   a.append_lens = p->append_lens;
   a.B = p->batch;
   a.page = p->page_size;
+  a.shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (a.page == (1 << s)) a.shift = s;
   a.req_pages = p->req_pages;
   a.req_stride = p->req_stride;
   a.R = p->num_rows;
@@ -285,8 +307,8 @@ extern "C" int atf_build_page_tables(const AtfPageTablesParams* p, atf_stream_t 
   if (smem > 47 * 1024 && cudaFuncSetAttribute(tables::tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                static_cast<int>(smem)) != cudaSuccess)
     return ATF_ERR_CUDA;
-  const long long most = a.cap_pages > a.cap_tokens ? a.cap_pages : a.cap_tokens;
-  long long grid = (most + tables::WARPS * tables::CHUNK - 1) / (tables::WARPS * tables::CHUNK);
+  const long long chunks = (a.cap_pages + tables::CHUNK - 1) / tables::CHUNK + (a.cap_tokens + tables::CHUNK - 1) / tables::CHUNK;
+  long long grid = (chunks + tables::WARPS - 1) / tables::WARPS;
   if (grid < 1) grid = 1;
   if (grid > 148) grid = 148;
   tables::tables_kernel<<<static_cast<unsigned>(grid), tables::THREADS, smem,
