@@ -76,8 +76,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
         q_pos / kv_pos0: the positions run() will be given (per request; defaults
         kv_len - 1 and 0). Under a snap16 window the work items are cut to equal
         bytes read at these distances; they steer the balance only, never the result.
-        kv_data_type: torch.float8_e4m3fn lays the schedule out for an e4m3 cache (any
-        plan runs with either cache, this one keeps ragged batches balanced).
+        kv_data_type: torch.float8_e4m3fn lays the schedule out for an e4m3 cache: equal
+        shares for the SMs whatever the requests' lengths.
         """
         if pos_encoding_mode != "NONE":
             raise NotImplementedError("RoPE is applied before the cache (pos_encoding_mode NONE)")

@@ -30,8 +30,9 @@
 // more than 8, so most stages need no maximum over lanes and no pass over O.
 //
 // CTA = (unit of atf_decode_plan, kv head): one producer warp with TMA boxes per
-// page slice (V rows of 128 bytes, and K's; under a window K as 32-byte slabs of
-// two levels, only those in the window), and 8 consumer warps in two quads that
+// page slice (rows of 128 bytes, always whole: HBM is read in lines of 128 bytes here,
+// and boxes of the 32 or 64 bytes that a window needs of a K row took as long, 4 x
+// 128K keys in pages of 64 170-176 us, as whole rows), and 8 consumer warps in two quads that
 // take 64-key stages in turn, 16 keys per warp. Two CTAs per SM. A unit holds
 // pieces of several requests, cut so that all units cost the same: one wave of
 // CTAs, equally long, whatever the requests' lengths; the producer runs through
@@ -54,7 +55,6 @@ using decode::ex2f;
 using decode::key_limit;
 using decode::ldsm_x4;
 using decode::ldsm_x4_t;
-using decode::levels_of;
 using decode::movmatrix_t;
 
 constexpr int STAGE_KEYS = 64;
@@ -64,9 +64,7 @@ constexpr int THREADS = (CONSUMERS + 1) * 32;
 // every phase of the slot's barrier (a parity wait one phase early returns at once).
 constexpr int NSTAGE = 4;
 static_assert(NSTAGE % 2 == 0, "a slot belongs to one quad");
-constexpr int SLABS = 4;                              // 32-byte slabs of a K row
-constexpr uint32_t SLAB_BYTES = STAGE_KEYS * 32;
-constexpr uint32_t K_BYTES = SLABS * SLAB_BYTES;
+constexpr uint32_t K_BYTES = STAGE_KEYS * 128;
 constexpr uint32_t V_BYTES = STAGE_KEYS * 128;
 constexpr uint32_t STAGE_BYTES = K_BYTES + V_BYTES;   // 16 KB
 constexpr uint32_t RING_BYTES = NSTAGE * STAGE_BYTES; // 64 KB
@@ -76,7 +74,8 @@ constexpr int MAX_UNIT_ITEMS = ATF_DECODE_UNIT_ITEMS;
 constexpr uint32_t OFF_MERGE = RING_BYTES;
 constexpr uint32_t OFF_STATS = OFF_MERGE + MERGE_BYTES;            // 3 x [CONSUMERS][16] floats
 constexpr uint32_t OFF_META = OFF_STATS + 3 * CONSUMERS * 16 * 4;  // Meta[MAX_UNIT_ITEMS]
-constexpr uint32_t OFF_SCALES = OFF_META + 32 * MAX_UNIT_ITEMS;    // float2[MAX_UNIT_PAGES]
+constexpr uint32_t OFF_LIM = OFF_META + 24 * MAX_UNIT_ITEMS;       // int[MAX_UNIT_ITEMS][8]
+constexpr uint32_t OFF_SCALES = OFF_LIM + 32 * MAX_UNIT_ITEMS;     // float2[MAX_UNIT_PAGES]
 constexpr uint32_t OFF_PAGES = OFF_SCALES + 8 * MAX_UNIT_PAGES;    // int[MAX_UNIT_PAGES]
 constexpr uint32_t OFF_BAR = OFF_PAGES + 4 * MAX_UNIT_PAGES;
 constexpr uint32_t OFF_ABORT = OFF_BAR + 8 * 2 * NSTAGE;
@@ -109,21 +108,14 @@ struct Args {
   int* err;
 };
 
-// K tensor maps. Under a window: over (32 bytes of a slab, token, slab, kv head,
-// page), map n-1 with the box {32, rows, n, 1, 1}. Without: n[0] alone, as V's.
-struct KMaps {
-  CUtensorMap n[SLABS];
-};
-
 // an item of the unit, as staged in shared memory
 struct Meta {
   int b, k_beg, k_end;
   int page0;     // first of its pages in the unit's list
   int list0;     // where those begin in `indices`
   int first;     // its first page within the request
-  long long zb;  // q_pos - kv_pos0
 };
-static_assert(sizeof(Meta) == 32, "two 16-byte words");
+static_assert(sizeof(Meta) == 24, "six ints");
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
@@ -152,7 +144,7 @@ __device__ __forceinline__ void consumers_sync() {
 // NT: tiles of 8 query heads (the group's size is at most 8 NT). WIN: a window.
 template <int NT, bool WIN>
 __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
-    decode_e4m3_kernel(const __grid_constant__ KMaps tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
+    decode_e4m3_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
   extern __shared__ uint8_t smem_raw[];
   // the split merge that follows on the stream may be scheduled now; it waits
   // for this grid's completion before reading the partial states
@@ -165,6 +157,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   volatile int* s_abort = reinterpret_cast<volatile int*>(sp + OFF_ABORT);
   int* s_total = reinterpret_cast<int*>(sp + OFF_ABORT + 4);  // pages of the unit, -1: refused
   Meta* s_meta = reinterpret_cast<Meta*>(sp + OFF_META);
+  int* s_lim = reinterpret_cast<int*>(sp + OFF_LIM);  // window: local key that level l is read from on
   int* s_pages = reinterpret_cast<int*>(sp + OFF_PAGES);
   float2* s_scale = reinterpret_cast<float2*>(sp + OFF_SCALES);  // (ks, log2 vs) of the unit's pages
 
@@ -201,7 +194,6 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         wrong = m.k_beg < 0 || m.k_end <= m.k_beg || (m.k_beg & 63) || m.k_end > len;
         m.first = m.k_beg >> a.page_shift;
         m.list0 = pg0 + m.first;
-        m.zb = len - 1;
         n = wrong ? 0 : ((m.k_end - 1) >> a.page_shift) - m.first + 1;
       }
       int sum = n;
@@ -227,8 +219,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
       fence_mbar_init();
     }
   } else if (warp == CONSUMERS) {
-    if (WIN ? lane < SLABS : lane == 0) tma_prefetch_desc(&tmK.n[lane]);
-    if (lane == SLABS) tma_prefetch_desc(&tmV);
+    if (lane == 0) tma_prefetch_desc(&tmK);
+    if (lane == 1) tma_prefetch_desc(&tmV);
   }
   __syncthreads();
   const int total_pages = *s_total;
@@ -249,16 +241,17 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   // Part 2: what a preceding kernel may have written (positions, query, pages,
   // scales) is read from here on.
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (WIN && tid < n_items) {
-    const int b = s_meta[tid].b;
-    const long long q_pos = a.q_pos != nullptr ? a.q_pos[b] : s_meta[tid].zb;
-    s_meta[tid].zb = q_pos - (a.kv_pos0 != nullptr ? a.kv_pos0[b] : 0);
+  if (WIN && tid < n_items * ATF_MAX_LEVELS) {
+    const int b = s_meta[tid >> 3].b, l = tid & 7;
+    const int np = a.indptr[b + 1] - a.indptr[b];  // an item's request is not empty
+    const long long len = static_cast<long long>(np - 1) * a.page_size + a.last_page_len[b];
+    const long long q_pos = a.q_pos != nullptr ? a.q_pos[b] : len - 1;
+    const long long zb = q_pos - (a.kv_pos0 != nullptr ? a.kv_pos0[b] : 0);
+    s_lim[tid] = l == 0 ? INT_MIN : key_limit(zb, a.zhi16[l]);
   }
   __syncthreads();
   const AbortCtl ab{s_abort, a.err};
   if (*s_abort != 0) return;
-  // the window of an item as limits on its local keys: level i is read from lim[i] on
-  auto limit = [&](const Meta& m, int l) { return l == 0 ? INT_MIN : key_limit(m.zb, a.zhi16[l]); };
 
   if (warp == CONSUMERS) {
     // ------------------------------------------------------------ producer
@@ -269,16 +262,11 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     bool ok = true;
     for (int i = 0; ok && i < n_items; ++i) {
       const Meta m = s_meta[i];
-      int lim[ATF_MAX_LEVELS];
-#pragma unroll
-      for (int l = 0; l < ATF_MAX_LEVELS; ++l) lim[l] = WIN ? limit(m, l) : INT_MIN;
       for (int k0 = m.k_beg; k0 < m.k_end; k0 += STAGE_KEYS) {
         ok = __all_sync(FULLMASK, mbar_wait(empty_bar(buf), ph, ab, kDevErrTimeout));
         if (!ok) break;
         const bool live = r0 < STAGE_KEYS && k0 + r0 < m.k_end;
-        int n_slab = SLABS;
-        if (WIN && live) n_slab = (levels_of(lim, min(k0 + r0 + R, m.k_end) - 1) + 1) >> 1;
-        uint32_t bytes = live ? static_cast<uint32_t>(R) * (is_v ? 128u : 32u * n_slab) : 0u;
+        uint32_t bytes = live ? static_cast<uint32_t>(R) * 128u : 0u;
 #pragma unroll
         for (int off = 4; off > 0; off >>= 1) bytes += __shfl_xor_sync(FULLMASK, bytes, off);  // lanes 0..7
         if (lane == 0) mbar_arrive_expect_tx(full_bar(buf), bytes);
@@ -288,13 +276,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
           const int page = s_pages[m.page0 + (n >> a.page_shift) - m.first];
           const int tok = n & (a.page_size - 1);
           const uint32_t st = sb + buf * STAGE_BYTES;
-          if (is_v)
-            tma_load_4d(st + K_BYTES + static_cast<uint32_t>(r0) * 128u, &tmV, full_bar(buf), 0, tok, hk, page);
-          else if (WIN)
-            tma_load_5d(st + static_cast<uint32_t>(r0) * 128u, &tmK.n[n_slab - 1], full_bar(buf), 0, tok, 0, hk,
-                        page);
-          else
-            tma_load_4d(st + static_cast<uint32_t>(r0) * 128u, &tmK.n[0], full_bar(buf), 0, tok, hk, page);
+          tma_load_4d(st + (is_v ? K_BYTES : 0u) + static_cast<uint32_t>(r0) * 128u, is_v ? &tmV : &tmK,
+                      full_bar(buf), 0, tok, hk, page);
         }
         __syncwarp();
         ++issued;
@@ -339,13 +322,6 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   uint32_t off[4];
 #pragma unroll
   for (int p = 0; p < 4; ++p) off[p] = row * 128u + 16u * ((2u * p + static_cast<uint32_t>(mi >> 1)) ^ (row & 7u));
-  // K under a window: slabs of 32-byte rows per slice, 16-byte halves swapped by bit
-  // 2 of the row
-  const uint32_t in_slice = row % R;
-  const uint32_t koff = (row - in_slice) * 128u + in_slice * 32u +
-                        16u * (static_cast<uint32_t>(mi >> 1) ^ ((in_slice >> 2) & 1u));
-  const uint32_t slab_stride = 32u * R;
-
   int cur = quad, buf = quad, ph = 0;  // this quad's next stage, its slot and parity
   int end = 0;                         // stages of the items so far
   bool ok = true;
@@ -353,9 +329,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   // same barriers)
   for (int i = 0; i < n_items; ++i) {
     const Meta m = s_meta[i];
-    // levels that every key of the last group read, and where the next one begins
-    // (keys come in rising order, their distance falls)
-    int Lmin = 0, next_lim = INT_MIN;
+    // levels that the keys up to next_lim - 1 read (keys come in rising order, their
+    // distance falls)
+    int levels = 0, next_lim = INT_MIN;
     // q as the B operand, heads as columns: in the MMA of level i, k-rows 2 t4,
     // 2 t4 + 1 are dims 16 i + 4 t4 + {0, 1} and k-rows 2 t4 + {8, 9} dims + {2, 3}
     uint32_t qb[NT][8][2];
@@ -420,57 +396,59 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) c[nt][e] = c2[nt][e] = 0.f;
-        if constexpr (!WIN) {
+        // levels that all keys of the group read, and that its newest reads: the same
+        // but where a level begins
+        int Lmax = ATF_MAX_LEVELS;
+        if (WIN) {
+          if (last >= next_lim) {
+            auto count = [&](int L, int key) {
+              while (L < ATF_MAX_LEVELS && key >= s_lim[8 * i + L]) ++L;
+              return L;
+            };
+            levels = count(levels, key0);
+            next_lim = levels < ATF_MAX_LEVELS ? s_lim[8 * i + levels] : INT_MAX;
+            Lmax = count(levels, last);
+          } else {
+            Lmax = levels;
+          }
+        }
+        if (!WIN || levels == Lmax) {
 #pragma unroll
-          for (int p = 0; p < SLABS; ++p) {
-            uint32_t r[4], a0, a1, a2, a3;
-            ldsm_x4(kb + off[p], r[0], r[1], r[2], r[3]);
-            e4m3x4_to_f16(r[0], a0, a2);
-            e4m3x4_to_f16(r[1], a1, a3);
+          for (int p = 0; p < 4; ++p) {
+            if (!WIN || 2 * p < Lmax) {
+              uint32_t r[4], a0, a1, a2, a3;
+              ldsm_x4(kb + off[p], r[0], r[1], r[2], r[3]);
+              e4m3x4_to_f16(r[0], a0, a2);
+              e4m3x4_to_f16(r[1], a1, a3);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(c[nt], a0, a1, a2, a3, qb[nt][2 * p][0], qb[nt][2 * p][1]);
-            e4m3x4_to_f16(r[2], a0, a2);
-            e4m3x4_to_f16(r[3], a1, a3);
+              for (int nt = 0; nt < NT; ++nt) mma_f16(c[nt], a0, a1, a2, a3, qb[nt][2 * p][0], qb[nt][2 * p][1]);
+              if (!WIN || 2 * p + 1 < Lmax) {
+                e4m3x4_to_f16(r[2], a0, a2);
+                e4m3x4_to_f16(r[3], a1, a3);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_f16(c2[nt], a0, a1, a2, a3, qb[nt][2 * p + 1][0], qb[nt][2 * p + 1][1]);
+                for (int nt = 0; nt < NT; ++nt)
+                  mma_f16(c2[nt], a0, a1, a2, a3, qb[nt][2 * p + 1][0], qb[nt][2 * p + 1][1]);
+              }
+            }
           }
         } else {
-          int Lmax = Lmin;
-          if (last >= next_lim) {  // the keys have come to another level
-            while (Lmin < ATF_MAX_LEVELS && key0 >= limit(m, Lmin)) ++Lmin;
-            next_lim = Lmin < ATF_MAX_LEVELS ? limit(m, Lmin) : INT_MAX;
-            Lmax = Lmin;
-            while (Lmax < ATF_MAX_LEVELS && last >= limit(m, Lmax)) ++Lmax;
-          }
+          // level by level: one that only the newer keys read counts from its limit on
 #pragma unroll
-          for (int p = 0; p < SLABS; ++p) {
-            if (2 * p < Lmax) {
-              uint32_t r[4];
-              ldsm_x4(kb + koff + p * slab_stride, r[0], r[1], r[2], r[3]);
+          for (int l = 0; l < ATF_MAX_LEVELS; ++l) {
+            if (l < Lmax) {
+              uint32_t r[4], a0, a1, a2, a3;
+              ldsm_x4(kb + off[l >> 1], r[0], r[1], r[2], r[3]);
+              e4m3x4_to_f16(r[2 * (l & 1)], a0, a2);
+              e4m3x4_to_f16(r[2 * (l & 1) + 1], a1, a3);
+              const int from = s_lim[8 * i + l];
 #pragma unroll
-              for (int hl = 0; hl < 2; ++hl) {
-                const int l = 2 * p + hl;
-                uint32_t a0, a1, a2, a3;
-                e4m3x4_to_f16(r[2 * hl], a0, a2);
-                e4m3x4_to_f16(r[2 * hl + 1], a1, a3);
-                if (l < Lmin) {
-#pragma unroll
-                  for (int nt = 0; nt < NT; ++nt)
-                    mma_f16(hl ? c2[nt] : c[nt], a0, a1, a2, a3, qb[nt][l][0], qb[nt][l][1]);
-                } else if (l < Lmax) {
-                  // a level that only the newer keys of the group read
-                  const int from = limit(m, l);
-#pragma unroll
-                  for (int nt = 0; nt < NT; ++nt) {
-                    float t[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma_f16(t, a0, a1, a2, a3, qb[nt][l][0], qb[nt][l][1]);
-                    c[nt][0] += key0 + g >= from ? t[0] : 0.f;
-                    c[nt][1] += key0 + g >= from ? t[1] : 0.f;
-                    c[nt][2] += key0 + g + 8 >= from ? t[2] : 0.f;
-                    c[nt][3] += key0 + g + 8 >= from ? t[3] : 0.f;
-                  }
-                }
+              for (int nt = 0; nt < NT; ++nt) {
+                float t[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_f16(t, a0, a1, a2, a3, qb[nt][l][0], qb[nt][l][1]);
+                c[nt][0] += key0 + g >= from ? t[0] : 0.f;
+                c[nt][1] += key0 + g >= from ? t[1] : 0.f;
+                c[nt][2] += key0 + g + 8 >= from ? t[2] : 0.f;
+                c[nt][3] += key0 + g + 8 >= from ? t[3] : 0.f;
               }
             }
           }
@@ -631,12 +609,11 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   }
 }
 
-// Units: the requests' 64-key blocks lie on one line, each with the cost of the
-// bytes a CTA reads for it (in 32-byte units: 4 for a V row, 1/2 per in-window level
-// of a K row) and each request's piece with a fixed cost for its state; unit u is
-// the part of the line up to (u + 1) / U of the whole. U fills the slots (two
-// resident CTAs per SM, over the kv heads) in as few waves as the units' limits
-// allow, with at least min_chunk_keys (64) keys per unit.
+// Units: the requests' 64-key blocks lie on one line, each key at the same cost (a
+// key's rows are read whole whatever the window) and each request's piece with that
+// of its state; unit u is the part of the line up to (u + 1) / U of the whole. U
+// fills the slots (two resident CTAs per SM, over the kv heads) in as few waves as
+// the units' limits allow, with at least min_chunk_keys (64) keys per unit.
 int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_host, int32_t items_capacity,
                int32_t* item_indptr_host, AtfDecodePlan* out) {
   const int B = p->batch_size, ps = p->page_size;
@@ -646,32 +623,15 @@ int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_hos
   cap = cap / 64 * 64;
   if (cap < 64) cap = 64;
   const long long min_keys = p->min_chunk_keys > 64 ? p->min_chunk_keys : 64;
-  const bool by_bytes = p->window == ATF_WINDOW_SNAP16;
-  constexpr long long ITEM_COST = 64 * 16;  // an item's state: about the time of 64 keys
-  struct Req {
-    long long len, lim[ATF_MAX_LEVELS];
-  };
-  std::vector<Req> reqs(static_cast<size_t>(B));
-  // cost of the keys [n0, n1) of a request, in 16-byte units
-  auto cost = [](const Req& r, long long n0, long long n1) {
-    long long c = 8 * (n1 - n0);
-    for (int i = 0; i < ATF_MAX_LEVELS; ++i) {
-      const long long lo = n0 > r.lim[i] ? n0 : r.lim[i];
-      if (n1 > lo) c += n1 - lo;
-    }
-    return c;
-  };
+  constexpr long long ITEM_COST = 64;  // an item's state takes about the time of 64 keys
+  std::vector<long long> lens(static_cast<size_t>(B));
   long long whole = 0, keys = 0;
   for (int b = 0; b < B; ++b) {
-    Req& r = reqs[static_cast<size_t>(b)];
     const int np = p->indptr_host[b + 1] - p->indptr_host[b];
-    r.len = np > 0 ? static_cast<long long>(np - 1) * ps + p->last_page_len_host[b] : 0;
-    const long long q_pos = p->q_pos_host != nullptr ? p->q_pos_host[b] : r.len - 1;
-    const long long pos0 = p->kv_pos0_host != nullptr ? p->kv_pos0_host[b] : 0;
-    for (int i = 0; i < ATF_MAX_LEVELS; ++i)
-      r.lim[i] = (!by_bytes || i == 0) ? LLONG_MIN / 4 : q_pos - pos0 - static_cast<long long>(p->zhi16[i]);
-    if (r.len > 0) whole += cost(r, 0, r.len) + ITEM_COST;
-    keys += r.len;
+    const long long len = np > 0 ? static_cast<long long>(np - 1) * ps + p->last_page_len_host[b] : 0;
+    lens[static_cast<size_t>(b)] = len;
+    if (len > 0) whole += len + ITEM_COST;
+    keys += len;
   }
   long long per_wave = slots / p->num_kv_heads;
   if (per_wave < 1) per_wave = 1;
@@ -685,10 +645,10 @@ int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_hos
   long long unit_pages = 0, unit_items = 0;
   bool open = false;
   for (int b = 0; b < B; ++b) {
-    const Req& r = reqs[static_cast<size_t>(b)];
+    const long long len = lens[static_cast<size_t>(b)];
     if (item_indptr_host != nullptr) item_indptr_host[b] = n;
     long long n0 = 0;
-    while (n0 < r.len) {
+    while (n0 < len) {
       // the unit in progress is full: by cost, by items or by pages
       if (!open || done * U >= whole * units || unit_items >= MAX_UNIT_ITEMS || unit_pages >= MAX_UNIT_PAGES) {
         if (items_host != nullptr) {
@@ -706,12 +666,9 @@ int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_hos
       room -= n0 % ps;
       if (room > cap) room = cap;
       room = room / 64 * 64;
-      long long ulo = n0 / 64 + 1, uhi = (r.len + 63) / 64;
-      while (ulo < uhi) {
-        const long long mid = ulo + (uhi - ulo) / 2;
-        if ((done + cost(r, n0, mid * 64 < r.len ? mid * 64 : r.len)) * U >= whole * units) uhi = mid; else ulo = mid + 1;
-      }
-      long long n1 = ulo * 64 < r.len ? ulo * 64 : r.len;
+      const long long share = (whole * units + U - 1) / U - done;  // keys that the unit still wants
+      long long n1 = share > 0 ? (n0 + share + 63) / 64 * 64 : n0 + 64;
+      if (n1 > len) n1 = len;
       if (room < 64) {  // no room for a block: the next unit takes it
         unit_pages = MAX_UNIT_PAGES;
         done -= n0 == 0 ? ITEM_COST : 0;
@@ -726,7 +683,7 @@ int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_hos
       }
       unit_pages += (n1 - 1) / ps - n0 / ps + 1;
       ++unit_items;
-      done += cost(r, n0, n1);
+      done += n1 - n0;
       longest = n1 - n0 > longest ? n1 - n0 : longest;
       n0 = n1;
       ++n;
@@ -819,22 +776,10 @@ extern "C" int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* 
     const uint64_t vdims[4] = {128, static_cast<uint64_t>(ps), hkv, npg};
     const uint64_t vstr[3] = {s_tok, s_head, s_page};
     const uint32_t vbox[4] = {128, rows, 1, 1};
-    decode8::KMaps tk;
-    CUtensorMap tv;
-    if (win) {
-      const uint64_t kdims[5] = {32, static_cast<uint64_t>(ps), decode8::SLABS, hkv, npg};
-      const uint64_t kstr[4] = {s_tok, 32, s_head, s_page};
-      for (uint32_t n = 1; n <= decode8::SLABS; ++n) {
-        const uint32_t box[5] = {32, rows, n, 1, 1};
-        // no promotion: the slabs out of the window are not fetched
-        if ((rc = encode_tiled_u8(&tk.n[n - 1], p->k_cache, 5, kdims, kstr, box, CU_TENSOR_MAP_SWIZZLE_32B,
-                                  CU_TENSOR_MAP_L2_PROMOTION_NONE)) != ATF_OK)
-          return rc;
-      }
-    } else if ((rc = encode_tiled_u8(&tk.n[0], p->k_cache, 4, vdims, vstr, vbox, CU_TENSOR_MAP_SWIZZLE_128B,
-                                     CU_TENSOR_MAP_L2_PROMOTION_L2_128B)) != ATF_OK) {
+    CUtensorMap tk, tv;
+    if ((rc = encode_tiled_u8(&tk, p->k_cache, 4, vdims, vstr, vbox, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_128B)) != ATF_OK)
       return rc;
-    }
     if ((rc = encode_tiled_u8(&tv, p->v_cache, 4, vdims, vstr, vbox, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B)) != ATF_OK)
       return rc;

@@ -203,11 +203,11 @@ typedef struct {
    * several items: the requests' keys, one after another, are cut into units of
    * equal cost (at most ATF_DECODE_UNIT_ITEMS items and ATF_DECODE_UNIT_PAGES
    * pages each), so that requests of different lengths keep the SMs equally busy.
-   * 0: one item per CTA. Both plans run with both kinds of cache. */
+   * 0: one item per CTA. Either plan runs with either cache. */
   int32_t units;
 } AtfDecodePlanParams;
 
-#define ATF_DECODE_UNIT_ITEMS 64
+#define ATF_DECODE_UNIT_ITEMS 32
 #define ATF_DECODE_UNIT_PAGES 1024
 
 typedef struct {
