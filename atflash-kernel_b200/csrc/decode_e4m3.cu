@@ -69,10 +69,13 @@ constexpr uint32_t V_BYTES = STAGE_KEYS * 128;
 constexpr uint32_t STAGE_BYTES = K_BYTES + V_BYTES;   // 16 KB
 constexpr uint32_t RING_BYTES = NSTAGE * STAGE_BYTES; // 64 KB
 constexpr uint32_t MERGE_BYTES = 16384;
+constexpr uint32_t Q_PITCH = 272;              // bytes of a staged q row (2-way bank conflicts at most)
+constexpr uint32_t Q_BYTES = 2 * 16 * Q_PITCH; // two items' rows
 constexpr int MAX_UNIT_PAGES = ATF_DECODE_UNIT_PAGES;
 constexpr int MAX_UNIT_ITEMS = ATF_DECODE_UNIT_ITEMS;
 constexpr uint32_t OFF_MERGE = RING_BYTES;
-constexpr uint32_t OFF_STATS = OFF_MERGE + MERGE_BYTES;            // 3 x [CONSUMERS][16] floats
+constexpr uint32_t OFF_Q = OFF_MERGE + MERGE_BYTES;
+constexpr uint32_t OFF_STATS = OFF_Q + Q_BYTES;            // 3 x [CONSUMERS][16] floats
 constexpr uint32_t OFF_META = OFF_STATS + 3 * CONSUMERS * 16 * 4;  // Meta[MAX_UNIT_ITEMS]
 constexpr uint32_t OFF_LIM = OFF_META + 24 * MAX_UNIT_ITEMS;       // int[MAX_UNIT_ITEMS][8]
 constexpr uint32_t OFF_SCALES = OFF_LIM + 32 * MAX_UNIT_ITEMS;     // float2[MAX_UNIT_PAGES]
@@ -297,6 +300,32 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   }
 
   // -------------------------------------------------------------- consumers
+  // An item's q is copied to shared memory while the item before it runs (the first
+  // one's before the loads of K and V fill the memory's queues), in two buffers by
+  // turns; rows past the group's heads are zero.
+  const int G = a.G, hq0 = hk * G;
+  auto copy_q = [&](int i) {
+    const int b = s_meta[i].b;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = 8 * nt + warp;
+      const __nv_bfloat16* src =
+          a.q + static_cast<long long>(b) * a.q_sb + static_cast<long long>(hq0 + h) * a.q_sh + 4 * lane;
+      const uint32_t dst = sb + OFF_Q + static_cast<uint32_t>((i & 1) * 16 + h) * Q_PITCH + 8u * lane;
+      if (h < G)
+        asm volatile(
+            "cp.async.ca.shared.global [%0], [%1], 4;\n\t"
+            "cp.async.ca.shared.global [%0+4], [%1+4], 4;" ::"r"(dst), "l"(src)
+            : "memory");
+    }
+  };
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+    if (8 * nt + warp >= G)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        *reinterpret_cast<uint2*>(sp + OFF_Q + (k * 16 + 8 * nt + warp) * Q_PITCH + 8 * lane) = make_uint2(0, 0);
+  copy_q(0);
   // the unit's scales, once, while the first pages are on their way
   for (int j = tid; j < total_pages; j += CONSUMERS * 32) {
     const int page = s_pages[j];
@@ -309,12 +338,11 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     }
     s_scale[j] = v;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   consumers_sync();
 
   const int g = lane >> 2, t4 = lane & 3;
-  const int G = a.G, hq0 = hk * G;
   const int quad = warp >> 2, wq = warp & 3;  // this warp: keys 16 wq .. of every second stage
-  const uint32_t R = static_cast<uint32_t>(a.rows);
   const int mi = lane >> 3, mr = lane & 7;
   // ldmatrix rows of the warp's 16 keys, matrices (keys 0-7, chunk c), (keys 8-15, c),
   // (0-7, c + 1), (8-15, c + 1). Rows of 128 bytes: 16-byte chunks XORed with the row.
@@ -338,16 +366,14 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     float qsl[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int h = 8 * nt + g;
-      const bool v0 = h < G;
-      const __nv_bfloat16* qrow =
-          a.q + static_cast<long long>(m.b) * a.q_sb + static_cast<long long>(hq0 + (v0 ? h : 0)) * a.q_sh;
+      const uint32_t* qrow =
+          reinterpret_cast<const uint32_t*>(sp + OFF_Q + ((i & 1) * 16 + 8 * nt + g) * Q_PITCH) + 2 * t4;
       float mx = 0.f;
 #pragma unroll
       for (int l = 0; l < 8; ++l)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t w = v0 ? *reinterpret_cast<const uint32_t*>(qrow + 16 * l + 4 * t4 + 2 * e) : 0u;
+          const uint32_t w = qrow[8 * l + e];
           qb[nt][l][e] = w;
           mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))));
         }
@@ -378,6 +404,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
     }
+    if (i + 1 < n_items) copy_q(i + 1);
     const int begin = end;
     end += (m.k_end - m.k_beg + STAGE_KEYS - 1) / STAGE_KEYS;
     while (cur < end) {
@@ -561,6 +588,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
       }
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
+      if (pass == 0) asm volatile("cp.async.wait_all;" ::: "memory");  // the next item's q
       consumers_sync();  // the buffer has been read
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -623,7 +651,7 @@ int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_hos
   cap = cap / 64 * 64;
   if (cap < 64) cap = 64;
   const long long min_keys = p->min_chunk_keys > 64 ? p->min_chunk_keys : 64;
-  constexpr long long ITEM_COST = 64;  // an item's state takes about the time of 64 keys
+  constexpr long long ITEM_COST = 288;  // keys in whose time an item starts and writes its state (2.8 us measured)
   std::vector<long long> lens(static_cast<size_t>(B));
   long long whole = 0, keys = 0;
   for (int b = 0; b < B; ++b) {
