@@ -46,144 +46,14 @@
 // TMEM columns: S_t at 128t, O_t at 256 + 128t; P_t at 128(1-t) + 64.
 #include <math.h>
 
-#include <algorithm>
-#include <cstring>
-#include <vector>
-
 #include "atf_internal.h"
 #include "atf_ptx.cuh"
+#include "prefill_common.cuh"
 #include "rope_math.cuh"
 
 namespace atf {
 namespace prefill {
 
-// MMA groups are issued from one asm block each, under a single elect: the MMA
-// warp shares its sub-partition with two softmax warps, so fewer instructions
-// per tcgen05.mma keep the tensor pipe fed.
-//
-// one elected lane issues the 8 PV MMAs (K = 128 keys) of a tile and the commit
-__device__ __forceinline__ void pv_group_asm(uint32_t o_tmem, uint32_t p_tmem, uint64_t vd, uint32_t idesc,
-                                             uint32_t acc0, uint32_t bar_addr) {
-  asm volatile(
-      "{\n\t.reg .pred pe, pa;\n\t.reg .b64 b;\n\t.reg .b32 a;\n\t"
-      "elect.sync _|pe, 0xffffffff;\n\t"
-      "setp.ne.b32 pa, %4, 0;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pa;\n\t"
-      "add.u32 a, %1, 8;\n\tadd.u64 b, %2, 128;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, 1;\n\t"
-      "add.u32 a, a, 8;\n\tadd.u64 b, b, 128;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, 1;\n\t"
-      "add.u32 a, a, 8;\n\tadd.u64 b, b, 128;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, 1;\n\t"
-      "add.u32 a, a, 8;\n\tadd.u64 b, b, 128;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, 1;\n\t"
-      "add.u32 a, a, 8;\n\tadd.u64 b, b, 128;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, 1;\n\t"
-      "add.u32 a, a, 8;\n\tadd.u64 b, b, 128;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, 1;\n\t"
-      "add.u32 a, a, 8;\n\tadd.u64 b, b, 128;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, 1;\n\t"
-      "@pe tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
-      ::"r"(o_tmem), "r"(p_tmem), "l"(vd), "r"(idesc), "r"(acc0), "r"(bar_addr)
-      : "memory");
-}
-// one elected lane issues the L (1..8) QK MMAs of a tile and the commit; level
-// i advances A and B by one 4 KB slab (descriptor start field += 256)
-__device__ __forceinline__ void qk_group_asm(uint32_t d_tmem, uint64_t qd, uint64_t kd, uint32_t idesc, int L,
-                                             uint32_t bar_addr) {
-  asm volatile(
-      "{\n\t.reg .pred pe, p1, p2, p3, p4, p5, p6, p7;\n\t.reg .b64 a, b;\n\t"
-      "elect.sync _|pe, 0xffffffff;\n\t"
-      "setp.gt.and.s32 p1, %4, 1, pe;\n\tsetp.gt.and.s32 p2, %4, 2, pe;\n\tsetp.gt.and.s32 p3, %4, 3, pe;\n\t"
-      "setp.gt.and.s32 p4, %4, 4, pe;\n\tsetp.gt.and.s32 p5, %4, 5, pe;\n\tsetp.gt.and.s32 p6, %4, 6, pe;\n\t"
-      "setp.gt.and.s32 p7, %4, 7, pe;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, 0;\n\t"
-      "add.u64 a, %1, 256;\n\tadd.u64 b, %2, 256;\n\t"
-      "@p1 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 256;\n\tadd.u64 b, b, 256;\n\t"
-      "@p2 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 256;\n\tadd.u64 b, b, 256;\n\t"
-      "@p3 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 256;\n\tadd.u64 b, b, 256;\n\t"
-      "@p4 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 256;\n\tadd.u64 b, b, 256;\n\t"
-      "@p5 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 256;\n\tadd.u64 b, b, 256;\n\t"
-      "@p6 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 256;\n\tadd.u64 b, b, 256;\n\t"
-      "@p7 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "@pe tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
-      ::"r"(d_tmem), "l"(qd), "l"(kd), "r"(idesc), "r"(L), "r"(bar_addr)
-      : "memory");
-}
-// The same with Q as two boxes of 64 dims in 128-byte rows (128-byte swizzle, 16
-// KB each): level i advances A by 32 bytes inside a row, and to the next box after
-// four levels.
-__device__ __forceinline__ void qk_group_rows_asm(uint32_t d_tmem, uint64_t qd, uint64_t kd, uint32_t idesc, int L,
-                                                  uint32_t bar_addr) {
-  asm volatile(
-      "{\n\t.reg .pred pe, p1, p2, p3, p4, p5, p6, p7;\n\t.reg .b64 a, b;\n\t"
-      "elect.sync _|pe, 0xffffffff;\n\t"
-      "setp.gt.and.s32 p1, %4, 1, pe;\n\tsetp.gt.and.s32 p2, %4, 2, pe;\n\tsetp.gt.and.s32 p3, %4, 3, pe;\n\t"
-      "setp.gt.and.s32 p4, %4, 4, pe;\n\tsetp.gt.and.s32 p5, %4, 5, pe;\n\tsetp.gt.and.s32 p6, %4, 6, pe;\n\t"
-      "setp.gt.and.s32 p7, %4, 7, pe;\n\t"
-      "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, 0;\n\t"
-      "add.u64 a, %1, 2;\n\tadd.u64 b, %2, 256;\n\t"
-      "@p1 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 2;\n\tadd.u64 b, b, 256;\n\t"
-      "@p2 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 2;\n\tadd.u64 b, b, 256;\n\t"
-      "@p3 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 1018;\n\tadd.u64 b, b, 256;\n\t"
-      "@p4 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 2;\n\tadd.u64 b, b, 256;\n\t"
-      "@p5 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 2;\n\tadd.u64 b, b, 256;\n\t"
-      "@p6 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "add.u64 a, a, 2;\n\tadd.u64 b, b, 256;\n\t"
-      "@p7 tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
-      "@pe tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
-      ::"r"(d_tmem), "l"(qd), "l"(kd), "r"(idesc), "r"(L), "r"(bar_addr)
-      : "memory");
-}
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-constexpr int BM = 128, BN = 128, HD = 128, NQ = 2, KST = 2, VST = 2;
-// Warps 10 and 11 have no role: they complete the third warpgroup so that the
-// register split below (setmaxnreg acts on whole warpgroups) can take
-// registers from the producer / MMA group and give them to the softmax groups.
-constexpr int WARP_LOAD = 8, WARP_MMA = 9, NUM_WARPS = 12, THREADS = NUM_WARPS * 32;
-// Registers per thread after the split. The block launches with THREADS x the
-// compiled count (168 under __launch_bounds__(THREADS, 1)); the host refuses to
-// launch unless 128 x REG_SMALL + 256 x REG_SOFTMAX fits in that.
-constexpr int REG_SMALL = 80, REG_SOFTMAX = 208;
-constexpr long long REG_SPLIT_TOTAL = 128LL * REG_SMALL + 256LL * REG_SOFTMAX;
-template <int N>
-__device__ __forceinline__ void reg_dealloc() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void reg_alloc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-constexpr uint32_t QHALF_BYTES = BM * 16;             // 2 KB
-constexpr uint32_t QSLAB_BYTES = 2 * QHALF_BYTES;     // 4 KB
-constexpr uint32_t QTILE_BYTES = 8 * QSLAB_BYTES;     // 32 KB
-constexpr uint32_t KHALF_BYTES = BN * 16;             // 2 KB
-constexpr uint32_t KSLAB_BYTES = 2 * KHALF_BYTES;     // 4 KB
-constexpr uint32_t KSTAGE_BYTES = 8 * KSLAB_BYTES;    // 32 KB
-// sorted-pair K tensor maps over (16 dims of a level, key, level, kv head,
-// batch); map L-1 moves the box {16, 128, L}: exactly the L in-window levels,
-// as [L][128 keys][32 B] with 32-byte swizzle
-struct KLevelMaps {
-  CUtensorMap lv[ATF_MAX_LEVELS];
-};
-constexpr uint32_t VBOX_BYTES = BN * 128;             // 16 KB
-constexpr uint32_t VSTAGE_BYTES = 2 * VBOX_BYTES;     // 32 KB
 constexpr uint32_t OFF_Q = 0;
 constexpr uint32_t OFF_K = OFF_Q + NQ * QTILE_BYTES;
 constexpr uint32_t OFF_V = OFF_K + KST * KSTAGE_BYTES;
@@ -208,10 +78,6 @@ constexpr uint32_t OFF_TMEM = OFF_ABORT + 16;
 constexpr uint32_t SMEM_USED = OFF_TMEM + 16;
 constexpr uint32_t SMEM_BYTES = SMEM_USED + 1024;  // slack for 1024-B alignment
 
-constexpr uint32_t IDESC_QK = make_idesc_bf16(128, BN, 0, 0);
-constexpr uint32_t IDESC_PV = make_idesc_bf16(128, HD, 0, 1);
-constexpr uint32_t FULL = 0xffffffffu;
-
 struct Args {
   int B, Sq, Sk, Hq, G, n_qblk;
   // query row ranges: range r covers rows [r_lo[r], r_hi[r]) in r_nblk[r] blocks
@@ -233,19 +99,7 @@ struct Args {
   const float* qcos;
   const float* qsin;
   long long cs_stride;
-  // ragged: the work items and their number, and the packed rows of q and k
-  const int* items;
-  int n_items;
-  long long total_q, total_k;
 };
-
-// One work item of a ragged batch: a block of 256 query rows of one sequence.
-// Rows and keys below are the sequence's own; the packed tensors hold them from
-// q_beg and k_beg on.
-struct Item {
-  int q_beg, q_len, k_beg, k_len, row, pad[3];
-};
-static_assert(sizeof(Item) == 32, "eight ints per item");
 
 // The window of one query tile (rows row0..row0+127) as key-tile limits, set
 // once per CTA and held in registers: key tile j reads level i when
@@ -253,9 +107,8 @@ static_assert(sizeof(Item) == 32, "eight ints per item");
 // - (128 j + 127)), and level i is read when z_min(j) <= zhi[i] (level 0
 // always: zhi[0] covers every distance), i.e. from
 // j = ceil((q_offset + row0 - 127 - zhi[i]) / 128) on.
-__device__ __forceinline__ void window_limits(const Args& a, long long q_offset, int row0,
-                                              int (&lim)[ATF_MAX_LEVELS]) {
-  const long long base = q_offset + row0 - (BN - 1);
+__device__ __forceinline__ void window_limits(const Args& a, int row0, int (&lim)[ATF_MAX_LEVELS]) {
+  const long long base = a.q_offset + row0 - (BN - 1);
 #pragma unroll
   for (int i = 0; i < ATF_MAX_LEVELS; ++i) {
     const long long x = base - a.zhi[i];
@@ -263,50 +116,18 @@ __device__ __forceinline__ void window_limits(const Args& a, long long q_offset,
     lim[i] = static_cast<int>(j > 0x7fffffffLL ? 0x7fffffffLL : j);
   }
 }
-// levels of key tile j: the L (1..8) in-window 16-dim levels of the pair
-__device__ __forceinline__ int levels_for(const int (&lim)[ATF_MAX_LEVELS], int j) {
-  int L = 0;
-#pragma unroll
-  for (int i = 0; i < ATF_MAX_LEVELS; ++i) L += j >= lim[i] ? 1 : 0;
-  return L;
-}
 // first key tile that needs per-element masks: a key past the query row
 // (causal) or past the end of the keys
-__device__ __forceinline__ int first_masked_tile(const Args& a, long long q_offset, int sk, int row0) {
-  long long jm = sk / BN;  // 128 j + 127 >= Sk from j = ceil((Sk - 127) / 128) = floor(Sk / 128)
+__device__ __forceinline__ int first_masked_tile(const Args& a, int row0) {
+  long long jm = a.Sk / BN;  // 128 j + 127 >= Sk from j = ceil((Sk - 127) / 128) = floor(Sk / 128)
   if (a.causal) {
-    const long long x = q_offset + row0 - (BN - 1);  // 128 j > x for a masked tile
+    const long long x = a.q_offset + row0 - (BN - 1);  // 128 j > x for a masked tile
     const long long jc = x < 0 ? 0 : x / BN + 1;
     if (jc < jm) jm = jc;
   }
   return static_cast<int>(jm > 0x7fffffffLL ? 0x7fffffffLL : jm);
 }
 
-// Column of the first element of half `hh` of level `i` along head_dim.
-// sorted-pair order: level i = dims [16i, 16i+16).
-// rotate_half order (HF): sorted pairs 8i..8i+7 are HF dims [56-8i, 64-8i) and
-// [120-8i, 128-8i).
-__device__ __forceinline__ int level_col(int layout, int i, int hh) {
-  return layout == ATF_LAYOUT_SORTED_PAIR ? 16 * i + 8 * hh : 64 * hh + 8 * (7 - i);
-}
-
-// Waits with no abort short-cut: used to drain this CTA's own asynchronous
-// copies / MMAs before the CTA's shared memory or TMEM is released.
-__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) {
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer_ns() - t0 > kWaitLimitNs) break;
-  }
-}
-
-// RAGGED: a batch of packed sequences of different lengths instead of a dense
-// one. The grid walks kv heads, then the plan's items (most key tiles first, so
-// that the last CTAs are the shortest), then the heads of the group; row and key
-// coordinates of the TMA boxes are offset to the sequence, so a tile's last box
-// may reach into the next one: its queries are not stored, its keys are masked,
-// and its V rows, whose P is 0, are cleared in shared memory before the product
-// (they may hold anything, NaN included).
-template <bool RAGGED>
 __global__ void __launch_bounds__(THREADS, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                    const __grid_constant__ KLevelMaps tmKL,
@@ -327,43 +148,17 @@ __global__ void __launch_bounds__(THREADS, 1)
   // resident together then read a single kv head's K/V, whose causal range
   // (256 B x 2 per key) stays in L2, so HBM sees each K/V byte about once.
   const int Hkv = a.Hq / a.G;
-  int row_base, row_end, bi, hk, h;
-  // first packed row of the sequence's queries and keys, its keys and the
-  // position of its query row 0
-  int q_tok = 0, k_tok = 0, sk = a.Sk;
-  long long q_offset = a.q_offset;
-  if constexpr (RAGGED) {
-    const int per_head = a.n_items * a.G;
-    const int rem = static_cast<int>(blockIdx.x) % per_head;
-    const Item it = reinterpret_cast<const Item*>(a.items)[rem / a.G];
-    if (it.q_beg < 0 || it.q_len < 0 || it.k_beg < 0 || it.k_len < 0 || it.row < 0 ||
-        static_cast<long long>(it.q_beg) + it.q_len > a.total_q ||
-        static_cast<long long>(it.k_beg) + it.k_len > a.total_k) {
-      if (threadIdx.x == 0 && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
-      return;
-    }
-    bi = 0;
-    hk = static_cast<int>(blockIdx.x) / per_head;
-    h = hk * a.G + rem % a.G;
-    row_base = it.row;
-    row_end = it.q_len;
-    q_tok = it.q_beg;
-    k_tok = it.k_beg;
-    sk = it.k_len;
-    q_offset = static_cast<long long>(it.k_len) - it.q_len;
-  } else {
-    const int per_group = a.n_qblk * a.G;
-    const int grp = static_cast<int>(blockIdx.x) / per_group;
-    const int rem = static_cast<int>(blockIdx.x) % per_group;
-    // blocks of the later row range first, each range's blocks latest rows first
-    const int qidx = a.n_qblk - 1 - rem / a.G;
-    const int rng = (a.nrange > 1 && qidx >= a.r_nblk[0]) ? 1 : 0;
-    row_base = a.r_lo[rng] + (qidx - (rng ? a.r_nblk[0] : 0)) * (BM * NQ);
-    row_end = rng ? a.r_hi[1] : a.r_hi[0];
-    bi = grp / Hkv;
-    hk = grp % Hkv;
-    h = hk * a.G + rem % a.G;
-  }
+  const int per_group = a.n_qblk * a.G;
+  const int grp = static_cast<int>(blockIdx.x) / per_group;
+  const int rem = static_cast<int>(blockIdx.x) % per_group;
+  // blocks of the later row range first, each range's blocks latest rows first
+  const int qidx = a.n_qblk - 1 - rem / a.G;
+  const int rng = (a.nrange > 1 && qidx >= a.r_nblk[0]) ? 1 : 0;
+  const int row_base = a.r_lo[rng] + (qidx - (rng ? a.r_nblk[0] : 0)) * (BM * NQ);
+  const int row_end = rng ? a.r_hi[1] : a.r_hi[0];
+  const int bi = grp / Hkv;
+  const int hk = grp % Hkv;
+  const int h = hk * a.G + rem % a.G;
   int row0[NQ], nk[NQ];
 #pragma unroll
   for (int t = 0; t < NQ; ++t) {
@@ -371,15 +166,15 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (row0[t] >= row_end) {
       nk[t] = 0;
     } else {
-      long long kend = a.causal ? q_offset + row0[t] + BM : sk;
-      if (kend > sk) kend = sk;
+      long long kend = a.causal ? a.q_offset + row0[t] + BM : a.Sk;
+      if (kend > a.Sk) kend = a.Sk;
       nk[t] = kend > 0 ? static_cast<int>((kend + BN - 1) / BN) : 0;
     }
   }
   const int nk_max = nk[0] > nk[1] ? nk[0] : nk[1];
   int lim[NQ][ATF_MAX_LEVELS];
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) window_limits(a, q_offset, row0[t], lim[t]);
+  for (int t = 0; t < NQ; ++t) window_limits(a, row0[t], lim[t]);
 
   if (threadIdx.x == 0) {
     *s_abort = (a.err != nullptr && *reinterpret_cast<volatile int*>(a.err) != 0) ? 1 : 0;
@@ -405,14 +200,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   if (warp == WARP_LOAD && lane == 0) {
     tma_prefetch_desc(&tmQ);
-    if constexpr (RAGGED) {  // only the maps that this call uses are there
-      if (a.layout != ATF_LAYOUT_SORTED_PAIR) tma_prefetch_desc(&tmK);
-      else
-        for (int L = a.window ? 0 : ATF_MAX_LEVELS - 1; L < ATF_MAX_LEVELS; ++L) tma_prefetch_desc(&tmKL.lv[L]);
-    } else {
-      tma_prefetch_desc(&tmK);
-      for (int L = 0; L < ATF_MAX_LEVELS; ++L) tma_prefetch_desc(&tmKL.lv[L]);
-    }
+    tma_prefetch_desc(&tmK);
+    for (int L = 0; L < ATF_MAX_LEVELS; ++L) tma_prefetch_desc(&tmKL.lv[L]);
     tma_prefetch_desc(&tmV);
   }
   if (warp == WARP_MMA) {
@@ -441,19 +230,12 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
           if (nk[t] == 0) continue;
-          if (RAGGED && a.layout == ATF_LAYOUT_SORTED_PAIR) {
-            // two boxes of 128-byte rows: a sixteenth of the 8-dim boxes' row pieces
-            tma_load_4d_elect(sb + OFF_Q + t * QTILE_BYTES, &tmQ, bar(B_Q), 0, q_tok + row0[t], h, bi);
-            tma_load_4d_elect(sb + OFF_Q + t * QTILE_BYTES + QTILE_BYTES / 2, &tmQ, bar(B_Q), 64, q_tok + row0[t], h,
-                              bi);
-            continue;
-          }
 #pragma unroll
           for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh)
               tma_load_4d_elect(sb + OFF_Q + t * QTILE_BYTES + i * QSLAB_BYTES + hh * QHALF_BYTES, &tmQ,
-                                bar(B_Q), level_col(a.layout, i, hh), q_tok + row0[t], h, bi);
+                                bar(B_Q), level_col(a.layout, i, hh), row0[t], h, bi);
         }
       }
       for (int j = 0; j < nk_max; ++j) {
@@ -471,25 +253,25 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (a.layout == ATF_LAYOUT_SORTED_PAIR) {
           // one 5-d box: the L in-window levels (dims 0..16L-1), one 4 KB slab each
           mbar_arrive_expect_tx_elect(bar(B_KFULL + ks), static_cast<uint32_t>(L) * KSLAB_BYTES);
-          if (elect_one_lane()) tma_load_5d(kdst, &tmKL.lv[L - 1], bar(B_KFULL + ks), 0, k_tok + j * BN, 0, hk, bi);
+          if (elect_one_lane()) tma_load_5d(kdst, &tmKL.lv[L - 1], bar(B_KFULL + ks), 0, j * BN, 0, hk, bi);
           __syncwarp();
         } else {
           // rotate_half: a level is two 8-dim chunks 64 dims apart, one box each
           mbar_arrive_expect_tx_elect(bar(B_KFULL + ks), static_cast<uint32_t>(L) * KSLAB_BYTES);
           for (int i = 0; i < L; ++i) {
             tma_load_4d_elect(kdst + i * KSLAB_BYTES, &tmK, bar(B_KFULL + ks), level_col(a.layout, i, 0),
-                              k_tok + j * BN, hk, bi);
+                              j * BN, hk, bi);
             tma_load_4d_elect(kdst + i * KSLAB_BYTES + KHALF_BYTES, &tmK, bar(B_KFULL + ks),
-                              level_col(a.layout, i, 1), k_tok + j * BN, hk, bi);
+                              level_col(a.layout, i, 1), j * BN, hk, bi);
           }
         }
         issued_k = j + 1;
         ok = __all_sync(FULL, mbar_wait_inl(bar(B_VEMPTY + vs), ((j / VST) & 1) ^ 1, ab, kDevErrTimeout));
         if (!ok) break;
         mbar_arrive_expect_tx_elect(bar(B_VFULL + vs), VSTAGE_BYTES);
-        tma_load_4d_elect(sb + OFF_V + vs * VSTAGE_BYTES, &tmV, bar(B_VFULL + vs), 0, k_tok + j * BN, hk, bi);
+        tma_load_4d_elect(sb + OFF_V + vs * VSTAGE_BYTES, &tmV, bar(B_VFULL + vs), 0, j * BN, hk, bi);
         tma_load_4d_elect(sb + OFF_V + vs * VSTAGE_BYTES + VBOX_BYTES, &tmV, bar(B_VFULL + vs), 64,
-                          k_tok + j * BN, hk, bi);
+                          j * BN, hk, bi);
         issued_v = j + 1;
       }
       // Drain: every copy this warp issued must land before shared memory is
@@ -506,7 +288,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       // the start-address field (all offsets stay inside the 14-bit field).
       const uint32_t tm = __shfl_sync(FULL, tmem, 0);
       const uint64_t qdesc0 = make_sdesc(sb + OFF_Q, QHALF_BYTES, 128, kLayoutNone);
-      const uint64_t qrows0 = make_sdesc(sb + OFF_Q, 16, 1024, kLayoutSw128);
       const uint64_t kdesc0 = make_sdesc(sb + OFF_K, KHALF_BYTES, 128, kLayoutNone);
       // sorted-pair K level slabs: 128 keys x 32 B, 32-byte swizzle (SBO = 8 rows)
       const uint64_t kdesc32 = make_sdesc(sb + OFF_K, 16, 256, kLayoutSw32);
@@ -519,10 +300,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t d_tmem = tm + static_cast<uint32_t>(t * 128);
         const uint64_t qd = qdesc0 + ((t * QTILE_BYTES) >> 4);
         const uint64_t kd = (sorted ? kdesc32 : kdesc0) + (((j % KST) * KSTAGE_BYTES) >> 4);
-        if (RAGGED && sorted)
-          qk_group_rows_asm(d_tmem, qrows0 + ((t * QTILE_BYTES) >> 4), kd, IDESC_QK, L, bar(B_SFULL + t));
-        else
-          qk_group_asm(d_tmem, qd, kd, IDESC_QK, L, bar(B_SFULL + t));
+        qk_group_asm(d_tmem, qd, kd, IDESC_QK, L, bar(B_SFULL + t));
       };
       // O_t += P_t(j) V_j; P_t sits in columns 64..127 of the other tile's S
       auto issue_PV = [&](int t, int j) {
@@ -566,20 +344,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int vs = j % VST;
         ok = __all_sync(FULL, mbar_wait_inl(bar(B_VFULL + vs), (j / VST) & 1, ab, kDevErrTimeout));
         if (!ok) break;
-        if constexpr (RAGGED) {
-          // V rows past the sequence's last key: another sequence's
-          const int live = sk - j * BN;
-          if (live < BN) {
-            uint8_t* v0 = sp + OFF_V + vs * VSTAGE_BYTES;
-            for (int e = live * 8 + lane; e < BN * 8; e += 32) {
-              *reinterpret_cast<uint4*>(v0 + 16 * e) = make_uint4(0, 0, 0, 0);
-              *reinterpret_cast<uint4*>(v0 + VBOX_BYTES + 16 * e) = make_uint4(0, 0, 0, 0);
-            }
-            // the MMAs read V through the async proxy
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-          }
-        }
         tc_fence_after();
         if (j < nk0) {
           ok = __all_sync(FULL, mbar_wait_inl(bar(B_PFULL + 0), j & 1, ab, kDevErrTimeout));
@@ -631,9 +395,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t tO = tmem + 256u + static_cast<uint32_t>(t * 128) + lane_off;
         const int my_row0 = t ? row0[1] : row0[0];
         const int my_nk = t ? nk[1] : nk[0];
-        const int j_mask = first_masked_tile(a, q_offset, sk, my_row0);
+        const int j_mask = first_masked_tile(a, my_row0);
         const int qrow = my_row0 + r;
-        const long long qpos = q_offset + qrow;
+        const long long qpos = a.q_offset + qrow;
         const float sl2 = a.scale_log2;
         if (a.qrot) {
           // RoPE at load: this thread's query row, rotated in fp32 at its position,
@@ -679,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int c = 0; c < BN; ++c) {
               const long long key = n0 + c;
-              if ((a.causal && key > qpos) || key >= sk) s[c] = -INFINITY;
+              if ((a.causal && key > qpos) || key >= a.Sk) s[c] = -INFINITY;
             }
           }
           // three-input max: 64 instructions for the 128 scores, 4 chains
@@ -773,7 +537,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const float inv = l > 0.f ? 1.0f / l : 0.f;
             const bool store = qrow < row_end;
             __nv_bfloat16* orow = a.out + static_cast<long long>(bi) * a.o_sb +
-                                  static_cast<long long>(q_tok + qrow) * a.o_ss +
+                                  static_cast<long long>(qrow) * a.o_ss +
                                   static_cast<long long>(h) * a.o_sh;
 #pragma unroll
             for (int c4 = 0; c4 < HD / 32; ++c4) {
@@ -783,10 +547,6 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int e = 0; e < 16; ++e)
                 pk[e] = pack_bf16x2(__uint_as_float(rr[2 * e]) * inv, __uint_as_float(rr[2 * e + 1]) * inv);
-              if constexpr (RAGGED) {  // a row without keys is 0, whatever V holds
-#pragma unroll
-                for (int e = 0; e < 16; ++e) pk[e] = qpos < 0 && a.causal ? 0u : pk[e];
-              }
               if (store) {
                 uint4* dst = reinterpret_cast<uint4*>(orow + 32 * c4);
 #pragma unroll
@@ -795,18 +555,8 @@ __global__ void __launch_bounds__(THREADS, 1)
               }
             }
             if (a.lse != nullptr && store)
-              a.lse[RAGGED ? static_cast<long long>(q_tok + qrow) * a.Hq + h
-                           : (static_cast<long long>(bi) * a.Hq + h) * a.Sq + qrow] =
+              a.lse[(static_cast<long long>(bi) * a.Hq + h) * a.Sq + qrow] =
                   (m2 + log2f(l)) * 0.69314718055994531f;
-          }
-        }
-        if constexpr (RAGGED) {
-          if (my_nk == 0 && qrow < row_end) {  // a tile whose rows have no keys
-            uint4* dst = reinterpret_cast<uint4*>(a.out + static_cast<long long>(q_tok + qrow) * a.o_ss +
-                                                  static_cast<long long>(h) * a.o_sh);
-#pragma unroll
-            for (int e = 0; e < HD / 8; ++e) dst[e] = make_uint4(0, 0, 0, 0);
-            if (a.lse != nullptr) a.lse[static_cast<long long>(q_tok + qrow) * a.Hq + h] = -INFINITY;
           }
         }
     }
@@ -817,24 +567,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-}
-
-template <bool RAGGED>
-static int launch(const CUtensorMap& tq, const CUtensorMap& tk, const KLevelMaps& tkl, const CUtensorMap& tv,
-                  const Args& a, long long grid, cudaStream_t st) {
-  if (cudaFuncSetAttribute(prefill_kernel<RAGGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(SMEM_BYTES)) != cudaSuccess)
-    return ATF_ERR_CUDA;
-  if (grid > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
-  // setmaxnreg.inc waits until the block's launch registers cover the split:
-  // never launch a build whose register count would leave it waiting
-  static const int launch_regs = [] {
-    cudaFuncAttributes fa{};
-    return cudaFuncGetAttributes(&fa, prefill_kernel<RAGGED>) == cudaSuccess ? fa.numRegs : 0;
-  }();
-  if (static_cast<long long>(launch_regs) * THREADS < REG_SPLIT_TOTAL) return ATF_ERR_UNSUPPORTED;
-  prefill_kernel<RAGGED><<<static_cast<unsigned>(grid), THREADS, SMEM_BYTES, st>>>(tq, tk, tkl, tv, a);
-  return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
 }
 
 }  // namespace prefill
@@ -975,140 +707,19 @@ extern "C" int atf_prefill_fwd(const AtfPrefillParams* p, atf_stream_t stream) {
   a.qsin = p->q_sin;
   a.cs_stride = p->q_cs_stride_pos;
 
-  a.items = nullptr;
-  a.n_items = 0;
-  a.total_q = a.total_k = 0;
-  return launch<false>(tq, tk, tkl, tv, a, static_cast<long long>(a.n_qblk) * a.B * a.Hq,
-                       reinterpret_cast<cudaStream_t>(stream));
-}
-
-extern "C" int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int32_t* items_host,
-                                       int32_t items_capacity, int32_t* num_items) {
-  using namespace atf::prefill;
-  if (p == nullptr || num_items == nullptr || p->qo_indptr_host == nullptr || p->kv_indptr_host == nullptr ||
-      p->batch_size < 1 || (items_host == nullptr && items_capacity > 0))
-    return ATF_ERR_INVALID_ARG;
-  long long n = 0;
-  for (int b = 0; b < p->batch_size; ++b) {
-    const long long nq = static_cast<long long>(p->qo_indptr_host[b + 1]) - p->qo_indptr_host[b];
-    const long long nk = static_cast<long long>(p->kv_indptr_host[b + 1]) - p->kv_indptr_host[b];
-    if (p->qo_indptr_host[b] < 0 || p->kv_indptr_host[b] < 0 || nq < 0 || nk < 0) return ATF_ERR_INVALID_ARG;
-    if (nq > (1ll << 30) || nk > (1ll << 30)) return ATF_ERR_UNSUPPORTED;
-    n += (nq + BM * NQ - 1) / (BM * NQ);
-  }
-  if (n > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
-  *num_items = static_cast<int32_t>(n);
-  if (items_host == nullptr) return ATF_OK;
-  if (n > items_capacity) return ATF_ERR_WORKSPACE;
-  struct Planned {
-    long long tiles;
-    Item it;
-  };
-  std::vector<Planned> all;
-  all.reserve(static_cast<size_t>(n));
-  for (int b = 0; b < p->batch_size; ++b) {
-    Planned x = {};
-    x.it.q_beg = p->qo_indptr_host[b];
-    x.it.q_len = p->qo_indptr_host[b + 1] - p->qo_indptr_host[b];
-    x.it.k_beg = p->kv_indptr_host[b];
-    x.it.k_len = p->kv_indptr_host[b + 1] - p->kv_indptr_host[b];
-    for (int row = 0; row < x.it.q_len; row += BM * NQ) {
-      x.it.row = row;
-      long long kend = p->causal ? static_cast<long long>(x.it.k_len) - x.it.q_len + row + BM * NQ : x.it.k_len;
-      kend = kend > x.it.k_len ? x.it.k_len : (kend < 0 ? 0 : kend);
-      x.tiles = (kend + BN - 1) / BN;
-      all.push_back(x);
-    }
-  }
-  std::stable_sort(all.begin(), all.end(), [](const Planned& x, const Planned& y) { return x.tiles > y.tiles; });
-  for (size_t i = 0; i < all.size(); ++i) std::memcpy(items_host + 8 * i, &all[i].it, sizeof(Item));
-  return ATF_OK;
-}
-
-extern "C" int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_stream_t stream) {
-  using namespace atf::prefill;
-  if (p == nullptr || p->q == nullptr || p->k == nullptr || p->v == nullptr || p->out == nullptr ||
-      p->items == nullptr)
-    return ATF_ERR_INVALID_ARG;
-  if (p->head_dim != ATF_HEAD_DIM) return ATF_ERR_UNSUPPORTED;
-  if (p->total_q < 1 || p->total_k < 1 || p->num_heads_q < 1 || p->num_heads_kv < 1 ||
-      p->num_heads_q % p->num_heads_kv != 0 || p->num_items < 0)
-    return ATF_ERR_INVALID_ARG;
-  if (p->total_q > 0x7fffffffLL - BM * NQ || p->total_k > 0x7fffffffLL - BN || p->num_heads_q > (1 << 20))
-    return ATF_ERR_UNSUPPORTED;
-  if (p->qk_layout != ATF_LAYOUT_SORTED_PAIR && p->qk_layout != ATF_LAYOUT_ROTATE_HALF) return ATF_ERR_INVALID_ARG;
-  if (p->window != ATF_WINDOW_OFF && p->window != ATF_WINDOW_SNAP16) return ATF_ERR_UNSUPPORTED;
-  if (!(p->softmax_scale > 0.f)) return ATF_ERR_INVALID_ARG;
-  if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->out) || !aligned16(p->items))
-    return ATF_ERR_ALIGNMENT;
-  const int64_t strides[8] = {p->q_stride_s, p->q_stride_h, p->k_stride_s, p->k_stride_h,
-                              p->v_stride_s, p->v_stride_h, p->o_stride_s, p->o_stride_h};
-  for (int i = 0; i < 8; ++i)
-    if (strides[i] < 0 || (strides[i] & 7) != 0) return ATF_ERR_ALIGNMENT;
-  if (p->window == ATF_WINDOW_SNAP16)
-    for (int i = 0; i < ATF_MAX_LEVELS; ++i)
-      if (p->zhi[i] < 0 || (i > 0 && p->zhi[i] > p->zhi[i - 1])) return ATF_ERR_INVALID_ARG;
-  int dev = 0;
-  int rc = check_device(&dev);
-  if (rc != ATF_OK) return rc;
-  if (p->num_items == 0) return ATF_OK;
-
-  // one batch of all packed rows; only the K maps that the call reads are encoded
-  CUtensorMap tq, tk, tv;
-  KLevelMaps tkl;
-  auto sane = [](int64_t stride, int64_t size) -> uint64_t {
-    return static_cast<uint64_t>(size == 1 ? 16 : stride * 2);
-  };
-  const bool sorted = p->qk_layout == ATF_LAYOUT_SORTED_PAIR;
-  const uint64_t nq = static_cast<uint64_t>(p->total_q), nk = static_cast<uint64_t>(p->total_k);
-  const uint64_t hq = static_cast<uint64_t>(p->num_heads_q), hkv = static_cast<uint64_t>(p->num_heads_kv);
-  {
-    const uint64_t dims[4] = {128, nq, hq, 1};
-    const uint64_t str[3] = {sane(p->q_stride_s, p->total_q), sane(p->q_stride_h, p->num_heads_q), 16};
-    const uint32_t box[4] = {sorted ? 64u : 8u, static_cast<uint32_t>(BM), 1, 1};
-    if ((rc = encode_tiled_bf16(&tq, p->q, 4, dims, str, box,
-                                sorted ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE)) != ATF_OK)
-      return rc;
-  }
-  const uint64_t ks = sane(p->k_stride_s, p->total_k), kh = sane(p->k_stride_h, p->num_heads_kv);
-  if (!sorted) {
-    const uint64_t dims[4] = {128, nk, hkv, 1};
-    const uint64_t str[3] = {ks, kh, 16};
-    const uint32_t box[4] = {8, static_cast<uint32_t>(BN), 1, 1};
-    if ((rc = encode_tiled_bf16(&tk, p->k, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_NONE)) != ATF_OK) return rc;
-  } else {
-    const uint64_t dims[5] = {16, nk, ATF_MAX_LEVELS, hkv, 1};
-    const uint64_t str[4] = {ks, 32, kh, 16};
-    for (int L = p->window ? 1 : ATF_MAX_LEVELS; L <= ATF_MAX_LEVELS; ++L) {
-      const uint32_t box[5] = {16, static_cast<uint32_t>(BN), static_cast<uint32_t>(L), 1, 1};
-      if ((rc = encode_tiled_bf16(&tkl.lv[L - 1], p->k, 5, dims, str, box, CU_TENSOR_MAP_SWIZZLE_32B)) != ATF_OK)
-        return rc;
-    }
-  }
-  {
-    const uint64_t dims[4] = {128, nk, hkv, 1};
-    const uint64_t str[3] = {sane(p->v_stride_s, p->total_k), sane(p->v_stride_h, p->num_heads_kv), 16};
-    const uint32_t box[4] = {64, static_cast<uint32_t>(BN), 1, 1};
-    if ((rc = encode_tiled_bf16(&tv, p->v, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) != ATF_OK) return rc;
-  }
-  Args a = {};
-  a.B = 1;
-  a.Hq = static_cast<int>(p->num_heads_q);
-  a.G = static_cast<int>(p->num_heads_q / p->num_heads_kv);
-  a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
-  a.causal = p->causal ? 1 : 0;
-  a.layout = p->qk_layout;
-  a.window = p->window == ATF_WINDOW_SNAP16 ? 1 : 0;
-  for (int i = 0; i < ATF_MAX_LEVELS; ++i) a.zhi[i] = p->zhi[i];
-  a.out = static_cast<__nv_bfloat16*>(p->out);
-  a.o_ss = p->o_stride_s;
-  a.o_sh = p->o_stride_h;
-  a.lse = p->lse;
-  a.err = p->error_flag;
-  a.items = p->items;
-  a.n_items = p->num_items;
-  a.total_q = p->total_q;
-  a.total_k = p->total_k;
-  return launch<true>(tq, tk, tkl, tv, a, static_cast<long long>(p->num_items) * a.Hq,
-                      reinterpret_cast<cudaStream_t>(stream));
+  if (cudaFuncSetAttribute(prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(SMEM_BYTES)) != cudaSuccess)
+    return ATF_ERR_CUDA;
+  const long long grid = static_cast<long long>(a.n_qblk) * a.B * a.Hq;
+  if (grid > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
+  // setmaxnreg.inc waits until the block's launch registers cover the split:
+  // never launch a build whose register count would leave it waiting
+  static const int launch_regs = [] {
+    cudaFuncAttributes fa{};
+    return cudaFuncGetAttributes(&fa, prefill_kernel) == cudaSuccess ? fa.numRegs : 0;
+  }();
+  if (static_cast<long long>(launch_regs) * THREADS < REG_SPLIT_TOTAL) return ATF_ERR_UNSUPPORTED;
+  prefill_kernel<<<static_cast<unsigned>(grid), THREADS, SMEM_BYTES,
+                   reinterpret_cast<cudaStream_t>(stream)>>>(tq, tk, tkl, tv, a);
+  return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
 }
