@@ -114,10 +114,9 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
         raise ValueError("kv_layout must be NHD or HND")
     if hk2 != hkv:
         raise ValueError("append_key heads do not match the cache")
-    bi = batch_indices.to(device=dev, dtype=torch.int32).contiguous()
-    ps = positions.to(device=dev, dtype=torch.int32).contiguous()
-    ip = kv_indptr.to(device=dev, dtype=torch.int32).contiguous()
-    ix = kv_indices.to(device=dev, dtype=torch.int32).contiguous()
+    bi, ps, ip, ix = (t if t.dtype == torch.int32 and t.device == dev and t.is_contiguous()
+                      else t.to(device=dev, dtype=torch.int32).contiguous()
+                      for t in (batch_indices, positions, kv_indptr, kv_indices))
     if bi.numel() != nnz or ps.numel() != nnz:
         raise ValueError("batch_indices and positions need one entry per appended token")
     if e4m3 and nnz == 0:

@@ -9,9 +9,13 @@
 //
 // A unit is (block of 256 query rows of a sequence, query head): two 128-row tiles.
 // The plan lists the blocks of all sequences by falling key count; units go kv head
-// by kv head, then block by block, then over the group's heads. Each of one CTA per
-// SM takes every 148th unit, forwards and backwards by turns, so that the CTAs' sums
-// of work are nearly equal.
+// by kv head, then block by block, then over the group's heads. The plan deals them
+// out in that order to one CTA per SM, each to the one with the least work so far
+// (a step of both tiles 1, of one tile 0.9, a unit's start and end 1.8), and the
+// kernel walks its list. (Every 148th unit to a CTA: 4 long chunks 780 us instead of
+// 730. CTAs that take the next unit from the hardware's queue with
+// clusterlaunchcontrol.try_cancel, handed on inside the CTA in shared memory, balanced
+// as well but ran each tile 5% slower: 4 x 4096 tokens, 24 heads, 464 against 440 us.)
 //
 // Why persistent: a block's fixed cost was 8 us against 2.1 us per key tile (start of
 // the CTA 0.8, barriers and TMEM 1.5, first loads 1.5, cold first step, a strided
@@ -38,6 +42,8 @@
 
 #include <algorithm>
 #include <cstring>
+#include <functional>
+#include <utility>
 #include <vector>
 
 #include "atf_internal.h"
@@ -125,6 +131,8 @@ struct Args {
   float* lse;
   int* err;
   const int* items;
+  const int* cta_units;  // [grid + 1]: where a CTA's units begin in `units`
+  const int* units;      // (kv head, item, head of the group) as one index
   int n_items, n_units;
   long long total_q, total_k;
 };
@@ -137,12 +145,22 @@ struct Unit {
   __device__ __forceinline__ int nk_max() const { return max(nk[0], nk[1]); }
 };
 
-// the CTA's n-th unit, -1 past its last: every gridDim.x-th one, backwards in odd rounds
-__device__ __forceinline__ int unit_index(const Args& a, int n) {
-  const int g = static_cast<int>(gridDim.x), c = static_cast<int>(blockIdx.x);
-  const long long u = static_cast<long long>(n) * g + ((n & 1) ? g - 1 - c : c);
-  return u < a.n_units ? static_cast<int>(u) : -1;
-}
+// a CTA's units, one after another; -1 past the last
+struct Walk {
+  const int* at;
+  int left;
+  __device__ __forceinline__ explicit Walk(const Args& a) {
+    const int b = __ldg(a.cta_units + blockIdx.x), e = __ldg(a.cta_units + blockIdx.x + 1);
+    at = a.units + b;
+    left = b >= 0 && e <= a.n_units ? e - b : 0;
+  }
+  __device__ __forceinline__ int next(const Args& a) {
+    if (left <= 0) return -1;
+    --left;
+    const int u = __ldg(at++);
+    return u >= 0 && u < a.n_units ? u : -1;
+  }
+};
 __device__ __forceinline__ Item load_item(const Args& a, int u) {
   const int rem = u % (a.n_items * a.G);
   const int4* p = reinterpret_cast<const int4*>(a.items) + 2 * (rem / a.G);
@@ -228,11 +246,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ---------------------------------------------------------------- producer
       int kc = 0, vc = 0, qc = 0;  // K and V stages and Q loads issued
       bool ok = true;
-      int u = unit_index(a, 0);
+      Walk walk(a);
+      int u = walk.next(a);
       Item it = u >= 0 ? load_item(a, u) : Item{};
-      for (int n = 0; ok && u >= 0; ++n) {
+      while (ok && u >= 0) {
         const Unit x = make_unit(a, u, it);
-        u = unit_index(a, n + 1);
+        u = walk.next(a);
         if (u >= 0) it = load_item(a, u);  // of the next unit
         const int nk_max = x.nk_max();
         if (nk_max == 0) continue;
@@ -305,11 +324,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       int kb = 0, vb = 0, qc = 0;               // stages and Q loads of the units before
       int sc0 = 0, sc1 = 0, oc0 = 0, oc1 = 0;   // S of each tile, and its units, before
       bool ok = true;
-      int u = unit_index(a, 0);
+      Walk walk(a);
+      int u = walk.next(a);
       Item it = u >= 0 ? load_item(a, u) : Item{};
-      for (int n = 0; ok && u >= 0; ++n) {
+      while (ok && u >= 0) {
         const Unit x = make_unit(a, u, it);
-        u = unit_index(a, n + 1);
+        u = walk.next(a);
         if (u >= 0) it = load_item(a, u);
         const int nk0 = x.nk[0], nk1 = x.nk[1], nk_max = x.nk_max();
         if (nk_max == 0) continue;
@@ -432,11 +452,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       const float sl2 = a.scale_log2;
       int mine = 0, other = 0, units = 0;  // S of this and of the other tile, and this tile's units, before
       bool ok = true;
-      int u = unit_index(a, 0);
+      Walk walk(a);
+      int u = walk.next(a);
       Item it = u >= 0 ? load_item(a, u) : Item{};
-      for (int n = 0; ok && u >= 0; ++n) {
+      while (ok && u >= 0) {
         const Unit x = make_unit(a, u, it);
-        u = unit_index(a, n + 1);
+        u = walk.next(a);
         if (u >= 0) it = load_item(a, u);
         const int my_nk = t ? x.nk[1] : x.nk[0], other_nk = t ? x.nk[0] : x.nk[1];
         const int row_w = x.row0 + t * BM + wq * 32;  // the warp's first row
@@ -619,11 +640,12 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 using namespace atf;
 
-extern "C" int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int32_t* items_host,
-                                       int32_t items_capacity, int32_t* num_items) {
+extern "C" int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int32_t* plan_host, int64_t capacity,
+                                       AtfPrefillRaggedPlan* out) {
   using namespace atf::ragged;
-  if (p == nullptr || num_items == nullptr || p->qo_indptr_host == nullptr || p->kv_indptr_host == nullptr ||
-      p->batch_size < 1 || (items_host == nullptr && items_capacity > 0))
+  if (p == nullptr || out == nullptr || p->qo_indptr_host == nullptr || p->kv_indptr_host == nullptr ||
+      p->batch_size < 1 || (plan_host == nullptr && capacity > 0) || p->num_heads_q < 1 || p->num_heads_kv < 1 ||
+      p->num_heads_q % p->num_heads_kv != 0 || p->num_sms < 0)
     return ATF_ERR_INVALID_ARG;
   long long n = 0;
   for (int b = 0; b < p->batch_size; ++b) {
@@ -633,13 +655,24 @@ extern "C" int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int3
     if (nq > (1ll << 30) || nk > (1ll << 30)) return ATF_ERR_UNSUPPORTED;
     n += (nq + BM * NQ - 1) / (BM * NQ);
   }
-  if (n > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
-  *num_items = static_cast<int32_t>(n);
-  if (items_host == nullptr) return ATF_OK;
-  if (n > items_capacity) return ATF_ERR_WORKSPACE;
+  const long long units = n * p->num_heads_q;
+  if (units > 0x3fffffffLL) return ATF_ERR_UNSUPPORTED;
+  int sms = p->num_sms;
+  if (sms == 0) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return ATF_ERR_CUDA;
+  }
+  const int ctas = static_cast<int>(units < sms ? units : sms);
+  out->num_items = static_cast<int32_t>(n);
+  out->num_ctas = ctas;
+  out->plan_ints = 8 * n + ctas + 1 + units;
+  if (plan_host == nullptr) return ATF_OK;
+  if (capacity < out->plan_ints) return ATF_ERR_WORKSPACE;
   struct Planned {
-    long long tiles;
     Item it;
+    int steps[NQ];  // key tiles of each query tile
   };
   std::vector<Planned> all;
   all.reserve(static_cast<size_t>(n));
@@ -651,32 +684,69 @@ extern "C" int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int3
     x.it.k_len = p->kv_indptr_host[b + 1] - p->kv_indptr_host[b];
     for (int row = 0; row < x.it.q_len; row += BM * NQ) {
       x.it.row = row;
-      long long kend = p->causal ? static_cast<long long>(x.it.k_len) - x.it.q_len + row + BM * NQ : x.it.k_len;
-      kend = kend > x.it.k_len ? x.it.k_len : (kend < 0 ? 0 : kend);
-      x.tiles = (kend + BN - 1) / BN;
+      for (int t = 0; t < NQ; ++t) {
+        long long kend = p->causal ? static_cast<long long>(x.it.k_len) - x.it.q_len + row + (t + 1) * BM : x.it.k_len;
+        if (kend > x.it.k_len) kend = x.it.k_len;
+        x.steps[t] = row + t * BM < x.it.q_len && kend > 0 ? static_cast<int>((kend + BN - 1) / BN) : 0;
+      }
       all.push_back(x);
     }
   }
-  std::stable_sort(all.begin(), all.end(), [](const Planned& x, const Planned& y) { return x.tiles > y.tiles; });
-  for (size_t i = 0; i < all.size(); ++i) std::memcpy(items_host + 8 * i, &all[i].it, sizeof(Item));
+  auto longest = [](const Planned& x) { return x.steps[0] > x.steps[1] ? x.steps[0] : x.steps[1]; };
+  std::stable_sort(all.begin(), all.end(),
+                   [&](const Planned& x, const Planned& y) { return longest(x) > longest(y); });
+  for (size_t i = 0; i < all.size(); ++i) std::memcpy(plan_host + 8 * i, &all[i].it, sizeof(Item));
+  int32_t* offsets = plan_host + 8 * n;
+  int32_t* list = offsets + ctas + 1;
+  if (ctas == 0) {
+    offsets[0] = 0;
+    return ATF_OK;
+  }
+  // Each unit, in order, to the CTA with the least work so far (ties: the lowest),
+  // in hundredths of a step of both tiles.
+  const int G = p->num_heads_q / p->num_heads_kv;
+  std::vector<int32_t> owner(static_cast<size_t>(units));
+  std::vector<long long> count(static_cast<size_t>(ctas), 0);
+  using Load = std::pair<long long, int>;
+  std::vector<Load> heap;
+  for (int c = 0; c < ctas; ++c) heap.emplace_back(0, c);
+  const auto more = std::greater<Load>();
+  std::make_heap(heap.begin(), heap.end(), more);
+  size_t u = 0;
+  for (int hk = 0; hk < p->num_heads_kv; ++hk)
+    for (const Planned& x : all) {
+      const int both = x.steps[0] < x.steps[1] ? x.steps[0] : x.steps[1];
+      const long long cost = 100ll * both + 90ll * (longest(x) - both) + 180;
+      for (int g = 0; g < G; ++g, ++u) {
+        std::pop_heap(heap.begin(), heap.end(), more);
+        heap.back().first += cost;
+        owner[u] = heap.back().second;
+        ++count[static_cast<size_t>(owner[u])];
+        std::push_heap(heap.begin(), heap.end(), more);
+      }
+    }
+  offsets[0] = 0;
+  for (int c = 0; c < ctas; ++c) offsets[c + 1] = offsets[c] + static_cast<int32_t>(count[static_cast<size_t>(c)]);
+  std::vector<int32_t> next(offsets, offsets + ctas);
+  for (size_t i = 0; i < owner.size(); ++i) list[next[static_cast<size_t>(owner[i])]++] = static_cast<int32_t>(i);
   return ATF_OK;
 }
 
 extern "C" int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_stream_t stream) {
   using namespace atf::ragged;
   if (p == nullptr || p->q == nullptr || p->k == nullptr || p->v == nullptr || p->out == nullptr ||
-      p->items == nullptr)
+      p->plan == nullptr)
     return ATF_ERR_INVALID_ARG;
   if (p->head_dim != ATF_HEAD_DIM) return ATF_ERR_UNSUPPORTED;
   if (p->total_q < 1 || p->total_k < 1 || p->num_heads_q < 1 || p->num_heads_kv < 1 ||
-      p->num_heads_q % p->num_heads_kv != 0 || p->num_items < 0)
+      p->num_heads_q % p->num_heads_kv != 0 || p->num_items < 0 || p->num_ctas < 0)
     return ATF_ERR_INVALID_ARG;
   if (p->total_q > 0x7fffffffLL - BM * NQ || p->total_k > 0x7fffffffLL - BN || p->num_heads_q > (1 << 20))
     return ATF_ERR_UNSUPPORTED;
   if (p->qk_layout != ATF_LAYOUT_SORTED_PAIR && p->qk_layout != ATF_LAYOUT_ROTATE_HALF) return ATF_ERR_INVALID_ARG;
   if (p->window != ATF_WINDOW_OFF && p->window != ATF_WINDOW_SNAP16) return ATF_ERR_UNSUPPORTED;
   if (!(p->softmax_scale > 0.f)) return ATF_ERR_INVALID_ARG;
-  if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->out) || !aligned16(p->items))
+  if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->out) || !aligned16(p->plan))
     return ATF_ERR_ALIGNMENT;
   const int64_t strides[8] = {p->q_stride_s, p->q_stride_h, p->k_stride_s, p->k_stride_h,
                               p->v_stride_s, p->v_stride_h, p->o_stride_s, p->o_stride_h};
@@ -688,7 +758,7 @@ extern "C" int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_strea
   int dev = 0;
   int rc = check_device(&dev);
   if (rc != ATF_OK) return rc;
-  if (p->num_items == 0) return ATF_OK;
+  if (p->num_items == 0 || p->num_ctas == 0) return ATF_OK;
 
   // one batch of all packed rows; only the K maps that the call reads are encoded
   CUtensorMap tq, tk, tv;
@@ -741,10 +811,12 @@ extern "C" int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_strea
   a.o_sh = p->o_stride_h;
   a.lse = p->lse;
   a.err = p->error_flag;
-  a.items = p->items;
-  a.n_items = p->num_items;
   const long long units = static_cast<long long>(p->num_items) * a.Hq;
-  if (units > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
+  if (units > 0x3fffffffLL) return ATF_ERR_UNSUPPORTED;
+  a.items = p->plan;
+  a.cta_units = p->plan + 8ll * p->num_items;
+  a.units = a.cta_units + p->num_ctas + 1;
+  a.n_items = p->num_items;
   a.n_units = static_cast<int>(units);
   a.total_q = p->total_q;
   a.total_k = p->total_k;
@@ -758,10 +830,7 @@ extern "C" int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_strea
     return cudaFuncGetAttributes(&fa, ragged_kernel) == cudaSuccess ? fa.numRegs : 0;
   }();
   if (static_cast<long long>(launch_regs) * THREADS < REG_SPLIT_TOTAL) return ATF_ERR_UNSUPPORTED;
-  int sms = 0;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1)
-    return ATF_ERR_CUDA;
-  const unsigned grid = static_cast<unsigned>(units < sms ? units : sms);
-  ragged_kernel<<<grid, THREADS, SMEM_BYTES, reinterpret_cast<cudaStream_t>(stream)>>>(tq, tk, tkl, tv, a);
+  ragged_kernel<<<static_cast<unsigned>(p->num_ctas), THREADS, SMEM_BYTES, reinterpret_cast<cudaStream_t>(stream)>>>(
+      tq, tk, tkl, tv, a);
   return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
 }
