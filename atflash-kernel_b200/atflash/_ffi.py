@@ -125,20 +125,15 @@ class AtfKvScales(ctypes.Structure):
 
 
 class AtfPrefillRaggedPlanParams(ctypes.Structure):
-    _fields_ = [("batch_size", _i32), ("qo_indptr_host", _vp), ("kv_indptr_host", _vp), ("num_heads_q", _i32),
-                ("num_heads_kv", _i32), ("num_sms", _i32), ("causal", ctypes.c_int)]
-
-
-class AtfPrefillRaggedPlan(ctypes.Structure):
-    _fields_ = [("num_items", _i32), ("num_ctas", _i32), ("plan_ints", _i64)]
+    _fields_ = [("batch_size", _i32), ("qo_indptr_host", _vp), ("kv_indptr_host", _vp), ("causal", ctypes.c_int)]
 
 
 class AtfPrefillRaggedParams(ctypes.Structure):
     _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("lse", _vp), ("total_q", _i64), ("total_k", _i64),
                 ("num_heads_q", _i64), ("num_heads_kv", _i64), ("head_dim", _i64), ("q_stride_s", _i64),
                 ("q_stride_h", _i64), ("k_stride_s", _i64), ("k_stride_h", _i64), ("v_stride_s", _i64),
-                ("v_stride_h", _i64), ("o_stride_s", _i64), ("o_stride_h", _i64), ("plan", _vp),
-                ("num_items", _i32), ("num_ctas", _i32), ("softmax_scale", _f32), ("causal", ctypes.c_int), ("qk_layout", ctypes.c_int),
+                ("v_stride_h", _i64), ("o_stride_s", _i64), ("o_stride_h", _i64), ("items", _vp),
+                ("num_items", _i32), ("softmax_scale", _f32), ("causal", ctypes.c_int), ("qk_layout", ctypes.c_int),
                 ("window", ctypes.c_int), ("zhi", _i32 * 8), ("error_flag", _vp)]
 
 
@@ -190,7 +185,7 @@ def load() -> ctypes.CDLL:
             lib.atf_ipc_import.argtypes = [_vp, _i64, P(_vp), P(_vp)]
             lib.atf_ipc_release.argtypes = [_vp]
             lib.atf_build_page_tables.argtypes = [P(AtfPageTablesParams), _vp]
-            lib.atf_prefill_ragged_plan.argtypes = [P(AtfPrefillRaggedPlanParams), P(_i32), _i64, P(AtfPrefillRaggedPlan)]
+            lib.atf_prefill_ragged_plan.argtypes = [P(AtfPrefillRaggedPlanParams), P(_i32), _i32, P(_i32)]
             lib.atf_prefill_ragged_fwd.argtypes = [P(AtfPrefillRaggedParams), _vp]
             lib.atf_decode_run_e4m3.argtypes = [P(AtfDecodeParams), P(AtfKvScales), _vp]
             lib.atf_paged_kv_append_e4m3.argtypes = [P(AtfAppendParams), P(AtfKvScales), _vp]

@@ -60,19 +60,17 @@ class BatchPrefillWithRaggedKVCacheWrapper:
         pp = _ffi.AtfPrefillRaggedPlanParams()
         pp.batch_size, pp.causal = len(cq) - 1, 1 if causal else 0
         pp.qo_indptr_host, pp.kv_indptr_host = cq.ctypes.data, ck.ctypes.data
-        pp.num_heads_q, pp.num_heads_kv = num_qo_heads, num_kv_heads
-        pp.num_sms = torch.cuda.get_device_properties(self._dev).multi_processor_count
-        size = _ffi.AtfPrefillRaggedPlan()
+        n = ctypes.c_int32(0)
         lib = _ffi.load()
-        _ffi.check("atf_prefill_ragged_plan", lib.atf_prefill_ragged_plan(ctypes.byref(pp), None, 0, ctypes.byref(size)))
-        plan = np.empty(size.plan_ints, dtype=np.int32)
+        _ffi.check("atf_prefill_ragged_plan", lib.atf_prefill_ragged_plan(ctypes.byref(pp), None, 0, ctypes.byref(n)))
+        items = np.zeros((max(1, n.value), 8), dtype=np.int32)
         _ffi.check("atf_prefill_ragged_plan", lib.atf_prefill_ragged_plan(
-            ctypes.byref(pp), plan.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), plan.size, ctypes.byref(size)))
-        self._schedule = torch.from_numpy(plan).to(self._dev)
+            ctypes.byref(pp), items.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), items.shape[0], ctypes.byref(n)))
+        self._items = torch.from_numpy(items).to(self._dev)
         t = _ffi.AtfPrefillRaggedParams()
         t.total_q, t.total_k = int(cq[-1]), int(ck[-1])
         t.num_heads_q, t.num_heads_kv, t.head_dim = num_qo_heads, num_kv_heads, head_dim
-        t.plan, t.num_items, t.num_ctas = self._schedule.data_ptr(), size.num_items, size.num_ctas
+        t.items, t.num_items = self._items.data_ptr(), n.value
         t.softmax_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim)
         t.causal, t.qk_layout = pp.causal, _LAYOUTS[qk_layout]
         t.window = _ffi.ATF_WINDOW_SNAP16 if zhi is not None else _ffi.ATF_WINDOW_OFF

@@ -97,7 +97,6 @@ extern "C" int64_t atf_params_size(const char* name) {
       {"AtfPageTablesParams", static_cast<int64_t>(sizeof(AtfPageTablesParams))},
       {"AtfKvScales", static_cast<int64_t>(sizeof(AtfKvScales))},
       {"AtfPrefillRaggedPlanParams", static_cast<int64_t>(sizeof(AtfPrefillRaggedPlanParams))},
-      {"AtfPrefillRaggedPlan", static_cast<int64_t>(sizeof(AtfPrefillRaggedPlan))},
       {"AtfPrefillRaggedParams", static_cast<int64_t>(sizeof(AtfPrefillRaggedParams))},
   };
   for (const Entry& e : kSizes)

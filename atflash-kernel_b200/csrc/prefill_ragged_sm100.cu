@@ -1,39 +1,28 @@
-// Causal or full attention over packed sequences of different lengths, for sm_100a:
-// the dense prefill's pipeline (prefill_sm100.cu) made persistent.
+// Causal or full attention over packed sequences of different lengths, for sm_100a.
 //
-// Mathematics, tiles and arithmetic are the dense kernel's: per query row an online
-// softmax in the log2 domain over 128-key tiles, S = Q K^T over the window's 16-dim
-// levels and O += P V on the tensor cores with both accumulators in TMEM, P in bf16.
-// A sequence's rows are those of a dense run of its own, bit for bit: the window is
+// Mathematics, tiles and pipeline are the dense prefill's (prefill_sm100.cu): per
+// query row an online softmax in the log2 domain over 128-key tiles, S = Q K^T over
+// the window's 16-dim levels and O += P V on the tensor cores with both accumulators
+// in TMEM, P in bf16; a producer warp, an MMA warp and two softmax groups. A
+// sequence's rows are those of a dense run of its own, bit for bit: the window is
 // quantised per (query tile, key tile) from the sequence's own first row and key.
 //
-// A unit is (block of 256 query rows of a sequence, query head): two 128-row tiles.
-// The plan lists the blocks of all sequences by falling key count; units go kv head
-// by kv head, then block by block, then over the group's heads. The plan deals them
-// out in that order to one CTA per SM, each to the one with the least work so far
-// (a step of both tiles 1, of one tile 0.9, a unit's start and end 1.8), and the
-// kernel walks its list. (Every 148th unit to a CTA: 4 long chunks 780 us instead of
-// 730. CTAs that take the next unit from the hardware's queue with
-// clusterlaunchcontrol.try_cancel, handed on inside the CTA in shared memory, balanced
-// as well but ran each tile 5% slower: 4 x 4096 tokens, 24 heads, 464 against 440 us.)
+// CTA = (block of 256 query rows of a sequence, query head). The plan lists the blocks
+// of all sequences by falling key count; the grid walks kv heads, then blocks, then
+// the heads of the group, so that CTAs resident together share K and V in L2 and the
+// last ones are the shortest.
 //
-// Why persistent: a block's fixed cost was 8 us against 2.1 us per key tile (start of
-// the CTA 0.8, barriers and TMEM 1.5, first loads 1.5, cold first step, a strided
-// epilogue 2.3 us; 64 sequences of 256 tokens, 28 heads: 170 us). Here barriers and
-// TMEM are set up once, and while a unit's last tiles are still in softmax and
-// epilogue the producer loads the next unit's Q, K and V and the MMA warp computes
-// its first scores. All barrier phases count on through the units.
-//   - Q has one buffer: free when the unit's last S = Q K^T has completed (Q_EMPTY).
-//   - O_t is free for the next unit's first O_t = P V once tile t's epilogue has read
-//     it from TMEM (OFREE).
-//   - S_t and the P in its upper half: the next unit's S is issued after every P V of
-//     this unit, by the same thread, so in order; P V waits for P, which follows the
-//     read of S.
-//   - a tile without keys (rows past the sequence, or before its first key) takes no
-//     part in a unit and advances no phase.
-// Q comes in rows of 128 bytes (two boxes of 64 dims, 128-byte swizzle; in
-// rotate_half order in the dense kernel's 8-dim boxes). Outputs go through shared
-// memory, 4 KB per warp, and leave in full 128-byte lines.
+// What bounds it: a step of two query tiles against a key tile takes 1.65 us (1.5 where
+// the window leaves half of K; exponentials and tensor work, as in the dense kernel),
+// and a CTA's start and end cost extra, which short sequences feel. So Q comes in
+// rows of 128 bytes (two boxes of 64 dims, 128-byte swizzle; 8-dim boxes as in the
+// dense kernel took 1-2 us longer; rotate_half keeps them), the item, the error flag,
+// the barriers and TMEM are set up side by side, and the outputs leave through shared
+// memory in whole lines. A persistent form of this kernel, whose next unit's loads
+// and scores ran under the epilogue, cost 2.5 us less per block but 0.3 us more per
+// step: its barrier phases and stages, counted on through the units, are no longer
+// known to be uniform, and the MMA warp's issue is what a step waits for. It lost
+// wherever a block has more than about 8 key tiles.
 //
 // A tile's last box may reach into the next sequence: its queries are not stored, its
 // keys are masked, and its V rows, whose P is 0, are cleared in shared memory before
@@ -42,8 +31,6 @@
 
 #include <algorithm>
 #include <cstring>
-#include <functional>
-#include <utility>
 #include <vector>
 
 #include "atf_internal.h"
@@ -89,30 +76,25 @@ __device__ __forceinline__ void qk_group_rows_asm(uint32_t d_tmem, uint64_t qd, 
 constexpr uint32_t OFF_Q = 0;
 constexpr uint32_t OFF_K = OFF_Q + NQ * QTILE_BYTES;
 constexpr uint32_t OFF_V = OFF_K + KST * KSTAGE_BYTES;
-constexpr uint32_t OFF_OUT = OFF_V + VST * VSTAGE_BYTES;  // 8 warps x [32 rows][128 B]
-constexpr uint32_t OUT_BYTES = 32 * 128;
-constexpr uint32_t OFF_BAR = OFF_OUT + 8 * OUT_BYTES;
+constexpr uint32_t OFF_BAR = OFF_V + VST * VSTAGE_BYTES;
 
 enum {
-  B_QFULL = 0,
-  B_QEMPTY,                   // the unit's last S has completed
-  B_KFULL,
+  B_Q = 0,
+  B_KFULL = 1,
   B_KEMPTY = B_KFULL + KST,
   B_VFULL = B_KEMPTY + KST,
   B_VEMPTY = B_VFULL + VST,
-  B_SFULL = B_VEMPTY + VST,   // [t], one phase per S_t
-  B_LOADED = B_SFULL + NQ,    // [t], one phase per S_t: its scores are in registers
-  B_PFULL = B_LOADED + NQ,    // [t], one phase per P_t
-  B_ODONE = B_PFULL + NQ,     // [t], one phase per O_t += P_t V
-  B_OFINAL = B_ODONE + NQ,    // [t], one phase per unit of tile t: its last O += P V done
-  B_OFREE = B_OFINAL + NQ,    // [t], one phase per unit of tile t: O has been read
-  B_FINAL = B_OFREE + NQ,
+  B_SFULL = B_VEMPTY + VST,   // [t]
+  B_PFULL = B_SFULL + NQ,     // [t]
+  B_ODONE = B_PFULL + NQ,     // [t], one phase per O += P V
+  B_OFINAL = B_ODONE + NQ,    // [t], single phase: the tile's last O += P V done
+  B_LOADED = B_OFINAL + NQ,   // [t], phase j: tile t's softmax has read S_t(j) into registers
+  B_FINAL = B_LOADED + NQ,
   NUM_BARS
 };
 constexpr uint32_t OFF_ABORT = OFF_BAR + 8 * NUM_BARS;
 constexpr uint32_t OFF_TMEM = OFF_ABORT + 16;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16 + 1024;  // slack for 1024-B alignment
-static_assert(SMEM_BYTES <= 227 * 1024, "one CTA per SM");
 
 // One work item of the plan: 256 query rows from `row` on of one sequence. Rows and
 // keys are the sequence's own; the packed tensors hold them from q_beg and k_beg on.
@@ -131,66 +113,10 @@ struct Args {
   float* lse;
   int* err;
   const int* items;
-  const int* cta_units;  // [grid + 1]: where a CTA's units begin in `units`
-  const int* units;      // (kv head, item, head of the group) as one index
-  int n_items, n_units;
+  int n_items;
   long long total_q, total_k;
 };
 
-struct Unit {
-  int q_tok, k_tok, sk, row_end, row0, hk, h;
-  int q_offset;  // position of the sequence's query row 0 among its keys (may be negative)
-  int nk[NQ];    // key tiles of each query tile
-
-  __device__ __forceinline__ int nk_max() const { return max(nk[0], nk[1]); }
-};
-
-// a CTA's units, one after another; -1 past the last
-struct Walk {
-  const int* at;
-  int left;
-  __device__ __forceinline__ explicit Walk(const Args& a) {
-    const int b = __ldg(a.cta_units + blockIdx.x), e = __ldg(a.cta_units + blockIdx.x + 1);
-    at = a.units + b;
-    left = b >= 0 && e <= a.n_units ? e - b : 0;
-  }
-  __device__ __forceinline__ int next(const Args& a) {
-    if (left <= 0) return -1;
-    --left;
-    const int u = __ldg(at++);
-    return u >= 0 && u < a.n_units ? u : -1;
-  }
-};
-__device__ __forceinline__ Item load_item(const Args& a, int u) {
-  const int rem = u % (a.n_items * a.G);
-  const int4* p = reinterpret_cast<const int4*>(a.items) + 2 * (rem / a.G);
-  const int4 x = __ldg(p), y = __ldg(p + 1);
-  return Item{x.x, x.y, x.z, x.w, y.x, {0, 0, 0}};
-}
-// An item outside the packed rows (a plan made for others) has no tiles and no rows.
-__device__ __forceinline__ Unit make_unit(const Args& a, int u, const Item& it) {
-  const int per_head = a.n_items * a.G, rem = u % per_head;
-  Unit x;
-  x.hk = u / per_head;
-  x.h = x.hk * a.G + rem % a.G;
-  const bool bad = it.q_beg < 0 || it.q_len < 0 || it.k_beg < 0 || it.k_len < 0 || it.row < 0 ||
-                   static_cast<long long>(it.q_beg) + it.q_len > a.total_q ||
-                   static_cast<long long>(it.k_beg) + it.k_len > a.total_k;
-  if (bad && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
-  x.q_tok = it.q_beg;
-  x.k_tok = it.k_beg;
-  x.sk = it.k_len;
-  x.row0 = it.row;
-  x.row_end = bad ? 0 : it.q_len;
-  x.q_offset = it.k_len - it.q_len;
-#pragma unroll
-  for (int t = 0; t < NQ; ++t) {
-    const int r = it.row + t * BM;
-    int kend = a.causal ? min(x.q_offset + r + BM, x.sk) : x.sk;
-    x.nk[t] = (r < x.row_end && kend > 0) ? (kend + BN - 1) / BN : 0;
-  }
-  return x;
-}
 // key tile j reads level i when j >= lim[i] (the dense kernel's rule)
 __device__ __forceinline__ void window_limits(const Args& a, int q_offset, int row0, int (&lim)[ATF_MAX_LEVELS]) {
   const long long base = static_cast<long long>(q_offset) + row0 - (BN - 1);
@@ -203,7 +129,8 @@ __device__ __forceinline__ void window_limits(const Args& a, int q_offset, int r
 
 __global__ void __launch_bounds__(THREADS, 1)
     ragged_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ KLevelMaps tmKL, const __grid_constant__ CUtensorMap tmV, const Args a) {
+                   const __grid_constant__ KLevelMaps tmKL,
+                   const __grid_constant__ CUtensorMap tmV, const Args a) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t sb = (raw_u32 + 1023u) & ~1023u;
@@ -211,20 +138,44 @@ __global__ void __launch_bounds__(THREADS, 1)
   volatile int* s_abort = reinterpret_cast<volatile int*>(sp + OFF_ABORT);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sp + OFF_TMEM);
   auto bar = [&](int i) -> uint32_t { return sb + OFF_BAR + 8u * static_cast<uint32_t>(i); };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool sorted = a.layout == ATF_LAYOUT_SORTED_PAIR;
 
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  // This CTA's unit. Its loads are issued side by side: thread 0's of the error flag
+  // does not hold up the barriers, and the barriers do not wait for the item.
+  const int per_head = a.n_items * a.G;
+  const int rem = static_cast<int>(blockIdx.x) % per_head;
+  const int hk = static_cast<int>(blockIdx.x) / per_head;
+  const int h = hk * a.G + rem % a.G;
+  const int4* src = reinterpret_cast<const int4*>(a.items) + 2 * (rem / a.G);
+  const int4 it0 = __ldg(src), it1 = __ldg(src + 1);
+  int err0 = 0;
+  if (threadIdx.x == 0 && a.err != nullptr) err0 = *reinterpret_cast<volatile int*>(a.err);
   if (threadIdx.x == 0) {
-    *s_abort = (a.err != nullptr && *reinterpret_cast<volatile int*>(a.err) != 0) ? 1 : 0;
-    for (int i = 0; i < NUM_BARS; ++i) {
-      const bool wide = (i >= B_LOADED && i < B_ODONE) || (i >= B_OFREE && i < B_FINAL);
-      mbar_init(bar(i), wide ? 128 : 1);  // LOADED, PFULL, OFREE: a whole softmax group
+    mbar_init(bar(B_Q), 1);
+    for (int s = 0; s < KST; ++s) {
+      mbar_init(bar(B_KFULL + s), 1);
+      mbar_init(bar(B_KEMPTY + s), 1);
     }
+    for (int s = 0; s < VST; ++s) {
+      mbar_init(bar(B_VFULL + s), 1);
+      mbar_init(bar(B_VEMPTY + s), 1);
+    }
+    for (int t = 0; t < NQ; ++t) {
+      mbar_init(bar(B_SFULL + t), 1);
+      mbar_init(bar(B_PFULL + t), 128);
+      mbar_init(bar(B_ODONE + t), 1);
+      mbar_init(bar(B_OFINAL + t), 1);
+      mbar_init(bar(B_LOADED + t), 128);
+    }
+    mbar_init(bar(B_FINAL), 1);
     fence_mbar_init();
   }
   if (warp == WARP_LOAD && lane == 0) {
     tma_prefetch_desc(&tmQ);
-    if (!sorted)
+    // only the maps that this call uses are there
+    if (a.layout != ATF_LAYOUT_SORTED_PAIR)
       tma_prefetch_desc(&tmK);
     else
       for (int L = a.window ? 0 : ATF_MAX_LEVELS - 1; L < ATF_MAX_LEVELS; ++L) tma_prefetch_desc(&tmKL.lv[L]);
@@ -234,6 +185,35 @@ __global__ void __launch_bounds__(THREADS, 1)
     tmem_alloc(smem_u32(s_tmem), 512);
     tmem_relinquish();
   }
+  // first packed row of the sequence's queries and keys, its keys, its rows and the
+  // position of its query row 0 among its keys (negative: rows without keys)
+  const int q_tok = it0.x, k_tok = it0.z, sk = it0.w, row_base = it1.x;
+  const int q_offset = it0.w - it0.y;
+  // an item outside the packed rows (a plan made for others) has no rows
+  const bool bad = it0.x < 0 || it0.y < 0 || it0.z < 0 || it0.w < 0 || it1.x < 0 ||
+                   static_cast<long long>(it0.x) + it0.y > a.total_q ||
+                   static_cast<long long>(it0.z) + it0.w > a.total_k;
+  const int row_end = bad ? 0 : it0.y;
+  if (threadIdx.x == 0) {
+    *s_abort = err0 != 0 ? 1 : 0;
+    if (bad && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
+  }
+  int row0[NQ], nk[NQ];
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    row0[t] = row_base + t * BM;
+    if (row0[t] >= row_end) {
+      nk[t] = 0;
+    } else {
+      const int kend = a.causal ? min(q_offset + row0[t] + BM, sk) : sk;
+      nk[t] = kend > 0 ? (kend + BN - 1) / BN : 0;
+    }
+  }
+  const int nk_max = nk[0] > nk[1] ? nk[0] : nk[1];
+  int lim[NQ][ATF_MAX_LEVELS];
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) window_limits(a, q_offset, row0[t], lim[t]);
+
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -244,148 +224,146 @@ __global__ void __launch_bounds__(THREADS, 1)
     reg_dealloc<REG_SMALL>();
     if (start_ok && warp == WARP_LOAD) {
       // ---------------------------------------------------------------- producer
-      int kc = 0, vc = 0, qc = 0;  // K and V stages and Q loads issued
+      // All 32 lanes run this loop with warp-uniform values; one elected lane
+      // issues each TMA / expect_tx.
+      int issued_k = 0, issued_v = 0;
       bool ok = true;
-      Walk walk(a);
-      int u = walk.next(a);
-      Item it = u >= 0 ? load_item(a, u) : Item{};
-      while (ok && u >= 0) {
-        const Unit x = make_unit(a, u, it);
-        u = walk.next(a);
-        if (u >= 0) it = load_item(a, u);  // of the next unit
-        const int nk_max = x.nk_max();
-        if (nk_max == 0) continue;
-        int lim[NQ][ATF_MAX_LEVELS];
+      {
+        uint32_t qbytes = 0;
 #pragma unroll
-        for (int t = 0; t < NQ; ++t) window_limits(a, x.q_offset, x.row0 + t * BM, lim[t]);
-        ok = __all_sync(FULL, mbar_wait_inl(bar(B_QEMPTY), (qc & 1) ^ 1, ab, kDevErrTimeout));
-        if (!ok) break;
-        mbar_arrive_expect_tx_elect(bar(B_QFULL), ((x.nk[0] > 0) + (x.nk[1] > 0)) * QTILE_BYTES);
+        for (int t = 0; t < NQ; ++t) qbytes += nk[t] > 0 ? QTILE_BYTES : 0u;
+        mbar_arrive_expect_tx_elect(bar(B_Q), qbytes);
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
-          if (x.nk[t] == 0) continue;
-          const uint32_t dst = sb + OFF_Q + t * QTILE_BYTES;
-          const int row = x.q_tok + x.row0 + t * BM;
-          if (sorted) {
-            tma_load_4d_elect(dst, &tmQ, bar(B_QFULL), 0, row, x.h, 0);
-            tma_load_4d_elect(dst + QTILE_BYTES / 2, &tmQ, bar(B_QFULL), 64, row, x.h, 0);
-          } else {
-            for (int i = 0; i < 16; ++i)
-              tma_load_4d_elect(dst + (i >> 1) * QSLAB_BYTES + (i & 1) * QHALF_BYTES, &tmQ, bar(B_QFULL),
-                                level_col(a.layout, i >> 1, i & 1), row, x.h, 0);
+          if (nk[t] == 0) continue;
+          if (a.layout == ATF_LAYOUT_SORTED_PAIR) {
+            // two boxes of 128-byte rows: an eighth of the 8-dim boxes' row pieces
+            tma_load_4d_elect(sb + OFF_Q + t * QTILE_BYTES, &tmQ, bar(B_Q), 0, q_tok + row0[t], h, 0);
+            tma_load_4d_elect(sb + OFF_Q + t * QTILE_BYTES + QTILE_BYTES / 2, &tmQ, bar(B_Q), 64, q_tok + row0[t], h,
+                              0);
+            continue;
           }
-        }
-        ++qc;
-        for (int j = 0; j < nk_max; ++j) {
-          const int ks = kc % KST, vs = vc % VST;
-          ok = __all_sync(FULL, mbar_wait_inl(bar(B_KEMPTY + ks), ((kc / KST) & 1) ^ 1, ab, kDevErrTimeout));
-          if (!ok) break;
-          int L = 0;
 #pragma unroll
-          for (int t = 0; t < NQ; ++t)
-            if (j < x.nk[t]) L = max(L, levels_for(lim[t], j));
-          const uint32_t kdst = sb + OFF_K + ks * KSTAGE_BYTES;
-          const int key = x.k_tok + j * BN;
-          mbar_arrive_expect_tx_elect(bar(B_KFULL + ks), static_cast<uint32_t>(L) * KSLAB_BYTES);
-          if (sorted) {
-            if (elect_one_lane()) tma_load_5d(kdst, &tmKL.lv[L - 1], bar(B_KFULL + ks), 0, key, 0, x.hk, 0);
-            __syncwarp();
-          } else {
-            for (int i = 0; i < L; ++i) {
-              tma_load_4d_elect(kdst + i * KSLAB_BYTES, &tmK, bar(B_KFULL + ks), level_col(a.layout, i, 0), key, x.hk,
-                                0);
-              tma_load_4d_elect(kdst + i * KSLAB_BYTES + KHALF_BYTES, &tmK, bar(B_KFULL + ks),
-                                level_col(a.layout, i, 1), key, x.hk, 0);
-            }
-          }
-          ++kc;
-          ok = __all_sync(FULL, mbar_wait_inl(bar(B_VEMPTY + vs), ((vc / VST) & 1) ^ 1, ab, kDevErrTimeout));
-          if (!ok) break;
-          const uint32_t vdst = sb + OFF_V + vs * VSTAGE_BYTES;
-          mbar_arrive_expect_tx_elect(bar(B_VFULL + vs), VSTAGE_BYTES);
-          tma_load_4d_elect(vdst, &tmV, bar(B_VFULL + vs), 0, key, x.hk, 0);
-          tma_load_4d_elect(vdst + VBOX_BYTES, &tmV, bar(B_VFULL + vs), 64, key, x.hk, 0);
-          ++vc;
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+              tma_load_4d_elect(sb + OFF_Q + t * QTILE_BYTES + i * QSLAB_BYTES + hh * QHALF_BYTES, &tmQ,
+                                bar(B_Q), level_col(a.layout, i, hh), q_tok + row0[t], h, 0);
         }
       }
-      // every copy issued lands before shared memory is released
-      if (qc > 0) drain_wait(bar(B_QFULL), (qc - 1) & 1);
-      for (int j = max(0, kc - KST); j < kc; ++j) drain_wait(bar(B_KFULL + j % KST), (j / KST) & 1);
-      for (int j = max(0, vc - VST); j < vc; ++j) drain_wait(bar(B_VFULL + j % VST), (j / VST) & 1);
+      for (int j = 0; j < nk_max; ++j) {
+        const int ks = j % KST, vs = j % VST;
+        ok = __all_sync(FULL, mbar_wait_inl(bar(B_KEMPTY + ks), ((j / KST) & 1) ^ 1, ab, kDevErrTimeout));
+        if (!ok) break;
+        int L = 0;
+#pragma unroll
+        for (int t = 0; t < NQ; ++t)
+          if (j < nk[t]) {
+            const int lt = levels_for(lim[t], j);
+            L = lt > L ? lt : L;
+          }
+        const uint32_t kdst = sb + OFF_K + ks * KSTAGE_BYTES;
+        if (a.layout == ATF_LAYOUT_SORTED_PAIR) {
+          // one 5-d box: the L in-window levels (dims 0..16L-1), one 4 KB slab each
+          mbar_arrive_expect_tx_elect(bar(B_KFULL + ks), static_cast<uint32_t>(L) * KSLAB_BYTES);
+          if (elect_one_lane()) tma_load_5d(kdst, &tmKL.lv[L - 1], bar(B_KFULL + ks), 0, k_tok + j * BN, 0, hk, 0);
+          __syncwarp();
+        } else {
+          // rotate_half: a level is two 8-dim chunks 64 dims apart, one box each
+          mbar_arrive_expect_tx_elect(bar(B_KFULL + ks), static_cast<uint32_t>(L) * KSLAB_BYTES);
+          for (int i = 0; i < L; ++i) {
+            tma_load_4d_elect(kdst + i * KSLAB_BYTES, &tmK, bar(B_KFULL + ks), level_col(a.layout, i, 0),
+                              k_tok + j * BN, hk, 0);
+            tma_load_4d_elect(kdst + i * KSLAB_BYTES + KHALF_BYTES, &tmK, bar(B_KFULL + ks),
+                              level_col(a.layout, i, 1), k_tok + j * BN, hk, 0);
+          }
+        }
+        issued_k = j + 1;
+        ok = __all_sync(FULL, mbar_wait_inl(bar(B_VEMPTY + vs), ((j / VST) & 1) ^ 1, ab, kDevErrTimeout));
+        if (!ok) break;
+        mbar_arrive_expect_tx_elect(bar(B_VFULL + vs), VSTAGE_BYTES);
+        tma_load_4d_elect(sb + OFF_V + vs * VSTAGE_BYTES, &tmV, bar(B_VFULL + vs), 0, k_tok + j * BN, hk, 0);
+        tma_load_4d_elect(sb + OFF_V + vs * VSTAGE_BYTES + VBOX_BYTES, &tmV, bar(B_VFULL + vs), 64,
+                          k_tok + j * BN, hk, 0);
+        issued_v = j + 1;
+      }
+      // Drain: every copy this warp issued must land before shared memory is
+      // released (no-op on the normal path, where the MMA warp consumed them).
+      drain_wait(bar(B_Q), 0);
+      for (int j = issued_k - KST; j < issued_k; ++j)
+        if (j >= 0) drain_wait(bar(B_KFULL + j % KST), (j / KST) & 1);
+      for (int j = issued_v - VST; j < issued_v; ++j)
+        if (j >= 0) drain_wait(bar(B_VFULL + j % VST), (j / VST) & 1);
       __syncwarp();
     } else if (start_ok && warp == WARP_MMA) {
       // ---------------------------------------------------------------- MMA issuer
+      // Descriptors are built once and advanced by adding (byte offset >> 4) to
+      // the start-address field (all offsets stay inside the 14-bit field).
       const uint32_t tm = __shfl_sync(FULL, tmem, 0);
+      const uint64_t qdesc0 = make_sdesc(sb + OFF_Q, QHALF_BYTES, 128, kLayoutNone);
       const uint64_t qrows0 = make_sdesc(sb + OFF_Q, 16, 1024, kLayoutSw128);
-      const uint64_t qslab0 = make_sdesc(sb + OFF_Q, QHALF_BYTES, 128, kLayoutNone);
-      const uint64_t kslab0 = make_sdesc(sb + OFF_K, KHALF_BYTES, 128, kLayoutNone);
-      const uint64_t kswz0 = make_sdesc(sb + OFF_K, 16, 256, kLayoutSw32);
+      const uint64_t kdesc0 = make_sdesc(sb + OFF_K, KHALF_BYTES, 128, kLayoutNone);
+      // sorted-pair K level slabs: 128 keys x 32 B, 32-byte swizzle (SBO = 8 rows)
+      const uint64_t kdesc32 = make_sdesc(sb + OFF_K, 16, 256, kLayoutSw32);
+      const bool sorted = a.layout == ATF_LAYOUT_SORTED_PAIR;
       const uint64_t vdesc0 = make_sdesc(sb + OFF_V, VBOX_BYTES, 1024, kLayoutSw128);
-      int kb = 0, vb = 0, qc = 0;               // stages and Q loads of the units before
-      int sc0 = 0, sc1 = 0, oc0 = 0, oc1 = 0;   // S of each tile, and its units, before
-      bool ok = true;
-      Walk walk(a);
-      int u = walk.next(a);
-      Item it = u >= 0 ? load_item(a, u) : Item{};
-      while (ok && u >= 0) {
-        const Unit x = make_unit(a, u, it);
-        u = walk.next(a);
-        if (u >= 0) it = load_item(a, u);
-        const int nk0 = x.nk[0], nk1 = x.nk[1], nk_max = x.nk_max();
-        if (nk_max == 0) continue;
-        int lim[NQ][ATF_MAX_LEVELS];
-#pragma unroll
-        for (int t = 0; t < NQ; ++t) window_limits(a, x.q_offset, x.row0 + t * BM, lim[t]);
-        int s_left = nk0 + nk1;
-        // S_t(j) into tile t's S columns; after the unit's last one Q is free
-        auto issue_S = [&](int t, int j) {
-          const int L = levels_for(lim[t], j);
-          const uint32_t d_tmem = tm + static_cast<uint32_t>(t * 128);
-          const uint64_t kd = (sorted ? kswz0 : kslab0) + ((((kb + j) % KST) * KSTAGE_BYTES) >> 4);
-          if (sorted)
-            qk_group_rows_asm(d_tmem, qrows0 + ((t * QTILE_BYTES) >> 4), kd, IDESC_QK, L, bar(B_SFULL + t));
-          else
-            qk_group_asm(d_tmem, qslab0 + ((t * QTILE_BYTES) >> 4), kd, IDESC_QK, L, bar(B_SFULL + t));
-          if (--s_left == 0) tc_commit_elect(bar(B_QEMPTY));
-        };
-        // O_t += P_t(j) V_j; P_t sits in columns 64..127 of the other tile's S
-        auto issue_PV = [&](int t, int j) {
-          const uint32_t o_tmem = tm + 256u + static_cast<uint32_t>(t * 128);
-          const uint32_t p_tmem = tm + static_cast<uint32_t>((1 - t) * 128 + 64);
-          const uint64_t vd = vdesc0 + ((((vb + j) % VST) * VSTAGE_BYTES) >> 4);
-          pv_group_asm(o_tmem, p_tmem, vd, IDESC_PV, j > 0 ? 1u : 0u, bar(B_ODONE + t));
-        };
-        auto wait = [&](int b, int phase) -> bool {
-          const bool w = __all_sync(FULL, mbar_wait_inl(bar(b), static_cast<uint32_t>(phase) & 1u, ab, kDevErrTimeout));
+      const int nk0 = nk[0], nk1 = nk[1];
+      // S_t(j) into tile t's S columns
+      auto issue_S = [&](int t, int j) {
+        const int L = levels_for(lim[t], j);
+        const uint32_t d_tmem = tm + static_cast<uint32_t>(t * 128);
+        const uint64_t qd = qdesc0 + ((t * QTILE_BYTES) >> 4);
+        const uint64_t kd = (sorted ? kdesc32 : kdesc0) + (((j % KST) * KSTAGE_BYTES) >> 4);
+        if (sorted)
+          qk_group_rows_asm(d_tmem, qrows0 + ((t * QTILE_BYTES) >> 4), kd, IDESC_QK, L, bar(B_SFULL + t));
+        else
+          qk_group_asm(d_tmem, qd, kd, IDESC_QK, L, bar(B_SFULL + t));
+      };
+      // O_t += P_t(j) V_j; P_t sits in columns 64..127 of the other tile's S
+      auto issue_PV = [&](int t, int j) {
+        const uint32_t o_tmem = tm + 256u + static_cast<uint32_t>(t * 128);
+        const uint32_t p_tmem = tm + static_cast<uint32_t>((1 - t) * 128 + 64);
+        const uint64_t vd = vdesc0 + (((j % VST) * VSTAGE_BYTES) >> 4);
+        pv_group_asm(o_tmem, p_tmem, vd, IDESC_PV, j > 0 ? 1u : 0u, bar(B_ODONE + t));
+      };
+      // K tiles are waited for in order, once each
+      int k_waited = -1;
+      auto kwait = [&](int j) -> bool {
+        while (k_waited < j) {
+          ++k_waited;
+          if (!__all_sync(FULL, mbar_wait_inl(bar(B_KFULL + k_waited % KST), (k_waited / KST) & 1, ab,
+                                          kDevErrTimeout)))
+            return false;
           tc_fence_after();
-          return w;
-        };
-        int k_waited = -1;  // K tiles are waited for in order, once each
-        auto kwait = [&](int j) -> bool {
-          while (k_waited < j) {
-            ++k_waited;
-            if (!wait(B_KFULL + (kb + k_waited) % KST, (kb + k_waited) / KST)) return false;
-          }
-          return true;
-        };
-        // A K stage is released after the last S that reads it: S_1(j) when tile 1
-        // has key tile j, else S_0(j).
-        ok = wait(B_QFULL, qc) && kwait(0);
-        if (ok) {
-          if (nk0 > 0) issue_S(0, 0);
-          if (nk1 > 0) issue_S(1, 0);
-          tc_commit_elect(bar(B_KEMPTY + kb % KST));
         }
-        // S_0(1) once tile 0 has read S_0(0)
-        if (ok && nk0 > 1 && (ok = kwait(1) && wait(B_LOADED + 0, sc0))) {
-          issue_S(0, 1);
-          if (1 >= nk1) tc_commit_elect(bar(B_KEMPTY + (kb + 1) % KST));
-        }
-        for (int j = 0; ok && j < nk_max; ++j) {
-          const int vs = (vb + j) % VST;
-          if (!(ok = wait(B_VFULL + vs, (vb + j) / VST))) break;
+        return true;
+      };
+      auto wait_loaded = [&](int t, int j) -> bool {
+        const bool w = __all_sync(FULL, mbar_wait_inl(bar(B_LOADED + t), j & 1, ab, kDevErrTimeout));
+        tc_fence_after();
+        return w;
+      };
+      // A K stage is released after the last S that reads it: S_1(j) when tile 1
+      // has key tile j, else S_0(j).
+      bool ok = __all_sync(FULL, mbar_wait_inl(bar(B_Q), 0, ab, kDevErrTimeout));
+      tc_fence_after();
+      if (ok && nk_max > 0 && (ok = kwait(0))) {
+        if (nk0 > 0) issue_S(0, 0);
+        if (nk1 > 0) issue_S(1, 0);
+        tc_commit_elect(bar(B_KEMPTY + 0));
+      }
+      // S_0(1) once tile 0 has read S_0(0)
+      if (ok && nk0 > 1 && (ok = kwait(1) && wait_loaded(0, 0))) {
+        issue_S(0, 1);
+        if (1 >= nk1) tc_commit_elect(bar(B_KEMPTY + 1 % KST));
+      }
+      for (int j = 0; ok && j < nk_max; ++j) {
+        const int vs = j % VST;
+        ok = __all_sync(FULL, mbar_wait_inl(bar(B_VFULL + vs), (j / VST) & 1, ab, kDevErrTimeout));
+        if (!ok) break;
+        {
           // V rows past the sequence's last key: another sequence's
-          const int live = x.sk - j * BN;
+          const int live = sk - j * BN;
           if (live < BN) {
             uint8_t* v0 = sp + OFF_V + vs * VSTAGE_BYTES;
             for (int e = live * 8 + lane; e < BN * 8; e += 32) {
@@ -396,41 +374,38 @@ __global__ void __launch_bounds__(THREADS, 1)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
           }
-          if (j < nk0) {
-            // (the first one overwrites O_0: the unit before it has been read)
-            if (!(ok = (j > 0 || wait(B_OFREE + 0, oc0 + 1)) && wait(B_PFULL + 0, sc0 + j))) break;
-            issue_PV(0, j);
-            if (j + 1 == nk0) tc_commit_elect(bar(B_OFINAL + 0));
-          }
-          // S_1(j+1) overwrites the columns P_0(j) occupies (O_0 += P_0(j) V_j was
-          // issued first; tcgen05.mma ops of one thread run in order) and needs
-          // tile 1 to have read S_1(j)
-          if (j + 1 < nk1) {
-            if (!(ok = kwait(j + 1) && wait(B_LOADED + 1, sc1 + j))) break;
-            issue_S(1, j + 1);
-            tc_commit_elect(bar(B_KEMPTY + (kb + j + 1) % KST));
-          }
-          if (j < nk1) {
-            if (!(ok = (j > 0 || wait(B_OFREE + 1, oc1 + 1)) && wait(B_PFULL + 1, sc1 + j))) break;
-            issue_PV(1, j);
-            if (j + 1 == nk1) tc_commit_elect(bar(B_OFINAL + 1));
-          }
-          // S_0(j+2): after O_1 += P_1(j) V_j (P_1(j) sits in S_0's columns) and
-          // tile 0's read of S_0(j+1)
-          if (j + 2 < nk0) {
-            if (!(ok = kwait(j + 2) && wait(B_LOADED + 0, sc0 + j + 1))) break;
-            issue_S(0, j + 2);
-            if (j + 2 >= nk1) tc_commit_elect(bar(B_KEMPTY + (kb + j + 2) % KST));
-          }
-          tc_commit_elect(bar(B_VEMPTY + vs));
         }
-        kb += nk_max;
-        vb += nk_max;
-        ++qc;
-        sc0 += nk0;
-        sc1 += nk1;
-        oc0 += nk0 > 0 ? 1 : 0;
-        oc1 += nk1 > 0 ? 1 : 0;
+        tc_fence_after();
+        if (j < nk0) {
+          ok = __all_sync(FULL, mbar_wait_inl(bar(B_PFULL + 0), j & 1, ab, kDevErrTimeout));
+          if (!ok) break;
+          tc_fence_after();
+          issue_PV(0, j);
+          if (j + 1 == nk0) tc_commit_elect(bar(B_OFINAL + 0));
+        }
+        // S_1(j+1) overwrites the columns P_0(j) occupies (O_0 += P_0(j) V_j was
+        // issued first; tcgen05.mma ops of one thread run in order) and needs
+        // tile 1 to have read S_1(j)
+        if (j + 1 < nk1) {
+          if (!(ok = kwait(j + 1) && wait_loaded(1, j))) break;
+          issue_S(1, j + 1);
+          tc_commit_elect(bar(B_KEMPTY + (j + 1) % KST));
+        }
+        if (j < nk1) {
+          ok = __all_sync(FULL, mbar_wait_inl(bar(B_PFULL + 1), j & 1, ab, kDevErrTimeout));
+          if (!ok) break;
+          tc_fence_after();
+          issue_PV(1, j);
+          if (j + 1 == nk1) tc_commit_elect(bar(B_OFINAL + 1));
+        }
+        // S_0(j+2): after O_1 += P_1(j) V_j (P_1(j) sits in S_0's columns) and
+        // tile 0's read of S_0(j+1)
+        if (j + 2 < nk0) {
+          if (!(ok = kwait(j + 2) && wait_loaded(0, j + 1))) break;
+          issue_S(0, j + 2);
+          if (j + 2 >= nk1) tc_commit_elect(bar(B_KEMPTY + (j + 2) % KST));
+        }
+        tc_commit_elect(bar(B_VEMPTY + vs));
       }
       // Every MMA issued by this CTA completes before TMEM is released.
       tc_commit_elect(bar(B_FINAL));
@@ -441,45 +416,26 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else {
     reg_alloc<REG_SOFTMAX>();
     if (start_ok) {
-      // ---------------------------------------------------------------- softmax
-      const int t = warp >> 2;
-      const int wq = warp & 3;
-      const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
-      const uint32_t tS = tmem + static_cast<uint32_t>(t * 128) + lane_off;
-      const uint32_t tP = tmem + static_cast<uint32_t>((1 - t) * 128 + 64) + lane_off;
-      const uint32_t tO = tmem + 256u + static_cast<uint32_t>(t * 128) + lane_off;
-      uint8_t* s_out = sp + OFF_OUT + warp * OUT_BYTES;
-      const float sl2 = a.scale_log2;
-      int mine = 0, other = 0, units = 0;  // S of this and of the other tile, and this tile's units, before
-      bool ok = true;
-      Walk walk(a);
-      int u = walk.next(a);
-      Item it = u >= 0 ? load_item(a, u) : Item{};
-      while (ok && u >= 0) {
-        const Unit x = make_unit(a, u, it);
-        u = walk.next(a);
-        if (u >= 0) it = load_item(a, u);
-        const int my_nk = t ? x.nk[1] : x.nk[0], other_nk = t ? x.nk[0] : x.nk[1];
-        const int row_w = x.row0 + t * BM + wq * 32;  // the warp's first row
+        // ---------------------------------------------------------------- softmax
+        const int t = warp >> 2;
+        const int wq = warp & 3;
+        const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+        const uint32_t tS = tmem + static_cast<uint32_t>(t * 128) + lane_off;
+        const uint32_t tP = tmem + static_cast<uint32_t>((1 - t) * 128 + 64) + lane_off;
+        const uint32_t tO = tmem + 256u + static_cast<uint32_t>(t * 128) + lane_off;
+        const int my_row0 = t ? row0[1] : row0[0];
+        const int my_nk = t ? nk[1] : nk[0];
+        const int row_w = my_row0 + wq * 32;  // the warp's first row
         const int qrow = row_w + lane;
-        if (my_nk == 0) {  // rows without keys (none, where the tile lies past the sequence)
-          if (qrow < x.row_end) {
-            uint4* dst = reinterpret_cast<uint4*>(a.out + static_cast<long long>(x.q_tok + qrow) * a.o_ss +
-                                                  static_cast<long long>(x.h) * a.o_sh);
-#pragma unroll
-            for (int e = 0; e < HD / 8; ++e) dst[e] = make_uint4(0, 0, 0, 0);
-            if (a.lse != nullptr) a.lse[static_cast<long long>(x.q_tok + qrow) * a.Hq + x.h] = -INFINITY;
-          }
-          other += other_nk;
-          continue;
-        }
-        // this row sees the keys before `seen`
-        const int seen = a.causal ? min(x.sk, x.q_offset + qrow + 1) : x.sk;
-        // first key tile with a key that a row of the tile does not see
-        const int j_mask = max(0, min(x.sk, a.causal ? x.q_offset + x.row0 + t * BM + 1 : x.sk)) / BN;
+        // this row sees the keys before `seen`; from key tile j_mask on, a row of the
+        // tile does not see every key
+        const int seen = a.causal ? min(sk, q_offset + qrow + 1) : sk;
+        const int j_mask = max(0, a.causal ? min(sk, q_offset + my_row0 + 1) : sk) / BN;
+        const float sl2 = a.scale_log2;
         float m2 = -INFINITY, l = 0.f;
+        bool ok = true;
         for (int j = 0; j < my_nk; ++j) {
-          ok = __all_sync(FULL, mbar_wait_inl(bar(B_SFULL + t), (mine + j) & 1, ab, kDevErrTimeout));
+          ok = __all_sync(FULL, mbar_wait_inl(bar(B_SFULL + t), j & 1, ab, kDevErrTimeout));
           if (!ok) break;
           tc_fence_after();
           float s[BN];
@@ -511,8 +467,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           mx0 = fmax3(mx0, s[BN - 4], s[BN - 3]);
           mx1 = fmax3(mx1, s[BN - 2], s[BN - 1]);
           const float mnew = fmaxf(m2, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sl2);
-          // Lazy rescale, as in the dense kernel: the running max only moves when it
-          // grows by more than 8 (log2 units).
+          // Lazy rescale: the running max only moves when it grows by more than
+          // 8 (log2 units), so P <= 2^8 stays exact enough in bf16 and O is
+          // rescaled rarely. The O update itself happens after P is stored.
           float alpha = 1.0f;
           bool need = false;
           if (j == 0) {
@@ -526,13 +483,15 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
           const float msub = (m2 == -INFINITY) ? 0.f : m2;
+          // exponentials, the row sum and the bf16 packing of P, two columns at a
+          // time with packed f32x2 arithmetic (half the FMA / add instructions)
           uint32_t pk[BN / 2];
           float2 ls0 = make_float2(0.f, 0.f), ls1 = make_float2(0.f, 0.f);
           const float2 sl2x2 = make_float2(sl2, sl2), negm = make_float2(-msub, -msub);
 #pragma unroll
           for (int c = 0; c < BN / 2; ++c) {
-            const float2 y = __ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sl2x2, negm);
-            const float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+            const float2 x = __ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sl2x2, negm);
+            const float2 p = make_float2(ex2_approx(x.x), ex2_approx(x.y));
             if (c & 1) ls1 = __fadd2_rn(ls1, p); else ls0 = __fadd2_rn(ls0, p);
             pk[c] = pack_bf16x2(p.x, p.y);
           }
@@ -546,14 +505,14 @@ __global__ void __launch_bounds__(THREADS, 1)
           // columns). Past the other tile's last key tile, wait for its last read
           // and for this tile's previous O += P V instead.
           {
-            const int want = j + t;
+            const int other_nk = t ? nk[0] : nk[1];
+            const int want = j + t;  // tile 0: S_1(j); tile 1: S_0(j + 1)
             bool w = true;
             if (want < other_nk) {
-              w = mbar_wait_inl(bar(B_LOADED + (t ^ 1)), (other + want) & 1, ab, kDevErrTimeout);
+              w = mbar_wait_inl(bar(B_LOADED + (t ^ 1)), want & 1, ab, kDevErrTimeout);
             } else {
-              if (other_nk > 0)
-                w = mbar_wait_inl(bar(B_LOADED + (t ^ 1)), (other + other_nk - 1) & 1, ab, kDevErrTimeout);
-              if (w && j > 0) w = mbar_wait_inl(bar(B_ODONE + t), (mine + j - 1) & 1, ab, kDevErrTimeout);
+              if (other_nk > 0) w = mbar_wait_inl(bar(B_LOADED + (t ^ 1)), (other_nk - 1) & 1, ab, kDevErrTimeout);
+              if (w && j > 0) w = mbar_wait_inl(bar(B_ODONE + t), (j - 1) & 1, ab, kDevErrTimeout);
             }
             ok = __all_sync(FULL, w);
             if (!ok) break;
@@ -561,9 +520,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           tmem_st64(tP, pk);
           if (__any_sync(FULL, need)) {
-            // O holds the sum up to tile j-1 once O += P(j-1) V has completed; the next
-            // one is not issued before this warpgroup arrives on PFULL below
-            ok = __all_sync(FULL, mbar_wait_inl(bar(B_ODONE + t), (mine + j - 1) & 1, ab, kDevErrTimeout));
+            // O holds the sum up to tile j-1 once PV(t, j-1) has completed (S_t(j) was
+            // issued after it, so at most that one is in flight); PV(t, j) is not
+            // issued before this warpgroup arrives on PFULL below.
+            ok = __all_sync(FULL, mbar_wait_inl(bar(B_ODONE + t), (j - 1) & 1, ab, kDevErrTimeout));
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -578,53 +538,56 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_fence_before();
           mbar_arrive(bar(B_PFULL + t));
         }
-        if (!ok) break;
-        ok = __all_sync(FULL, mbar_wait_inl(bar(B_OFINAL + t), units & 1, ab, kDevErrTimeout));
-        if (!ok) break;
-        tc_fence_after();
-        const float inv = l > 0.f ? 1.0f / l : 0.f;
-        const bool keyless = seen <= 0;  // 0, whatever V holds
-        const int nrows = min(32, x.row_end - row_w);  // rows of this warp to store
-        __nv_bfloat16* orow = a.out + static_cast<long long>(x.q_tok + row_w) * a.o_ss +
-                              static_cast<long long>(x.h) * a.o_sh;
+        if (ok && my_nk > 0) {
+          ok = __all_sync(FULL, mbar_wait_inl(bar(B_OFINAL + t), 0, ab, kDevErrTimeout));
+          if (ok) {
+            tc_fence_after();
+            const float inv = l > 0.f ? 1.0f / l : 0.f;
+            const bool keyless = seen <= 0;             // 0, whatever V holds
+            const int nrows = min(32, row_end - row_w);  // rows of this warp to store
+            // Through the tile's own Q in shared memory (its last product has read it):
+            // rows of 128 bytes, 16-byte chunks XORed with the row, then eight lanes per
+            // row, so that whole 128-byte lines leave.
+            uint8_t* s_out = sp + OFF_Q + t * QTILE_BYTES + wq * (32 * 128);
+            __nv_bfloat16* orow = a.out + static_cast<long long>(q_tok + row_w) * a.o_ss +
+                                  static_cast<long long>(h) * a.o_sh;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {  // 64 dims
+            for (int half = 0; half < 2; ++half) {  // 64 dims
 #pragma unroll
-          for (int c4 = 0; c4 < 2; ++c4) {
-            uint32_t rr[32];
-            tmem_ld32(tO + static_cast<uint32_t>(64 * half + 32 * c4), rr);
-            if (half == 1 && c4 == 1) {  // O_t has been read
-              tc_fence_before();
-              mbar_arrive(bar(B_OFREE + t));
+              for (int c4 = 0; c4 < 2; ++c4) {
+                uint32_t rr[32];
+                tmem_ld32(tO + static_cast<uint32_t>(64 * half + 32 * c4), rr);
+                uint32_t pk[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  pk[e] = keyless ? 0u
+                                  : pack_bf16x2(__uint_as_float(rr[2 * e]) * inv, __uint_as_float(rr[2 * e + 1]) * inv);
+#pragma unroll
+                for (int v4 = 0; v4 < 4; ++v4)
+                  *reinterpret_cast<uint4*>(s_out + lane * 128 + 16 * ((4 * c4 + v4) ^ (lane & 7))) =
+                      make_uint4(pk[4 * v4], pk[4 * v4 + 1], pk[4 * v4 + 2], pk[4 * v4 + 3]);
+              }
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + (lane >> 3), c = lane & 7;
+                const uint4 v = *reinterpret_cast<const uint4*>(s_out + r * 128 + 16 * (c ^ (r & 7)));
+                if (r < nrows)
+                  *reinterpret_cast<uint4*>(orow + static_cast<long long>(r) * a.o_ss + 64 * half + 8 * c) = v;
+              }
+              __syncwarp();
             }
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              pk[e] = keyless ? 0u
-                              : pack_bf16x2(__uint_as_float(rr[2 * e]) * inv, __uint_as_float(rr[2 * e + 1]) * inv);
-            // rows of 128 bytes, 16-byte chunks XORed with the row
-#pragma unroll
-            for (int v4 = 0; v4 < 4; ++v4)
-              *reinterpret_cast<uint4*>(s_out + lane * 128 + 16 * ((4 * c4 + v4) ^ (lane & 7))) =
-                  make_uint4(pk[4 * v4], pk[4 * v4 + 1], pk[4 * v4 + 2], pk[4 * v4 + 3]);
+            if (a.lse != nullptr && qrow < row_end)
+              a.lse[static_cast<long long>(q_tok + qrow) * a.Hq + h] = (m2 + log2f(l)) * 0.69314718055994531f;
           }
-          __syncwarp();
-          // eight lanes per row: 128 bytes in one line
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int r = 4 * k + (lane >> 3), c = lane & 7;
-            const uint4 v = *reinterpret_cast<const uint4*>(s_out + r * 128 + 16 * (c ^ (r & 7)));
-            if (r < nrows)
-              *reinterpret_cast<uint4*>(orow + static_cast<long long>(r) * a.o_ss + 64 * half + 8 * c) = v;
-          }
-          __syncwarp();
         }
-        if (a.lse != nullptr && qrow < x.row_end)
-          a.lse[static_cast<long long>(x.q_tok + qrow) * a.Hq + x.h] = (m2 + log2f(l)) * 0.69314718055994531f;
-        mine += my_nk;
-        other += other_nk;
-        ++units;
-      }
+        if (my_nk == 0 && qrow < row_end) {  // a tile whose rows have no keys
+          uint4* dst = reinterpret_cast<uint4*>(a.out + static_cast<long long>(q_tok + qrow) * a.o_ss +
+                                                static_cast<long long>(h) * a.o_sh);
+#pragma unroll
+          for (int e = 0; e < HD / 8; ++e) dst[e] = make_uint4(0, 0, 0, 0);
+          if (a.lse != nullptr) a.lse[static_cast<long long>(q_tok + qrow) * a.Hq + h] = -INFINITY;
+        }
     }
   }
 
@@ -640,12 +603,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 using namespace atf;
 
-extern "C" int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int32_t* plan_host, int64_t capacity,
-                                       AtfPrefillRaggedPlan* out) {
+extern "C" int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int32_t* items_host,
+                                       int32_t items_capacity, int32_t* num_items) {
   using namespace atf::ragged;
-  if (p == nullptr || out == nullptr || p->qo_indptr_host == nullptr || p->kv_indptr_host == nullptr ||
-      p->batch_size < 1 || (plan_host == nullptr && capacity > 0) || p->num_heads_q < 1 || p->num_heads_kv < 1 ||
-      p->num_heads_q % p->num_heads_kv != 0 || p->num_sms < 0)
+  if (p == nullptr || num_items == nullptr || p->qo_indptr_host == nullptr || p->kv_indptr_host == nullptr ||
+      p->batch_size < 1 || (items_host == nullptr && items_capacity > 0))
     return ATF_ERR_INVALID_ARG;
   long long n = 0;
   for (int b = 0; b < p->batch_size; ++b) {
@@ -655,24 +617,13 @@ extern "C" int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int3
     if (nq > (1ll << 30) || nk > (1ll << 30)) return ATF_ERR_UNSUPPORTED;
     n += (nq + BM * NQ - 1) / (BM * NQ);
   }
-  const long long units = n * p->num_heads_q;
-  if (units > 0x3fffffffLL) return ATF_ERR_UNSUPPORTED;
-  int sms = p->num_sms;
-  if (sms == 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-      return ATF_ERR_CUDA;
-  }
-  const int ctas = static_cast<int>(units < sms ? units : sms);
-  out->num_items = static_cast<int32_t>(n);
-  out->num_ctas = ctas;
-  out->plan_ints = 8 * n + ctas + 1 + units;
-  if (plan_host == nullptr) return ATF_OK;
-  if (capacity < out->plan_ints) return ATF_ERR_WORKSPACE;
+  if (n > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
+  *num_items = static_cast<int32_t>(n);
+  if (items_host == nullptr) return ATF_OK;
+  if (n > items_capacity) return ATF_ERR_WORKSPACE;
   struct Planned {
+    long long tiles;
     Item it;
-    int steps[NQ];  // key tiles of each query tile
   };
   std::vector<Planned> all;
   all.reserve(static_cast<size_t>(n));
@@ -684,69 +635,32 @@ extern "C" int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int3
     x.it.k_len = p->kv_indptr_host[b + 1] - p->kv_indptr_host[b];
     for (int row = 0; row < x.it.q_len; row += BM * NQ) {
       x.it.row = row;
-      for (int t = 0; t < NQ; ++t) {
-        long long kend = p->causal ? static_cast<long long>(x.it.k_len) - x.it.q_len + row + (t + 1) * BM : x.it.k_len;
-        if (kend > x.it.k_len) kend = x.it.k_len;
-        x.steps[t] = row + t * BM < x.it.q_len && kend > 0 ? static_cast<int>((kend + BN - 1) / BN) : 0;
-      }
+      long long kend = p->causal ? static_cast<long long>(x.it.k_len) - x.it.q_len + row + BM * NQ : x.it.k_len;
+      kend = kend > x.it.k_len ? x.it.k_len : (kend < 0 ? 0 : kend);
+      x.tiles = (kend + BN - 1) / BN;
       all.push_back(x);
     }
   }
-  auto longest = [](const Planned& x) { return x.steps[0] > x.steps[1] ? x.steps[0] : x.steps[1]; };
-  std::stable_sort(all.begin(), all.end(),
-                   [&](const Planned& x, const Planned& y) { return longest(x) > longest(y); });
-  for (size_t i = 0; i < all.size(); ++i) std::memcpy(plan_host + 8 * i, &all[i].it, sizeof(Item));
-  int32_t* offsets = plan_host + 8 * n;
-  int32_t* list = offsets + ctas + 1;
-  if (ctas == 0) {
-    offsets[0] = 0;
-    return ATF_OK;
-  }
-  // Each unit, in order, to the CTA with the least work so far (ties: the lowest),
-  // in hundredths of a step of both tiles.
-  const int G = p->num_heads_q / p->num_heads_kv;
-  std::vector<int32_t> owner(static_cast<size_t>(units));
-  std::vector<long long> count(static_cast<size_t>(ctas), 0);
-  using Load = std::pair<long long, int>;
-  std::vector<Load> heap;
-  for (int c = 0; c < ctas; ++c) heap.emplace_back(0, c);
-  const auto more = std::greater<Load>();
-  std::make_heap(heap.begin(), heap.end(), more);
-  size_t u = 0;
-  for (int hk = 0; hk < p->num_heads_kv; ++hk)
-    for (const Planned& x : all) {
-      const int both = x.steps[0] < x.steps[1] ? x.steps[0] : x.steps[1];
-      const long long cost = 100ll * both + 90ll * (longest(x) - both) + 180;
-      for (int g = 0; g < G; ++g, ++u) {
-        std::pop_heap(heap.begin(), heap.end(), more);
-        heap.back().first += cost;
-        owner[u] = heap.back().second;
-        ++count[static_cast<size_t>(owner[u])];
-        std::push_heap(heap.begin(), heap.end(), more);
-      }
-    }
-  offsets[0] = 0;
-  for (int c = 0; c < ctas; ++c) offsets[c + 1] = offsets[c] + static_cast<int32_t>(count[static_cast<size_t>(c)]);
-  std::vector<int32_t> next(offsets, offsets + ctas);
-  for (size_t i = 0; i < owner.size(); ++i) list[next[static_cast<size_t>(owner[i])]++] = static_cast<int32_t>(i);
+  std::stable_sort(all.begin(), all.end(), [](const Planned& x, const Planned& y) { return x.tiles > y.tiles; });
+  for (size_t i = 0; i < all.size(); ++i) std::memcpy(items_host + 8 * i, &all[i].it, sizeof(Item));
   return ATF_OK;
 }
 
 extern "C" int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_stream_t stream) {
   using namespace atf::ragged;
   if (p == nullptr || p->q == nullptr || p->k == nullptr || p->v == nullptr || p->out == nullptr ||
-      p->plan == nullptr)
+      p->items == nullptr)
     return ATF_ERR_INVALID_ARG;
   if (p->head_dim != ATF_HEAD_DIM) return ATF_ERR_UNSUPPORTED;
   if (p->total_q < 1 || p->total_k < 1 || p->num_heads_q < 1 || p->num_heads_kv < 1 ||
-      p->num_heads_q % p->num_heads_kv != 0 || p->num_items < 0 || p->num_ctas < 0)
+      p->num_heads_q % p->num_heads_kv != 0 || p->num_items < 0)
     return ATF_ERR_INVALID_ARG;
   if (p->total_q > 0x7fffffffLL - BM * NQ || p->total_k > 0x7fffffffLL - BN || p->num_heads_q > (1 << 20))
     return ATF_ERR_UNSUPPORTED;
   if (p->qk_layout != ATF_LAYOUT_SORTED_PAIR && p->qk_layout != ATF_LAYOUT_ROTATE_HALF) return ATF_ERR_INVALID_ARG;
   if (p->window != ATF_WINDOW_OFF && p->window != ATF_WINDOW_SNAP16) return ATF_ERR_UNSUPPORTED;
   if (!(p->softmax_scale > 0.f)) return ATF_ERR_INVALID_ARG;
-  if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->out) || !aligned16(p->plan))
+  if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->out) || !aligned16(p->items))
     return ATF_ERR_ALIGNMENT;
   const int64_t strides[8] = {p->q_stride_s, p->q_stride_h, p->k_stride_s, p->k_stride_h,
                               p->v_stride_s, p->v_stride_h, p->o_stride_s, p->o_stride_h};
@@ -758,7 +672,7 @@ extern "C" int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_strea
   int dev = 0;
   int rc = check_device(&dev);
   if (rc != ATF_OK) return rc;
-  if (p->num_items == 0 || p->num_ctas == 0) return ATF_OK;
+  if (p->num_items == 0) return ATF_OK;
 
   // one batch of all packed rows; only the K maps that the call reads are encoded
   CUtensorMap tq, tk, tv;
@@ -811,15 +725,12 @@ extern "C" int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_strea
   a.o_sh = p->o_stride_h;
   a.lse = p->lse;
   a.err = p->error_flag;
-  const long long units = static_cast<long long>(p->num_items) * a.Hq;
-  if (units > 0x3fffffffLL) return ATF_ERR_UNSUPPORTED;
-  a.items = p->plan;
-  a.cta_units = p->plan + 8ll * p->num_items;
-  a.units = a.cta_units + p->num_ctas + 1;
+  a.items = p->items;
   a.n_items = p->num_items;
-  a.n_units = static_cast<int>(units);
   a.total_q = p->total_q;
   a.total_k = p->total_k;
+  const long long units = static_cast<long long>(p->num_items) * a.Hq;
+  if (units > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
   if (cudaFuncSetAttribute(ragged_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(SMEM_BYTES)) != cudaSuccess)
     return ATF_ERR_CUDA;
@@ -830,7 +741,7 @@ extern "C" int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_strea
     return cudaFuncGetAttributes(&fa, ragged_kernel) == cudaSuccess ? fa.numRegs : 0;
   }();
   if (static_cast<long long>(launch_regs) * THREADS < REG_SPLIT_TOTAL) return ATF_ERR_UNSUPPORTED;
-  ragged_kernel<<<static_cast<unsigned>(p->num_ctas), THREADS, SMEM_BYTES, reinterpret_cast<cudaStream_t>(stream)>>>(
+  ragged_kernel<<<static_cast<unsigned>(units), THREADS, SMEM_BYTES, reinterpret_cast<cudaStream_t>(stream)>>>(
       tq, tk, tkl, tv, a);
   return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
 }

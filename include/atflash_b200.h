@@ -149,22 +149,13 @@ typedef struct {
   int32_t batch_size;
   const int32_t* qo_indptr_host; /* [batch+1] (host) */
   const int32_t* kv_indptr_host; /* [batch+1] (host) */
-  int32_t num_heads_q, num_heads_kv;
-  int32_t num_sms; /* 0: query the current device */
   int causal;
 } AtfPrefillRaggedPlanParams;
 
-typedef struct {
-  int32_t num_items; /* blocks of 256 query rows */
-  int32_t num_ctas;
-  int64_t plan_ints; /* int32 that the plan takes */
-} AtfPrefillRaggedPlan;
-
-/* The schedule of a packed batch, built on the host: the items (8 int32 each, the
- * ones with the most key tiles first), num_ctas + 1 offsets and the units (item x
- * query head) of each CTA, dealt out to equal work. plan_host NULL: sizes only. */
-int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int32_t* plan_host, int64_t capacity,
-                            AtfPrefillRaggedPlan* out);
+/* The work items of a packed batch: 8 int32 each, blocks of 256 query rows, the
+ * ones with the most key tiles first. items_host NULL: only *num_items is set. */
+int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int32_t* items_host,
+                            int32_t items_capacity, int32_t* num_items);
 
 typedef struct {
   const void* q; /* bf16 [total_q, Hq, 128] */
@@ -174,8 +165,8 @@ typedef struct {
   float* lse;    /* optional fp32 [total_q, Hq], natural log */
   int64_t total_q, total_k, num_heads_q, num_heads_kv, head_dim;
   int64_t q_stride_s, q_stride_h, k_stride_s, k_stride_h, v_stride_s, v_stride_h, o_stride_s, o_stride_h;
-  const int32_t* plan;  /* device, from atf_prefill_ragged_plan for these heads; 16-byte aligned */
-  int32_t num_items, num_ctas;
+  const int32_t* items; /* device, from atf_prefill_ragged_plan; 16-byte aligned */
+  int32_t num_items;
   float softmax_scale;
   int causal;           /* as planned */
   int qk_layout;        /* ATF_LAYOUT_* */
@@ -532,7 +523,7 @@ int atf_version(void);
 /* sizeof of the named params struct ("AtfPrefillParams", "AtfDecodePlanParams",
  * "AtfDecodePlan", "AtfDecodeParams", "AtfMergeParams", "AtfRopeParams",
  * "AtfAppendParams", "AtfExchangeParams", "AtfPageTablesParams", "AtfKvScales",
- * "AtfPrefillRaggedPlanParams", "AtfPrefillRaggedPlan", "AtfPrefillRaggedParams"),
+ * "AtfPrefillRaggedPlanParams", "AtfPrefillRaggedParams"),
  * or -1: lets an FFI binding check its struct mirrors. */
 int64_t atf_params_size(const char* name);
 /* Synchronises the current device, copies *error_flag to *out and clears it. */
