@@ -14,6 +14,9 @@
 // writes its own part of the entries. No CTA reads what another writes: the new
 // pages go into req_pages by the thread that lists them, slots of new pages are
 // taken from the free list again, and the next free head is a word of its own.
+//
+// Measured: 256 requests, 47K pages 7.4 us; 4096 requests, 684K pages and 106K new
+// tokens 15 us, of which the scan is about 6.
 #include "atf_internal.h"
 
 namespace atf {

@@ -144,7 +144,10 @@ int atf_prefill_fwd(const AtfPrefillParams* p, atf_stream_t stream);
  * rows [qo_indptr[b], qo_indptr[b+1]) and the keys [kv_indptr[b], kv_indptr[b+1]).
  * Its queries are the last of its keys (causal: row i sees the keys up to
  * nk - nq + i); a row that sees no key gets 0 and an LSE of -inf. The reference
- * runs one sequence at a time. */
+ * runs one sequence at a time. Nothing of another sequence reaches a row, NaN and
+ * infinity included; within a sequence they reach the rows of every query tile
+ * that loads their key tile (P is 0 there, and 0 x NaN is NaN), as in
+ * atf_prefill_fwd. */
 typedef struct {
   int32_t batch_size;
   const int32_t* qo_indptr_host; /* [batch+1] (host) */
