@@ -29,31 +29,80 @@ def get_batch_indices_positions(append_indptr: torch.Tensor, seq_lens: torch.Ten
     return batch.to(torch.int32), pos.to(torch.int32)
 
 
-def check_e4m3_cache(kc: torch.Tensor, vc: torch.Tensor, kv_scales, kv_layout: str) -> None:
-    """Pages and scales of an e4m3 cache: the append's and the decode's checks."""
+def check_e4m3_cache(kc: torch.Tensor, vc: torch.Tensor, kv_scales, kv_layout: str) -> Tuple[tuple, tuple, _ffi.AtfKvScales]:
+    """Pages and scales of an e4m3 cache, the append's and the decode's checks. Returns
+    (pages, page size, kv heads), the byte strides (page, token, head) and the scales
+    for the C call. (Sizes and strides are read once: on a short step the checks'
+    host time is the call's.)"""
     if kc.dtype != torch.float8_e4m3fn or vc.dtype != torch.float8_e4m3fn:
         raise ValueError("with kv_scales the cache pages must be float8_e4m3fn")
-    if kc.dim() != 4 or kc.shape != vc.shape or kc.stride() != vc.stride():
+    shape, st = kc.shape, kc.stride()
+    if len(shape) != 4 or shape != vc.shape or st != vc.stride():
         raise ValueError("k and v pages must have the same 4-d shape and strides")
-    if kc.shape[-1] != 128 or kc.stride(-1) != 1:
+    if shape[3] != 128 or st[3] != 1:
         raise ValueError("the cache pages must have a contiguous head_dim of 128")
+    if kv_layout == "NHD":
+        size, strides = (shape[0], shape[1], shape[2]), st[:3]
+    elif kv_layout == "HND":
+        size, strides = (shape[0], shape[2], shape[1]), (st[0], st[2], st[1])
+    else:
+        raise ValueError("kv_layout must be NHD or HND")
     if not isinstance(kv_scales, (tuple, list)) or len(kv_scales) != 2:
         raise ValueError("kv_scales is (k_scales, v_scales)")
     ks, vs = kv_scales
-    want = (kc.shape[0], kc.shape[1 if kv_layout == "HND" else 2])
-    for t in (ks, vs):
-        if not t.is_cuda or t.device != kc.device or t.dtype != torch.float32 or tuple(t.shape) != want:
-            raise ValueError(f"k_scales and v_scales must be float32 {want} tensors (pages, kv heads) on {kc.device}")
-    if ks.stride() != vs.stride():
+    want, dev, ss = (size[0], size[2]), kc.device, ks.stride()
+    if (ks.shape != want or vs.shape != want or ks.dtype != torch.float32 or vs.dtype != torch.float32
+            or ks.device != dev or vs.device != dev):
+        raise ValueError(f"k_scales and v_scales must be float32 {want} tensors (pages, kv heads) on {dev}")
+    if ss != vs.stride():
         raise ValueError("k_scales and v_scales must have the same strides")
+    return size, strides, _ffi.AtfKvScales(ks.data_ptr(), vs.data_ptr(), ss[0], ss[1])
 
 
-def e4m3_scales(kv_scales) -> _ffi.AtfKvScales:
-    ks, vs = kv_scales
-    sc = _ffi.AtfKvScales()
-    sc.k_scale, sc.v_scale = ks.data_ptr(), vs.data_ptr()
-    sc.stride_page, sc.stride_head = ks.stride(0), ks.stride(1)
-    return sc
+def _dev_i32(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    if t.dtype == torch.int32 and t.device == dev and t.is_contiguous():
+        return t
+    return t.to(device=dev, dtype=torch.int32).contiguous()
+
+
+def _append_e4m3(k: torch.Tensor, v: torch.Tensor, batch_indices, positions, kc, vc, kv_indices, kv_indptr, kv_layout,
+                 rope, rope_positions, out_layout, kv_scales) -> None:
+    dev = _runtime.require_cuda(k, v, kc, vc)
+    (npages, page, hkv), (s_page, s_tok, s_head), scales = check_e4m3_cache(kc, vc, kv_scales, kv_layout)
+    shape, st = k.shape, k.stride()
+    if (len(shape) != 3 or shape[2] != 128 or st[2] != 1 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16):
+        raise ValueError("keys and values must be (tokens, kv heads, 128) bf16 with a contiguous head_dim")
+    if v.shape != shape or v.stride() != st:
+        raise ValueError("append_key and append_value must have the same shape and strides")
+    nnz = shape[0]
+    if shape[1] != hkv:
+        raise ValueError("append_key heads do not match the cache")
+    layout = _LAYOUTS[out_layout]
+    bi, ps = _dev_i32(batch_indices, dev), _dev_i32(positions, dev)
+    ip, ix = _dev_i32(kv_indptr, dev), _dev_i32(kv_indices, dev)
+    if bi.numel() != nnz or ps.numel() != nnz:
+        raise ValueError("batch_indices and positions need one entry per appended token")
+    if nnz == 0:
+        return
+    p = _ffi.AtfAppendParams(k.data_ptr(), v.data_ptr(), nnz, st[0], st[1], bi.data_ptr(), ps.data_ptr(), kc.data_ptr(),
+                             vc.data_ptr(), npages, s_page, s_tok, s_head, hkv, 128, page, ip.numel() - 1,
+                             ip.data_ptr(), ix.data_ptr())
+    p.out_layout = layout
+    p.error_flag = _runtime.error_flag(dev).data_ptr()
+    if rope is not None:
+        cos, sin = rope
+        cst, csh = cos.stride(), cos.shape
+        if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(csh) != 2 or csh != sin.shape
+                or csh[1] < 64 or cst != sin.stride() or cst[1] != 1 or cos.device != dev or sin.device != dev):
+            raise ValueError("cos/sin must be matching fp32 (n_pos, >=64) tables")
+        p.cos, p.sin, p.cs_stride_pos, p.n_pos = cos.data_ptr(), sin.data_ptr(), cst[0], csh[0]
+        if rope_positions is not None:
+            rp = rope_positions.to(device=dev, dtype=torch.int64).contiguous()
+            if rp.numel() != nnz:
+                raise ValueError("rope_positions needs one entry per appended token")
+            p.rope_positions = rp.data_ptr()
+    _runtime.launch("atf_paged_kv_append_e4m3", _ffi.load().atf_paged_kv_append_e4m3, dev, ctypes.byref(p),
+                    ctypes.byref(scales))
 
 
 def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, batch_indices: torch.Tensor,
@@ -81,15 +130,15 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
         kc, vc = paged_kv_cache
     else:
         kc, vc = paged_kv_cache[:, 0], paged_kv_cache[:, 1]
+    if kv_scales is not None:
+        _append_e4m3(append_key, append_value, batch_indices, positions, kc, vc, kv_indices, kv_indptr, kv_layout, rope,
+                     rope_positions, out_layout, kv_scales)
+        return
     dev = _runtime.require_cuda(append_key, append_value, kc, vc)
-    e4m3 = kv_scales is not None
-    if not e4m3 and torch.float8_e4m3fn in (kc.dtype, vc.dtype):
+    if torch.float8_e4m3fn in (kc.dtype, vc.dtype):
         raise ValueError("float8_e4m3fn pages need kv_scales")
-    if e4m3:
-        check_e4m3_cache(kc, vc, kv_scales, kv_layout)
     k_level_major = kc.dim() == 5
-    bf16 = (append_key, append_value) if e4m3 else (append_key, append_value, vc) + (() if k_level_major else (kc,))
-    for t in bf16:
+    for t in (append_key, append_value, vc) + (() if k_level_major else (kc,)):
         if t.dtype != torch.bfloat16 or t.stride(-1) != 1 or t.shape[-1] != 128:
             raise ValueError("keys, values and cache pages must be bf16 with a contiguous head_dim of 128")
     if append_key.shape != append_value.shape or append_key.stride() != append_value.stride():
@@ -114,13 +163,10 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
         raise ValueError("kv_layout must be NHD or HND")
     if hk2 != hkv:
         raise ValueError("append_key heads do not match the cache")
-    bi, ps, ip, ix = (t if t.dtype == torch.int32 and t.device == dev and t.is_contiguous()
-                      else t.to(device=dev, dtype=torch.int32).contiguous()
-                      for t in (batch_indices, positions, kv_indptr, kv_indices))
+    bi, ps = _dev_i32(batch_indices, dev), _dev_i32(positions, dev)
+    ip, ix = _dev_i32(kv_indptr, dev), _dev_i32(kv_indices, dev)
     if bi.numel() != nnz or ps.numel() != nnz:
         raise ValueError("batch_indices and positions need one entry per appended token")
-    if e4m3 and nnz == 0:
-        return
     p = _ffi.AtfAppendParams()
     p.append_k, p.append_v, p.nnz = append_key.data_ptr(), append_value.data_ptr(), nnz
     p.a_stride_n, p.a_stride_h = append_key.stride(0), append_key.stride(1)
@@ -150,11 +196,6 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
             raise ValueError("level-major k pages do not match the v pages")
         p.k_level_major = 1
         p.k_stride_page, p.k_stride_head, p.k_stride_level = kc.stride(0), kc.stride(1), kc.stride(2)
-    if e4m3:
-        sc = e4m3_scales(kv_scales)
-        _runtime.launch("atf_paged_kv_append_e4m3", _ffi.load().atf_paged_kv_append_e4m3, dev, ctypes.byref(p),
-                        ctypes.byref(sc))
-        return
     with torch.cuda.device(dev):
         rc = _ffi.load().atf_paged_kv_append(ctypes.byref(p), _runtime.stream_handle(dev))
     _ffi.check("atf_paged_kv_append", rc)

@@ -18,7 +18,7 @@ import numpy as np
 import torch
 
 from . import _ffi, _runtime
-from .append import check_e4m3_cache, e4m3_scales
+from .append import check_e4m3_cache
 from .window_table import KERNEL_CAP, WindowTable, zhi_slice_vec8
 
 _LAYOUTS = {"sorted_pair": _ffi.ATF_LAYOUT_SORTED_PAIR, "rotate_half": _ffi.ATF_LAYOUT_ROTATE_HALF}
@@ -239,19 +239,11 @@ class BatchDecodeWithPagedKVCacheWrapper:
             kc, vc = paged_kv_cache
         else:
             kc, vc = paged_kv_cache[:, 0], paged_kv_cache[:, 1]
-        dev = _runtime.require_cuda(q, kc, vc)
         if kv_scales is not None:
-            if q.dtype != torch.bfloat16:
-                raise TypeError("q must be bfloat16")
-            check_e4m3_cache(kc, vc, kv_scales, self._kv_layout)
-            if exchange is not None:
-                raise NotImplementedError("the KV-sharded exchange reads bfloat16 caches")
-            if P["page_size"] not in (16, 32, 64, 128, 256):
-                raise NotImplementedError("an e4m3 cache has pages of 16, 32, 64, 128 or 256 tokens")
-            if P["window"] == _ffi.ATF_WINDOW_VEC8 or (P["window"] != _ffi.ATF_WINDOW_OFF
-                                                       and P["layout"] != _ffi.ATF_LAYOUT_SORTED_PAIR):
-                raise NotImplementedError("an e4m3 cache takes snap16 windows over sorted pairs")
-        elif kc.dtype != torch.bfloat16 or vc.dtype != torch.bfloat16 or q.dtype != torch.bfloat16:
+            return self._run_e4m3(q, kc, vc, kv_scales, out, lse, return_lse, enable_pdl, q_pos, kv_pos0, out_dtype,
+                                  exchange)
+        dev = _runtime.require_cuda(q, kc, vc)
+        if kc.dtype != torch.bfloat16 or vc.dtype != torch.bfloat16 or q.dtype != torch.bfloat16:
             raise TypeError("q and the KV cache must be bfloat16 (float8_e4m3fn pages need kv_scales)")
         # K pages are either laid out like V (4-d, NHD / HND) or level-major:
         # (P, Hkv, 8 levels, page, 16) in sorted-pair order, so that a page's
@@ -323,14 +315,63 @@ class BatchDecodeWithPagedKVCacheWrapper:
                                                          _runtime.stream_handle(dev))
             _ffi.check("atf_decode_run_exchange", rc)
             return (out, lse) if return_lse else out
-        if kv_scales is not None:
-            sc = e4m3_scales(kv_scales)
-            _runtime.launch("atf_decode_run_e4m3", _ffi.load().atf_decode_run_e4m3, dev, ctypes.byref(a),
-                            ctypes.byref(sc))
-            return (out, lse) if return_lse else out
         with torch.cuda.device(dev):
             rc = _ffi.load().atf_decode_run(ctypes.byref(a), _runtime.stream_handle(dev))
         _ffi.check("atf_decode_run", rc)
+        return (out, lse) if return_lse else out
+
+    def _run_e4m3(self, q, kc, vc, kv_scales, out, lse, return_lse, enable_pdl, q_pos, kv_pos0, out_dtype, exchange):
+        """run() over float8_e4m3fn pages with their scales."""
+        P = self._plan
+        if exchange is not None:
+            raise NotImplementedError("the KV-sharded exchange reads bfloat16 caches")
+        dev = _runtime.require_cuda(q, kc, vc)
+        if q.dtype != torch.bfloat16:
+            raise TypeError("q must be bfloat16")
+        (npages, page, hkv), strides, scales = check_e4m3_cache(kc, vc, kv_scales, self._kv_layout)
+        if page != P["page_size"] or hkv != P["Hkv"]:
+            raise ValueError("KV cache shape does not match the plan")
+        if page not in (16, 32, 64, 128, 256):
+            raise NotImplementedError("an e4m3 cache has pages of 16, 32, 64, 128 or 256 tokens")
+        if P["window"] != _ffi.ATF_WINDOW_OFF and (P["window"] == _ffi.ATF_WINDOW_VEC8
+                                                   or P["layout"] != _ffi.ATF_LAYOUT_SORTED_PAIR):
+            raise NotImplementedError("an e4m3 cache takes snap16 windows over sorted pairs")
+        shape, qst = (P["B"], P["Hq"], 128), q.stride()
+        if q.shape != shape or qst[2] != 1:
+            raise ValueError(f"q must be {shape} with a contiguous head_dim axis")
+        if out is None:
+            if out_dtype not in (None, torch.bfloat16, torch.float32):
+                raise TypeError("out_dtype must be bfloat16 or float32")
+            out = torch.empty(shape, dtype=out_dtype or torch.bfloat16, device=dev)
+        elif (out.shape != shape or out.dtype not in (torch.bfloat16, torch.float32) or out.device != dev
+              or (out_dtype is not None and out.dtype != out_dtype) or out.stride(2) != 1):
+            raise ValueError(f"out must be a {shape} bfloat16 or float32 tensor on {dev} with a contiguous head_dim axis")
+        if lse is None:
+            if return_lse:
+                lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
+        elif lse.shape != shape[:2] or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous():
+            raise ValueError(f"lse must be a contiguous float32 {shape[:2]} tensor on {dev}")
+        a = _ffi.AtfDecodeParams.from_buffer_copy(self._tmpl)
+        ost = out.stride()
+        a.q, a.q_stride_b, a.q_stride_h = q.data_ptr(), qst[0], qst[1]
+        a.k_cache, a.v_cache, a.num_pages = kc.data_ptr(), vc.data_ptr(), npages
+        a.kv_stride_page, a.kv_stride_token, a.kv_stride_head = strides
+        a.out, a.o_stride_b, a.o_stride_h = out.data_ptr(), ost[0], ost[1]
+        a.out_dtype = _ffi.ATF_DTYPE_F32 if out.dtype == torch.float32 else _ffi.ATF_DTYPE_BF16
+        if lse is not None:
+            a.lse_out = lse.data_ptr()
+        keep = []
+        for name, pos in (("q_pos", q_pos), ("kv_pos0", kv_pos0)):
+            if pos is not None:
+                pos = pos.to(device=dev, dtype=torch.int64).contiguous()
+                if pos.numel() != shape[0]:
+                    raise ValueError(f"{name} must have one entry per request")
+                keep.append(pos)
+                setattr(a, name, pos.data_ptr())
+        if enable_pdl:
+            a.enable_pdl = 1
+        _runtime.launch("atf_decode_run_e4m3", _ffi.load().atf_decode_run_e4m3, dev, ctypes.byref(a),
+                        ctypes.byref(scales))
         return (out, lse) if return_lse else out
 
     forward = run

@@ -60,6 +60,7 @@ def build_page_tables(kv_lens: torch.Tensor, append_lens: torch.Tensor, req_page
     if B < 1 or B > _ffi.ATF_TABLES_MAX_BATCH:
         raise ValueError(f"between 1 and {_ffi.ATF_TABLES_MAX_BATCH} requests")
     kv_lens, append_lens = _i32(kv_lens, "kv_lens"), _i32(append_lens, "append_lens", B)
+    num_tokens, max_pages = int(num_tokens), int(max_pages)
     if req_pages.dim() != 2 or req_pages.dtype != torch.int32 or (req_pages.shape[1] > 1 and req_pages.stride(1) != 1):
         raise ValueError("req_pages must be an int32 (rows, pages) tensor with contiguous rows")
     if req_pages.shape[0] < 1 or (req_rows is None and req_pages.shape[0] < B):
@@ -83,29 +84,34 @@ def build_page_tables(kv_lens: torch.Tensor, append_lens: torch.Tensor, req_page
         rows = _i32(req_rows, "req_rows", B)
         keep.append(rows)
         p.req_rows = rows.data_ptr()
-    head_out = None
     if free_pages is not None:
         _runtime.require_cuda(kv_lens, free_pages, free_head)
         free_pages = _i32(free_pages, "free_pages")
         free_head = _i32(free_head, "free_head", 1)
         keep += [free_pages, free_head]
-        head_out = torch.empty(1, dtype=torch.int32, device=dev)
         # an empty list still has a head: any valid address will do for its pages
         p.free_pages = free_pages.data_ptr() or free_head.data_ptr()
-        p.free_head, p.free_head_out, p.num_free = free_head.data_ptr(), head_out.data_ptr(), free_pages.numel()
-    # one allocation for the 32-bit outputs
-    sizes = (B + 1, max_pages, B, B + 1, num_tokens, num_tokens)
-    buf = torch.empty(sum(sizes), dtype=torch.int32, device=dev)
+        p.free_head, p.num_free = free_head.data_ptr(), free_pages.numel()
+    # one allocation for the 32-bit outputs, in the order of PageTables
+    sizes = (B + 1, max_pages, B, B + 1, num_tokens, num_tokens, 1)
+    buf = torch.empty(3 * B + 3 + max_pages + 2 * num_tokens, dtype=torch.int32, device=dev)
     slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    p.max_pages, p.max_tokens = int(max_pages), int(num_tokens)
+    p.max_pages, p.max_tokens = max_pages, num_tokens
     at = buf.data_ptr()
     p.indptr = at
-    p.indices = at + 4 * (B + 1)
-    p.last_page_len = p.indices + 4 * max_pages
-    p.append_indptr = p.last_page_len + 4 * B
-    p.batch_indices = p.append_indptr + 4 * (B + 1)
-    p.positions = p.batch_indices + 4 * num_tokens
+    at += 4 * (B + 1)
+    p.indices = at
+    at += 4 * max_pages
+    p.last_page_len = at
+    at += 4 * B
+    p.append_indptr = at
+    at += 4 * (B + 1)
+    p.batch_indices = at
+    p.positions = at + 4 * num_tokens
+    if free_pages is not None:
+        p.free_head_out = at + 8 * num_tokens
     p.slot_mapping = slots.data_ptr()
     p.error_flag = _runtime.error_flag(dev).data_ptr()
     _runtime.launch("atf_build_page_tables", _ffi.load().atf_build_page_tables, dev, ctypes.byref(p))
-    return PageTables(*buf.split_with_sizes(sizes), slots, head_out)
+    indptr, indices, last, aptr, bidx, pos, head = buf.split_with_sizes(sizes)
+    return PageTables(indptr, indices, last, aptr, bidx, pos, slots, head if free_pages is not None else None)
