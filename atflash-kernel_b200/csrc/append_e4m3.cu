@@ -18,16 +18,19 @@
 // What bounds it: HBM for prompts (2 x 256 bytes read and 2 x 128 written per
 // token and head); for one token per request the chain of dependent loads (token
 // -> page list -> row). A CTA covers a window of tokens: its first warp finds the
-// runs that begin there, their pages and lengths once, and all warps then go
-// through the tasks. The window shrinks with the token count so that a decode
-// step's tokens spread over the SMs.
+// runs that begin there, their pages and lengths once, while the others fetch the
+// tokens' rows of angles for all heads (RoPE); then all warps go through the tasks.
+// The window shrinks with the token count so that a decode step's tokens spread over
+// the SMs.
 //
-// Measured: 64K tokens x 8 heads in pages of 16 74 us (90% of HBM), with RoPE 108:
-// its products and the rows of angles, from L2, for every head; 64 tokens x 8 heads
-// 4.5 us. What cost most on the way: rows loaded one after another behind their
-// bounds checks (170 us), and a division per element in the unrolled rounding (130).
+// Measured: 64K tokens x 8 heads in pages of 16 74 us (90% of HBM), with RoPE 98: the
+// products of its rotation (107 with the angles read from L2 for every head); 64 tokens
+// x 8 heads 4.5 us. What cost most on the way: rows loaded one after another behind
+// their bounds checks (170 us), and a division per element in the unrolled rounding
+// (130). CTAs of 4 warps: 96-102 us, but 18-19 instead of 13 for pages of 64.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "atf_internal.h"
@@ -156,13 +159,15 @@ __device__ __forceinline__ Words load_row(const __nv_bfloat16* row, int c, bool 
   return x;
 }
 // the 8 pairs rotated as in rope_math.cuh (separately rounded products, then bf16),
-// as words in the order they are written; cr and sr: the position's table rows
-__device__ __forceinline__ Words rotate(const Words& in, const float* cr, const float* sr, int c, bool sorted) {
+// as words in the order they are written; row(f): the position's table rows, cos in
+// the 16-byte words 0 .. 15 and sin in 16 .. 31
+template <typename Row>
+__device__ __forceinline__ Words rotate(const Words& in, Row row, int c, bool sorted) {
   float cv[8], sv[8];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
-    const float4 c4 = *reinterpret_cast<const float4*>(cr + 8 * c + 4 * q);
-    const float4 s4 = *reinterpret_cast<const float4*>(sr + 8 * c + 4 * q);
+    const float4 c4 = row(2 * c + q);
+    const float4 s4 = row(16 + 2 * c + q);
     cv[4 * q] = c4.x; cv[4 * q + 1] = c4.y; cv[4 * q + 2] = c4.z; cv[4 * q + 3] = c4.w;
     sv[4 * q] = s4.x; sv[4 * q + 1] = s4.y; sv[4 * q + 2] = s4.z; sv[4 * q + 3] = s4.w;
   }
@@ -279,16 +284,43 @@ __device__ __forceinline__ int find_runs(const Args& a, long long i0, Run* runs,
   return __popc(goods);
 }
 
+// position of a token in the tables, inside them
+__device__ __forceinline__ long long angle_row(const Args& a, long long i) {
+  const long long rp = a.rope_pos != nullptr ? a.rope_pos[i] : a.positions[i];
+  return rp < 0 ? 0 : (rp >= a.n_pos ? a.n_pos - 1 : rp);
+}
+// word f of a staged row: even words of the two halves of cos (or sin) would share
+// banks, so the second half's are swapped with their neighbours
+__device__ __forceinline__ int angle_slot(int f) { return f ^ ((f >> 3) & 1); }
+
+// The angles of the window's tokens, read once for all heads, by the warps that
+// wait for find_runs meanwhile
+__device__ __forceinline__ void stage_angles(const Args& a, long long i0, float4 (*rows)[32], int warp, int lane) {
+  const int tokens = static_cast<int>(min(static_cast<long long>(a.window), a.nnz - i0));
+  // lane k holds the row of this warp's k-th token
+  const int mine = (warp - 1) + lane * (WARPS - 1);
+  const long long rp = mine < tokens ? angle_row(a, i0 + mine) : 0;
+  for (int k = 0, t = warp - 1; t < tokens; ++k, t += WARPS - 1) {
+    const long long at = __shfl_sync(0xffffffffu, rp, k) * a.cs_stride + 4 * (lane & 15);
+    const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(&rows[t][angle_slot(lane)]));
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"((lane < 16 ? a.cs : a.sn) + at) : "memory");
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 template <bool ROPE>
 __global__ void __launch_bounds__(THREADS, 3) append_e4m3_kernel(const Args a) {
   __shared__ Run s_run[MAX_WINDOW];
   __shared__ int s_n;
   __shared__ float s_max[2][WARPS];
+  __shared__ __align__(16) float4 s_angle[ROPE ? MAX_WINDOW : 1][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long i0 = static_cast<long long>(blockIdx.x) * a.window;
   if (warp == 0) {
     const int n = find_runs(a, i0, s_run, lane);
     if (lane == 0) s_n = n;
+  } else if (ROPE) {
+    stage_angles(a, i0, s_angle, warp, lane);
   }
   __syncthreads();
   // this CTA's heads: a block's y takes `heads` of them
@@ -326,9 +358,15 @@ __global__ void __launch_bounds__(THREADS, 3) append_e4m3_kernel(const Args a) {
       if (rot) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          long long rp = a.rope_pos != nullptr ? a.rope_pos[i0 + run.i + r[u]] : run.pos + r[u];
-          rp = rp < 0 ? 0 : (rp >= a.n_pos ? a.n_pos - 1 : rp);
-          w[u] = rotate(w[u], a.cs + rp * a.cs_stride, a.sn + rp * a.cs_stride, c, a.sorted != 0);
+          const int t = run.i + r[u];
+          if (t < a.window) {
+            w[u] = rotate(w[u], [&](int f) { return s_angle[t][angle_slot(f)]; }, c, a.sorted != 0);
+          } else {  // the run goes on past the window
+            const long long at = angle_row(a, i0 + t) * a.cs_stride;
+            w[u] = rotate(w[u], [&](int f) {
+              return *reinterpret_cast<const float4*>((f < 16 ? a.cs : a.sn) + at + 4 * (f & 15));
+            }, c, a.sorted != 0);
+          }
         }
       }
     };
@@ -455,11 +493,15 @@ extern "C" int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvSca
   const long long blocks = (a.nnz + a.window - 1) / a.window;
   if (blocks > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // few CTAs with more tasks than warps: the heads go to several
+  // Few CTAs that begin a run (pages longer than the window: not all do) with more
+  // tasks than warps: the heads go to several (13 prompts in pages of 64, 4 heads:
+  // 13.4 us undivided, 10.0 divided; dividing further, or more CTAs than this, gave
+  // nothing or cost 1.8 us at pages of 16)
   const long long runs = a.window / p->page_size + 1;  // that a window may begin, for one request
   const long long at_once = append8::WARPS / a.share;
   int split = 1;
-  while (split < a.H && blocks * split < 2 * 148 && runs * ((a.H + split - 1) / split) * 2 > at_once) split <<= 1;
+  const long long busy = (blocks * std::min(a.window, p->page_size) + p->page_size - 1) / p->page_size;
+  while (split < a.H && busy * split < 2 * 148 && runs * ((a.H + split - 1) / split) * 2 > at_once) split <<= 1;
   a.heads = (a.H + split - 1) / split;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((a.H + a.heads - 1) / a.heads));
   if (rope)
