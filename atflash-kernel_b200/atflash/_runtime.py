@@ -22,6 +22,12 @@ def error_flag(device: torch.device) -> torch.Tensor:
     return t
 
 
+def error_flag_ptr(device: torch.device) -> int:
+    """Address of error_flag(device); of a flag that is there, without the lock."""
+    t = _flags.get(device.index)
+    return (error_flag(device) if t is None else t).data_ptr()
+
+
 def check_device_errors(device=None) -> int:
     """Synchronise `device`, return (and clear) its kernel error flag.
 

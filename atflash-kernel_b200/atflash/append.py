@@ -88,7 +88,7 @@ def _append_e4m3(k: torch.Tensor, v: torch.Tensor, batch_indices, positions, kc,
                              vc.data_ptr(), npages, s_page, s_tok, s_head, hkv, 128, page, ip.numel() - 1,
                              ip.data_ptr(), ix.data_ptr())
     p.out_layout = layout
-    p.error_flag = _runtime.error_flag(dev).data_ptr()
+    p.error_flag = _runtime.error_flag_ptr(dev)
     if rope is not None:
         cos, sin = rope
         cst, csh = cos.stride(), cos.shape

@@ -95,18 +95,20 @@ class BatchPrefillWithRaggedKVCacheWrapper:
             raise ValueError(f"the plan is on {self._dev}, the tensors are on {dev}")
         if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
             raise TypeError("q, k, v must be bfloat16")
-        if tuple(q.shape) != (nq, hq, 128) or tuple(k.shape) != (nk, hkv, 128) or k.shape != v.shape:
+        shape = (nq, hq, 128)
+        if q.shape != shape or k.shape != (nk, hkv, 128) or k.shape != v.shape:
             raise ValueError(f"planned for q ({nq}, {hq}, 128) and k, v ({nk}, {hkv}, 128)")
-        if q.stride(-1) != 1 or k.stride(-1) != 1 or v.stride(-1) != 1:
+        qst, kst, vst = q.stride(), k.stride(), v.stride()
+        if qst[2] != 1 or kst[2] != 1 or vst[2] != 1:
             raise ValueError("the head_dim axis must be contiguous")
         if out is None:
-            out = torch.empty((nq, hq, 128), dtype=torch.bfloat16, device=dev)
-        elif (tuple(out.shape) != (nq, hq, 128) or out.dtype != torch.bfloat16 or out.device != dev
+            out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        elif (out.shape != shape or out.dtype != torch.bfloat16 or out.device != dev
               or out.stride(-1) != 1):
             raise ValueError(f"out must be a bf16 ({nq}, {hq}, 128) tensor on {dev} with a contiguous head_dim axis")
         if return_lse and lse is None:
             lse = torch.empty((nq, hq), dtype=torch.float32, device=dev)
-        if lse is not None and (tuple(lse.shape) != (nq, hq) or lse.dtype != torch.float32 or lse.device != dev
+        if lse is not None and (lse.shape != (nq, hq) or lse.dtype != torch.float32 or lse.device != dev
                                 or not lse.is_contiguous()):
             raise ValueError(f"lse must be a contiguous float32 ({nq}, {hq}) tensor on {dev}")
         if nk == 0:  # no keys at all
@@ -116,10 +118,11 @@ class BatchPrefillWithRaggedKVCacheWrapper:
         elif nq > 0:
             p = _ffi.AtfPrefillRaggedParams.from_buffer_copy(t)
             p.q, p.k, p.v, p.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-            p.lse = lse.data_ptr() if lse is not None else None
-            p.q_stride_s, p.q_stride_h, _ = q.stride()
-            p.k_stride_s, p.k_stride_h, _ = k.stride()
-            p.v_stride_s, p.v_stride_h, _ = v.stride()
+            if lse is not None:
+                p.lse = lse.data_ptr()
+            p.q_stride_s, p.q_stride_h, _ = qst
+            p.k_stride_s, p.k_stride_h, _ = kst
+            p.v_stride_s, p.v_stride_h, _ = vst
             p.o_stride_s, p.o_stride_h, _ = out.stride()
             _runtime.launch("atf_prefill_ragged_fwd", _ffi.load().atf_prefill_ragged_fwd, dev, ctypes.byref(p))
         return (out, lse) if return_lse else out

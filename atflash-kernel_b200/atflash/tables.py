@@ -61,11 +61,13 @@ def build_page_tables(kv_lens: torch.Tensor, append_lens: torch.Tensor, req_page
         raise ValueError(f"between 1 and {_ffi.ATF_TABLES_MAX_BATCH} requests")
     kv_lens, append_lens = _i32(kv_lens, "kv_lens"), _i32(append_lens, "append_lens", B)
     num_tokens, max_pages = int(num_tokens), int(max_pages)
-    if req_pages.dim() != 2 or req_pages.dtype != torch.int32 or (req_pages.shape[1] > 1 and req_pages.stride(1) != 1):
+    shape, st = req_pages.shape, req_pages.stride()
+    if len(shape) != 2 or req_pages.dtype != torch.int32 or (shape[1] > 1 and st[1] != 1):
         raise ValueError("req_pages must be an int32 (rows, pages) tensor with contiguous rows")
-    if req_pages.shape[0] < 1 or (req_rows is None and req_pages.shape[0] < B):
+    R, M = shape
+    if R < 1 or (req_rows is None and R < B):
         raise ValueError("req_pages needs a row for each request")
-    if req_pages.shape[0] > 1 and req_pages.stride(0) < req_pages.shape[1]:
+    if R > 1 and st[0] < M:
         raise ValueError("the rows of req_pages must not overlap")
     if page_size < 1 or num_tokens < 0 or max_pages < 0:
         raise ValueError("page_size must be positive, num_tokens and max_pages not negative")
@@ -73,45 +75,33 @@ def build_page_tables(kv_lens: torch.Tensor, append_lens: torch.Tensor, req_page
         raise ValueError("num_tokens and max_pages must be under 2^30")
     if (free_pages is None) != (free_head is None):
         raise ValueError("free_pages and free_head go together")
-    keep = [kv_lens, append_lens]
-    p = _ffi.AtfPageTablesParams()
-    p.kv_lens, p.append_lens, p.batch, p.page_size = kv_lens.data_ptr(), append_lens.data_ptr(), B, int(page_size)
-    p.req_pages = req_pages.data_ptr() or kv_lens.data_ptr()  # no columns: never read
-    p.req_stride = req_pages.stride(0) if req_pages.shape[0] > 1 else max(1, req_pages.shape[1])
-    p.num_rows, p.max_req_pages = req_pages.shape
+    rows_ptr = free_ptr = head_ptr = num_free = 0
     if req_rows is not None:
         _runtime.require_cuda(kv_lens, req_rows)
-        rows = _i32(req_rows, "req_rows", B)
-        keep.append(rows)
-        p.req_rows = rows.data_ptr()
+        req_rows = _i32(req_rows, "req_rows", B)
+        rows_ptr = req_rows.data_ptr()
     if free_pages is not None:
         _runtime.require_cuda(kv_lens, free_pages, free_head)
         free_pages = _i32(free_pages, "free_pages")
         free_head = _i32(free_head, "free_head", 1)
-        keep += [free_pages, free_head]
         # an empty list still has a head: any valid address will do for its pages
-        p.free_pages = free_pages.data_ptr() or free_head.data_ptr()
-        p.free_head, p.num_free = free_head.data_ptr(), free_pages.numel()
+        head_ptr, num_free = free_head.data_ptr(), free_pages.numel()
+        free_ptr = free_pages.data_ptr() or head_ptr
     # one allocation for the 32-bit outputs, in the order of PageTables
-    sizes = (B + 1, max_pages, B, B + 1, num_tokens, num_tokens, 1)
     buf = torch.empty(3 * B + 3 + max_pages + 2 * num_tokens, dtype=torch.int32, device=dev)
     slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    p.max_pages, p.max_tokens = max_pages, num_tokens
-    at = buf.data_ptr()
-    p.indptr = at
-    at += 4 * (B + 1)
-    p.indices = at
-    at += 4 * max_pages
-    p.last_page_len = at
-    at += 4 * B
-    p.append_indptr = at
-    at += 4 * (B + 1)
-    p.batch_indices = at
-    p.positions = at + 4 * num_tokens
-    if free_pages is not None:
-        p.free_head_out = at + 8 * num_tokens
-    p.slot_mapping = slots.data_ptr()
-    p.error_flag = _runtime.error_flag(dev).data_ptr()
+    indptr = buf.data_ptr()
+    indices = indptr + 4 * (B + 1)
+    last = indices + 4 * max_pages
+    aptr = last + 4 * B
+    bidx = aptr + 4 * (B + 1)
+    pos = bidx + 4 * num_tokens
+    lens_ptr = kv_lens.data_ptr()
+    # (req_pages without columns is never read: any valid address will do)
+    p = _ffi.AtfPageTablesParams(
+        lens_ptr, append_lens.data_ptr(), B, int(page_size), req_pages.data_ptr() or lens_ptr, st[0] if R > 1 else max(1, M),
+        R, M, rows_ptr, free_ptr, head_ptr, pos + 4 * num_tokens if head_ptr else 0, num_free, max_pages, num_tokens,
+        indptr, indices, last, aptr, bidx, pos, slots.data_ptr(), _runtime.error_flag_ptr(dev))
     _runtime.launch("atf_build_page_tables", _ffi.load().atf_build_page_tables, dev, ctypes.byref(p))
-    indptr, indices, last, aptr, bidx, pos, head = buf.split_with_sizes(sizes)
-    return PageTables(indptr, indices, last, aptr, bidx, pos, slots, head if free_pages is not None else None)
+    out = buf.split_with_sizes((B + 1, max_pages, B, B + 1, num_tokens, num_tokens, 1))
+    return PageTables(*out[:6], slots, out[6] if head_ptr else None)
