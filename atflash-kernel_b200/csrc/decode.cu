@@ -956,7 +956,13 @@ extern "C" int atf_decode_plan(const AtfDecodePlanParams* p, int32_t* items_host
   // key counts would leave the CTAs nearest the query the slowest. Cuts fall on
   // multiples of 64 keys (a stage).
   const long long slots = 2ll * sms;
-  if (p->units) return decode8::plan_units(p, slots, items_host, items_capacity, item_indptr_host, out);
+  if (p->units) {
+    try {
+      return decode8::plan_units(p, slots, items_host, items_capacity, item_indptr_host, out);
+    } catch (...) {  // no host memory for the schedule
+      return ATF_ERR_WORKSPACE;
+    }
+  }
   const long long min_chunk = p->min_chunk_keys > 0 ? p->min_chunk_keys : 256;
   long long cap = decode_tma::MAX_ITEM_KEYS;
   if (p->max_chunk_keys > 0 && p->max_chunk_keys < cap) cap = p->max_chunk_keys;

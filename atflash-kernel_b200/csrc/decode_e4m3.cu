@@ -39,13 +39,15 @@
 // item per CTA, 55 so). The producer runs through the pieces without a stop while
 // the consumers write each piece's state (2.8 us of a CTA's time per piece).
 //
-// Measured: 8 x 128K keys, 24 / 8 heads 335 us in HND pages (98% of the copy
-// bandwidth), 355 in NHD pages of 16 (boxes of 2 KB), window on 365; 37 requests up to
-// 20011 keys (28 / 4 heads) 55 us, 80%: the SMs' shares end between 44 and 52 us.
+// Measured: 8 x 128K keys, 24 / 8 heads, window on 325 us in HND pages of 64 (the
+// copy bandwidth, rows read whole), 360 in NHD pages of 16 (boxes of 2 KB); 37 requests
+// up to 20011 keys (28 / 4 heads) 55 us, 80%: the SMs' shares end between 44 and 52 us;
+// 3 requests up to 300 keys 8.2 us with the merge.
 #include <cuda_fp16.h>
 #include <limits.h>
 #include <math.h>
 
+#include <algorithm>
 #include <vector>
 
 #include "atf_internal.h"
@@ -108,7 +110,7 @@ struct Args {
   const float* vs;
   long long ss_page, ss_head;
   long long num_pages;
-  int Hq, G, page_size, page_shift, rows;
+  int Hq, Hkv, G, page_size, page_shift, rows;
   float scale_log2;
   int zhi16[ATF_MAX_LEVELS];
   float* part_o;
@@ -170,10 +172,12 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   float2* s_scale = reinterpret_cast<float2*>(sp + OFF_SCALES);  // (ks, log2 vs) of the unit's pages
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int hk = blockIdx.y;
+  // Heads run fastest over the grid: a plan with units has rows that name none, and
+  // their blocks, which leave at once, come after every block that works.
+  const int hk = static_cast<int>(blockIdx.x) % a.Hkv;
   // The unit's items: row x of the plan names its first item (1-based; 0: the
   // row is a unit of its own, negative: no unit).
-  const int x = blockIdx.x;
+  const int x = static_cast<int>(blockIdx.x) / a.Hkv;
   const int tag = a.items[4 * x + 3];
   const int next = x + 1 < a.num_items ? a.items[4 * x + 7] : 0;
   if (tag < 0) return;
@@ -645,90 +649,141 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   }
 }
 
-// Units: the requests' 64-key blocks lie on one line, each key at the same cost (a
-// key's rows are read whole whatever the window) and each request's piece with that
-// of its state; unit u is the part of the line up to (u + 1) / U of the whole. U
-// fills the slots (two resident CTAs per SM, over the kv heads) in as few waves as
-// the units' limits allow, with at least min_chunk_keys (64) keys per unit.
+// keys in whose time an item starts and writes its state (2.8 us measured)
+constexpr long long ITEM_COST = 288;
+
+struct Piece {  // an item; opens: the first of its unit
+  int b;
+  long long k0, k1;
+  bool opens;
+};
+
+// the cost of the dearest unit, in keys
+long long longest_unit(const std::vector<Piece>& pieces) {
+  long long most = 0, unit = 0;
+  for (const Piece& p : pieces) {
+    unit = (p.opens ? 0 : unit) + p.k1 - p.k0 + ITEM_COST;
+    most = std::max(most, unit);
+  }
+  return most;
+}
+
+// Requests cut into items of at most `chunk` keys, each a unit.
+std::vector<Piece> cut_evenly(const std::vector<long long>& lens, long long chunk) {
+  std::vector<Piece> out;
+  for (size_t b = 0; b < lens.size(); ++b) {
+    const long long n = (lens[b] + chunk - 1) / chunk;
+    for (long long i = 0; i < n; ++i)
+      out.push_back({static_cast<int>(b), i * chunk, std::min(lens[b], (i + 1) * chunk), true});
+  }
+  return out;
+}
+
+// The requests' keys on one line, each at the same cost (a key's rows are read whole
+// whatever the window) and each request with that of its state: unit u is the part up
+// to (u + 1) / U of the whole. An item costs a
+// start of its own, so a request is not begun for the last keys that a unit wants, nor
+// are its own last ones left to the next unit, up to `slack` keys.
+std::vector<Piece> cut_in_units(const std::vector<long long>& lens, long long U, long long whole, long long cap, int ps) {
+  const long long slack = std::min(ITEM_COST / 2, whole / (2 * U));
+  std::vector<Piece> out;
+  long long units = 0, done = 0;  // done: cost of everything cut so far
+  long long unit_pages = 0, unit_items = 0;
+  for (size_t b = 0; b < lens.size(); ++b) {
+    const long long len = lens[b];
+    long long n0 = 0;
+    while (n0 < len) {
+      // the unit in progress is full: by cost, by items or by pages
+      bool opens = units == 0 || done * U >= whole * units || unit_items >= MAX_UNIT_ITEMS || unit_pages >= MAX_UNIT_PAGES;
+      if (n0 == 0 && whole * units - done * U < slack * U) opens = true;
+      if (opens) {
+        ++units;
+        unit_pages = unit_items = 0;
+      }
+      // (an item begins at a multiple of 64, so inside a page of 128 or 256)
+      long long room = (MAX_UNIT_PAGES - unit_pages) * static_cast<long long>(ps) - n0 % ps;
+      room = std::min(room, cap) / 64 * 64;
+      if (room < 64) {  // no room for a block: the next unit takes it
+        unit_pages = MAX_UNIT_PAGES;
+        continue;
+      }
+      done += n0 == 0 ? ITEM_COST : 0;
+      // the first 64-key boundary at which the unit has its share, or the end
+      const long long share = (whole * units + U - 1) / U - done;  // keys that the unit still wants
+      long long n1 = share > 0 ? (n0 + share + 63) / 64 * 64 : n0 + 64;
+      if (len - n1 < slack) n1 = len;
+      if (n1 - n0 > room) n1 = n0 + room;
+      out.push_back({static_cast<int>(b), n0, n1, opens});
+      unit_pages += (n1 - 1) / ps - n0 / ps + 1;
+      ++unit_items;
+      done += n1 - n0;
+      n0 = n1;
+    }
+  }
+  return out;
+}
+
+// U fills the slots (two resident CTAs per SM, over the kv heads) in as few waves as
+// the units' limits allow, with at least min_chunk_keys (64) keys per item.
 int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_host, int32_t items_capacity,
                int32_t* item_indptr_host, AtfDecodePlan* out) {
   const int B = p->batch_size, ps = p->page_size;
-  long long cap = static_cast<long long>(MAX_UNIT_PAGES) * ps;  // keys of an item
-  if (cap > 16384) cap = 16384;
+  const long long unit_cap = std::min(MAX_UNIT_PAGES * static_cast<long long>(ps), 16384ll);
+  long long cap = unit_cap;  // keys of an item
   if (p->max_chunk_keys > 0 && p->max_chunk_keys < cap) cap = p->max_chunk_keys;
-  cap = cap / 64 * 64;
-  if (cap < 64) cap = 64;
-  const long long min_keys = p->min_chunk_keys > 64 ? p->min_chunk_keys : 64;
-  constexpr long long ITEM_COST = 288;  // keys in whose time an item starts and writes its state (2.8 us measured)
+  cap = std::max(cap / 64 * 64, 64ll);
+  const long long min_keys = p->min_chunk_keys > 64 ? std::min((p->min_chunk_keys + 63ll) / 64 * 64, cap) : 64;
   std::vector<long long> lens(static_cast<size_t>(B));
-  long long whole = 0, keys = 0;
+  long long whole = 0, keys = 0, pieces = 0, most = 0;  // pieces: the most that are worth an item
   for (int b = 0; b < B; ++b) {
     const int np = p->indptr_host[b + 1] - p->indptr_host[b];
     const long long len = np > 0 ? static_cast<long long>(np - 1) * ps + p->last_page_len_host[b] : 0;
     lens[static_cast<size_t>(b)] = len;
     if (len > 0) whole += len + ITEM_COST;
     keys += len;
+    most = std::max(most, len);
+    pieces += (len + min_keys - 1) / min_keys;
   }
-  long long per_wave = slots / p->num_kv_heads;
-  if (per_wave < 1) per_wave = 1;
-  const long long unit_cap = MAX_UNIT_PAGES * static_cast<long long>(ps) < 16384 ? MAX_UNIT_PAGES * static_cast<long long>(ps) : 16384;
-  long long waves = (keys + per_wave * unit_cap - 1) / (per_wave * unit_cap);
-  long long U = per_wave * (waves < 1 ? 1 : waves);
-  if (U > (keys + min_keys - 1) / min_keys) U = (keys + min_keys - 1) / min_keys;
-  if (U < 1) U = 1;
-  int n = 0, units = 0;
-  long long longest = 0, done = 0;       // cost of everything cut so far
-  long long unit_pages = 0, unit_items = 0;
-  bool open = false;
-  for (int b = 0; b < B; ++b) {
-    const long long len = lens[static_cast<size_t>(b)];
-    if (item_indptr_host != nullptr) item_indptr_host[b] = n;
-    long long n0 = 0;
-    while (n0 < len) {
-      // the unit in progress is full: by cost, by items or by pages
-      if (!open || done * U >= whole * units || unit_items >= MAX_UNIT_ITEMS || unit_pages >= MAX_UNIT_PAGES) {
-        if (items_host != nullptr) {
-          if (units >= items_capacity) return ATF_ERR_WORKSPACE;
-          items_host[4 * units + 3] = n + 1;
-        }
-        ++units;
-        unit_pages = unit_items = 0;
-        open = true;
-      }
-      done += n0 == 0 ? ITEM_COST : 0;
-      // the first 64-key boundary at which the unit has its share, or the end
-      long long room = (MAX_UNIT_PAGES - unit_pages) * static_cast<long long>(ps);
-      // (an item begins at a multiple of 64, so inside a page of 128 or 256)
-      room -= n0 % ps;
-      if (room > cap) room = cap;
-      room = room / 64 * 64;
-      const long long share = (whole * units + U - 1) / U - done;  // keys that the unit still wants
-      long long n1 = share > 0 ? (n0 + share + 63) / 64 * 64 : n0 + 64;
-      if (n1 > len) n1 = len;
-      if (room < 64) {  // no room for a block: the next unit takes it
-        unit_pages = MAX_UNIT_PAGES;
-        done -= n0 == 0 ? ITEM_COST : 0;
-        continue;
-      }
-      if (n1 - n0 > room) n1 = n0 + room;
-      if (items_host != nullptr) {
-        if (n >= items_capacity) return ATF_ERR_WORKSPACE;
-        items_host[4 * n + 0] = b;
-        items_host[4 * n + 1] = static_cast<int32_t>(n0);
-        items_host[4 * n + 2] = static_cast<int32_t>(n1);
-      }
-      unit_pages += (n1 - 1) / ps - n0 / ps + 1;
-      ++unit_items;
-      done += n1 - n0;
-      longest = n1 - n0 > longest ? n1 - n0 : longest;
-      n0 = n1;
-      ++n;
+  const long long per_wave = std::max(slots / p->num_kv_heads, 1ll);
+  const long long waves = std::max((keys + per_wave * unit_cap - 1) / (per_wave * unit_cap), 1ll);
+  const long long U = std::max(std::min(per_wave * waves, pieces), 1ll);
+  std::vector<Piece> cut = cut_in_units(lens, U, whole, cap, ps);
+  // Where the requests fit one wave as units of one item: the smallest such items,
+  // taken where they end sooner (30 requests of 3 keys 50 -> 9.1 us, 50 of up to 300
+  // keys 14.4 -> 11.0, 3 of up to 300 10.5 -> 8.2).
+  auto items_of = [&](long long chunk) {
+    long long n = 0;
+    for (const long long len : lens) n += (len + chunk - 1) / chunk;
+    return n;
+  };
+  if (items_of(cap) <= per_wave) {
+    long long lo = min_keys / 64, hi = cap / 64;  // in blocks of 64 keys; hi fits
+    while (lo < hi) {
+      const long long mid = (lo + hi) / 2;
+      if (items_of(mid * 64) <= per_wave) hi = mid; else lo = mid + 1;
     }
+    if (std::min(hi * 64, most) + ITEM_COST < longest_unit(cut)) cut = cut_evenly(lens, hi * 64);
+  }
+  const long long n = static_cast<long long>(cut.size());
+  if (items_host != nullptr && n > items_capacity) return ATF_ERR_WORKSPACE;
+  long long longest = 0, units = 0;
+  int b = 0;  // offsets up to here are written
+  for (long long i = 0; i < n; ++i) {
+    const Piece& c = cut[static_cast<size_t>(i)];
+    longest = std::max(longest, c.k1 - c.k0);
+    if (item_indptr_host != nullptr)
+      for (; b <= c.b; ++b) item_indptr_host[b] = static_cast<int32_t>(i);
+    if (items_host == nullptr) continue;
+    items_host[4 * i + 0] = c.b;
+    items_host[4 * i + 1] = static_cast<int32_t>(c.k0);
+    items_host[4 * i + 2] = static_cast<int32_t>(c.k1);
+    if (c.opens) items_host[4 * units++ + 3] = static_cast<int32_t>(i + 1);
   }
   if (items_host != nullptr)
-    for (int i = units; i < n; ++i) items_host[4 * i + 3] = -1;
-  if (item_indptr_host != nullptr) item_indptr_host[B] = n;
-  out->num_items = n;
+    for (; units < n; ++units) items_host[4 * units + 3] = -1;
+  if (item_indptr_host != nullptr)
+    for (; b <= B; ++b) item_indptr_host[b] = static_cast<int32_t>(n);
+  out->num_items = static_cast<int32_t>(n);
   out->chunk_keys = static_cast<int32_t>(longest);
   out->partial_o_floats = static_cast<int64_t>(n) * p->num_qo_heads * ATF_HEAD_DIM;
   out->partial_lse_floats = static_cast<int64_t>(n) * p->num_qo_heads;
@@ -792,6 +847,7 @@ extern "C" int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* 
     a.ss_head = sc->stride_head;
     a.num_pages = p->num_pages;
     a.Hq = p->num_qo_heads;
+    a.Hkv = p->num_kv_heads;
     a.G = G;
     a.page_size = ps;
     a.page_shift = 0;
@@ -823,7 +879,9 @@ extern "C" int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* 
                       : (win ? decode8::decode_e4m3_kernel<1, true> : decode8::decode_e4m3_kernel<1, false>);
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, decode8::SMEM_BYTES) != cudaSuccess)
       return ATF_ERR_CUDA;
-    const dim3 grid(static_cast<unsigned>(p->num_items), static_cast<unsigned>(p->num_kv_heads));
+    const long long blocks = static_cast<long long>(p->num_items) * p->num_kv_heads;
+    if (blocks > INT_MAX) return ATF_ERR_UNSUPPORTED;
+    const dim3 grid(static_cast<unsigned>(blocks));
     if (launch_pdl(kern, grid, decode8::THREADS, decode8::SMEM_BYTES, st, p->enable_pdl != 0, tk, tv, a) !=
         cudaSuccess)
       return ATF_ERR_CUDA;

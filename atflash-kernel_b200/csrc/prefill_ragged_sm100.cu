@@ -626,7 +626,11 @@ extern "C" int atf_prefill_ragged_plan(const AtfPrefillRaggedPlanParams* p, int3
     Item it;
   };
   std::vector<Planned> all;
-  all.reserve(static_cast<size_t>(n));
+  try {
+    all.reserve(static_cast<size_t>(n));
+  } catch (...) {  // no host memory for the schedule
+    return ATF_ERR_WORKSPACE;
+  }
   for (int b = 0; b < p->batch_size; ++b) {
     Planned x = {};
     x.it.q_beg = p->qo_indptr_host[b];

@@ -157,6 +157,21 @@ def test_units_share_ragged_requests_evenly():
     assert max(cost) <= sum(cost) / units + 64 + 288 and min(cost[:-1]) >= sum(cost) / units - 64 - 288
 
 
+@pytest.mark.parametrize("lens,hkv", [([3] * 30, 2), ([1], 1), ([300, 64, 1], 8), ([0, 65, 0, 1000], 4)])
+def test_units_of_few_keys_hold_one_item(lens, hkv):
+    """What fits one wave runs side by side, not one item after another."""
+    ffi, lib = _lib()
+    items, _ = _units(ffi, lib, lens, 32, hkv)
+    assert np.array_equal(items[:, 3], np.arange(1, len(items) + 1))
+    assert len(items) <= 2 * 148 // hkv and max(items[:, 2] - items[:, 1]) <= 64
+
+
+def test_units_do_not_begin_a_request_for_its_first_keys_only():
+    ffi, lib = _lib()
+    items, _ = _units(ffi, lib, [100] * 64, 16, 8)  # 37 units at once
+    assert len(items) == 64
+
+
 @pytest.mark.parametrize("seed", range(20))
 def test_ragged_items_cover_every_row_once(seed):
     ffi, lib = _lib()
