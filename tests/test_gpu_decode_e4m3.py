@@ -119,6 +119,15 @@ def test_decode_e4m3_window_and_splits(page, hkv, group, chunk):
     _close(_run(cache, q, indptr, indices, last, page, hkv, "NHD", window_table=Z16, max_chunk_keys=chunk), want)
 
 
+@pytest.mark.parametrize("hkv,group", [(8, 1), (2, 8), (1, 11)])
+def test_decode_e4m3_many_short_requests(hkv, group):
+    """More rows than the split merge's blocks fill at once, empty requests among them."""
+    g = np.random.default_rng(hkv)
+    lens = [int(x) for x in g.integers(0, 90, 180)] + [0, 1500]
+    cache, q, indptr, indices, last = _setup(lens, 16, hkv, group, "NHD", 5)
+    _close(_run(cache, q, indptr, indices, last, 16, hkv, "NHD"), _exact(cache, q, indptr, indices, lens, "NHD"))
+
+
 def test_decode_e4m3_positions_and_layouts():
     """Explicit positions move the window; without one the pair order is free."""
     lens = [600, 33]
