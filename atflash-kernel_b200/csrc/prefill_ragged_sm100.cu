@@ -8,9 +8,11 @@
 // quantised per (query tile, key tile) from the sequence's own first row and key.
 //
 // CTA = (block of 256 query rows of a sequence, query head). The plan lists the blocks
-// of all sequences by falling key count; the grid walks kv heads, then blocks, then
-// the heads of the group, so that CTAs resident together share K and V in L2 and the
-// last ones are the shortest.
+// of all sequences by falling key count. Where K and V of all heads fit L2 beside the
+// rest, the grid walks blocks, then heads: the longest start first and the last ones
+// are the shortest (one prompt of 2500, 24 / 8 heads, 65 -> 45 us; of 8000 383 -> 350).
+// Else it walks kv heads, then blocks, then the heads of the group, so that CTAs
+// resident together share K and V in L2 (both ways within 3% at 100 MB and more).
 //
 // What bounds it: a step of two query tiles against a key tile takes 1.65 us (1.5 where
 // the window leaves half of K; exponentials and tensor work, as in the dense kernel),
@@ -104,7 +106,7 @@ struct Item {
 static_assert(sizeof(Item) == 32, "eight ints per item");
 
 struct Args {
-  int Hq, G;
+  int Hq, G, walk;
   float scale_log2;
   int causal, layout, window;
   int zhi[ATF_MAX_LEVELS];
@@ -144,11 +146,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   // This CTA's unit. Its loads are issued side by side: thread 0's of the error flag
   // does not hold up the barriers, and the barriers do not wait for the item.
-  const int per_head = a.n_items * a.G;
-  const int rem = static_cast<int>(blockIdx.x) % per_head;
-  const int hk = static_cast<int>(blockIdx.x) / per_head;
-  const int h = hk * a.G + rem % a.G;
-  const int4* src = reinterpret_cast<const int4*>(a.items) + 2 * (rem / a.G);
+  const int per_walk = a.n_items * a.walk;  // a walk over the items, with `walk` heads
+  const int rem = static_cast<int>(blockIdx.x) % per_walk;
+  const int h = static_cast<int>(blockIdx.x) / per_walk * a.walk + rem % a.walk;
+  const int hk = h / a.G;
+  const int4* src = reinterpret_cast<const int4*>(a.items) + 2 * (rem / a.walk);
   const int4 it0 = __ldg(src), it1 = __ldg(src + 1);
   int err0 = 0;
   if (threadIdx.x == 0 && a.err != nullptr) err0 = *reinterpret_cast<volatile int*>(a.err);
@@ -718,6 +720,8 @@ extern "C" int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_strea
   }
   Args a = {};
   a.Hq = static_cast<int>(p->num_heads_q);
+  const bool in_l2 = p->total_k * p->num_heads_kv * 512 <= (64ll << 20);
+  a.walk = in_l2 ? a.Hq : static_cast<int>(p->num_heads_q / p->num_heads_kv);
   a.G = static_cast<int>(p->num_heads_q / p->num_heads_kv);
   a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
   a.causal = p->causal ? 1 : 0;
