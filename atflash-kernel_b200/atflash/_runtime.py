@@ -59,6 +59,25 @@ def launch(name: str, fn, device: torch.device, *args) -> None:
         _ffi.check(name, rc)
 
 
+class PlanTensors:
+    """The device tensors of a plan. Runs use them on their own current stream, which
+    need not be the one they were allocated on: each stream is recorded with the
+    allocator, so that tensors dropped by a new plan are not handed out again before the
+    runs that read them have ended."""
+
+    def __init__(self, device: torch.device, *tensors: torch.Tensor):
+        self._idx, self._tensors, self._streams = device.index, tensors, set()
+
+    def use(self) -> None:
+        """Before a launch that reads the tensors on the current stream."""
+        raw = torch._C._cuda_getCurrentRawStream(self._idx)
+        if raw not in self._streams:
+            stream = torch.cuda.current_stream(self._idx)
+            for t in self._tensors:
+                t.record_stream(stream)
+            self._streams.add(raw)
+
+
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
     dev = None
     for t in tensors:

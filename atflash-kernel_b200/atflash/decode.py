@@ -174,6 +174,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
             "window": mode, "zhi16": zhi16, "zhi8": zhi8, "layout": _LAYOUTS[qk_layout],
             "kv_lens": kv_lens,
         }
+        self._held = _runtime.PlanTensors(dev, *(self._plan[k] for k in ("items", "item_indptr", "indptr", "indices",
+                                                                         "last_page_len")))
         # everything of the launch parameters that the plan fixes, filled once;
         # run() copies this template and sets the per-call pointers only
         P = self._plan
@@ -305,6 +307,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
         # table reads) overlaps the previous kernel on the stream; opt-in, since a
         # kernel that writes the page table must not directly precede the decode
         a.enable_pdl = 1 if enable_pdl else 0
+        self._held.use()
         if k_level_major:
             a.k_level_major = 1
             a.k_stride_page, a.k_stride_head, a.k_stride_level = kc.stride(0), kc.stride(1), kc.stride(2)
@@ -370,6 +373,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
                 setattr(a, name, pos.data_ptr())
         if enable_pdl:
             a.enable_pdl = 1
+        self._held.use()
         _runtime.launch("atf_decode_run_e4m3", _ffi.load().atf_decode_run_e4m3, dev, ctypes.byref(a),
                         ctypes.byref(scales))
         return (out, lse) if return_lse else out

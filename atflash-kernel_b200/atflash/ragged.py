@@ -67,6 +67,7 @@ class BatchPrefillWithRaggedKVCacheWrapper:
         _ffi.check("atf_prefill_ragged_plan", lib.atf_prefill_ragged_plan(
             ctypes.byref(pp), items.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), items.shape[0], ctypes.byref(n)))
         self._items = torch.from_numpy(items).to(self._dev)
+        self._held = _runtime.PlanTensors(self._dev, self._items)
         t = _ffi.AtfPrefillRaggedParams()
         t.total_q, t.total_k = int(cq[-1]), int(ck[-1])
         t.num_heads_q, t.num_heads_kv, t.head_dim = num_qo_heads, num_kv_heads, head_dim
@@ -124,6 +125,7 @@ class BatchPrefillWithRaggedKVCacheWrapper:
             p.k_stride_s, p.k_stride_h, _ = kst
             p.v_stride_s, p.v_stride_h, _ = vst
             p.o_stride_s, p.o_stride_h, _ = out.stride()
+            self._held.use()
             _runtime.launch("atf_prefill_ragged_fwd", _ffi.load().atf_prefill_ragged_fwd, dev, ctypes.byref(p))
         return (out, lse) if return_lse else out
 

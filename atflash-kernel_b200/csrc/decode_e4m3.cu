@@ -110,7 +110,7 @@ struct Args {
   const float* vs;
   long long ss_page, ss_head;
   long long num_pages;
-  int Hq, Hkv, G, page_size, page_shift, rows;
+  int B, Hq, Hkv, G, page_size, page_shift, rows;
   float scale_log2;
   int zhi16[ATF_MAX_LEVELS];
   float* part_o;
@@ -185,8 +185,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   const int n_items = (tag > 0 ? (next > 0 ? next - 1 : a.num_items) : x + 1) - it0;
   // Prologue, part 1: only the plan and the page table, which no kernel of this
   // step writes (it runs before the previous kernel's end under programmatic
-  // dependent launch). An item starts on a 64-key boundary and lies inside its
-  // request; the unit's pages fit the list. Else it is reported and skipped.
+  // dependent launch). An item names a request of the batch, starts on a 64-key
+  // boundary and lies inside its request; the unit's pages fit the list. Else it is
+  // reported and skipped.
   if (warp == 0) {
     int total = 0;
     bool bad = n_items < 1 || n_items > MAX_UNIT_ITEMS || it0 < 0 || it0 + n_items > a.num_items;
@@ -200,7 +201,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         m.b = row.x;
         m.k_beg = row.y;
         m.k_end = row.z;
-        const int pg0 = a.indptr[m.b], npages = a.indptr[m.b + 1] - pg0;
+        const bool known = m.b >= 0 && m.b < a.B;
+        const int pg0 = known ? a.indptr[m.b] : 0, npages = known ? a.indptr[m.b + 1] - pg0 : 0;
         const long long len =
             npages > 0 ? static_cast<long long>(npages - 1) * a.page_size + a.last_page_len[m.b] : 0;
         wrong = m.k_beg < 0 || m.k_end <= m.k_beg || (m.k_beg & 63) || m.k_end > len;
@@ -894,6 +896,7 @@ extern "C" int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* 
     a.ss_page = sc->stride_page;
     a.ss_head = sc->stride_head;
     a.num_pages = p->num_pages;
+    a.B = p->batch_size;
     a.Hq = p->num_qo_heads;
     a.Hkv = p->num_kv_heads;
     a.G = G;
