@@ -53,8 +53,11 @@ def build_page_tables(kv_lens: torch.Tensor, append_lens: torch.Tensor, req_page
 
     num_tokens and max_pages are the sizes of the token outputs and of indices: the
     step's totals, or capacities (a fixed shape for a CUDA graph): entries past the
-    end are -1. Bad lengths or rows, an exhausted free list and exceeded
-    capacities are reported by ``atflash.check_device_errors()`` (code 2)."""
+    end are -1. Bad lengths or rows, an exhausted free list, pages that req_pages should
+    hold but does not (negative entries) and exceeded capacities are reported by
+    ``atflash.check_device_errors()`` (code 2). A capacity cuts the lists only: req_pages
+    gets, and free_head counts, every new page of the step, so that the same call with
+    the same free_head and larger capacities completes it."""
     dev = _runtime.require_cuda(kv_lens, append_lens, req_pages)
     B = kv_lens.numel()
     if B < 1 or B > _ffi.ATF_TABLES_MAX_BATCH:

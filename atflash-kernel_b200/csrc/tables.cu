@@ -149,14 +149,15 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
   }
   for (int b = b0; b < b1; ++b) {  // each thread turns its own run into offsets
     const int n = s_page[b], app = s_tok[b];
-    s_page[b] = min(before[0], a.cap_pages);
+    s_page[b] = before[0];
     s_tok[b] = min(before[1], a.cap_tokens);
     s_new[b] = before[2];
     before[0] = add(before[0], n);
     before[1] = add(before[1], app);
     before[2] = add(before[2], n - s_have[b]);
   }
-  const int n_pages = min(total[0], a.cap_pages), n_tok = min(total[1], a.cap_tokens);
+  // pages past the list's capacity still go to their requests' rows: they are taken
+  const int all_pages = total[0], n_pages = min(all_pages, a.cap_pages), n_tok = min(total[1], a.cap_tokens);
   if (first_cta) {
     if (tid == 0) {
       a.indptr[a.B] = n_pages;
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
   __syncthreads();
   if (first_cta)
     for (int b = tid; b < a.B; b += THREADS) {
-      a.indptr[b] = s_page[b];
+      a.indptr[b] = min(s_page[b], a.cap_pages);
       a.aptr[b] = s_tok[b];
     }
 
@@ -180,16 +181,17 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
     const long long at = static_cast<long long>(head) + s_new[b] + (j - s_have[b]);
     return head >= 0 && at < a.F ? __ldg(a.free_pages + at) : -1;
   };
+  bool missing = false;  // a page that a request should hold is not in its row
   // A warp takes chunks of 128 entries, four per lane, whose loads are issued
   // together: searches for the chunk's ends, and from them short ones per entry.
   const int gw = static_cast<int>(blockIdx.x) * WARPS + warp, nw = static_cast<int>(gridDim.x) * WARPS;
-  const int page_chunks = (a.cap_pages + CHUNK - 1) / CHUNK, tok_chunks = (a.cap_tokens + CHUNK - 1) / CHUNK;
+  const int page_chunks = (max(a.cap_pages, all_pages) + CHUNK - 1) / CHUNK, tok_chunks = (a.cap_tokens + CHUNK - 1) / CHUNK;
   for (int ch = gw; ch < page_chunks; ch += nw) {
     const long long e0 = static_cast<long long>(ch) * CHUNK;
     int lo = 0, hi = 0;
-    if (e0 < n_pages) {
+    if (e0 < all_pages) {
       lo = bracket(s_page, 0, a.B, static_cast<int>(e0));
-      hi = bracket(s_page, lo, a.B, static_cast<int>(min(e0 + CHUNK, static_cast<long long>(n_pages)) - 1)) + 1;
+      hi = bracket(s_page, lo, a.B, static_cast<int>(min(e0 + CHUNK, static_cast<long long>(all_pages)) - 1)) + 1;
     }
     int id[PER_LANE];
     int32_t* put[PER_LANE];
@@ -198,13 +200,14 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
       const long long e = e0 + 32 * k + lane;
       id[k] = -1;
       put[k] = nullptr;
-      if (e < n_pages) {
+      if (e < all_pages) {
         const int b = bracket(s_page, lo, hi, static_cast<int>(e));
         const int j = static_cast<int>(e) - s_page[b];
         const long long row = a.req_rows != nullptr ? __ldg(a.req_rows + b) : b;
         int32_t* at = a.req_pages + row * a.req_stride + j;
         if (j < s_have[b]) {
           id[k] = *at;
+          missing |= id[k] < 0;
         } else {
           id[k] = new_page(b, j);
           put[k] = at;
@@ -218,6 +221,7 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
       if (e < a.cap_pages) a.indices[e] = id[k];
     }
   }
+  if (missing && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
   // (tokens go to the last warps first, which have the fewest chunks of pages)
   for (int ch = nw - 1 - gw; ch < tok_chunks; ch += nw) {
     const long long t0 = static_cast<long long>(ch) * CHUNK;

@@ -484,8 +484,12 @@ typedef struct {
  * launch without a host synchronisation. A request with a negative length, more
  * new tokens than tokens, more than max_req_pages pages or a row out of range
  * counts as empty; a page that the free list cannot give is -1, as are its slots;
- * pages and tokens past a capacity are cut off. Each of these sets *error_flag
- * to 2. Requests of one call use different rows. */
+ * entries past a capacity are cut off the lists (indices, or the token outputs).
+ * The rows of req_pages and *free_head_out do not depend on the capacities: a step
+ * whose lists were cut has taken all its pages, and the same call with the same
+ * *free_head and larger capacities gives the whole lists. Each of these, and a page
+ * that a request should hold already but whose entry is negative, sets *error_flag to
+ * 2. Requests of one call use different rows. */
 int atf_build_page_tables(const AtfPageTablesParams* p, atf_stream_t stream);
 
 /* ------------------------------------------------------------------ e4m3 paged cache */
