@@ -31,8 +31,11 @@ def error_flag_ptr(device: torch.device) -> int:
 def check_device_errors(device=None) -> int:
     """Synchronise `device`, return (and clear) its kernel error flag.
 
-    Non-zero means a bounded device wait expired and a kernel returned early;
-    its outputs are not valid."""
+    2 is an index report: a call left out lengths, pages, rows or items that do not fit
+    (its documentation says which); later calls run as ever. Any other non-zero
+    value means that a bounded device wait expired and a kernel returned early: its
+    outputs are not valid, nor are those of attention calls since, which return
+    without computing until this function clears the flag."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     flag = error_flag(dev)
     out = ctypes.c_int(0)

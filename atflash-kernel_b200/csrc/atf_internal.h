@@ -11,7 +11,8 @@ namespace atf {
 
 // Error code a bounded device wait writes to the caller's error flag.
 constexpr int kDevErrTimeout = 1;
-// Error code the paged-KV append writes for a token whose page index is out of range.
+// Error code for indices out of range: lengths, pages, rows or items of a call that its
+// kernel reports and leaves out.
 constexpr int kDevErrIndex = 2;
 
 // Encodes a tiled TMA descriptor through the driver entry point (loaded once).

@@ -7,6 +7,8 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include "atf_internal.h"
+
 namespace atf {
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -49,6 +51,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // limit records `code` in the caller's device error flag and in shared memory;
 // every later wait in the CTA (and in CTAs that start afterwards and see the
 // global flag) returns false at once, so the kernel drains instead of hanging.
+// An index report in the flag is about the arguments of one call, an ordinary
+// event for an engine (a free list that ran out): it stops no kernel.
 struct AbortCtl {
   volatile int* smem_flag;
   int* gflag;  // may be null
@@ -56,9 +60,20 @@ struct AbortCtl {
 
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s per wait
 
+// whether a kernel that finds this flag at its start returns at once
+__device__ __forceinline__ bool stops(const int* gflag) {
+  if (gflag == nullptr) return false;
+  const int v = *reinterpret_cast<const volatile int*>(gflag);
+  return v != 0 && v != kDevErrIndex;
+}
+// a wait that ran out, in place of an index report if there is one
+__device__ __forceinline__ void record_wait(int* gflag, int code) {
+  if (gflag != nullptr) atomicExch(gflag, code);
+}
+
 __device__ __forceinline__ bool aborted(const AbortCtl& a) {
   if (*a.smem_flag) return true;
-  if (a.gflag != nullptr && *reinterpret_cast<volatile int*>(a.gflag) != 0) {
+  if (a.gflag != nullptr && *reinterpret_cast<volatile int*>(a.gflag) == kDevErrTimeout) {
     *a.smem_flag = 1;
     return true;
   }
@@ -74,7 +89,7 @@ static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity
       if (aborted(a)) return false;
       if (globaltimer_ns() - t0 > kWaitLimitNs) {
         *a.smem_flag = 1;
-        if (a.gflag != nullptr) atomicCAS(a.gflag, 0, code);
+        record_wait(a.gflag, code);
         return false;
       }
     }
@@ -101,7 +116,7 @@ __device__ __forceinline__ bool mbar_wait_inl(uint32_t bar, uint32_t parity, con
       if (aborted(a)) return false;
       if (globaltimer_ns() - t0 > kWaitLimitNs) {
         *a.smem_flag = 1;
-        if (a.gflag != nullptr) atomicCAS(a.gflag, 0, code);
+        record_wait(a.gflag, code);
         return false;
       }
     }

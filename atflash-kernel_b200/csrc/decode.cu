@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   const int hq0 = hk * G;
   const int nst = (k_end - k_beg + STAGE_KEYS - 1) / STAGE_KEYS;
   if (tid == 0) {
-    *s_abort = (args.err != nullptr && *reinterpret_cast<volatile int*>(args.err) != 0) ? 1 : 0;
+    *s_abort = stops(args.err) ? 1 : 0;
     for (int s = 0; s < NSTAGE_MAX; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), CONSUMERS);

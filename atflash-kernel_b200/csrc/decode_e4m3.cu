@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     }
     if (lane == 0) {
       *s_total = bad ? -1 : total;
-      *s_abort = (a.err != nullptr && *reinterpret_cast<volatile int*>(a.err) != 0) ? 1 : 0;
+      *s_abort = stops(a.err) ? 1 : 0;
       if (bad && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
       for (int s = 0; s < NSTAGE; ++s) {
         mbar_init(full_bar(s), 1);

@@ -192,7 +192,7 @@ static __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const Ar
       for (int q = 0; q < a.P; ++q) {
         while (ld_acquire_sys_u64(a.wait_flags + q) < target) {
           if (globaltimer_ns() - t0 > kWaitLimitNs) {
-            if (a.err != nullptr) atomicCAS(a.err, 0, kDevErrTimeout);
+            record_wait(a.err, kDevErrTimeout);
             break;
           }
         }
@@ -320,7 +320,7 @@ static __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_exchange_kernel
       if (q == x.rank) continue;
       while (ld_acquire_sys_u64(flags + q) < target) {
         if (globaltimer_ns() - t0 > kWaitLimitNs) {
-          if (x.err != nullptr) atomicCAS(x.err, 0, kDevErrTimeout);
+          record_wait(x.err, kDevErrTimeout);
           break;
         }
       }

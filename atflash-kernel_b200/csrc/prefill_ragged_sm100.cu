@@ -152,8 +152,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int hk = h / a.G;
   const int4* src = reinterpret_cast<const int4*>(a.items) + 2 * (rem / a.walk);
   const int4 it0 = __ldg(src), it1 = __ldg(src + 1);
-  int err0 = 0;
-  if (threadIdx.x == 0 && a.err != nullptr) err0 = *reinterpret_cast<volatile int*>(a.err);
+  const bool stop0 = threadIdx.x == 0 && stops(a.err);
   if (threadIdx.x == 0) {
     mbar_init(bar(B_Q), 1);
     for (int s = 0; s < KST; ++s) {
@@ -197,7 +196,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                    static_cast<long long>(it0.z) + it0.w > a.total_k;
   const int row_end = bad ? 0 : it0.y;
   if (threadIdx.x == 0) {
-    *s_abort = err0 != 0 ? 1 : 0;
+    *s_abort = stop0 ? 1 : 0;
     if (bad && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
   }
   int row0[NQ], nk[NQ];

@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   for (int t = 0; t < NQ; ++t) window_limits(a, row0[t], lim[t]);
 
   if (threadIdx.x == 0) {
-    *s_abort = (a.err != nullptr && *reinterpret_cast<volatile int*>(a.err) != 0) ? 1 : 0;
+    *s_abort = stops(a.err) ? 1 : 0;
     // Q arrives by TMA (one expect_tx arrival), or rotated by the softmax threads
     mbar_init(bar(B_Q), a.qrot ? NQ * 128 : 1);
     for (int s = 0; s < KST; ++s) {

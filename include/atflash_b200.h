@@ -19,7 +19,10 @@
  *  - head_dim is 128. GQA group sizes 1..16 (1/2/3/4/7/8 are the tested ones).
  *  - Device-side waits are bounded. A wait that expires writes a non-zero code
  *    to params->error_flag (if not NULL) and the kernel returns early; read it
- *    with atf_read_error_flag() after synchronising.
+ *    with atf_read_error_flag() after synchronising. Until it is cleared, attention
+ *    kernels given that flag return without computing. Code 2 is an index report
+ *    (lengths, pages, rows or items that a call left out): it stops no kernel, and a
+ *    wait that expires replaces it.
  *
  * Reference interfaces each entry point replaces (paths inside the reference
  * project):
@@ -520,7 +523,7 @@ int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvScales* s, atf
  * sizes 16, 32, 64, 128 and 256; window off (either pair order) or 16-snap over
  * sorted pairs; no level-major K: anything else is ATF_ERR_UNSUPPORTED. A scale
  * may be any non-negative number. A page id outside the cache is not read and sets
- * *error_flag to 2 (the call's outputs are not valid then). */
+ * *error_flag to 2 (the outputs of that request are not valid then). */
 int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* s, atf_stream_t stream);
 
 /* ------------------------------------------------------------------ misc */
