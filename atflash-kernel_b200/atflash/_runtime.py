@@ -62,6 +62,14 @@ def launch(name: str, fn, device: torch.device, *args) -> None:
         _ffi.check(name, rc)
 
 
+def narrow_i32(t: torch.Tensor, device: torch.device, top: int = 0x7fffffff) -> torch.Tensor:
+    """An index tensor as contiguous int32 on `device`. 64-bit values that do not fit
+    become -1 or `top`, which the kernels report, instead of another valid index."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-1, top)
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
 class PlanTensors:
     """The device tensors of a plan. Runs use them on their own current stream, which
     need not be the one they were allocated on: each stream is recorded with the

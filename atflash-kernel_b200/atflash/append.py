@@ -59,10 +59,10 @@ def check_e4m3_cache(kc: torch.Tensor, vc: torch.Tensor, kv_scales, kv_layout: s
     return size, strides, _ffi.AtfKvScales(ks.data_ptr(), vs.data_ptr(), ss[0], ss[1])
 
 
-def _dev_i32(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+def _dev_i32(t: torch.Tensor, dev: torch.device, top: int = 0x7fffffff) -> torch.Tensor:
     if t.dtype == torch.int32 and t.device == dev and t.is_contiguous():
         return t
-    return t.to(device=dev, dtype=torch.int32).contiguous()
+    return _runtime.narrow_i32(t, dev, top)
 
 
 def _append_e4m3(k: torch.Tensor, v: torch.Tensor, batch_indices, positions, kc, vc, kv_indices, kv_indptr, kv_layout,
@@ -79,7 +79,7 @@ def _append_e4m3(k: torch.Tensor, v: torch.Tensor, batch_indices, positions, kc,
         raise ValueError("append_key heads do not match the cache")
     layout = _LAYOUTS[out_layout]
     bi, ps = _dev_i32(batch_indices, dev), _dev_i32(positions, dev)
-    ip, ix = _dev_i32(kv_indptr, dev), _dev_i32(kv_indices, dev)
+    ip, ix = _dev_i32(kv_indptr, dev, kv_indices.numel()), _dev_i32(kv_indices, dev)
     if bi.numel() != nnz or ps.numel() != nnz:
         raise ValueError("batch_indices and positions need one entry per appended token")
     if nnz == 0:
@@ -164,7 +164,7 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
     if hk2 != hkv:
         raise ValueError("append_key heads do not match the cache")
     bi, ps = _dev_i32(batch_indices, dev), _dev_i32(positions, dev)
-    ip, ix = _dev_i32(kv_indptr, dev), _dev_i32(kv_indices, dev)
+    ip, ix = _dev_i32(kv_indptr, dev, kv_indices.numel()), _dev_i32(kv_indices, dev)
     if bi.numel() != nnz or ps.numel() != nnz:
         raise ValueError("batch_indices and positions need one entry per appended token")
     p = _ffi.AtfAppendParams()

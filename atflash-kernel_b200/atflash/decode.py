@@ -167,7 +167,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
             "items": torch.from_numpy(items).to(dev, non_blocking=False),
             "item_indptr": torch.from_numpy(item_indptr).to(dev),
             "indptr": torch.from_numpy(indptr_h).to(dev),
-            "indices": idx_dev.to(device=dev, dtype=torch.int32).contiguous(),
+            "indices": _runtime.narrow_i32(idx_dev, dev),
             "last_page_len": torch.from_numpy(lpl_h).to(dev),
             "po_floats": plan.partial_o_floats, "pl_floats": plan.partial_lse_floats,
             "sm_scale": float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim),

@@ -33,7 +33,7 @@ def _i32(t: torch.Tensor, name: str, n: Optional[int] = None) -> torch.Tensor:
     if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or (n is not None and t.numel() != n):
         raise ValueError(f"{name} must be a 1-d integer tensor" + (f" of {n} entries" if n is not None else ""))
     if t.dtype != torch.int32 or not t.is_contiguous():
-        t = t.to(torch.int32).contiguous()
+        t = _runtime.narrow_i32(t, t.device)
     return t
 
 
