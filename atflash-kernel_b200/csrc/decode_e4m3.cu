@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         const long long at = static_cast<long long>(it0 + i) * a.Hq + hq0 + rw;
         *reinterpret_cast<float4*>(a.part_o + at * 128 + pass * DP + d) =
             make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
-        if (pass == 0 && d == 0) a.part_lse[at] = L > 0.f ? ms + log2f(L) : -INFINITY;
+        if (pass == 0 && d == 0) a.part_lse[at] = L == 0.f ? -INFINITY : ms + log2f(L);  // NaN stays
       }
     }
   }
@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) merge_rows_kernel(const merge:
   const float inv = L > 0.f ? 1.0f / L : 0.f;
   merge::store_row(a.out, static_cast<long long>(b) * a.o_sb + static_cast<long long>(h) * a.o_sh, a.out_f32, a.lse_out,
                    row, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv),
-                   L > 0.f ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY);
+                   L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f);
 }
 
 // keys in whose time an item starts and writes its state (2.8 us measured)

@@ -64,7 +64,7 @@ __device__ __forceinline__ void st_release_sys_u64(unsigned long long* p, unsign
 // pl[lb + i * sl] (log2 when lse_log2, else natural log) and its O at
 // po + ob + i * so. Every thread of the block calls it; the result is in warp
 // 0: lane l holds O dims 4l..4l+3 (normalised) in *o, and *lse is the row's
-// LSE (natural log; -inf when no part has weight).
+// LSE (natural log; -inf when no part has weight, NaN when a part's is).
 __device__ __forceinline__ void merge_row(const float* po, const float* pl, long long lb, long long sl,
                                           long long ob, long long so, int n, int lse_log2, float4* o,
                                           float* lse) {
@@ -137,7 +137,7 @@ __device__ __forceinline__ void merge_row(const float* po, const float* pl, long
     }
     const float inv = L > 0.f ? 1.0f / L : 0.f;
     *o = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-    *lse = L > 0.f ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY;
+    *lse = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
   }
 }
 
