@@ -718,14 +718,27 @@ long long longest_unit(const std::vector<Piece>& pieces) {
   return most;
 }
 
-// Requests cut into items of at most `chunk` keys, each a unit.
-std::vector<Piece> cut_evenly(const std::vector<long long>& lens, long long chunk) {
+// Keys of the next item of a request with `left` keys, where `want` (a multiple of 64,
+// at most room) would do for the balance: an item holds at least min_keys, and leaves as
+// many to the next one or none, as far as the request and `room` allow. (At the least
+// min_keys, 64, a last item may be shorter.)
+long long item_keys(long long left, long long want, long long room, long long min_keys) {
+  const long long n = std::min(std::max(want, min_keys), room);
+  if (left <= n) return left;
+  if (min_keys <= 64 || left - n >= min_keys) return n;
+  if (left <= room) return left;
+  const long long less = (left - min_keys) / 64 * 64;
+  return less >= min_keys ? less : n;
+}
+
+// Requests cut into items of about `chunk` keys, each a unit.
+std::vector<Piece> cut_evenly(const std::vector<long long>& lens, long long chunk, long long cap, long long min_keys) {
   std::vector<Piece> out;
-  for (size_t b = 0; b < lens.size(); ++b) {
-    const long long n = (lens[b] + chunk - 1) / chunk;
-    for (long long i = 0; i < n; ++i)
-      out.push_back({static_cast<int>(b), i * chunk, std::min(lens[b], (i + 1) * chunk), true});
-  }
+  for (size_t b = 0; b < lens.size(); ++b)
+    for (long long n0 = 0, n; n0 < lens[b]; n0 += n) {
+      n = item_keys(lens[b] - n0, chunk, cap, min_keys);
+      out.push_back({static_cast<int>(b), n0, n0 + n, true});
+    }
   return out;
 }
 
@@ -734,7 +747,8 @@ std::vector<Piece> cut_evenly(const std::vector<long long>& lens, long long chun
 // to (u + 1) / U of the whole. An item costs a
 // start of its own, so a request is not begun for the last keys that a unit wants, nor
 // are its own last ones left to the next unit, up to `slack` keys.
-std::vector<Piece> cut_in_units(const std::vector<long long>& lens, long long U, long long whole, long long cap, int ps) {
+std::vector<Piece> cut_in_units(const std::vector<long long>& lens, long long U, long long whole, long long cap,
+                                long long min_keys, int ps) {
   const long long slack = std::min(ITEM_COST / 2, whole / (2 * U));
   std::vector<Piece> out;
   long long units = 0, done = 0;  // done: cost of everything cut so far
@@ -753,28 +767,31 @@ std::vector<Piece> cut_in_units(const std::vector<long long>& lens, long long U,
       // (an item begins at a multiple of 64, so inside a page of 128 or 256)
       long long room = (MAX_UNIT_PAGES - unit_pages) * static_cast<long long>(ps) - n0 % ps;
       room = std::min(room, cap) / 64 * 64;
-      if (room < 64) {  // no room for a block: the next unit takes it
+      const long long left = len - n0, start = n0 == 0 ? ITEM_COST : 0;
+      // the first 64-key boundary at which the unit has its share, or the end
+      const long long share = (whole * units + U - 1) / U - done - start;  // keys that the unit still wants
+      long long n = std::max((share + 63) / 64 * 64, min_keys);
+      if (left - n < slack) n = left;
+      n = item_keys(left, n, room, min_keys);
+      // no room for a block, or for items of min_keys: the next unit takes it
+      const bool cramped = min_keys > 64 && unit_items > 0 && (n < std::min(min_keys, left) || (n < left && left - n < min_keys));
+      if (room < 64 || cramped) {
         unit_pages = MAX_UNIT_PAGES;
         continue;
       }
-      done += n0 == 0 ? ITEM_COST : 0;
-      // the first 64-key boundary at which the unit has its share, or the end
-      const long long share = (whole * units + U - 1) / U - done;  // keys that the unit still wants
-      long long n1 = share > 0 ? (n0 + share + 63) / 64 * 64 : n0 + 64;
-      if (len - n1 < slack) n1 = len;
-      if (n1 - n0 > room) n1 = n0 + room;
-      out.push_back({static_cast<int>(b), n0, n1, opens});
-      unit_pages += (n1 - 1) / ps - n0 / ps + 1;
+      out.push_back({static_cast<int>(b), n0, n0 + n, opens});
+      unit_pages += (n0 + n - 1) / ps - n0 / ps + 1;
       ++unit_items;
-      done += n1 - n0;
-      n0 = n1;
+      done += start + n;
+      n0 += n;
     }
   }
   return out;
 }
 
 // U fills the slots (two resident CTAs per SM, over the kv heads) in as few waves as
-// the units' limits allow, with at least min_chunk_keys (64) keys per item.
+// the units' limits allow, with at least min_chunk_keys (64) keys per item where its
+// request has them.
 int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_host, int32_t items_capacity,
                int32_t* item_indptr_host, AtfDecodePlan* out) {
   const int B = p->batch_size, ps = p->page_size;
@@ -784,20 +801,19 @@ int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_hos
   cap = std::max(cap / 64 * 64, 64ll);
   const long long min_keys = p->min_chunk_keys > 64 ? std::min((p->min_chunk_keys + 63ll) / 64 * 64, cap) : 64;
   std::vector<long long> lens(static_cast<size_t>(B));
-  long long whole = 0, keys = 0, pieces = 0, most = 0;  // pieces: the most that are worth an item
+  long long whole = 0, keys = 0, pieces = 0;  // pieces: the most that are worth an item
   for (int b = 0; b < B; ++b) {
     const int np = p->indptr_host[b + 1] - p->indptr_host[b];
     const long long len = np > 0 ? static_cast<long long>(np - 1) * ps + p->last_page_len_host[b] : 0;
     lens[static_cast<size_t>(b)] = len;
     if (len > 0) whole += len + ITEM_COST;
     keys += len;
-    most = std::max(most, len);
     pieces += (len + min_keys - 1) / min_keys;
   }
   const long long per_wave = std::max(slots / p->num_kv_heads, 1ll);
   const long long waves = std::max((keys + per_wave * unit_cap - 1) / (per_wave * unit_cap), 1ll);
   const long long U = std::max(std::min(per_wave * waves, pieces), 1ll);
-  std::vector<Piece> cut = cut_in_units(lens, U, whole, cap, ps);
+  std::vector<Piece> cut = cut_in_units(lens, U, whole, cap, min_keys, ps);
   // Where the requests fit one wave as units of one item: the smallest such items,
   // taken where they end sooner (30 requests of 3 keys 50 -> 9.1 us, 50 of up to 300
   // keys 14.4 -> 11.0, 3 of up to 300 10.5 -> 8.2).
@@ -812,7 +828,8 @@ int plan_units(const AtfDecodePlanParams* p, long long slots, int32_t* items_hos
       const long long mid = (lo + hi) / 2;
       if (items_of(mid * 64) <= per_wave) hi = mid; else lo = mid + 1;
     }
-    if (std::min(hi * 64, most) + ITEM_COST < longest_unit(cut)) cut = cut_evenly(lens, hi * 64);
+    std::vector<Piece> even = cut_evenly(lens, hi * 64, cap, min_keys);
+    if (longest_unit(even) < longest_unit(cut)) cut.swap(even);
   }
   const long long n = static_cast<long long>(cut.size());
   if (items_host != nullptr && n > items_capacity) return ATF_ERR_WORKSPACE;

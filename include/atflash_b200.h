@@ -194,7 +194,7 @@ typedef struct {
   const int32_t* indptr_host;        /* [batch+1] page ranges per request (host) */
   const int32_t* last_page_len_host; /* [batch] (host) */
   int32_t num_sms;        /* 0: query the current device */
-  int32_t min_chunk_keys; /* 0: default (256) */
+  int32_t min_chunk_keys; /* keys of an item where its request has them; 0: default (256; 64 with units) */
   int32_t max_chunk_keys; /* 0: unlimited; forces at least ceil(len/max) splits */
   /* Optional window of the run (ATF_WINDOW_SNAP16 with its zhi16 table): the
    * items are then cut to equal bytes read (V rows plus in-window K levels)
