@@ -450,6 +450,12 @@ extern "C" int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvSca
       (p->a_stride_n & 7) || (p->a_stride_h & 7) || (p->kv_stride_page & 15) || (p->kv_stride_token & 15) ||
       (p->kv_stride_head & 15))
     return ATF_ERR_ALIGNMENT;
+  // pages and scales are written: one element that stands for several (a broadcast
+  // axis) would take whichever task came last
+  if ((p->num_pages > 1 && (s->stride_page == 0 || p->kv_stride_page == 0)) ||
+      (p->num_kv_heads > 1 && (s->stride_head == 0 || p->kv_stride_head == 0)) ||
+      (p->page_size > 1 && p->kv_stride_token == 0))
+    return ATF_ERR_INVALID_ARG;
   if (p->nnz == 0) return ATF_OK;
   int dev = 0;
   int rc = check_device(&dev);

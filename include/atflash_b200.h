@@ -514,7 +514,8 @@ typedef struct {
  * at slot 0 sets the scale to want, any other to max(scale, want), and where that
  * is more than the scale was, the rows before the run are rounded again under
  * the new one. Rows are rounded to nearest even, saturating at 448 s. With RoPE the
- * rows of cos and sin are 16-byte aligned. */
+ * rows of cos and sin are 16-byte aligned. Pages and scales are written, so none of
+ * their strides is 0 over an axis longer than 1. */
 int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvScales* s, atf_stream_t stream);
 
 /* atf_decode_run over an e4m3 cache: k_cache / v_cache hold e4m3 bytes (strides
