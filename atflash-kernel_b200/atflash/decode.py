@@ -30,6 +30,14 @@ def _host_i32(t) -> np.ndarray:
     return np.asarray(t, dtype=np.int32).copy()
 
 
+def _check_e4m3_form(page: int, window: int, layout: int) -> None:
+    """What the decode over an e4m3 cache takes."""
+    if page not in (16, 32, 64, 128, 256):
+        raise NotImplementedError("an e4m3 cache has pages of 16, 32, 64, 128 or 256 tokens")
+    if window != _ffi.ATF_WINDOW_OFF and (window == _ffi.ATF_WINDOW_VEC8 or layout != _ffi.ATF_LAYOUT_SORTED_PAIR):
+        raise NotImplementedError("an e4m3 cache takes snap16 windows over sorted pairs")
+
+
 class BatchDecodeWithPagedKVCacheWrapper:
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD",
                  use_cuda_graph: bool = False, use_tensor_cores: bool = False,
@@ -77,7 +85,9 @@ class BatchDecodeWithPagedKVCacheWrapper:
         kv_len - 1 and 0). Under a snap16 window the work items are cut to equal
         bytes read at these distances; they steer the balance only, never the result.
         kv_data_type: torch.float8_e4m3fn lays the schedule out for an e4m3 cache: equal
-        shares for the SMs whatever the requests' lengths.
+        shares for the SMs whatever the requests' lengths. Such a cache has pages of 16,
+        32, 64, 128 or 256 tokens, and no window or a snap16 window over sorted pairs
+        (the append and the page tables take any page size).
         """
         if pos_encoding_mode != "NONE":
             raise NotImplementedError("RoPE is applied before the cache (pos_encoding_mode NONE)")
@@ -133,6 +143,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
                     raise ValueError("zhi levels must be non-negative and non-increasing")
                 zhi16[0] = max(zhi16[0], KERNEL_CAP)
                 mode = _ffi.ATF_WINDOW_SNAP16
+        if pp.units:
+            _check_e4m3_form(page_size, mode, _LAYOUTS[qk_layout])
         pp.window = mode
         for i in range(8):
             pp.zhi16[i] = zhi16[i]
@@ -334,11 +346,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
         (npages, page, hkv), strides, scales = check_e4m3_cache(kc, vc, kv_scales, self._kv_layout)
         if page != P["page_size"] or hkv != P["Hkv"]:
             raise ValueError("KV cache shape does not match the plan")
-        if page not in (16, 32, 64, 128, 256):
-            raise NotImplementedError("an e4m3 cache has pages of 16, 32, 64, 128 or 256 tokens")
-        if P["window"] != _ffi.ATF_WINDOW_OFF and (P["window"] == _ffi.ATF_WINDOW_VEC8
-                                                   or P["layout"] != _ffi.ATF_LAYOUT_SORTED_PAIR):
-            raise NotImplementedError("an e4m3 cache takes snap16 windows over sorted pairs")
+        _check_e4m3_form(page, P["window"], P["layout"])
         shape, qst = (P["B"], P["Hq"], 128), q.stride()
         if q.shape != shape or qst[2] != 1:
             raise ValueError(f"q must be {shape} with a contiguous head_dim axis")
