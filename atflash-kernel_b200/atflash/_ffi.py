@@ -19,6 +19,7 @@ ATF_WINDOW_OFF, ATF_WINDOW_SNAP16, ATF_WINDOW_VEC8 = 0, 1, 2
 ATF_DTYPE_BF16, ATF_DTYPE_F32 = 0, 1
 ATF_NOALLOC_MAX_PARTIAL_ROWS = 16384
 ATF_TABLES_MAX_BATCH = 8192
+ATF_VERSION = 101  # of the header whose structs are mirrored here
 
 EXPORTED = ("atf_window_widths", "atf_window_zhi16", "atf_window_zhi8", "atf_window_deff",
             "atf_prefill_fwd", "atf_decode_plan", "atf_decode_run", "atf_decode_run_noalloc", "atf_lse_merge",
@@ -160,6 +161,9 @@ def load() -> ctypes.CDLL:
                 raise ImportError(f"{_LIB_PATH} is missing: build it with "
                                   "`python atflash-kernel_b200/build.py` (no CPU fallback exists)")
             lib = ctypes.CDLL(_LIB_PATH)
+            if lib.atf_version() != ATF_VERSION:
+                raise ImportError(f"{_LIB_PATH} has version {lib.atf_version()} of the C interface, the package "
+                                  f"{ATF_VERSION}: build it again with `python atflash-kernel_b200/build.py`")
             P = ctypes.POINTER
             lib.atf_window_widths.argtypes = [ctypes.c_int, ctypes.c_double, ctypes.c_double, P(_f32)]
             lib.atf_window_zhi16.argtypes = [P(_f32), ctypes.c_int, _i64, P(_i32)]

@@ -77,7 +77,7 @@ int check_device(int* device_out) {
 
 using namespace atf;
 
-extern "C" int atf_version(void) { return 100; }
+extern "C" int atf_version(void) { return ATF_VERSION; }
 
 extern "C" int64_t atf_params_size(const char* name) {
   if (name == nullptr) return -1;

@@ -530,6 +530,11 @@ int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* s, atf_stre
 /* ------------------------------------------------------------------ misc */
 
 const char* atf_status_string(int status);
+/* ATF_VERSION of the library. A caller compiled against another version's header may
+ * pass shorter params structs than the library reads, so it should refuse to run.
+ *   100: the first
+ *   101: AtfDecodePlanParams ends in `units` */
+#define ATF_VERSION 101
 int atf_version(void);
 /* sizeof of the named params struct ("AtfPrefillParams", "AtfDecodePlanParams",
  * "AtfDecodePlan", "AtfDecodeParams", "AtfMergeParams", "AtfRopeParams",
