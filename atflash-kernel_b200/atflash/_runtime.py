@@ -18,6 +18,10 @@ def error_flag(device: torch.device) -> torch.Tensor:
         t = _flags.get(idx)
         if t is None:
             t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+            # kernels on any stream read it from now on (a capture cannot wait: its fill
+            # is the graph's first node)
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(idx).synchronize()
             _flags[idx] = t
     return t
 

@@ -111,3 +111,14 @@ def test_an_expired_wait_stops_attention_until_it_is_read():
     assert _runtime.selftest_wait_timeout(torch.device(DEV)) == 1
     got = _run(calls)
     assert atflash.check_device_errors() == 0 and all(torch.equal(got[n], want[n]) for n in calls)
+
+
+def test_a_new_flag_is_clear_for_every_stream(monkeypatch):
+    """The flag's first value is there before a kernel on another stream can read it."""
+    from atflash import _runtime
+    monkeypatch.setattr(_runtime, "_flags", {})
+    torch.cuda.synchronize()
+    torch.cuda._sleep(400_000_000)
+    flag = _runtime.error_flag(torch.device(DEV))
+    assert torch.cuda.current_stream().query()  # the fill has run, not only been queued
+    assert flag.item() == 0
