@@ -25,8 +25,10 @@
 // The scale of V in the exponent keeps P V free of its range: with m the running
 // maximum of s and M that of s + log2 vs (both log2 units), l = sum 2^(s - m) and
 // O = sum 2^(s + log2 vs - M) v; the row is O / l * 2^(M - m). The second
-// exponential costs 4 ex2 per thread and group. P is rounded to f16 (11 bits,
-// where the bf16 decode keeps 8). m and M move only when a score exceeds them by
+// exponential costs 4 ex2 per thread and group. P is rounded to f16: 11 bits (where
+// the bf16 decode keeps 8) down to 2^-21 of the largest p vs of the warp's keys, and
+// an absolute 2^-32 of that per key below (f16's subnormals; M is kept 7 lower than
+// the maximum for this). m and M move only when a score exceeds them by
 // more than 8, so most stages need no maximum over lanes and no pass over O.
 //
 // CTA = (unit of atf_decode_plan, kv head): one producer warp with TMA boxes per
@@ -91,7 +93,10 @@ constexpr uint32_t OFF_BAR = OFF_PAGES + 4 * MAX_UNIT_PAGES;
 constexpr uint32_t OFF_ABORT = OFF_BAR + 8 * 2 * NSTAGE;
 constexpr uint32_t SMEM_BYTES = OFF_ABORT + 16 + 1024;
 constexpr uint32_t FULLMASK = 0xffffffffu;
-constexpr float LAZY = 8.f;      // P <= 2^8: exact enough in f16, far from its largest value
+constexpr float LAZY = 8.f;      // a maximum moves when a score exceeds it by more
+// P's maximum is kept this much lower, so that P <= 2^15 (LAZY + RISE), just below f16's
+// largest value, and small weights have the most room above its subnormals
+constexpr float RISE = 7.f;
 constexpr float LOWEST = -1e30f; // a running maximum before any key
 static_assert((OFF_META & 15) == 0 && (OFF_SCALES & 7) == 0 && (OFF_BAR & 7) == 0, "shared memory layout");
 static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
@@ -506,7 +511,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float mx = fmaxf(c[nt][e], c[nt][e + 2]) - LAZY;
-            need |= mx > m_s[nt][e] || mx + sc.y > m_u[nt][e];
+            need |= mx > m_s[nt][e] || mx + (sc.y - RISE) > m_u[nt][e];
           }
         }
         if (__any_sync(FULLMASK, need)) {
@@ -517,7 +522,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
               float mh = fmaxf(c[nt][e], c[nt][e + 2]);  // over the group's 16 keys
 #pragma unroll
               for (int of = 4; of < 32; of <<= 1) mh = fmaxf(mh, __shfl_xor_sync(FULLMASK, mh, of));
-              const float ns = fmaxf(m_s[nt][e], mh), nu = fmaxf(m_u[nt][e], mh + sc.y);
+              const float ns = fmaxf(m_s[nt][e], mh), nu = fmaxf(m_u[nt][e], mh + (sc.y - RISE));
               l_run[nt][e] *= ex2f(m_s[nt][e] - ns);
               const float al = ex2f(m_u[nt][e] - nu);
               m_s[nt][e] = ns;
