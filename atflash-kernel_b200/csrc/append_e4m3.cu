@@ -112,7 +112,7 @@ __device__ __forceinline__ float mul_odd(float x, float r) {
   return __fmaf_rn(x, r, -q) != 0.f ? __uint_as_float(__float_as_uint(q) | 1u) : q;
 }
 
-// the 16 elements under a scale that is no power of two (another program's), divided
+// the 16 elements under a scale that is no such power of two (another program's), divided
 // by it; out of line, since this kernel writes powers of two only
 __device__ __noinline__ uint4 divide_words(uint4 lo, uint4 hi, float s) {
   const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
@@ -127,9 +127,10 @@ __device__ __noinline__ uint4 divide_words(uint4 lo, uint4 hi, float s) {
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
-// the 16 elements under scale s: for a power of two the product with 1/s is exact
+// the 16 elements under scale s: for a power of two up to 2^126 the product with 1/s is
+// exact (the inverse of 2^127 is no normal number)
 __device__ __forceinline__ void round_words(const Words& x, float s, uint32_t (&o)[4]) {
-  if ((__float_as_uint(s) & 0x7fffffu) != 0) {
+  if ((__float_as_uint(s) & 0x7fffffu) != 0 || __float_as_uint(s) >= 0x7f000000u) {
     const uint4 v = divide_words(make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]),
                                  make_uint4(x.w[4], x.w[5], x.w[6], x.w[7]), s);
     o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
