@@ -207,7 +207,6 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
         int32_t* at = a.req_pages + row * a.req_stride + j;
         if (j < s_have[b]) {
           id[k] = *at;
-          missing |= id[k] < 0;
         } else {
           id[k] = new_page(b, j);
           put[k] = at;
@@ -218,6 +217,7 @@ __global__ void __launch_bounds__(THREADS) tables_kernel(const Args a) {
     for (int k = 0; k < PER_LANE; ++k) {
       const long long e = e0 + 32 * k + lane;
       if (put[k] != nullptr) *put[k] = id[k];
+      else missing |= id[k] < 0 && e < all_pages;
       if (e < a.cap_pages) a.indices[e] = id[k];
     }
   }
