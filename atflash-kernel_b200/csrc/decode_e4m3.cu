@@ -41,10 +41,10 @@
 // item per CTA, 55 so). The producer runs through the pieces without a stop while
 // the consumers write each piece's state (2.8 us of a CTA's time per piece).
 //
-// Measured: 8 x 128K keys, 24 / 8 heads, window on 325 us in HND pages of 64 (the
-// copy bandwidth, rows read whole), 360 in NHD pages of 16 (boxes of 2 KB); 37 requests
-// up to 20011 keys (28 / 4 heads) 55 us, 80%: the SMs' shares end between 44 and 52 us;
-// 3 requests up to 300 keys 8.2 us with the merge.
+// Measured: 8 x 128K keys, 24 / 8 heads, window on 326 us in HND pages of 64 (the
+// copy bandwidth, rows read whole; off 316), 361 in NHD pages of 16 (boxes of 2 KB; off
+// 350); 37 requests up to 20011 keys (28 / 4 heads) 56 us, 80%: the SMs' shares end
+// between 44 and 52 us; 3 requests up to 300 keys 8.1 us with the merge.
 #include <cuda_fp16.h>
 #include <limits.h>
 #include <math.h>
@@ -188,9 +188,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   if (tag < 0) return;
   const int it0 = tag > 0 ? tag - 1 : x;
   const int n_items = (tag > 0 ? (next > 0 ? next - 1 : a.num_items) : x + 1) - it0;
-  // Prologue, part 1: only the plan and the page table, which no kernel of this
-  // step writes (it runs before the previous kernel's end under programmatic
-  // dependent launch). An item names a request of the batch, starts on a 64-key
+  // Prologue, part 1: only the plan and the page table, which the kernel just before
+  // does not write where programmatic dependent launch is on (this part runs before
+  // that kernel's end). An item names a request of the batch, starts on a 64-key
   // boundary and lies inside its request; the unit's pages fit the list. Else it is
   // reported and skipped.
   if (warp == 0) {

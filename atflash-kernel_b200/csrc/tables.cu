@@ -16,7 +16,7 @@
 // taken from the free list again, and the next free head is a word of its own.
 //
 // Measured: 256 requests, 47K pages 7.4 us; 4096 requests, 684K pages and 106K new
-// tokens 15 us, of which the scan is about 6.
+// tokens 15.3 us, of which the scan is about 6 and the searches 9.
 #include "atf_internal.h"
 
 namespace atf {
