@@ -300,8 +300,8 @@ int atf_decode_run(const AtfDecodeParams* p, atf_stream_t stream);
  *    plans return ATF_ERR_WORKSPACE and launch nothing; plan them with a larger
  *    min_chunk_keys, or use atf_decode_run.
  *  - Nothing in the scratch has to start at zero: each call writes every row it
- *    reads. The caller's error_flag, when given, must be zero on entry, as for
- *    atf_decode_run.
+ *    reads. The caller's error_flag, when given, must hold no expired wait on
+ *    entry, as for atf_decode_run.
  *  - All calls on one device share the scratch. Calls that overlap on the GPU
  *    (on different streams with no ordering between them, or from several
  *    threads) race and corrupt each other's output. Issue them on one stream,
