@@ -123,9 +123,9 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
     kv_scales = (k_scales, v_scales), fp32 (num_pages, Hkv): the cache pages are
     float8_e4m3fn (not level-major) and each (page, kv head) has one scale, which
     the call sets for pages it begins and raises for pages it goes on filling
-    (``atf_paged_kv_append_e4m3``; expanded pages or scales are refused). The tokens of a request are then adjacent and in
-    position order, as ``build_page_tables`` and ``get_batch_indices_positions`` list
-    them; a batch index of -1 is padding."""
+    (``atf_paged_kv_append_e4m3``; expanded pages or scales are refused). The tokens of
+    a request are then adjacent and in position order, as ``build_page_tables`` and
+    ``get_batch_indices_positions`` list them; a batch index of -1 is padding."""
     if isinstance(paged_kv_cache, (tuple, list)):
         kc, vc = paged_kv_cache
     else:

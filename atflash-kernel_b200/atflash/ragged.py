@@ -29,9 +29,9 @@ def _host_indptr(x, name: str) -> np.ndarray:
 
 
 class BatchPrefillWithRaggedKVCacheWrapper:
-    """plan() once per batch of sequences, run() for each layer, on any stream. Sequence b holds
-    the rows [qo_indptr[b], qo_indptr[b+1]) of q and [kv_indptr[b], kv_indptr[b+1])
-    of k and v; its queries are the last of its keys."""
+    """plan() once per batch of sequences, run() for each layer, on any stream. Sequence
+    b holds the rows [qo_indptr[b], qo_indptr[b+1]) of q and [kv_indptr[b],
+    kv_indptr[b+1]) of k and v; its queries are the last of its keys."""
 
     def __init__(self, device="cuda"):
         self._dev = torch.device(device)
@@ -142,8 +142,8 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q=Non
     optional ATFlash window table: a plan and a run of
     ``BatchPrefillWithRaggedKVCacheWrapper`` (keep the wrapper to plan once for all
     layers: the plan reads the cu_seqlens on the host, and cost 0.05 to 0.14 ms of each
-    call with 4 to 16 sequences). max_seqlen_* are accepted for call compatibility. Returns out, or (out, softmax_lse (Hq, total_q), None)
-    when return_attn_probs."""
+    call with 4 to 16 sequences). max_seqlen_* are accepted for call compatibility.
+    Returns out, or (out, softmax_lse (Hq, total_q), None) when return_attn_probs."""
     if dropout_p != 0.0:
         raise NotImplementedError("dropout is not supported")
     if tuple(window_size) != (-1, -1):
