@@ -10,11 +10,14 @@
     BatchDecodeWithPagedKVCacheWrapper
                    windowed paged-KV GQA decode (split-KV + LSE merge)
     rope_pack      fused RoPE + pair-order pack (pre-RoPE HF q/k -> kernel layout)
+    qk_norm_rope   RMS norms of the q and k heads with their RoPE in one pass
     append_paged_kv_cache
-                   write new K/V tokens into a paged cache (RoPE + pack on K); bf16
+                   write new K/V tokens into a paged cache (norm, RoPE + pack on K); bf16
                    pages, or e4m3 pages with a scale for each page and kv head
     build_page_tables
                    page tables and slot maps of a step from the requests' lengths
+    fork_requests / free_requests / compact_pages / PageCopier / copy_pages
+                   pages that requests share: tables, holders, free list and copies
     dist           zig-zag sharded prefill and KV-sharded decode over torch.distributed
     hf             transformers AttentionInterface function (import atflash.hf)
 
@@ -26,6 +29,8 @@ from ._ffi import AtfError, lib_path
 from ._runtime import check_device_errors
 from .append import append_paged_kv_cache, get_batch_indices_positions
 from .decode import BatchDecodeWithPagedKVCacheWrapper, lse_merge
+from .norm import qk_norm_rope
+from .pages import PageCopier, PageMoves, compact_pages, copy_pages, fork_requests, free_requests
 from .prefill import _flash_attn_fwd, flash_attn_func, prefill_fwd
 from .ragged import BatchPrefillWithRaggedKVCacheWrapper, flash_attn_varlen_func
 from .rope import cos_sin_table, inv_freq, rope_pack
@@ -49,4 +54,5 @@ __all__ = ["window_table", "WindowTable", "flash_attn_func", "prefill_fwd", "_fl
            "BatchDecodeWithPagedKVCacheWrapper", "lse_merge", "rope_pack", "cos_sin_table",
            "inv_freq", "check_device_errors", "dist", "AtfError", "append_paged_kv_cache",
            "get_batch_indices_positions", "build_page_tables", "PageTables",
-           "BatchPrefillWithRaggedKVCacheWrapper", "flash_attn_varlen_func"]
+           "BatchPrefillWithRaggedKVCacheWrapper", "flash_attn_varlen_func", "qk_norm_rope",
+           "fork_requests", "free_requests", "compact_pages", "PageMoves", "PageCopier", "copy_pages"]

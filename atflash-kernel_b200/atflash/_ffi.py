@@ -19,6 +19,7 @@ ATF_WINDOW_OFF, ATF_WINDOW_SNAP16, ATF_WINDOW_VEC8 = 0, 1, 2
 ATF_DTYPE_BF16, ATF_DTYPE_F32 = 0, 1
 ATF_NOALLOC_MAX_PARTIAL_ROWS = 16384
 ATF_TABLES_MAX_BATCH = 8192
+ATF_PAGES_MAX_ROWS, ATF_COMPACT_MAX_PAGES = 32768, 1048576
 ATF_VERSION = 101  # of the header whose structs are mirrored here
 
 EXPORTED = ("atf_window_widths", "atf_window_zhi16", "atf_window_zhi8", "atf_window_deff",
@@ -28,7 +29,8 @@ EXPORTED = ("atf_window_widths", "atf_window_zhi16", "atf_window_zhi8", "atf_win
             "atf_exchange_region_bytes", "atf_state_push", "atf_state_merge", "atf_decode_run_exchange",
             "atf_ipc_export", "atf_ipc_import", "atf_ipc_release",
             "atf_build_page_tables", "atf_paged_kv_append_e4m3", "atf_decode_run_e4m3",
-            "atf_prefill_ragged_plan", "atf_prefill_ragged_fwd")
+            "atf_prefill_ragged_plan", "atf_prefill_ragged_fwd", "atf_qk_norm_rope", "atf_paged_kv_append_norm",
+            "atf_fork_requests", "atf_free_requests", "atf_compact_pages", "atf_copy_pages")
 ATF_IPC_HANDLE_BYTES = 64
 
 _i64, _i32, _f32, _vp = ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p
@@ -105,6 +107,53 @@ class AtfAppendParams(ctypes.Structure):
                 ("k_stride_head", _i64), ("k_stride_level", _i64)]
 
 
+class AtfKNorm(ctypes.Structure):
+    _fields_ = [("weight", _vp), ("weight_dtype", ctypes.c_int), ("eps", _f32)]
+
+
+class AtfQkNormParams(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp), ("batch", _i64), ("seqlen", _i64),
+                ("num_heads_q", _i64), ("num_heads_k", _i64), ("head_dim", _i64),
+                ("q_stride_b", _i64), ("q_stride_s", _i64), ("q_stride_h", _i64),
+                ("k_stride_b", _i64), ("k_stride_s", _i64), ("k_stride_h", _i64),
+                ("q_out_stride_b", _i64), ("q_out_stride_s", _i64), ("q_out_stride_h", _i64),
+                ("k_out_stride_b", _i64), ("k_out_stride_s", _i64), ("k_out_stride_h", _i64),
+                ("q_weight", _vp), ("k_weight", _vp), ("weight_dtype", ctypes.c_int), ("eps", _f32),
+                ("cos", _vp), ("sin", _vp), ("cs_stride_pos", _i64), ("n_pos", _i64), ("positions", _vp),
+                ("positions_64", ctypes.c_int), ("pos_stride_b", _i64), ("pos_stride_s", _i64),
+                ("pos_offset", _i64), ("out_layout", ctypes.c_int)]
+
+
+class AtfForkParams(ctypes.Structure):
+    _fields_ = [("parents", _vp), ("children", _vp), ("kv_lens", _vp), ("batch", _i32), ("page_size", _i32),
+                ("req_pages", _vp), ("req_stride", _i64), ("num_rows", _i32), ("max_req_pages", _i32),
+                ("shared", _vp), ("num_pages", _i32), ("free_pages", _vp), ("free_head", _vp),
+                ("free_head_out", _vp), ("num_free", _i32), ("src", _vp), ("dst", _vp), ("error_flag", _vp)]
+
+
+class AtfFreeParams(ctypes.Structure):
+    _fields_ = [("req_rows", _vp), ("kv_lens", _vp), ("batch", _i32), ("page_size", _i32), ("req_pages", _vp),
+                ("req_stride", _i64), ("num_rows", _i32), ("max_req_pages", _i32), ("shared", _vp),
+                ("num_pages", _i32), ("free_pages", _vp), ("free_head", _vp), ("free_head_out", _vp),
+                ("num_free", _i32), ("error_flag", _vp)]
+
+
+class AtfCompactParams(ctypes.Structure):
+    _fields_ = [("req_rows", _vp), ("kv_lens", _vp), ("batch", _i32), ("page_size", _i32), ("req_pages", _vp),
+                ("req_stride", _i64), ("num_rows", _i32), ("max_req_pages", _i32), ("shared", _vp),
+                ("num_pages", _i32), ("max_moves", _i32), ("free_pages", _vp), ("free_head_out", _vp),
+                ("num_free", _i32), ("src", _vp), ("dst", _vp), ("error_flag", _vp)]
+
+
+class AtfPageTensor(ctypes.Structure):
+    _fields_ = [("base", _vp), ("page_stride_bytes", _i64), ("page_bytes", _i64)]
+
+
+class AtfCopyPagesParams(ctypes.Structure):
+    _fields_ = [("tensors_host", _vp), ("num_tensors", _i32), ("num_pages", _i32), ("src", _vp), ("dst", _vp),
+                ("num_pairs", _i32), ("error_flag", _vp)]
+
+
 class AtfExchangeParams(ctypes.Structure):
     _fields_ = [("o", _vp), ("lse", _vp), ("o_stride_b", _i64), ("o_stride_h", _i64), ("batch", _i32),
                 ("num_heads", _i32), ("world", _i32), ("rank", _i32), ("peer_base", _vp), ("base", _vp),
@@ -164,6 +213,10 @@ def load() -> ctypes.CDLL:
             if lib.atf_version() != ATF_VERSION:
                 raise ImportError(f"{_LIB_PATH} has version {lib.atf_version()} of the C interface, the package "
                                   f"{ATF_VERSION}: build it again with `python atflash-kernel_b200/build.py`")
+            lacking = [name for name in EXPORTED if not hasattr(lib, name)]
+            if lacking:
+                raise ImportError(f"{_LIB_PATH} lacks {', '.join(lacking)}: build it again with "
+                                  "`python atflash-kernel_b200/build.py`")
             P = ctypes.POINTER
             lib.atf_window_widths.argtypes = [ctypes.c_int, ctypes.c_double, ctypes.c_double, P(_f32)]
             lib.atf_window_zhi16.argtypes = [P(_f32), ctypes.c_int, _i64, P(_i32)]
@@ -193,6 +246,12 @@ def load() -> ctypes.CDLL:
             lib.atf_prefill_ragged_fwd.argtypes = [P(AtfPrefillRaggedParams), _vp]
             lib.atf_decode_run_e4m3.argtypes = [P(AtfDecodeParams), P(AtfKvScales), _vp]
             lib.atf_paged_kv_append_e4m3.argtypes = [P(AtfAppendParams), P(AtfKvScales), _vp]
+            lib.atf_paged_kv_append_norm.argtypes = [P(AtfAppendParams), P(AtfKvScales), P(AtfKNorm), _vp]
+            lib.atf_qk_norm_rope.argtypes = [P(AtfQkNormParams), _vp]
+            lib.atf_fork_requests.argtypes = [P(AtfForkParams), _vp]
+            lib.atf_free_requests.argtypes = [P(AtfFreeParams), _vp]
+            lib.atf_compact_pages.argtypes = [P(AtfCompactParams), _vp]
+            lib.atf_copy_pages.argtypes = [P(AtfCopyPagesParams), _vp]
             for name in EXPORTED:
                 if name not in ("atf_status_string", "atf_params_size", "atf_exchange_region_bytes"):
                     getattr(lib, name).restype = ctypes.c_int

@@ -11,6 +11,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _ffi, _runtime
+from .norm import check_norm, refuse_gradients
 
 _LAYOUTS = {"sorted_pair": _ffi.ATF_LAYOUT_SORTED_PAIR, "rotate_half": _ffi.ATF_LAYOUT_ROTATE_HALF}
 
@@ -65,8 +66,18 @@ def _dev_i32(t: torch.Tensor, dev: torch.device, top: int = 0x7fffffff) -> torch
     return _runtime.narrow_i32(t, dev, top)
 
 
+def _k_norm(k_norm, rope, key: torch.Tensor, dev: torch.device) -> _ffi.AtfKNorm:
+    if not isinstance(k_norm, (tuple, list)) or len(k_norm) != 2:
+        raise ValueError("k_norm is (weight, eps)")
+    weight, eps = k_norm
+    if rope is None:
+        raise ValueError("k_norm needs rope: the norm stands before the rotation")
+    refuse_gradients(weight, key)
+    return _ffi.AtfKNorm(weight.data_ptr(), check_norm(weight, eps, dev, "k_norm's weight"), eps)
+
+
 def _append_e4m3(k: torch.Tensor, v: torch.Tensor, batch_indices, positions, kc, vc, kv_indices, kv_indptr, kv_layout,
-                 rope, rope_positions, out_layout, kv_scales) -> None:
+                 rope, rope_positions, out_layout, kv_scales, k_norm) -> None:
     dev = _runtime.require_cuda(k, v, kc, vc)
     (npages, page, hkv), (s_page, s_tok, s_head), scales = check_e4m3_cache(kc, vc, kv_scales, kv_layout)
     shape, st = k.shape, k.stride()
@@ -78,6 +89,7 @@ def _append_e4m3(k: torch.Tensor, v: torch.Tensor, batch_indices, positions, kc,
     if shape[1] != hkv:
         raise ValueError("append_key heads do not match the cache")
     layout = _LAYOUTS[out_layout]
+    norm = _k_norm(k_norm, rope, k, dev) if k_norm is not None else None
     bi, ps = _dev_i32(batch_indices, dev), _dev_i32(positions, dev)
     ip, ix = _dev_i32(kv_indptr, dev, kv_indices.numel()), _dev_i32(kv_indices, dev)
     if bi.numel() != nnz or ps.numel() != nnz:
@@ -101,6 +113,10 @@ def _append_e4m3(k: torch.Tensor, v: torch.Tensor, batch_indices, positions, kc,
             if rp.numel() != nnz:
                 raise ValueError("rope_positions needs one entry per appended token")
             p.rope_positions = rp.data_ptr()
+    if norm is not None:
+        _runtime.launch("atf_paged_kv_append_norm", _ffi.load().atf_paged_kv_append_norm, dev, ctypes.byref(p),
+                        ctypes.byref(scales), ctypes.byref(norm))
+        return
     _runtime.launch("atf_paged_kv_append_e4m3", _ffi.load().atf_paged_kv_append_e4m3, dev, ctypes.byref(p),
                     ctypes.byref(scales))
 
@@ -110,7 +126,8 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
                           kv_indptr: torch.Tensor, kv_last_page_len: Optional[torch.Tensor] = None,
                           kv_layout: str = "NHD", *, rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
                           rope_positions: Optional[torch.Tensor] = None, out_layout: str = "sorted_pair",
-                          kv_scales: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> None:
+                          kv_scales: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                          k_norm: Optional[Tuple[torch.Tensor, float]] = None) -> None:
     """append_key / append_value (nnz, Hkv, 128) bf16; token i goes to request
     batch_indices[i] at KV position positions[i]. paged_kv_cache = (k_pages,
     v_pages) or one tensor with a k/v axis at dim 1; kv_layout "NHD" or "HND".
@@ -125,14 +142,18 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
     the call sets for pages it begins and raises for pages it goes on filling
     (``atf_paged_kv_append_e4m3``; expanded pages or scales are refused). The tokens of
     a request are then adjacent and in position order, as ``build_page_tables`` and
-    ``get_batch_indices_positions`` list them; a batch index of -1 is padding."""
+    ``get_batch_indices_positions`` list them; a batch index of -1 is padding.
+
+    k_norm = (weight, eps), with rope: each K row is RMS-normed before it is rotated, with
+    128 bf16 or fp32 weights, in fp32 and rounded once to bf16, as by ``qk_norm_rope``; e4m3
+    pages hold the rounding of that bf16 row. There is no backward pass."""
     if isinstance(paged_kv_cache, (tuple, list)):
         kc, vc = paged_kv_cache
     else:
         kc, vc = paged_kv_cache[:, 0], paged_kv_cache[:, 1]
     if kv_scales is not None:
         _append_e4m3(append_key, append_value, batch_indices, positions, kc, vc, kv_indices, kv_indptr, kv_layout, rope,
-                     rope_positions, out_layout, kv_scales)
+                     rope_positions, out_layout, kv_scales, k_norm)
         return
     dev = _runtime.require_cuda(append_key, append_value, kc, vc)
     if torch.float8_e4m3fn in (kc.dtype, vc.dtype):
@@ -163,6 +184,7 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
         raise ValueError("kv_layout must be NHD or HND")
     if hk2 != hkv:
         raise ValueError("append_key heads do not match the cache")
+    norm = _k_norm(k_norm, rope, append_key, dev) if k_norm is not None else None
     bi, ps = _dev_i32(batch_indices, dev), _dev_i32(positions, dev)
     ip, ix = _dev_i32(kv_indptr, dev, kv_indices.numel()), _dev_i32(kv_indices, dev)
     if bi.numel() != nnz or ps.numel() != nnz:
@@ -196,6 +218,10 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
             raise ValueError("level-major k pages do not match the v pages")
         p.k_level_major = 1
         p.k_stride_page, p.k_stride_head, p.k_stride_level = kc.stride(0), kc.stride(1), kc.stride(2)
+    if norm is not None:
+        _runtime.launch("atf_paged_kv_append_norm", _ffi.load().atf_paged_kv_append_norm, dev, ctypes.byref(p), None,
+                        ctypes.byref(norm))
+        return
     with torch.cuda.device(dev):
         rc = _ffi.load().atf_paged_kv_append(ctypes.byref(p), _runtime.stream_handle(dev))
     _ffi.check("atf_paged_kv_append", rc)

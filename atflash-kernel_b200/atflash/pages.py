@@ -1,0 +1,224 @@
+"""Cache pages that requests share: fork requests, free them, compact the pool and copy
+pages, over the tables of ``build_page_tables`` (req_pages, free_pages, free_head).
+
+``shared`` (int32, one entry per page, zeros to begin with) counts the holders of a page
+beyond the first. It is 0 for a free page and for a page of one request, so pages that
+``build_page_tables`` takes from the free list need no entry. A request writes into its
+last page only, and a fork gives the child a copy of a last page that is partly filled,
+so a page with several holders is never written.
+
+Index reports of these calls go to ``atflash.check_device_errors()`` (code 2). The
+reference serves one request and has no counterpart."""
+import ctypes
+from dataclasses import dataclass
+from typing import Optional, Sequence
+
+import torch
+
+from . import _ffi, _runtime
+
+
+@dataclass
+class PageMoves:
+    """src, dst int32: pages to copy (-1 on both sides: none), for ``PageCopier.copy``;
+    free_head (1): the next free list position."""
+    src: torch.Tensor
+    dst: torch.Tensor
+    free_head: torch.Tensor
+
+
+def _list(t: torch.Tensor, name: str, dev: torch.device, n: Optional[int] = None) -> torch.Tensor:
+    """An index list that a call reads, as contiguous int32."""
+    if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or (n is not None and t.numel() != n):
+        raise ValueError(f"{name} must be a 1-d integer tensor" + (f" of {n} entries" if n is not None else ""))
+    if t.device != dev:
+        raise ValueError("all tensors must be on the same device")
+    return t if t.dtype == torch.int32 and t.is_contiguous() else _runtime.narrow_i32(t, dev)
+
+
+def _state(t: torch.Tensor, name: str, dev: torch.device, least: int = 1) -> torch.Tensor:
+    """A tensor that a call changes in place: taken as it is."""
+    if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < least:
+        raise ValueError(f"{name} must be a contiguous 1-d int32 tensor" + (f" of {least} entries or more" if least > 1 else ""))
+    if t.device != dev:
+        raise ValueError("all tensors must be on the same device")
+    return t
+
+
+def _table(p, req_pages: torch.Tensor, batch: int, page_size: int) -> torch.device:
+    """Fills the request table's fields of a params struct."""
+    dev = _runtime.require_cuda(req_pages)
+    shape, st = req_pages.shape, req_pages.stride()
+    if len(shape) != 2 or req_pages.dtype != torch.int32 or (shape[1] > 1 and st[1] != 1):
+        raise ValueError("req_pages must be an int32 (rows, pages) tensor with contiguous rows")
+    if shape[0] < 1 or shape[1] < 1 or shape[0] > _ffi.ATF_PAGES_MAX_ROWS:
+        raise ValueError(f"req_pages must have between 1 and {_ffi.ATF_PAGES_MAX_ROWS} rows, of one page or more")
+    if shape[0] > 1 and st[0] < shape[1]:
+        raise ValueError("the rows of req_pages must not overlap")
+    if batch < 1 or batch > _ffi.ATF_TABLES_MAX_BATCH:
+        raise ValueError(f"between 1 and {_ffi.ATF_TABLES_MAX_BATCH} requests")
+    if batch * shape[1] >= 1 << 30:
+        raise ValueError("requests x pages must be under 2^30")
+    if page_size < 1:
+        raise ValueError("page_size must be positive")
+    p.batch, p.page_size, p.req_pages = batch, int(page_size), req_pages.data_ptr()
+    p.req_stride, p.num_rows, p.max_req_pages = (st[0] if shape[0] > 1 else shape[1]), shape[0], shape[1]
+    p.error_flag = _runtime.error_flag_ptr(dev)
+    return dev
+
+
+def _rows(req_rows: Optional[torch.Tensor], req_pages: torch.Tensor, batch: int, dev: torch.device):
+    if req_rows is not None:
+        return _list(req_rows, "req_rows", dev, batch)
+    if req_pages.shape[0] < batch:
+        raise ValueError("req_pages needs a row for each request")
+    return None
+
+
+def fork_requests(parents: torch.Tensor, children: torch.Tensor, kv_lens: torch.Tensor, req_pages: torch.Tensor,
+                  page_size: int, *, free_pages: torch.Tensor, free_head: torch.Tensor,
+                  shared: torch.Tensor) -> PageMoves:
+    """Fork requests in one launch: row children[i] of req_pages gets the pages that hold
+    the first kv_lens[i] tokens of row parents[i]. Full pages are shared (one holder more in
+    `shared`, in place); a last page that is partly filled becomes a page of the child's
+    own from free_pages[free_head:], in the order of the children, and a pair (src, dst)
+    to copy in every layer's cache before the child is read. A row may be the parent of
+    many. kv_lens[i] may be less than the parent's length (a shared prefix).
+
+    The child's row must hold no pages yet (free it first); entries past its pages stay.
+    A row is a child at most once and no child is a parent: entries against that, rows or
+    lengths out of range are left out. A page that the free list cannot give is -1 in the
+    row, and its pair is -1. Each is reported (code 2). src and dst have one entry per
+    child, -1 where there is nothing to copy; free_head itself stays."""
+    p = _ffi.AtfForkParams()
+    n = parents.numel()
+    dev = _table(p, req_pages, n, page_size)
+    parents, children = _list(parents, "parents", dev), _list(children, "children", dev, n)
+    kv_lens = _list(kv_lens, "kv_lens", dev, n)
+    free_pages, free_head = _list(free_pages, "free_pages", dev), _list(free_head, "free_head", dev, 1)
+    _state(shared, "shared", dev)
+    out = torch.empty(2 * n + 1, dtype=torch.int32, device=dev)
+    src = out.data_ptr()
+    p.parents, p.children, p.kv_lens = parents.data_ptr(), children.data_ptr(), kv_lens.data_ptr()
+    p.shared, p.num_pages = shared.data_ptr(), shared.numel()
+    # an empty list still has a head: any valid address will do for its pages
+    p.free_pages, p.free_head, p.num_free = free_pages.data_ptr() or free_head.data_ptr(), free_head.data_ptr(), \
+        free_pages.numel()
+    p.src, p.dst, p.free_head_out = src, src + 4 * n, src + 8 * n
+    _runtime.launch("atf_fork_requests", _ffi.load().atf_fork_requests, dev, ctypes.byref(p))
+    return PageMoves(*out.split_with_sizes((n, n, 1)))
+
+
+def free_requests(req_rows: Optional[torch.Tensor], kv_lens: torch.Tensor, req_pages: torch.Tensor, page_size: int, *,
+                  free_pages: torch.Tensor, free_head: torch.Tensor,
+                  shared: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Free requests in one launch: row req_rows[i] (default i) of req_pages gives up the
+    ceil(kv_lens[i] / page_size) pages of its kv_lens[i] tokens, and its entries become -1.
+    Each page loses one holder; the n that have none left go back to the free list,
+    free_pages[free_head - n : free_head], in place, in the order of the requests (a page
+    that several of them held at its last one). Returns the next free_head; free_head
+    itself stays. Without `shared` every page has one holder.
+
+    A row that is named twice (its first entry counts), rows and lengths out of range,
+    page ids outside the cache, a page given up more often than it was held and a list
+    without room are reported (code 2) and left out."""
+    p = _ffi.AtfFreeParams()
+    n = kv_lens.numel()
+    dev = _table(p, req_pages, n, page_size)
+    kv_lens = _list(kv_lens, "kv_lens", dev)
+    req_rows = _rows(req_rows, req_pages, n, dev)
+    _state(free_pages, "free_pages", dev)
+    free_head = _list(free_head, "free_head", dev, 1)
+    out = torch.empty(1, dtype=torch.int32, device=dev)
+    if req_rows is not None:
+        p.req_rows = req_rows.data_ptr()
+    if shared is not None:
+        _state(shared, "shared", dev)
+        p.shared, p.num_pages = shared.data_ptr(), shared.numel()
+    p.kv_lens, p.free_pages, p.num_free = kv_lens.data_ptr(), free_pages.data_ptr(), free_pages.numel()
+    p.free_head, p.free_head_out = free_head.data_ptr(), out.data_ptr()
+    _runtime.launch("atf_free_requests", _ffi.load().atf_free_requests, dev, ctypes.byref(p))
+    return out
+
+
+def compact_pages(kv_lens: torch.Tensor, req_pages: torch.Tensor, page_size: int, num_pages: int, *, max_moves: int,
+                  free_pages: torch.Tensor, req_rows: Optional[torch.Tensor] = None,
+                  shared: Optional[torch.Tensor] = None) -> PageMoves:
+    """Move pages in use towards the start of the cache, in one launch. kv_lens (and
+    req_rows, default i) name every request that holds pages; the L pages that they hold
+    out of num_pages end up as pages 0 .. L-1: the highest page at or above L moves to the
+    lowest free one, the next to the next, at most max_moves of them (a later call goes
+    on). req_pages and `shared` follow, in place; src and dst (max_moves) are the pairs
+    to copy in every layer's cache, -1 past the last; free_pages (num_pages entries or
+    more) becomes the list of all other pages, rising, at its end, and free_head in the
+    result points to its first.
+
+    Pages that no named request holds count as free. Rows, lengths and page ids out of
+    range are reported (code 2) and left out. At most 2^20 pages."""
+    p = _ffi.AtfCompactParams()
+    n, num_pages, max_moves = kv_lens.numel(), int(num_pages), int(max_moves)
+    dev = _table(p, req_pages, n, page_size)
+    if num_pages < 1 or num_pages > _ffi.ATF_COMPACT_MAX_PAGES:
+        raise ValueError(f"between 1 and {_ffi.ATF_COMPACT_MAX_PAGES} pages")
+    if max_moves < 0 or max_moves > num_pages:
+        raise ValueError("max_moves must be between 0 and num_pages")
+    kv_lens = _list(kv_lens, "kv_lens", dev)
+    req_rows = _rows(req_rows, req_pages, n, dev)
+    _state(free_pages, "free_pages", dev, num_pages)
+    out = torch.empty(2 * max_moves + 1, dtype=torch.int32, device=dev)
+    src = out.data_ptr()
+    if req_rows is not None:
+        p.req_rows = req_rows.data_ptr()
+    if shared is not None:
+        p.shared = _state(shared, "shared", dev, num_pages).data_ptr()
+    p.kv_lens, p.num_pages, p.max_moves = kv_lens.data_ptr(), num_pages, max_moves
+    p.free_pages, p.num_free = free_pages.data_ptr(), free_pages.numel()
+    p.src, p.dst, p.free_head_out = src, src + 4 * max_moves, src + 8 * max_moves
+    _runtime.launch("atf_compact_pages", _ffi.load().atf_compact_pages, dev, ctypes.byref(p))
+    return PageMoves(*out.split_with_sizes((max_moves, max_moves, 1)))
+
+
+class PageCopier:
+    """Copies pages in every tensor of a cache at once: the K and V pages of all layers
+    and, for e4m3 pages, their scales. Made once for a cache (it keeps the tensors, whose
+    first axis is the page); copy() is one launch per 256 tensors."""
+
+    def __init__(self, caches: Sequence[torch.Tensor]):
+        caches = list(caches)
+        if not caches:
+            raise ValueError("at least one cache tensor")
+        self._dev = _runtime.require_cuda(*caches)
+        self._pages = caches[0].shape[0] if caches[0].dim() > 0 else 0
+        desc = (_ffi.AtfPageTensor * len(caches))()
+        for d, t in zip(desc, caches):
+            if t.dim() < 1 or t.shape[0] != self._pages or t.numel() == 0:
+                raise ValueError("the first axis of every cache tensor is the page, of the same number")
+            dense = 1  # a page's own elements lie together, in any order of the axes
+            for size, stride in sorted(zip(t.shape[1:], t.stride()[1:]), key=lambda x: (x[1], x[0])):
+                if size > 1:
+                    if stride != dense:
+                        raise ValueError("a page's elements must lie together in memory")
+                    dense *= size
+            if self._pages > 1 and t.stride(0) < dense:
+                raise ValueError("the pages of a cache tensor must not overlap")
+            es = t.element_size()
+            d.base, d.page_stride_bytes, d.page_bytes = t.data_ptr(), t.stride(0) * es, dense * es
+        self._caches, self._desc = caches, desc
+
+    def copy(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Page src[i] of every tensor to page dst[i]; -1 on both sides is no copy, and
+        other ids outside the cache are reported by ``atflash.check_device_errors()`` (code 2)
+        and left out. The pages of dst differ from one another and are none of src's, as in
+        the lists of ``fork_requests`` and ``compact_pages``; src may name a page twice."""
+        src = _list(src, "src", self._dev)
+        dst = _list(dst, "dst", self._dev, src.numel())
+        if src.numel() == 0:
+            return
+        p = _ffi.AtfCopyPagesParams(ctypes.addressof(self._desc), len(self._desc), self._pages, src.data_ptr(),
+                                    dst.data_ptr(), src.numel(), _runtime.error_flag_ptr(self._dev))
+        _runtime.launch("atf_copy_pages", _ffi.load().atf_copy_pages, self._dev, ctypes.byref(p))
+
+
+def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:
+    """``PageCopier(caches).copy(src, dst)``, for a single copy."""
+    PageCopier(caches).copy(src, dst)

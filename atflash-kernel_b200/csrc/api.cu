@@ -98,6 +98,13 @@ extern "C" int64_t atf_params_size(const char* name) {
       {"AtfKvScales", static_cast<int64_t>(sizeof(AtfKvScales))},
       {"AtfPrefillRaggedPlanParams", static_cast<int64_t>(sizeof(AtfPrefillRaggedPlanParams))},
       {"AtfPrefillRaggedParams", static_cast<int64_t>(sizeof(AtfPrefillRaggedParams))},
+      {"AtfQkNormParams", static_cast<int64_t>(sizeof(AtfQkNormParams))},
+      {"AtfKNorm", static_cast<int64_t>(sizeof(AtfKNorm))},
+      {"AtfForkParams", static_cast<int64_t>(sizeof(AtfForkParams))},
+      {"AtfFreeParams", static_cast<int64_t>(sizeof(AtfFreeParams))},
+      {"AtfCompactParams", static_cast<int64_t>(sizeof(AtfCompactParams))},
+      {"AtfPageTensor", static_cast<int64_t>(sizeof(AtfPageTensor))},
+      {"AtfCopyPagesParams", static_cast<int64_t>(sizeof(AtfCopyPagesParams))},
   };
   for (const Entry& e : kSizes)
     if (std::strcmp(e.n, name) == 0) return e.size;

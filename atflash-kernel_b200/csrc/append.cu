@@ -9,7 +9,11 @@
 // to page kv_indices[kv_indptr[b] + pos / page], slot pos % page. A token
 // whose page index lies outside the request's pages or the cache is skipped
 // and reported through the error flag (kDevErrIndex).
+//
+// With k_norm_weight, K is normed before it is rotated (norm_math.cuh): the 8 threads of a
+// row are neighbouring lanes, which share its sum of squares.
 #include "atf_internal.h"
+#include "norm_math.cuh"
 #include "rope_math.cuh"
 
 namespace atf {
@@ -35,8 +39,12 @@ struct Args {
   int* err;
   int k_lm;                              // level-major K pages
   long long k_s_page, k_s_head, k_s_level;
+  const void* norm_w;
+  int norm_f32;
+  float eps;
 };
 
+template <bool NORM>
 __global__ void append_kernel(const Args a) {
   const long long gid = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (gid >= a.nnz * a.H * 8) return;
@@ -81,6 +89,22 @@ __global__ void append_kernel(const Args a) {
   long long rp = a.rope_pos != nullptr ? a.rope_pos[i] : pos;
   if (rp < 0) rp = 0;
   if (rp >= a.n_pos) rp = a.n_pos - 1;
+  if (NORM) {
+    // a row's 8 threads take the same branches up to here, so the group is whole
+    const unsigned group = 0xffu << (threadIdx.x & 24);
+    float x1[8], x2[8], w1[8], w2[8], cv[8], sv[8];
+    normmath::unpack(*reinterpret_cast<const uint4*>(a.ak + src + 8 * c), x1);
+    normmath::unpack(*reinterpret_cast<const uint4*>(a.ak + src + 64 + 8 * c), x2);
+    normmath::weights8(a.norm_w, a.norm_f32 != 0, 8 * c, w1);
+    normmath::weights8(a.norm_w, a.norm_f32 != 0, 64 + 8 * c, w2);
+    normmath::load8(a.cs + rp * a.cs_stride + 8 * c, cv);
+    normmath::load8(a.sn + rp * a.cs_stride + 8 * c, sv);
+    normmath::normalise(x1, x2, w1, w2, a.eps, group);
+    uint32_t o[8];
+    normmath::rotate(x1, x2, cv, sv, a.sorted != 0, o);
+    normmath::store_pairs(a.kc + kdst, c, a.sorted != 0, lstride, o);
+    return;
+  }
   ropemath::rotate_chunk(a.ak + src, a.cs + rp * a.cs_stride, a.sn + rp * a.cs_stride, a.kc + kdst, c,
                          a.sorted != 0, lstride);
 }
@@ -91,6 +115,16 @@ __global__ void append_kernel(const Args a) {
 using namespace atf;
 
 extern "C" int atf_paged_kv_append(const AtfAppendParams* p, atf_stream_t stream) {
+  return append_bf16(p, nullptr, stream);
+}
+
+extern "C" int atf_paged_kv_append_norm(const AtfAppendParams* p, const AtfKvScales* s, const AtfKNorm* n,
+                                        atf_stream_t stream) {
+  if (n == nullptr) return ATF_ERR_INVALID_ARG;
+  return s != nullptr ? append_e4m3(p, s, n, stream) : append_bf16(p, n, stream);
+}
+
+int atf::append_bf16(const AtfAppendParams* p, const AtfKNorm* norm, atf_stream_t stream) {
   if (p == nullptr || p->append_k == nullptr || p->append_v == nullptr || p->batch_indices == nullptr ||
       p->positions == nullptr || p->k_cache == nullptr || p->v_cache == nullptr ||
       p->kv_indptr == nullptr || p->kv_indices == nullptr)
@@ -113,10 +147,12 @@ extern "C" int atf_paged_kv_append(const AtfAppendParams* p, atf_stream_t stream
       !aligned16(p->v_cache) || (p->a_stride_n & 7) || (p->a_stride_h & 7) || (p->kv_stride_page & 7) ||
       (p->kv_stride_token & 7) || (p->kv_stride_head & 7))
     return ATF_ERR_ALIGNMENT;
+  int rc = norm_args_ok(p, norm);
+  if (rc != ATF_OK) return rc;
   const long long total = p->nnz * p->num_kv_heads * 8;
   if (total == 0) return ATF_OK;
   int dev = 0;
-  int rc = check_device(&dev);
+  rc = check_device(&dev);
   if (rc != ATF_OK) return rc;
   append::Args a;
   a.ak = static_cast<const __nv_bfloat16*>(p->append_k);
@@ -152,7 +188,13 @@ extern "C" int atf_paged_kv_append(const AtfAppendParams* p, atf_stream_t stream
   const int threads = 256;
   const long long blocks = (total + threads - 1) / threads;
   if (blocks > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
-  append::append_kernel<<<static_cast<unsigned>(blocks), threads, 0,
-                          reinterpret_cast<cudaStream_t>(stream)>>>(a);
+  a.norm_w = norm != nullptr ? norm->weight : nullptr;
+  a.norm_f32 = norm != nullptr && norm->weight_dtype == ATF_DTYPE_F32 ? 1 : 0;
+  a.eps = norm != nullptr ? norm->eps : 0.f;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (a.norm_w != nullptr)
+    append::append_kernel<true><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
+  else
+    append::append_kernel<false><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
 }

@@ -35,6 +35,7 @@
 #include <type_traits>
 
 #include "atf_internal.h"
+#include "norm_math.cuh"
 #include "rope_math.cuh"
 
 namespace atf {
@@ -66,6 +67,9 @@ struct Args {
   const int64_t* rope_pos;
   int sorted;
   int* err;
+  const void* norm_w;
+  int norm_f32;
+  float eps;
 };
 
 // exponent e of the smallest power of two with amax <= 448 * 2^e, in [-126, 120]:
@@ -162,9 +166,11 @@ __device__ __forceinline__ Words load_row(const __nv_bfloat16* row, int c, bool 
 }
 // the 8 pairs rotated as in rope_math.cuh (separately rounded products, then bf16),
 // as words in the order they are written; row(f): the position's table rows, cos in
-// the 16-byte words 0 .. 15 and sin in 16 .. 31
-template <typename Row>
-__device__ __forceinline__ Words rotate(const Words& in, Row row, int c, bool sorted) {
+// the 16-byte words 0 .. 15 and sin in 16 .. 31. With a norm, the pairs are normed first
+// over the 8 lanes of the row, under weights w1 and w2.
+template <bool NORM, typename Row>
+__device__ __forceinline__ Words rotate(const Words& in, Row row, int c, bool sorted, const float (&w1)[NORM ? 8 : 1],
+                                        const float (&w2)[NORM ? 8 : 1], float eps) {
   float cv[8], sv[8];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
@@ -173,26 +179,12 @@ __device__ __forceinline__ Words rotate(const Words& in, Row row, int c, bool so
     cv[4 * q] = c4.x; cv[4 * q + 1] = c4.y; cv[4 * q + 2] = c4.z; cv[4 * q + 3] = c4.w;
     sv[4 * q] = s4.x; sv[4 * q + 1] = s4.y; sv[4 * q + 2] = s4.z; sv[4 * q + 3] = s4.w;
   }
-  float r1[8], r2[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t l2 = in.w[e >> 1], h2 = in.w[4 + (e >> 1)];
-    const float x1 = (e & 1) ? __uint_as_float(l2 & 0xffff0000u) : __uint_as_float(l2 << 16);
-    const float x2 = (e & 1) ? __uint_as_float(h2 & 0xffff0000u) : __uint_as_float(h2 << 16);
-    r1[e] = __fsub_rn(__fmul_rn(x1, cv[e]), __fmul_rn(x2, sv[e]));
-    r2[e] = __fadd_rn(__fmul_rn(x2, cv[e]), __fmul_rn(x1, sv[e]));
-  }
+  float x1[8], x2[8];
+  normmath::unpack(make_uint4(in.w[0], in.w[1], in.w[2], in.w[3]), x1);
+  normmath::unpack(make_uint4(in.w[4], in.w[5], in.w[6], in.w[7]), x2);
+  if constexpr (NORM) normmath::normalise(x1, x2, w1, w2, eps, 0xffu << (threadIdx.x & 24));
   Words x;
-  if (sorted) {  // pairs in falling order, (x1, x2) adjacent
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x.w[7 - e] = ropemath::pack_rn(r1[e], r2[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x.w[e] = ropemath::pack_rn(r1[2 * e], r1[2 * e + 1]);
-      x.w[4 + e] = ropemath::pack_rn(r2[2 * e], r2[2 * e + 1]);
-    }
-  }
+  normmath::rotate(x1, x2, cv, sv, sorted, x.w);
   return x;
 }
 
@@ -310,8 +302,9 @@ __device__ __forceinline__ void stage_angles(const Args& a, long long i0, float4
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <bool ROPE>
-__global__ void __launch_bounds__(THREADS, 3) append_e4m3_kernel(const Args a) {
+// (the norm's weights take 16 registers more)
+template <bool ROPE, bool NORM>
+__global__ void __launch_bounds__(THREADS, NORM ? 2 : 3) append_e4m3_kernel(const Args a) {
   __shared__ Run s_run[MAX_WINDOW];
   __shared__ int s_n;
   __shared__ float s_max[2][WARPS];
@@ -330,6 +323,11 @@ __global__ void __launch_bounds__(THREADS, 3) append_e4m3_kernel(const Args a) {
   const int tasks = s_n * nh * 2;
   const int W = a.share, wi = warp & (W - 1), slots = WARPS / W;
   const int c = lane & 7, r0 = wi * WARP_ROWS + (lane >> 3), step = W * WARP_ROWS;
+  float w1[NORM ? 8 : 1] = {}, w2[NORM ? 8 : 1] = {};  // of this lane's pairs
+  if constexpr (NORM) {
+    normmath::weights8(a.norm_w, a.norm_f32 != 0, 8 * c, w1);
+    normmath::weights8(a.norm_w, a.norm_f32 != 0, 64 + 8 * c, w2);
+  }
   int turn = 0;
   for (int base = 0; base < tasks; base += slots, turn ^= 1) {
     const int task = base + warp / W;
@@ -362,12 +360,12 @@ __global__ void __launch_bounds__(THREADS, 3) append_e4m3_kernel(const Args a) {
         for (int u = 0; u < U; ++u) {
           const int t = run.i + r[u];
           if (t < a.window) {
-            w[u] = rotate(w[u], [&](int f) { return s_angle[t][angle_slot(f)]; }, c, a.sorted != 0);
+            w[u] = rotate<NORM>(w[u], [&](int f) { return s_angle[t][angle_slot(f)]; }, c, a.sorted != 0, w1, w2, a.eps);
           } else {  // the run goes on past the window
             const long long at = angle_row(a, i0 + t) * a.cs_stride;
-            w[u] = rotate(w[u], [&](int f) {
+            w[u] = rotate<NORM>(w[u], [&](int f) {
               return *reinterpret_cast<const float4*>((f < 16 ? a.cs : a.sn) + at + 4 * (f & 15));
-            }, c, a.sorted != 0);
+            }, c, a.sorted != 0, w1, w2, a.eps);
           }
         }
       }
@@ -435,6 +433,10 @@ __global__ void __launch_bounds__(THREADS, 3) append_e4m3_kernel(const Args a) {
 using namespace atf;
 
 extern "C" int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvScales* s, atf_stream_t stream) {
+  return append_e4m3(p, s, nullptr, stream);
+}
+
+int atf::append_e4m3(const AtfAppendParams* p, const AtfKvScales* s, const AtfKNorm* norm, atf_stream_t stream) {
   if (p == nullptr || s == nullptr || p->append_k == nullptr || p->append_v == nullptr ||
       p->batch_indices == nullptr || p->positions == nullptr || p->k_cache == nullptr || p->v_cache == nullptr ||
       p->kv_indptr == nullptr || p->kv_indices == nullptr || s->k_scale == nullptr || s->v_scale == nullptr)
@@ -447,6 +449,8 @@ extern "C" int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvSca
   if (rope && (p->n_pos < 1 || p->cs_stride_pos < 64)) return ATF_ERR_INVALID_ARG;
   if (p->out_layout != ATF_LAYOUT_SORTED_PAIR && p->out_layout != ATF_LAYOUT_ROTATE_HALF)
     return ATF_ERR_INVALID_ARG;
+  int rc = norm_args_ok(p, norm);
+  if (rc != ATF_OK) return rc;
   if (rope && (!aligned16(p->cos) || !aligned16(p->sin) || (p->cs_stride_pos & 3))) return ATF_ERR_ALIGNMENT;
   if (!aligned16(p->append_k) || !aligned16(p->append_v) || !aligned16(p->k_cache) || !aligned16(p->v_cache) ||
       (p->a_stride_n & 7) || (p->a_stride_h & 7) || (p->kv_stride_page & 15) || (p->kv_stride_token & 15) ||
@@ -460,7 +464,7 @@ extern "C" int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvSca
     return ATF_ERR_INVALID_ARG;
   if (p->nnz == 0) return ATF_OK;
   int dev = 0;
-  int rc = check_device(&dev);
+  rc = check_device(&dev);
   if (rc != ATF_OK) return rc;
   append8::Args a;
   a.ak = static_cast<const __nv_bfloat16*>(p->append_k);
@@ -512,9 +516,14 @@ extern "C" int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvSca
   while (split < a.H && busy * split < 2 * 148 && runs * ((a.H + split - 1) / split) * 2 > at_once) split <<= 1;
   a.heads = (a.H + split - 1) / split;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((a.H + a.heads - 1) / a.heads));
-  if (rope)
-    append8::append_e4m3_kernel<true><<<grid, append8::THREADS, 0, st>>>(a);
+  a.norm_w = norm != nullptr ? norm->weight : nullptr;
+  a.norm_f32 = norm != nullptr && norm->weight_dtype == ATF_DTYPE_F32 ? 1 : 0;
+  a.eps = norm != nullptr ? norm->eps : 0.f;
+  if (a.norm_w != nullptr)
+    append8::append_e4m3_kernel<true, true><<<grid, append8::THREADS, 0, st>>>(a);
+  else if (rope)
+    append8::append_e4m3_kernel<true, false><<<grid, append8::THREADS, 0, st>>>(a);
   else
-    append8::append_e4m3_kernel<false><<<grid, append8::THREADS, 0, st>>>(a);
+    append8::append_e4m3_kernel<false, false><<<grid, append8::THREADS, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
 }

@@ -32,6 +32,22 @@ int check_device(int* device_out);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// The K norm of an append (optional): it stands before a rotation, and its weights are
+// read 16 bytes at a time.
+inline int norm_args_ok(const AtfAppendParams* p, const AtfKNorm* n) {
+  if (n == nullptr) return ATF_OK;
+  if (n->weight == nullptr || p->cos == nullptr || !(n->eps > 0.f) ||
+      (n->weight_dtype != ATF_DTYPE_BF16 && n->weight_dtype != ATF_DTYPE_F32))
+    return ATF_ERR_INVALID_ARG;
+  if (!aligned16(n->weight) || !aligned16(p->cos) || !aligned16(p->sin) || (p->cs_stride_pos & 3) != 0)
+    return ATF_ERR_ALIGNMENT;
+  return ATF_OK;
+}
+
+// The appends, with an optional norm of K (append.cu, append_e4m3.cu)
+int append_bf16(const AtfAppendParams* p, const AtfKNorm* norm, atf_stream_t stream);
+int append_e4m3(const AtfAppendParams* p, const AtfKvScales* s, const AtfKNorm* norm, atf_stream_t stream);
+
 // atf_decode_run's checks and its split-KV kernel launch, without the merge
 // (decode.cu); atf_decode_run and atf_decode_run_exchange add their merges.
 int decode_launch_split(const AtfDecodeParams* p, cudaStream_t st);

@@ -417,6 +417,38 @@ typedef struct {
  * contraction), rounded to bf16, written in the requested pair order. */
 int atf_rope_pack(const AtfRopeParams* p, atf_stream_t stream);
 
+/* ------------------------------------------------------------------ norm + RoPE */
+
+/* RMS norms of the query and key heads with their rotation. No counterpart in the
+ * reference, whose models have none. */
+typedef struct {
+  const void* q; /* bf16 [B, S, Hq, 128], pre-norm, rotate_half pair order (not read when Hq = 0) */
+  const void* k; /* bf16 [B, S, Hk, 128] (not read when Hk = 0) */
+  void* q_out;   /* bf16, q's shape; may be q itself (with its strides), else overlaps no input */
+  void* k_out;
+  int64_t batch, seqlen, num_heads_q, num_heads_k, head_dim;
+  int64_t q_stride_b, q_stride_s, q_stride_h, k_stride_b, k_stride_s, k_stride_h;
+  int64_t q_out_stride_b, q_out_stride_s, q_out_stride_h, k_out_stride_b, k_out_stride_s, k_out_stride_h;
+  const void* q_weight; /* [128] */
+  const void* k_weight;
+  int weight_dtype;     /* ATF_DTYPE_* of both */
+  float eps;            /* positive */
+  const float* cos;     /* fp32 [n_pos, >= 64], rows 16-byte aligned */
+  const float* sin;
+  int64_t cs_stride_pos, n_pos;
+  const void* positions; /* optional device int32 or int64; default pos_offset + s */
+  int positions_64;
+  int64_t pos_stride_b, pos_stride_s; /* of positions, elements (0: shared along the axis) */
+  int64_t pos_offset;
+  int out_layout; /* ATF_LAYOUT_* */
+} AtfQkNormParams;
+
+/* y = x w / sqrt(mean(x^2) + eps) over each row's 128 elements, then the rotation of
+ * atf_rope_pack on y at the token's position (clamped into the tables), all in fp32,
+ * rounded once to bf16 and written in the requested pair order. A row whose squares
+ * overflow fp32 (elements over 1e18) gives 0. */
+int atf_qk_norm_rope(const AtfQkNormParams* p, atf_stream_t stream);
+
 /* ------------------------------------------------------------------ paged-KV append */
 
 typedef struct {
@@ -495,6 +527,114 @@ typedef struct {
  * 2. Requests of one call use different rows. */
 int atf_build_page_tables(const AtfPageTablesParams* p, atf_stream_t stream);
 
+/* ------------------------------------------------------------------ shared pages */
+
+/* Requests that hold pages together, over the tables of atf_build_page_tables
+ * (req_pages, free_pages, free_head). shared[p] counts the holders of page p beyond the
+ * first: 0 for a free page and for one of a single request, so a page taken by
+ * atf_build_page_tables needs no entry of its own. Every id is checked before it is
+ * used; what a call leaves out (rows or lengths out of range, a row named twice, page
+ * ids outside the cache) sets *error_flag to 2. No counterpart in the reference, which
+ * serves one request. */
+#define ATF_PAGES_MAX_ROWS 32768
+#define ATF_COMPACT_MAX_PAGES 1048576
+
+typedef struct {
+  const int32_t* parents;  /* device [batch]: row of req_pages */
+  const int32_t* children; /* device [batch]: row that the fork fills */
+  const int32_t* kv_lens;  /* device [batch]: tokens that the child takes over */
+  int32_t batch, page_size;
+  int32_t* req_pages;      /* device [num_rows, >= max_req_pages] */
+  int64_t req_stride;
+  int32_t num_rows, max_req_pages;
+  int32_t* shared;         /* device [num_pages] */
+  int32_t num_pages;
+  const int32_t* free_pages; /* device [num_free] */
+  const int32_t* free_head;  /* device [1] */
+  int32_t* free_head_out;    /* device [1], another word */
+  int32_t num_free;
+  int32_t* src;            /* device [batch]: page to copy for each child, or -1 */
+  int32_t* dst;
+  int* error_flag;
+} AtfForkParams;
+
+/* Fork batch children in one launch: child i's first kv_lens[i] / page_size entries are
+ * its parent's (one holder more each); a remainder of tokens gets a page of its own from
+ * free_pages[*free_head ..], in the order of the children, and a pair (src, dst) to copy
+ * with atf_copy_pages. The rest of the child's row stays. A row is a child once, and
+ * no child is a parent; an entry against that (each but a row's first) is left out. A
+ * page that the free list cannot give is -1 in the row, and its pair is -1. */
+int atf_fork_requests(const AtfForkParams* p, atf_stream_t stream);
+
+typedef struct {
+  const int32_t* req_rows; /* optional device [batch]: row of each request (default i) */
+  const int32_t* kv_lens;  /* device [batch] */
+  int32_t batch, page_size;
+  int32_t* req_pages;
+  int64_t req_stride;
+  int32_t num_rows, max_req_pages;
+  int32_t* shared;         /* optional device [num_pages]; NULL: every page has one holder */
+  int32_t num_pages;
+  int32_t* free_pages;     /* device [num_free] */
+  const int32_t* free_head;
+  int32_t* free_head_out;  /* another word */
+  int32_t num_free;
+  int* error_flag;
+} AtfFreeParams;
+
+/* Free the first ceil(kv_lens[i] / page_size) pages of batch requests in one launch: each
+ * page loses a holder per entry, and one that has none left goes back to the free
+ * list: n such pages to free_pages[*free_head - n .. *free_head), by their last entry in the
+ * call, and *free_head_out = *free_head - n. The entries become -1. A page given up more often
+ * than it was held is freed once and reported. */
+int atf_free_requests(const AtfFreeParams* p, atf_stream_t stream);
+
+typedef struct {
+  const int32_t* req_rows; /* optional device [batch] */
+  const int32_t* kv_lens;  /* device [batch]: of every request that holds pages */
+  int32_t batch, page_size;
+  int32_t* req_pages;
+  int64_t req_stride;
+  int32_t num_rows, max_req_pages;
+  int32_t* shared;         /* optional device [num_pages] */
+  int32_t num_pages;       /* up to ATF_COMPACT_MAX_PAGES */
+  int32_t max_moves;
+  int32_t* free_pages;     /* device [num_free], num_free >= num_pages */
+  int32_t* free_head_out;
+  int32_t num_free;
+  int32_t* src;            /* device [max_moves] */
+  int32_t* dst;
+  int* error_flag;
+} AtfCompactParams;
+
+/* Move the L pages that the requests hold towards the first L of the cache: the
+ * highest one at or above L to the lowest free one, and so on, at most max_moves. The
+ * tables and counts are changed, the pairs to copy are in src and dst (-1 past the last),
+ * and the free list becomes the pages that no request holds, rising, at its end. */
+int atf_compact_pages(const AtfCompactParams* p, atf_stream_t stream);
+
+typedef struct {
+  void* base;
+  int64_t page_stride_bytes;
+  int64_t page_bytes; /* of a page's own data, without gaps */
+} AtfPageTensor;
+
+#define ATF_COPY_MAX_TENSORS 256 /* per launch: more tensors take more launches */
+
+typedef struct {
+  const AtfPageTensor* tensors_host; /* [num_tensors] (host) */
+  int32_t num_tensors, num_pages;    /* every tensor has num_pages pages */
+  const int32_t* src;                /* device [num_pairs], -1 on both sides: no copy */
+  const int32_t* dst;
+  int32_t num_pairs;
+  int* error_flag;
+} AtfCopyPagesParams;
+
+/* Copy page src[i] to page dst[i] of every tensor. The pages of dst differ from one
+ * another and are none of src's, as those of a fork or a compaction are (which copy
+ * comes last is not defined otherwise); a page may be the src of several. */
+int atf_copy_pages(const AtfCopyPagesParams* p, atf_stream_t stream);
+
 /* ------------------------------------------------------------------ e4m3 paged cache */
 
 /* An e4m3 cache keeps one fp32 scale for each (page, kv head) of K and of V: an
@@ -527,6 +667,20 @@ int atf_paged_kv_append_e4m3(const AtfAppendParams* p, const AtfKvScales* s, atf
  * *error_flag to 2 (the outputs of that request are not valid then). */
 int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* s, atf_stream_t stream);
 
+/* The norm of K at an append. */
+typedef struct {
+  const void* weight; /* [128], 16-byte aligned */
+  int weight_dtype;   /* ATF_DTYPE_* */
+  float eps;          /* positive */
+} AtfKNorm;
+
+/* atf_paged_kv_append (s NULL) or atf_paged_kv_append_e4m3 of a K that is normed first:
+ * x w / sqrt(mean(x^2) + eps) over each row, then the rotation (p->cos and p->sin are
+ * required, their rows 16-byte aligned), in fp32 and rounded once to bf16; e4m3
+ * pages hold the rounding of that bf16 row. */
+int atf_paged_kv_append_norm(const AtfAppendParams* p, const AtfKvScales* s, const AtfKNorm* n,
+                             atf_stream_t stream);
+
 /* ------------------------------------------------------------------ misc */
 
 const char* atf_status_string(int status);
@@ -539,7 +693,9 @@ int atf_version(void);
 /* sizeof of the named params struct ("AtfPrefillParams", "AtfDecodePlanParams",
  * "AtfDecodePlan", "AtfDecodeParams", "AtfMergeParams", "AtfRopeParams",
  * "AtfAppendParams", "AtfExchangeParams", "AtfPageTablesParams", "AtfKvScales",
- * "AtfPrefillRaggedPlanParams", "AtfPrefillRaggedParams"),
+ * "AtfPrefillRaggedPlanParams", "AtfPrefillRaggedParams", "AtfQkNormParams",
+ * "AtfKNorm", "AtfForkParams", "AtfFreeParams", "AtfCompactParams", "AtfPageTensor",
+ * "AtfCopyPagesParams"),
  * or -1: lets an FFI binding check its struct mirrors. */
 int64_t atf_params_size(const char* name);
 /* Synchronises the current device, copies *error_flag to *out and clears it. */
