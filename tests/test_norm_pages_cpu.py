@@ -53,7 +53,7 @@ def test_append_norm_refuses_bad_arguments():
     p, n, s = ffi.AtfAppendParams(), ffi.AtfKNorm(), ffi.AtfKvScales()
     p.append_k = p.append_v = p.batch_indices = p.positions = p.k_cache = p.v_cache = p.kv_indptr = p.kv_indices = 256
     p.head_dim, p.num_kv_heads, p.page_size, p.batch_size, p.num_pages = 128, 1, 16, 1, 1
-    s.k_scale = s.v_scale = 256
+    s.k_scale = s.v_scale = p.kv_stride_token = 256
     s.stride_page = s.stride_head = 1
     for scales in (None, ctypes.byref(s)):
         call = lambda: lib.atf_paged_kv_append_norm(ctypes.byref(p), scales, ctypes.byref(n), None)
