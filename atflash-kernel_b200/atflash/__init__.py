@@ -30,6 +30,7 @@ from ._runtime import check_device_errors
 from .append import append_paged_kv_cache, get_batch_indices_positions
 from .decode import BatchDecodeWithPagedKVCacheWrapper, lse_merge
 from .norm import qk_norm_rope
+from .paged import BatchPrefillWithPagedKVCacheWrapper
 from .pages import PageCopier, PageMoves, compact_pages, copy_pages, fork_requests, free_requests
 from .prefill import _flash_attn_fwd, flash_attn_func, prefill_fwd
 from .ragged import BatchPrefillWithRaggedKVCacheWrapper, flash_attn_varlen_func
@@ -55,4 +56,4 @@ __all__ = ["window_table", "WindowTable", "flash_attn_func", "prefill_fwd", "_fl
            "inv_freq", "check_device_errors", "dist", "AtfError", "append_paged_kv_cache",
            "get_batch_indices_positions", "build_page_tables", "PageTables",
            "BatchPrefillWithRaggedKVCacheWrapper", "flash_attn_varlen_func", "qk_norm_rope",
-           "fork_requests", "free_requests", "compact_pages", "PageMoves", "PageCopier", "copy_pages"]
+           "BatchPrefillWithPagedKVCacheWrapper", "fork_requests", "free_requests", "compact_pages", "PageMoves", "PageCopier", "copy_pages"]

@@ -19,6 +19,7 @@ ATF_WINDOW_OFF, ATF_WINDOW_SNAP16, ATF_WINDOW_VEC8 = 0, 1, 2
 ATF_DTYPE_BF16, ATF_DTYPE_F32 = 0, 1
 ATF_NOALLOC_MAX_PARTIAL_ROWS = 16384
 ATF_TABLES_MAX_BATCH = 8192
+ATF_PAGED_ITEM_INTS = 12
 ATF_PAGES_MAX_ROWS, ATF_COMPACT_MAX_PAGES = 32768, 1048576
 ATF_VERSION = 101  # of the header whose structs are mirrored here
 
@@ -29,7 +30,8 @@ EXPORTED = ("atf_window_widths", "atf_window_zhi16", "atf_window_zhi8", "atf_win
             "atf_exchange_region_bytes", "atf_state_push", "atf_state_merge", "atf_decode_run_exchange",
             "atf_ipc_export", "atf_ipc_import", "atf_ipc_release",
             "atf_build_page_tables", "atf_paged_kv_append_e4m3", "atf_decode_run_e4m3",
-            "atf_prefill_ragged_plan", "atf_prefill_ragged_fwd", "atf_qk_norm_rope", "atf_paged_kv_append_norm",
+            "atf_prefill_ragged_plan", "atf_prefill_ragged_fwd",
+            "atf_prefill_paged_plan", "atf_prefill_paged_fwd", "atf_qk_norm_rope", "atf_paged_kv_append_norm",
             "atf_fork_requests", "atf_free_requests", "atf_compact_pages", "atf_copy_pages")
 ATF_IPC_HANDLE_BYTES = 64
 
@@ -187,6 +189,29 @@ class AtfPrefillRaggedParams(ctypes.Structure):
                 ("window", ctypes.c_int), ("zhi", _i32 * 8), ("error_flag", _vp)]
 
 
+class AtfPrefillPagedPlanParams(ctypes.Structure):
+    _fields_ = [("batch_size", _i32), ("num_qo_heads", _i32), ("num_kv_heads", _i32), ("page_size", _i32),
+                ("qo_indptr_host", _vp), ("kv_indptr_host", _vp), ("last_page_len_host", _vp),
+                ("causal", ctypes.c_int), ("num_sms", _i32)]
+
+
+class AtfPrefillPagedPlan(ctypes.Structure):
+    _fields_ = [("num_items", _i32), ("num_wide", _i32), ("num_rows", _i32), ("num_parts", _i32),
+                ("partial_o_floats", _i64), ("partial_lse_floats", _i64)]
+
+
+class AtfPrefillPagedParams(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k_cache", _vp), ("v_cache", _vp), ("out", _vp), ("lse", _vp), ("total_q", _i64),
+                ("num_pages", _i64), ("num_heads_q", _i64), ("num_heads_kv", _i64), ("head_dim", _i64),
+                ("q_stride_s", _i64), ("q_stride_h", _i64), ("o_stride_s", _i64), ("o_stride_h", _i64),
+                ("k_stride_page", _i64), ("k_stride_token", _i64), ("k_stride_head", _i64),
+                ("v_stride_page", _i64), ("v_stride_token", _i64), ("v_stride_head", _i64),
+                ("page_size", _i32), ("num_indices", _i32), ("indices", _vp), ("items", _vp), ("rows", _vp),
+                ("num_items", _i32), ("num_wide", _i32), ("num_rows", _i32), ("num_parts", _i32),
+                ("partial_o", _vp), ("partial_lse", _vp), ("softmax_scale", _f32), ("causal", ctypes.c_int),
+                ("window", ctypes.c_int), ("zhi", _i32 * 8), ("error_flag", _vp)]
+
+
 class AtfError(RuntimeError):
     """A non-zero status from the C ABI."""
 
@@ -246,6 +271,9 @@ def load() -> ctypes.CDLL:
             lib.atf_prefill_ragged_fwd.argtypes = [P(AtfPrefillRaggedParams), _vp]
             lib.atf_decode_run_e4m3.argtypes = [P(AtfDecodeParams), P(AtfKvScales), _vp]
             lib.atf_paged_kv_append_e4m3.argtypes = [P(AtfAppendParams), P(AtfKvScales), _vp]
+            lib.atf_prefill_paged_plan.argtypes = [P(AtfPrefillPagedPlanParams), P(_i32), _i32, P(_i32), _i32,
+                                                   P(AtfPrefillPagedPlan)]
+            lib.atf_prefill_paged_fwd.argtypes = [P(AtfPrefillPagedParams), _vp]
             lib.atf_paged_kv_append_norm.argtypes = [P(AtfAppendParams), P(AtfKvScales), P(AtfKNorm), _vp]
             lib.atf_qk_norm_rope.argtypes = [P(AtfQkNormParams), _vp]
             lib.atf_fork_requests.argtypes = [P(AtfForkParams), _vp]

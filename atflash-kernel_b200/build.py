@@ -17,8 +17,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "atflash", "_lib")
 LIB = os.path.join(OUT_DIR, "libatflash_b200.so")
-SOURCES = ["api.cu", "prefill_sm100.cu", "prefill_ragged_sm100.cu", "decode.cu", "decode_e4m3.cu", "decode_noalloc.cu",
-           "exchange.cu", "rope.cu", "append.cu", "append_e4m3.cu", "tables.cu", "pages.cu", "qk_norm.cu",
+SOURCES = ["api.cu", "prefill_sm100.cu", "prefill_ragged_sm100.cu", "prefill_paged_sm100.cu", "decode.cu",
+           "decode_e4m3.cu", "decode_noalloc.cu", "exchange.cu", "rope.cu", "append.cu", "append_e4m3.cu", "tables.cu", "pages.cu", "qk_norm.cu",
            "selftest.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

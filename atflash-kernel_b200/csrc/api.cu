@@ -98,6 +98,9 @@ extern "C" int64_t atf_params_size(const char* name) {
       {"AtfKvScales", static_cast<int64_t>(sizeof(AtfKvScales))},
       {"AtfPrefillRaggedPlanParams", static_cast<int64_t>(sizeof(AtfPrefillRaggedPlanParams))},
       {"AtfPrefillRaggedParams", static_cast<int64_t>(sizeof(AtfPrefillRaggedParams))},
+      {"AtfPrefillPagedPlanParams", static_cast<int64_t>(sizeof(AtfPrefillPagedPlanParams))},
+      {"AtfPrefillPagedPlan", static_cast<int64_t>(sizeof(AtfPrefillPagedPlan))},
+      {"AtfPrefillPagedParams", static_cast<int64_t>(sizeof(AtfPrefillPagedParams))},
       {"AtfQkNormParams", static_cast<int64_t>(sizeof(AtfQkNormParams))},
       {"AtfKNorm", static_cast<int64_t>(sizeof(AtfKNorm))},
       {"AtfForkParams", static_cast<int64_t>(sizeof(AtfForkParams))},

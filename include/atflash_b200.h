@@ -186,6 +186,64 @@ typedef struct {
  * own. */
 int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_stream_t stream);
 
+/* Paged prefill: attention of each request's new tokens (one, a few or thousands) over
+ * its pages. q [total_q, Hq, 128] holds the requests' tokens one after another, the tokens
+ * of request b at [qo_indptr[b], qo_indptr[b+1]); they are the last of its keys (causal:
+ * token i sees the keys up to nk - nq + i), which are already in the pages. A row that
+ * sees no key gets 0 and an LSE of -inf. The window is quantised per tile of 128 tokens and
+ * 128 keys of a request, as in atf_prefill_ragged_fwd. Pages past the last key and rows past it in
+ * its page are not used, whatever they hold. No counterpart in the reference, whose
+ * prefill reads contiguous K and V. */
+typedef struct {
+  int32_t batch_size, num_qo_heads, num_kv_heads, page_size; /* pages of 16, 32, 64, 128 or 256 */
+  const int32_t* qo_indptr_host;     /* [batch+1] (host) */
+  const int32_t* kv_indptr_host;     /* [batch+1] pages (host) */
+  const int32_t* last_page_len_host; /* [batch] (host) */
+  int causal;
+  int32_t num_sms;                   /* 0: 148 */
+} AtfPrefillPagedPlanParams;
+
+#define ATF_PAGED_ITEM_INTS 12
+
+typedef struct {
+  int32_t num_items, num_wide; /* items; the first num_wide have a head of their own each */
+  int32_t num_rows;            /* tokens whose keys several items share */
+  int32_t num_parts;           /* states of tokens in the workspace */
+  int64_t partial_o_floats, partial_lse_floats;
+} AtfPrefillPagedPlan;
+
+/* The work items: ATF_PAGED_ITEM_INTS int32 each, and 4 int32 for each of num_rows. NULL
+ * buffers: only *out is set. */
+int atf_prefill_paged_plan(const AtfPrefillPagedPlanParams* p, int32_t* items_host, int32_t items_capacity,
+                           int32_t* rows_host, int32_t rows_capacity, AtfPrefillPagedPlan* out);
+
+typedef struct {
+  const void* q;       /* bf16 [total_q, Hq, 128] */
+  const void* k_cache; /* bf16 pages, NHD or HND through the strides; K in q's pair order */
+  const void* v_cache;
+  void* out;           /* bf16 [total_q, Hq, 128] */
+  float* lse;          /* optional fp32 [total_q, Hq], natural log */
+  int64_t total_q, num_pages, num_heads_q, num_heads_kv, head_dim;
+  int64_t q_stride_s, q_stride_h, o_stride_s, o_stride_h;
+  int64_t k_stride_page, k_stride_token, k_stride_head;
+  int64_t v_stride_page, v_stride_token, v_stride_head;
+  int32_t page_size, num_indices;
+  const int32_t* indices; /* device [num_indices]: page ids, as kv_indptr orders them */
+  const int32_t* items;   /* device, from the plan; 16-byte aligned */
+  const int32_t* rows;    /* device, from the plan; 16-byte aligned (NULL when num_rows = 0) */
+  int32_t num_items, num_wide, num_rows, num_parts;
+  float* partial_o;       /* workspace, 16-byte aligned (NULL when num_parts = 0) */
+  float* partial_lse;
+  float softmax_scale;
+  int causal;             /* as planned */
+  int window;             /* ATF_WINDOW_OFF, or ATF_WINDOW_SNAP16 over sorted pairs */
+  int32_t zhi[ATF_MAX_LEVELS]; /* level 0 is always read */
+  int* error_flag;        /* optional; 2: an item outside the tensors was skipped, or a page id
+                             outside the cache (the outputs of its request are not valid) */
+} AtfPrefillPagedParams;
+
+int atf_prefill_paged_fwd(const AtfPrefillPagedParams* p, atf_stream_t stream);
+
 /* ------------------------------------------------------------------ decode */
 
 typedef struct {
@@ -693,7 +751,8 @@ int atf_version(void);
 /* sizeof of the named params struct ("AtfPrefillParams", "AtfDecodePlanParams",
  * "AtfDecodePlan", "AtfDecodeParams", "AtfMergeParams", "AtfRopeParams",
  * "AtfAppendParams", "AtfExchangeParams", "AtfPageTablesParams", "AtfKvScales",
- * "AtfPrefillRaggedPlanParams", "AtfPrefillRaggedParams", "AtfQkNormParams",
+ * "AtfPrefillRaggedPlanParams", "AtfPrefillRaggedParams", "AtfPrefillPagedPlanParams",
+ * "AtfPrefillPagedPlan", "AtfPrefillPagedParams", "AtfQkNormParams",
  * "AtfKNorm", "AtfForkParams", "AtfFreeParams", "AtfCompactParams", "AtfPageTensor",
  * "AtfCopyPagesParams"),
  * or -1: lets an FFI binding check its struct mirrors. */
