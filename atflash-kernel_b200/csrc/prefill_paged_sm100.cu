@@ -99,7 +99,8 @@ enum {
   NUM_BARS
 };
 constexpr uint32_t OFF_STATE = OFF_BAR + 8 * ((NUM_BARS + 1) / 2 * 2);  // [t][128] of (max, sum)
-constexpr uint32_t OFF_ABORT = OFF_STATE + NQ * BM * 8;
+constexpr uint32_t OFF_PLACE = OFF_STATE + NQ * BM * 8;                 // Place
+constexpr uint32_t OFF_ABORT = OFF_PLACE + 48;
 constexpr uint32_t OFF_TMEM = OFF_ABORT + 16;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16 + 1024;  // slack for 1024-B alignment
 
@@ -150,12 +151,20 @@ struct Unit {
   uint8_t* sp;
   uint32_t tmem;
   AbortCtl ab;
-  int q_tok, sk, q_offset, row0, n0, n1, kt0, page_beg, part, n_parts, page_end;
+  int sk, q_offset, row0, n0, n1, kt0, page_beg, page_end;
   int nk[NQ];       // key tiles of each group
-  int h, hk, packed, P;
+  int hk, P;        // heads side by side in a tile
   int lim[NQ][ATF_MAX_LEVELS];
   __device__ __forceinline__ uint32_t bar(int i) const { return sb + OFF_BAR + 8u * static_cast<uint32_t>(i); }
 };
+
+// Where the rows go, in shared memory: the softmax groups have no registers left for it
+// until their loop is done.
+struct Place {
+  int q_tok, row0, part, n_parts, head0, P, n0, n1;
+  int nk[NQ], pad[2];
+};
+static_assert(sizeof(Place) == 48, "its room in shared memory");
 
 // The key tile of a group's i-th step, and its place in the order of all loads
 template <bool SPLIT_KEYS>
@@ -330,16 +339,16 @@ __device__ __forceinline__ void issue_mmas(const Args& a, const Unit& u, int lan
 // per row, so that whole 128-byte lines leave. get(c4, v): dims [32 c4, 32 c4 + 32) of
 // this lane's row.
 template <typename Get>
-__device__ __forceinline__ void store_half(const Args& a, const Unit& u, int half, int tok0, int first_row, int n_rows,
+__device__ __forceinline__ void store_half(const Args& a, const Place& to, int half, int tok0, int first_row, int n_rows,
                                            uint8_t* stage, int lane, Get&& get) {
   const int lr = lane >> 3, c = lane & 7;
   // (token, head) of a row of the tile
   auto place = [&](int r, int* tok, int* head) {
-    *tok = tok0 + (u.packed ? r / u.P : r);
-    *head = u.packed ? u.hk * a.G + r % u.P : u.h;
+    *tok = tok0 + r / to.P;
+    *head = to.head0 + r % to.P;
   };
   float v[32];
-  if (u.part < 0) {
+  if (to.part < 0) {
 #pragma unroll
     for (int c4 = 0; c4 < 2; ++c4) {
       get(2 * half + c4, v);
@@ -357,7 +366,7 @@ __device__ __forceinline__ void store_half(const Args& a, const Unit& u, int hal
       if (first_row + r < n_rows) {
         int tok, head;
         place(first_row + r, &tok, &head);
-        *reinterpret_cast<uint4*>(a.out + static_cast<long long>(u.q_tok + tok) * a.o_ss +
+        *reinterpret_cast<uint4*>(a.out + static_cast<long long>(to.q_tok + tok) * a.o_ss +
                                   static_cast<long long>(head) * a.o_sh + 64 * half + 8 * c) = x;
       }
     }
@@ -379,7 +388,7 @@ __device__ __forceinline__ void store_half(const Args& a, const Unit& u, int hal
       if (first_row + r < n_rows) {
         int tok, head;
         place(first_row + r, &tok, &head);
-        const long long slot = u.part + static_cast<long long>(tok - u.row0) * u.n_parts;
+        const long long slot = to.part + static_cast<long long>(tok - to.row0) * to.n_parts;
         *reinterpret_cast<float4*>(a.part_o + (slot * a.Hq + head) * 128 + 64 * half + 32 * c4 + 4 * c) = x;
       }
     }
@@ -396,17 +405,14 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
   const uint32_t tO = u.tmem + 256u + static_cast<uint32_t>(t * 128) + lane_off;
   const int my_nk = t ? u.nk[1] : u.nk[0], other_nk = t ? u.nk[0] : u.nk[1];
   const int tok0 = u.row0 + (!SPLIT_KEYS && t ? u.n0 : 0);      // the tile's first token
-  const int n_tok = !SPLIT_KEYS && t ? u.n1 : u.n0, n_rows = n_tok * u.P;
-  const int r = wq * 32 + lane, tok = tok0 + (u.packed ? r / u.P : r);
-  // this row sees the keys before `seen`; from key tile j_mask on, a row of the tile does
-  // not see every key
-  const int seen = a.causal ? min(u.sk, u.q_offset + tok + 1) : u.sk;
-  const int j_mask = max(0, a.causal ? min(u.sk, u.q_offset + tok0 + 1) : u.sk) / BN;
+  // keys that this row still sees from the step's key tile on, and that the tile's first row
+  // sees: under 128, some row of the tile does not see every key
+  int left = (a.causal ? min(u.sk, u.q_offset + tok0 + (wq * 32 + lane) / u.P + 1) : u.sk) - (u.kt0 + nth<SPLIT_KEYS>(t, 0)) * BN;
+  int left0 = (a.causal ? min(u.sk, u.q_offset + tok0 + 1) : u.sk) - (u.kt0 + nth<SPLIT_KEYS>(t, 0)) * BN;
   const float sl2 = a.scale_log2;
   float m2 = -INFINITY, l = 0.f;
   bool ok = true;
   for (int i = 0; i < my_nk; ++i) {
-    const int j = u.kt0 + nth<SPLIT_KEYS>(t, i);
     ok = __all_sync(FULL, mbar_wait_inl(u.bar(B_SFULL + t), i & 1, u.ab, kDevErrTimeout));
     if (!ok) break;
     tc_fence_after();
@@ -421,11 +427,12 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
     // other group may store its P there
     tc_fence_before();
     mbar_arrive(u.bar(B_LOADED + t));
-    if (j >= j_mask) {
-      const int left = seen - j * BN;
+    if (left0 < BN) {
 #pragma unroll
       for (int c = 0; c < BN; ++c) s[c] = c < left ? s[c] : -INFINITY;
     }
+    left -= (SPLIT_KEYS ? 2 : 1) * BN;
+    left0 -= (SPLIT_KEYS ? 2 : 1) * BN;
     // three-input max: 64 instructions for the 128 scores, 4 chains
     float mx0 = fmax3(s[0], s[1], s[2]), mx1 = fmax3(s[3], s[4], s[5]);
     float mx2 = fmax3(s[6], s[7], s[8]), mx3 = fmax3(s[9], s[10], s[11]);
@@ -511,15 +518,19 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
 
   float lse2;  // log2 of the row's sum
   uint8_t* stage;
+  const int r = wq * 32 + lane;
+  const Place& to = *reinterpret_cast<const Place*>(u.sp + OFF_PLACE);
+  const int out0 = to.row0 + (!SPLIT_KEYS && t ? to.n0 : 0), n_rows = (!SPLIT_KEYS && t ? to.n1 : to.n0) * to.P;
   if (SPLIT_KEYS) {
     // both groups' states of the row: (max, sum) through shared memory, O from TMEM, where
     // the row has the same lane in both. Group t stores half t of the dims.
     float2* state = reinterpret_cast<float2*>(u.sp + OFF_STATE);
     state[t * BM + r] = make_float2(m2, l);
-    if (ok && my_nk > 0) ok = __all_sync(FULL, mbar_wait_inl(u.bar(B_OFINAL + t), 0, u.ab, kDevErrTimeout));
-    if (ok && other_nk > 0) ok = __all_sync(FULL, mbar_wait_inl(u.bar(B_OFINAL + (t ^ 1)), 0, u.ab, kDevErrTimeout));
+#pragma unroll
+    for (int k = 0; k < NQ; ++k)
+      if (ok && to.nk[k] > 0) ok = __all_sync(FULL, mbar_wait_inl(u.bar(B_OFINAL + k), 0, u.ab, kDevErrTimeout));
     // (without keys nothing has read Q, whose place the outputs take)
-    if (ok && u.nk[0] == 0) ok = __all_sync(FULL, mbar_wait_inl(u.bar(B_Q), 0, u.ab, kDevErrTimeout));
+    if (ok && to.nk[0] == 0) ok = __all_sync(FULL, mbar_wait_inl(u.bar(B_Q), 0, u.ab, kDevErrTimeout));
     tc_fence_after();
     __syncwarp();
     asm volatile("bar.sync 1, 256;" ::: "memory");  // every softmax thread of the CTA comes here
@@ -529,14 +540,14 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
     const float w0 = s0.x == -INFINITY ? 0.f : ex2_approx(s0.x - m), w1 = s1.x == -INFINITY ? 0.f : ex2_approx(s1.x - m);
     l = s0.y * w0 + s1.y * w1;
     lse2 = m + log2f(l);
-    const bool keyless = seen <= u.kt0 * BN;
-    const float inv = l > 0.f && !keyless ? 1.0f / l : 0.f;
+    const bool keyless = m == -INFINITY;  // 0, whatever V holds
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
     const float f0 = w0 * inv, f1 = w1 * inv;
-    const uint32_t tO0 = u.tmem + 256u + lane_off;
+    const uint32_t tO0 = tO - static_cast<uint32_t>(t * 128);
     stage = u.sp + OFF_Q + warp * 4096;
-    store_half(a, u, t, tok0, wq * 32, n_rows, stage, lane, [&](int c4, float (&v)[32]) {
+    store_half(a, to, t, out0, wq * 32, n_rows, stage, lane, [&](int c4, float (&v)[32]) {
       uint32_t rr[32];
-      if (u.nk[0] > 0) {  // (the same for every thread of the CTA)
+      if (to.nk[0] > 0) {  // (the same for every thread of the CTA)
         tmem_ld32(tO0 + static_cast<uint32_t>(32 * c4), rr);
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = keyless ? 0.f : __uint_as_float(rr[e]) * f0;
@@ -544,7 +555,7 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = 0.f;
       }
-      if (u.nk[1] > 0) {
+      if (to.nk[1] > 0) {
         tmem_ld32(tO0 + static_cast<uint32_t>(128 + 32 * c4), rr);
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = keyless ? 0.f : fmaf(__uint_as_float(rr[e]), f1, v[e]);
@@ -552,13 +563,13 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
     });
     if (t != 0) return;
   } else {
-    if (!ok || n_tok == 0) return;
+    if (!ok || n_rows == 0) return;
     if (my_nk > 0) {
       if (!__all_sync(FULL, mbar_wait_inl(u.bar(B_OFINAL + t), 0, u.ab, kDevErrTimeout))) return;
       tc_fence_after();
     }
-    const bool keyless = seen <= u.kt0 * BN;  // 0, whatever V holds
-    const float inv = l > 0.f && !keyless ? 1.0f / l : 0.f;
+    const bool keyless = m2 == -INFINITY;  // 0, whatever V holds
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
     lse2 = m2 + log2f(l);
     // through the tile's own Q in shared memory (its last product has read it; a tile without
     // keys has no products)
@@ -566,7 +577,7 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
     if (my_nk == 0 && !__all_sync(FULL, mbar_wait_inl(u.bar(B_Q), 0, u.ab, kDevErrTimeout))) return;
 #pragma unroll
     for (int half = 0; half < 2; ++half)
-      store_half(a, u, half, tok0, wq * 32, n_rows, stage, lane, [&](int c4, float (&v)[32]) {
+      store_half(a, to, half, out0, wq * 32, n_rows, stage, lane, [&](int c4, float (&v)[32]) {
         if (my_nk > 0) {
           uint32_t rr[32];
           tmem_ld32(tO + static_cast<uint32_t>(32 * c4), rr);
@@ -579,11 +590,11 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
       });
   }
   if (r < n_rows) {
-    const int head = u.packed ? u.hk * a.G + r % u.P : u.h;
-    if (u.part >= 0)
-      a.part_lse[(u.part + static_cast<long long>(tok - u.row0) * u.n_parts) * a.Hq + head] = lse2;
+    const int tok = out0 + r / to.P, head = to.head0 + r % to.P;
+    if (to.part >= 0)
+      a.part_lse[(to.part + static_cast<long long>(tok - to.row0) * to.n_parts) * a.Hq + head] = lse2;
     else if (a.lse != nullptr)
-      a.lse[static_cast<long long>(u.q_tok + tok) * a.Hq + head] = lse2 * 0.69314718055994531f;
+      a.lse[static_cast<long long>(to.q_tok + tok) * a.Hq + head] = lse2 * 0.69314718055994531f;
   }
 }
 
@@ -601,16 +612,16 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int lane = threadIdx.x & 31;
 
   // This CTA's item and head: unpacked items go by query heads, packed ones by kv heads
-  int item;
+  int item, h;
   const int bid = static_cast<int>(blockIdx.x), wide = a.n_wide * a.Hq;
   if (bid < wide) {
     const int per_walk = a.n_wide * a.walk, rem = bid % per_walk;
-    u.h = bid / per_walk * a.walk + rem % a.walk;
-    u.hk = u.h / a.G;
+    h = bid / per_walk * a.walk + rem % a.walk;
+    u.hk = h / a.G;
     item = rem / a.walk;
   } else {
     u.hk = (bid - wide) % a.Hkv;
-    u.h = u.hk * a.G;
+    h = u.hk * a.G;
     item = a.n_wide + (bid - wide) / a.Hkv;
   }
   const int4* src = reinterpret_cast<const int4*>(a.items) + 3 * item;
@@ -647,7 +658,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   // the merge of the states may be launched: it waits for this grid before it reads them
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  u.q_tok = it0.x;
   u.sk = it0.z;
   u.q_offset = it0.z - it0.y;  // position of the request's query 0 among its keys (negative: rows without keys)
   u.page_beg = it0.w;
@@ -655,19 +665,17 @@ __global__ void __launch_bounds__(THREADS, 1)
   u.n0 = it1.y;
   u.n1 = it1.z;
   u.kt0 = it2.x;
-  u.part = it2.z;
-  u.n_parts = it2.w;
-  u.packed = (it1.w & PACKED) != 0 ? 1 : 0;
-  u.P = u.packed ? a.G : 1;
+  const bool packed = (it1.w & PACKED) != 0;
+  u.P = packed ? a.G : 1;
   const bool split = (it1.w & SPLIT) != 0;
-  const int tile_tokens = u.packed ? a.T : BM;
+  const int tile_tokens = packed ? a.T : BM;
   // An item outside the query rows, the page list or the workspace (a plan made for
   // others) has no rows.
   const long long last_tok = static_cast<long long>(it1.x) + it1.y + it1.z;
   const bool bad = it0.x < 0 || it0.y < 0 || it0.z < 0 || it0.w < 0 || it1.x < 0 || it1.y < 1 || it1.z < 0 ||
                    it1.y > tile_tokens || it1.z > tile_tokens || (split && it1.z != 0) || last_tok > it0.y ||
                    it0.x + static_cast<long long>(it0.y) > a.total_q || it2.x < 0 || it2.y < it2.x ||
-                   (u.packed != 0) != (bid >= wide) ||
+                   packed != (bid >= wide) ||
                    it0.w + (static_cast<long long>(it0.z) + a.page - 1) / a.page > a.num_indices ||
                    (it2.z >= 0 && (it2.w < 1 || it2.z + (static_cast<long long>(it1.y) + it1.z - 1) * it2.w >= a.parts));
   if (bad) u.n0 = u.n1 = 0;
@@ -689,6 +697,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     u.nk[1] = u.nk[0] / 2;
     u.nk[0] -= u.nk[1];
   }
+  if (threadIdx.x == 0)
+    *reinterpret_cast<Place*>(u.sp + OFF_PLACE) =
+        Place{it0.x, u.row0, it2.z, it2.w, h, u.P, u.n0, u.n1, {u.nk[0], u.nk[1]}, {0, 0}};
 
   tc_fence_before();
   __syncthreads();
@@ -707,7 +718,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int half = 0; half < 2; ++half)
           tma_load_4d_elect(u.sb + OFF_Q + t * QTILE_BYTES + half * QBOX_BYTES, bid < wide ? &tmQ : &tmQP, u.bar(B_Q),
-                            64 * half, u.h, u.q_tok + u.row0 + (t ? u.n0 : 0), 0);
+                            64 * half, h, it0.x + u.row0 + (t ? u.n0 : 0), 0);
       __syncwarp();
       if (split)
         produce<true>(a, u, &tmK, true, lane);
