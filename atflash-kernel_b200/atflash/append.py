@@ -158,70 +158,66 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
     dev = _runtime.require_cuda(append_key, append_value, kc, vc)
     if torch.float8_e4m3fn in (kc.dtype, vc.dtype):
         raise ValueError("float8_e4m3fn pages need kv_scales")
-    k_level_major = kc.dim() == 5
-    for t in (append_key, append_value, vc) + (() if k_level_major else (kc,)):
-        if t.dtype != torch.bfloat16 or t.stride(-1) != 1 or t.shape[-1] != 128:
-            raise ValueError("keys, values and cache pages must be bf16 with a contiguous head_dim of 128")
-    if append_key.shape != append_value.shape or append_key.stride() != append_value.stride():
+    # (sizes and strides are read once: on a short step the checks' host time is the call's)
+    kcs, vcs, kct, vct = kc.shape, vc.shape, kc.stride(), vc.stride()
+    shape, st = append_key.shape, append_key.stride()
+    k_level_major = len(kcs) == 5
+    bf16 = torch.bfloat16
+    if (append_key.dtype != bf16 or append_value.dtype != bf16 or vc.dtype != bf16 or kc.dtype != bf16
+            or shape[-1] != 128 or vcs[-1] != 128 or st[-1] != 1 or vct[-1] != 1
+            or (not k_level_major and (kcs[-1] != 128 or kct[-1] != 1))):
+        raise ValueError("keys, values and cache pages must be bf16 with a contiguous head_dim of 128")
+    if shape != append_value.shape or st != append_value.stride():
         raise ValueError("append_key and append_value must have the same shape and strides")
     if k_level_major:
         # (P, Hkv, 8 levels, page, 16) sorted-pair K pages (see BatchDecodeWithPagedKVCacheWrapper.run)
-        if (kc.dtype != torch.bfloat16 or kc.shape[2] != 8 or kc.shape[4] != 16 or kc.stride(4) != 1
-                or kc.stride(3) != 16 or vc.dim() != 4 or kc.shape[0] != vc.shape[0]):
+        if (kcs[2] != 8 or kcs[4] != 16 or kct[4] != 1 or kct[3] != 16 or len(vcs) != 4 or kcs[0] != vcs[0]):
             raise ValueError("level-major k pages must be (P, Hkv, 8, page, 16) bf16 with 16-element rows")
         if rope is not None and out_layout != "sorted_pair":
             raise ValueError("level-major k pages hold sorted-pair K")
-    elif kc.shape != vc.shape or kc.stride() != vc.stride() or kc.dim() != 4:
+    elif kcs != vcs or kct != vct or len(kcs) != 4:
         raise ValueError("k and v pages must have the same 4-d shape and strides")
-    nnz, hkv, _ = append_key.shape
+    nnz, hkv, _ = shape
     if kv_layout == "NHD":
-        npages, page, hk2, _ = vc.shape
-        s_page, s_tok, s_head = vc.stride(0), vc.stride(1), vc.stride(2)
+        npages, page, hk2, _ = vcs
+        s_page, s_tok, s_head, _ = vct
     elif kv_layout == "HND":
-        npages, hk2, page, _ = vc.shape
-        s_page, s_head, s_tok = vc.stride(0), vc.stride(1), vc.stride(2)
+        npages, hk2, page, _ = vcs
+        s_page, s_head, s_tok, _ = vct
     else:
         raise ValueError("kv_layout must be NHD or HND")
     if hk2 != hkv:
         raise ValueError("append_key heads do not match the cache")
+    layout = _LAYOUTS[out_layout]
     norm = _k_norm(k_norm, rope, append_key, dev) if k_norm is not None else None
     bi, ps = _dev_i32(batch_indices, dev), _dev_i32(positions, dev)
     ip, ix = _dev_i32(kv_indptr, dev, kv_indices.numel()), _dev_i32(kv_indices, dev)
     if bi.numel() != nnz or ps.numel() != nnz:
         raise ValueError("batch_indices and positions need one entry per appended token")
-    p = _ffi.AtfAppendParams()
-    p.append_k, p.append_v, p.nnz = append_key.data_ptr(), append_value.data_ptr(), nnz
-    p.a_stride_n, p.a_stride_h = append_key.stride(0), append_key.stride(1)
-    p.batch_indices, p.positions = bi.data_ptr(), ps.data_ptr()
-    p.k_cache, p.v_cache, p.num_pages = kc.data_ptr(), vc.data_ptr(), npages
-    p.kv_stride_page, p.kv_stride_token, p.kv_stride_head = s_page, s_tok, s_head
-    p.num_kv_heads, p.head_dim, p.page_size, p.batch_size = hkv, 128, page, ip.numel() - 1
-    p.kv_indptr, p.kv_indices = ip.data_ptr(), ix.data_ptr()
-    keep = [bi, ps, ip, ix]
+    p = _ffi.AtfAppendParams(append_key.data_ptr(), append_value.data_ptr(), nnz, st[0], st[1], bi.data_ptr(),
+                             ps.data_ptr(), kc.data_ptr(), vc.data_ptr(), npages, s_page, s_tok, s_head, hkv, 128, page,
+                             ip.numel() - 1, ip.data_ptr(), ix.data_ptr())
     if rope is not None:
         cos, sin = rope
-        if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() != 2
-                or cos.shape[1] < 64 or cos.stride() != sin.stride() or cos.stride(1) != 1 or cos.device != dev
-                or sin.device != dev):
+        cst, csh = cos.stride(), cos.shape
+        if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or csh != sin.shape or len(csh) != 2
+                or csh[1] < 64 or cst != sin.stride() or cst[1] != 1 or cos.device != dev or sin.device != dev):
             raise ValueError("cos/sin must be matching fp32 (n_pos, >=64) tables")
-        p.cos, p.sin, p.cs_stride_pos, p.n_pos = cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0]
+        p.cos, p.sin, p.cs_stride_pos, p.n_pos = cos.data_ptr(), sin.data_ptr(), cst[0], csh[0]
         if rope_positions is not None:
             rp = rope_positions.to(device=dev, dtype=torch.int64).contiguous()
             if rp.numel() != nnz:
                 raise ValueError("rope_positions needs one entry per appended token")
-            keep.append(rp)
             p.rope_positions = rp.data_ptr()
-    p.out_layout = _LAYOUTS[out_layout]
-    p.error_flag = _runtime.error_flag(dev).data_ptr()
+    p.out_layout = layout
+    p.error_flag = _runtime.error_flag_ptr(dev)
     if k_level_major:
-        if kc.shape[1] != hkv or kc.shape[3] != page:
+        if kcs[1] != hkv or kcs[3] != page:
             raise ValueError("level-major k pages do not match the v pages")
         p.k_level_major = 1
-        p.k_stride_page, p.k_stride_head, p.k_stride_level = kc.stride(0), kc.stride(1), kc.stride(2)
+        p.k_stride_page, p.k_stride_head, p.k_stride_level = kct[0], kct[1], kct[2]
     if norm is not None:
         _runtime.launch("atf_paged_kv_append_norm", _ffi.load().atf_paged_kv_append_norm, dev, ctypes.byref(p), None,
                         ctypes.byref(norm))
-        return
-    with torch.cuda.device(dev):
-        rc = _ffi.load().atf_paged_kv_append(ctypes.byref(p), _runtime.stream_handle(dev))
-    _ffi.check("atf_paged_kv_append", rc)
+    else:
+        _runtime.launch("atf_paged_kv_append", _ffi.load().atf_paged_kv_append, dev, ctypes.byref(p))

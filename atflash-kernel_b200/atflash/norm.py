@@ -12,44 +12,52 @@ import torch
 from . import _ffi, _runtime
 
 _LAYOUTS = {"sorted_pair": _ffi.ATF_LAYOUT_SORTED_PAIR, "rotate_half": _ffi.ATF_LAYOUT_ROTATE_HALF}
+_ROW, _ONE = (128,), (1,)
 _WEIGHTS = {torch.bfloat16: _ffi.ATF_DTYPE_BF16, torch.float32: _ffi.ATF_DTYPE_F32}
 
 
 def check_norm(weight: torch.Tensor, eps: float, dev: torch.device, name: str) -> int:
     """Checks a norm's weights and eps; returns the weights' ATF_DTYPE."""
     dtype = _WEIGHTS.get(weight.dtype)
-    if dtype is None or weight.shape != (128,) or weight.stride(0) != 1 or weight.device != dev:
+    if dtype is None or weight.shape != _ROW or weight.stride() != _ONE or weight.device != dev:
         raise ValueError(f"{name} must be 128 contiguous bf16 or fp32 weights on {dev}")
-    if not (eps > 0.0 and math.isfinite(eps) and ctypes.c_float(eps).value > 0.0):
+    if not 1e-38 <= eps < math.inf:  # (a normal fp32 number)
         raise ValueError("the norm's eps must be a positive number")
     return dtype
 
 
 def refuse_gradients(*tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("atflash has no backward pass: call it under torch.no_grad() or with detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("atflash has no backward pass: call it under torch.no_grad() or with detached tensors")
 
 
-def _heads(x: torch.Tensor, name: str) -> Tuple[int, int, int, Tuple[int, int, int]]:
-    """(batch, seqlen, heads) and the strides of a (B, S, H, 128) or (T, H, 128) tensor."""
+def _heads(x: torch.Tensor, name: str) -> Tuple[torch.Size, Tuple[int, int, int]]:
+    """The shape of a (B, S, H, 128) or (T, H, 128) tensor and its strides (batch, token, head)."""
     shape, st = x.shape, x.stride()
-    if x.dtype != torch.bfloat16 or len(shape) not in (3, 4) or shape[-1] != 128 or st[-1] != 1:
+    n = len(shape)
+    if x.dtype != torch.bfloat16 or (n != 3 and n != 4) or shape[-1] != 128 or st[-1] != 1:
         raise ValueError(f"{name} must be (B, S, H, 128) or (T, H, 128) bf16 with a contiguous last axis")
-    if len(shape) == 3:
-        return 1, shape[0], shape[1], (0, st[0], st[1])
-    return shape[0], shape[1], shape[2], st[:3]
+    return shape, ((0, st[0], st[1]) if n == 3 else st[:3])
 
 
-def _output(out: Optional[torch.Tensor], x: torch.Tensor, name: str) -> torch.Tensor:
-    if out is None:
-        return torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
-    if out.shape != x.shape or out.dtype != torch.bfloat16 or out.device != x.device or out.stride(-1) != 1:
+def _output(out: torch.Tensor, x: torch.Tensor, name: str) -> Tuple[int, int, int]:
+    """Checks a caller's output; returns its strides (batch, token, head)."""
+    shape, st = out.shape, out.stride()
+    if shape != x.shape or out.dtype != torch.bfloat16 or out.device != x.device or st[-1] != 1:
         raise ValueError(f"{name} must be a bf16 {tuple(x.shape)} tensor on {x.device} with a contiguous last axis")
-    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+    if any(n > 1 and s == 0 for n, s in zip(shape, st)):
         raise ValueError(f"{name} must not be expanded: its rows are written")
-    if out.data_ptr() == x.data_ptr() and out.stride() != x.stride() and out.numel() > 0:
+    if out.data_ptr() == x.data_ptr() and st != x.stride() and out.numel() > 0:
         raise ValueError(f"{name} over its own input needs the input's strides")
-    return out
+    return (0, st[0], st[1]) if len(shape) == 3 else st[:3]
+
+
+def _fresh(shape: torch.Size) -> Tuple[int, int, int]:
+    """The strides (batch, token, head) of a new tensor."""
+    row = shape[-2] * 128
+    return (0 if len(shape) == 3 else shape[1] * row), row, 128
 
 
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.Tensor, k_weight: Optional[torch.Tensor],
@@ -71,47 +79,50 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.Ten
         raise ValueError("k and k_weight go together")
     refuse_gradients(q, k, q_weight, k_weight)
     dev = _runtime.require_cuda(q, cos, sin)
-    B, S, hq, qst = _heads(q, "q")
+    shape, qst = _heads(q, "q")
+    tokens = shape[:-2]
+    B, S = tokens if len(tokens) == 2 else (1, tokens[0])
     wt = check_norm(q_weight, eps, dev, "q_weight")
-    if out_layout not in _LAYOUTS:
+    layout = _LAYOUTS.get(out_layout)
+    if layout is None:
         raise ValueError(f"out_layout must be one of {sorted(_LAYOUTS)}")
     csh, cst = cos.shape, cos.stride()
     if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(csh) != 2 or csh != sin.shape or csh[0] < 1
             or csh[1] < 64 or cst != sin.stride() or cst[1] != 1):
         raise ValueError("cos/sin must be matching fp32 (n_pos, >=64) tables with a contiguous last axis")
-    q_out = _output(q_out, q, "q_out")
-    p = _ffi.AtfQkNormParams()
-    p.q, p.q_out, p.q_weight = q.data_ptr(), q_out.data_ptr(), q_weight.data_ptr()
-    p.batch, p.seqlen, p.num_heads_q, p.head_dim = B, S, hq, 128
-    p.q_stride_b, p.q_stride_s, p.q_stride_h = qst
-    _, _, _, ost = _heads(q_out, "q_out")
-    p.q_out_stride_b, p.q_out_stride_s, p.q_out_stride_h = ost
+    if q_out is None:
+        q_out, ost = torch.empty(shape, dtype=torch.bfloat16, device=dev), _fresh(shape)
+    else:
+        ost = _output(q_out, q, "q_out")
+    k_ptr = k_out_ptr = k_w = hk = 0
+    kst = kost = (0, 0, 0)
     if k is not None:
         if k.device != dev:
             raise ValueError("all tensors must be on the same device")
-        kb, ks, hk, kst = _heads(k, "k")
-        if (kb, ks) != (B, S) or k.dim() != q.dim():
+        kshape, kst = _heads(k, "k")
+        if kshape[:-2] != tokens:
             raise ValueError("q and k must hold the same tokens")
         if check_norm(k_weight, eps, dev, "k_weight") != wt:
             raise ValueError("q_weight and k_weight must have the same type")
-        k_out = _output(k_out, k, "k_out")
-        p.k, p.k_out, p.k_weight, p.num_heads_k = k.data_ptr(), k_out.data_ptr(), k_weight.data_ptr(), hk
-        p.k_stride_b, p.k_stride_s, p.k_stride_h = kst
-        _, _, _, ost = _heads(k_out, "k_out")
-        p.k_out_stride_b, p.k_out_stride_s, p.k_out_stride_h = ost
-    p.weight_dtype, p.eps, p.out_layout = wt, eps, _LAYOUTS[out_layout]
-    p.cos, p.sin, p.cs_stride_pos, p.n_pos = cos.data_ptr(), sin.data_ptr(), cst[0], csh[0]
-    p.pos_offset = int(pos_offset)
+        if k_out is None:
+            k_out, kost = torch.empty(kshape, dtype=torch.bfloat16, device=dev), _fresh(kshape)
+        else:
+            kost = _output(k_out, k, "k_out")
+        k_ptr, k_out_ptr, k_w, hk = k.data_ptr(), k_out.data_ptr(), k_weight.data_ptr(), kshape[-2]
+    pos, pos64, pst = 0, 0, (0, 0)
     if positions is not None:
         ps = positions.shape
         if (positions.dtype not in (torch.int32, torch.int64) or positions.device != dev
-                or (ps != (S,) and (q.dim() == 3 or ps != (B, S)))):
+                or (ps != tokens and ps != (S,))):
             raise ValueError(f"positions must be int32 or int64 on {dev}, one per token")
         st = positions.stride()
-        p.positions, p.positions_64 = positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0
-        p.pos_stride_b, p.pos_stride_s = (0, st[0]) if len(ps) == 1 else st
-    if csh[0] == 1:
-        p.cs_stride_pos = max(64, cst[0] & ~3)  # the only row's stride is any
+        pos, pos64 = positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0
+        pst = (0, st[0]) if len(ps) == 1 else st
     if B * S > 0:  # (tensors without tokens have no address)
+        p = _ffi.AtfQkNormParams(
+            q.data_ptr(), k_ptr, q_out.data_ptr(), k_out_ptr, B, S, shape[-2], hk, 128, *qst, *kst, *ost, *kost,
+            q_weight.data_ptr(), k_w, wt, eps, cos.data_ptr(), sin.data_ptr(),
+            # (the only row's stride is any)
+            cst[0] if csh[0] > 1 else max(64, cst[0] & ~3), csh[0], pos, pos64, *pst, int(pos_offset), layout)
         _runtime.launch("atf_qk_norm_rope", _ffi.load().atf_qk_norm_rope, dev, ctypes.byref(p))
     return q_out, k_out

@@ -11,7 +11,7 @@ Index reports of these calls go to ``atflash.check_device_errors()`` (code 2). T
 reference serves one request and has no counterpart."""
 import ctypes
 from dataclasses import dataclass
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -29,48 +29,49 @@ class PageMoves:
 
 def _list(t: torch.Tensor, name: str, dev: torch.device, n: Optional[int] = None) -> torch.Tensor:
     """An index list that a call reads, as contiguous int32."""
-    if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or (n is not None and t.numel() != n):
+    shape = t.shape
+    if len(shape) != 1 or (n is not None and shape[0] != n) or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be a 1-d integer tensor" + (f" of {n} entries" if n is not None else ""))
     if t.device != dev:
         raise ValueError("all tensors must be on the same device")
     return t if t.dtype == torch.int32 and t.is_contiguous() else _runtime.narrow_i32(t, dev)
 
 
-def _state(t: torch.Tensor, name: str, dev: torch.device, least: int = 1) -> torch.Tensor:
-    """A tensor that a call changes in place: taken as it is."""
-    if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < least:
+def _state(t: torch.Tensor, name: str, dev: torch.device, least: int = 1) -> int:
+    """A tensor that a call changes in place, taken as it is; returns its number of entries."""
+    shape = t.shape
+    if len(shape) != 1 or shape[0] < least or t.dtype != torch.int32 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-d int32 tensor" + (f" of {least} entries or more" if least > 1 else ""))
     if t.device != dev:
         raise ValueError("all tensors must be on the same device")
-    return t
+    return shape[0]
 
 
-def _table(p, req_pages: torch.Tensor, batch: int, page_size: int) -> torch.device:
-    """Fills the request table's fields of a params struct."""
+def _table(req_pages: torch.Tensor, batch: int, page_size: int) -> Tuple[torch.device, Tuple[int, int, int, int]]:
+    """Checks the request table; returns its device, and its address, row stride, rows and
+    pages per row."""
     dev = _runtime.require_cuda(req_pages)
     shape, st = req_pages.shape, req_pages.stride()
     if len(shape) != 2 or req_pages.dtype != torch.int32 or (shape[1] > 1 and st[1] != 1):
         raise ValueError("req_pages must be an int32 (rows, pages) tensor with contiguous rows")
-    if shape[0] < 1 or shape[1] < 1 or shape[0] > _ffi.ATF_PAGES_MAX_ROWS:
+    rows, width = shape
+    if rows < 1 or width < 1 or rows > _ffi.ATF_PAGES_MAX_ROWS:
         raise ValueError(f"req_pages must have between 1 and {_ffi.ATF_PAGES_MAX_ROWS} rows, of one page or more")
-    if shape[0] > 1 and st[0] < shape[1]:
+    if rows > 1 and st[0] < width:
         raise ValueError("the rows of req_pages must not overlap")
     if batch < 1 or batch > _ffi.ATF_TABLES_MAX_BATCH:
         raise ValueError(f"between 1 and {_ffi.ATF_TABLES_MAX_BATCH} requests")
-    if batch * shape[1] >= 1 << 30:
+    if batch * width >= 1 << 30:
         raise ValueError("requests x pages must be under 2^30")
     if page_size < 1:
         raise ValueError("page_size must be positive")
-    p.batch, p.page_size, p.req_pages = batch, int(page_size), req_pages.data_ptr()
-    p.req_stride, p.num_rows, p.max_req_pages = (st[0] if shape[0] > 1 else shape[1]), shape[0], shape[1]
-    p.error_flag = _runtime.error_flag_ptr(dev)
-    return dev
+    return dev, (req_pages.data_ptr(), st[0] if rows > 1 else width, rows, width)
 
 
-def _rows(req_rows: Optional[torch.Tensor], req_pages: torch.Tensor, batch: int, dev: torch.device):
+def _rows(req_rows: Optional[torch.Tensor], rows: int, batch: int, dev: torch.device) -> Optional[torch.Tensor]:
     if req_rows is not None:
         return _list(req_rows, "req_rows", dev, batch)
-    if req_pages.shape[0] < batch:
+    if rows < batch:
         raise ValueError("req_pages needs a row for each request")
     return None
 
@@ -90,21 +91,19 @@ def fork_requests(parents: torch.Tensor, children: torch.Tensor, kv_lens: torch.
     lengths out of range are left out. A page that the free list cannot give is -1 in the
     row, and its pair is -1. Each is reported (code 2). src and dst have one entry per
     child, -1 where there is nothing to copy; free_head itself stays."""
-    p = _ffi.AtfForkParams()
     n = parents.numel()
-    dev = _table(p, req_pages, n, page_size)
+    dev, table = _table(req_pages, n, page_size)
     parents, children = _list(parents, "parents", dev), _list(children, "children", dev, n)
     kv_lens = _list(kv_lens, "kv_lens", dev, n)
     free_pages, free_head = _list(free_pages, "free_pages", dev), _list(free_head, "free_head", dev, 1)
-    _state(shared, "shared", dev)
+    num_pages = _state(shared, "shared", dev)
     out = torch.empty(2 * n + 1, dtype=torch.int32, device=dev)
-    src = out.data_ptr()
-    p.parents, p.children, p.kv_lens = parents.data_ptr(), children.data_ptr(), kv_lens.data_ptr()
-    p.shared, p.num_pages = shared.data_ptr(), shared.numel()
-    # an empty list still has a head: any valid address will do for its pages
-    p.free_pages, p.free_head, p.num_free = free_pages.data_ptr() or free_head.data_ptr(), free_head.data_ptr(), \
-        free_pages.numel()
-    p.src, p.dst, p.free_head_out = src, src + 4 * n, src + 8 * n
+    src, head = out.data_ptr(), free_head.data_ptr()
+    p = _ffi.AtfForkParams(
+        parents.data_ptr(), children.data_ptr(), kv_lens.data_ptr(), n, int(page_size), *table, shared.data_ptr(), num_pages,
+        # an empty list still has a head: any valid address will do for its pages
+        free_pages.data_ptr() or head, head, src + 8 * n, free_pages.shape[0], src, src + 4 * n,
+        _runtime.error_flag_ptr(dev))
     _runtime.launch("atf_fork_requests", _ffi.load().atf_fork_requests, dev, ctypes.byref(p))
     return PageMoves(*out.split_with_sizes((n, n, 1)))
 
@@ -122,21 +121,18 @@ def free_requests(req_rows: Optional[torch.Tensor], kv_lens: torch.Tensor, req_p
     A row that is named twice (its first entry counts), rows and lengths out of range,
     page ids outside the cache, a page given up more often than it was held and a list
     without room are reported (code 2) and left out."""
-    p = _ffi.AtfFreeParams()
     n = kv_lens.numel()
-    dev = _table(p, req_pages, n, page_size)
+    dev, table = _table(req_pages, n, page_size)
     kv_lens = _list(kv_lens, "kv_lens", dev)
-    req_rows = _rows(req_rows, req_pages, n, dev)
-    _state(free_pages, "free_pages", dev)
+    req_rows = _rows(req_rows, table[2], n, dev)
+    num_free = _state(free_pages, "free_pages", dev)
     free_head = _list(free_head, "free_head", dev, 1)
+    num_pages = _state(shared, "shared", dev) if shared is not None else 0
     out = torch.empty(1, dtype=torch.int32, device=dev)
-    if req_rows is not None:
-        p.req_rows = req_rows.data_ptr()
-    if shared is not None:
-        _state(shared, "shared", dev)
-        p.shared, p.num_pages = shared.data_ptr(), shared.numel()
-    p.kv_lens, p.free_pages, p.num_free = kv_lens.data_ptr(), free_pages.data_ptr(), free_pages.numel()
-    p.free_head, p.free_head_out = free_head.data_ptr(), out.data_ptr()
+    p = _ffi.AtfFreeParams(
+        req_rows.data_ptr() if req_rows is not None else None, kv_lens.data_ptr(), n, int(page_size), *table,
+        shared.data_ptr() if shared is not None else None, num_pages, free_pages.data_ptr(), free_head.data_ptr(),
+        out.data_ptr(), num_free, _runtime.error_flag_ptr(dev))
     _runtime.launch("atf_free_requests", _ffi.load().atf_free_requests, dev, ctypes.byref(p))
     return out
 
@@ -155,25 +151,23 @@ def compact_pages(kv_lens: torch.Tensor, req_pages: torch.Tensor, page_size: int
 
     Pages that no named request holds count as free. Rows, lengths and page ids out of
     range are reported (code 2) and left out. At most 2^20 pages."""
-    p = _ffi.AtfCompactParams()
     n, num_pages, max_moves = kv_lens.numel(), int(num_pages), int(max_moves)
-    dev = _table(p, req_pages, n, page_size)
+    dev, table = _table(req_pages, n, page_size)
     if num_pages < 1 or num_pages > _ffi.ATF_COMPACT_MAX_PAGES:
         raise ValueError(f"between 1 and {_ffi.ATF_COMPACT_MAX_PAGES} pages")
     if max_moves < 0 or max_moves > num_pages:
         raise ValueError("max_moves must be between 0 and num_pages")
     kv_lens = _list(kv_lens, "kv_lens", dev)
-    req_rows = _rows(req_rows, req_pages, n, dev)
-    _state(free_pages, "free_pages", dev, num_pages)
+    req_rows = _rows(req_rows, table[2], n, dev)
+    num_free = _state(free_pages, "free_pages", dev, num_pages)
+    if shared is not None:
+        _state(shared, "shared", dev, num_pages)
     out = torch.empty(2 * max_moves + 1, dtype=torch.int32, device=dev)
     src = out.data_ptr()
-    if req_rows is not None:
-        p.req_rows = req_rows.data_ptr()
-    if shared is not None:
-        p.shared = _state(shared, "shared", dev, num_pages).data_ptr()
-    p.kv_lens, p.num_pages, p.max_moves = kv_lens.data_ptr(), num_pages, max_moves
-    p.free_pages, p.num_free = free_pages.data_ptr(), free_pages.numel()
-    p.src, p.dst, p.free_head_out = src, src + 4 * max_moves, src + 8 * max_moves
+    p = _ffi.AtfCompactParams(
+        req_rows.data_ptr() if req_rows is not None else None, kv_lens.data_ptr(), n, int(page_size), *table,
+        shared.data_ptr() if shared is not None else None, num_pages, max_moves, free_pages.data_ptr(),
+        src + 8 * max_moves, num_free, src, src + 4 * max_moves, _runtime.error_flag_ptr(dev))
     _runtime.launch("atf_compact_pages", _ffi.load().atf_compact_pages, dev, ctypes.byref(p))
     return PageMoves(*out.split_with_sizes((max_moves, max_moves, 1)))
 
@@ -203,7 +197,7 @@ class PageCopier:
                 raise ValueError("the pages of a cache tensor must not overlap")
             es = t.element_size()
             d.base, d.page_stride_bytes, d.page_bytes = t.data_ptr(), t.stride(0) * es, dense * es
-        self._caches, self._desc = caches, desc
+        self._caches, self._desc, self._desc_ptr = caches, desc, ctypes.addressof(desc)
 
     def copy(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Page src[i] of every tensor to page dst[i]; -1 on both sides is no copy, and
@@ -211,11 +205,12 @@ class PageCopier:
         and left out. The pages of dst differ from one another and are none of src's, as in
         the lists of ``fork_requests`` and ``compact_pages``; src may name a page twice."""
         src = _list(src, "src", self._dev)
-        dst = _list(dst, "dst", self._dev, src.numel())
-        if src.numel() == 0:
+        n = src.shape[0]
+        dst = _list(dst, "dst", self._dev, n)
+        if n == 0:
             return
-        p = _ffi.AtfCopyPagesParams(ctypes.addressof(self._desc), len(self._desc), self._pages, src.data_ptr(),
-                                    dst.data_ptr(), src.numel(), _runtime.error_flag_ptr(self._dev))
+        p = _ffi.AtfCopyPagesParams(self._desc_ptr, len(self._desc), self._pages, src.data_ptr(), dst.data_ptr(), n,
+                                    _runtime.error_flag_ptr(self._dev))
         _runtime.launch("atf_copy_pages", _ffi.load().atf_copy_pages, self._dev, ctypes.byref(p))
 
 

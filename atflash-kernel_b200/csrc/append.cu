@@ -10,8 +10,7 @@
 // whose page index lies outside the request's pages or the cache is skipped
 // and reported through the error flag (kDevErrIndex).
 //
-// With k_norm_weight, K is normed before it is rotated (norm_math.cuh): the 8 threads of a
-// row are neighbouring lanes, which share its sum of squares.
+// append_norm_kernel norms K before it rotates it.
 #include "atf_internal.h"
 #include "norm_math.cuh"
 #include "rope_math.cuh"
@@ -42,9 +41,9 @@ struct Args {
   const void* norm_w;
   int norm_f32;
   float eps;
+  unsigned units;  // of 4 U heads per token
 };
 
-template <bool NORM>
 __global__ void append_kernel(const Args a) {
   const long long gid = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (gid >= a.nnz * a.H * 8) return;
@@ -89,24 +88,82 @@ __global__ void append_kernel(const Args a) {
   long long rp = a.rope_pos != nullptr ? a.rope_pos[i] : pos;
   if (rp < 0) rp = 0;
   if (rp >= a.n_pos) rp = a.n_pos - 1;
-  if (NORM) {
-    // a row's 8 threads take the same branches up to here, so the group is whole
-    const unsigned group = 0xffu << (threadIdx.x & 24);
-    float x1[8], x2[8], w1[8], w2[8], cv[8], sv[8];
-    normmath::unpack(*reinterpret_cast<const uint4*>(a.ak + src + 8 * c), x1);
-    normmath::unpack(*reinterpret_cast<const uint4*>(a.ak + src + 64 + 8 * c), x2);
-    normmath::weights8(a.norm_w, a.norm_f32 != 0, 8 * c, w1);
-    normmath::weights8(a.norm_w, a.norm_f32 != 0, 64 + 8 * c, w2);
-    normmath::load8(a.cs + rp * a.cs_stride + 8 * c, cv);
-    normmath::load8(a.sn + rp * a.cs_stride + 8 * c, sv);
-    normmath::normalise(x1, x2, w1, w2, a.eps, group);
-    uint32_t o[8];
-    normmath::rotate(x1, x2, cv, sv, a.sorted != 0, o);
-    normmath::store_pairs(a.kc + kdst, c, a.sorted != 0, lstride, o);
-    return;
-  }
   ropemath::rotate_chunk(a.ak + src, a.cs + rp * a.cs_stride, a.sn + rp * a.cs_stride, a.kc + kdst, c,
                          a.sorted != 0, lstride);
+}
+
+// With a norm of K in front of the rotation (norm_math.cuh). A warp takes 4 U heads of a
+// token, 8 lanes a row as above, so that the token's page is looked up and its angles are
+// read once for them, while their rows are on the way.
+//
+// HBM-bound for prompts: 64K tokens x 8 heads take 96 us into pages of 16 (91% of HBM), 107
+// into level-major ones, whose K leaves in pieces of 32 bytes. A thread per (row, 8 pairs)
+// as above took 129 / 120 us (115 / 104 with the loads in front of the lookup), 4 heads a
+// warp 119 / 107, 8 heads with more registers and fewer CTAs 123 / 111. A step's tokens (too
+// few for two CTAs an SM) go by 4 heads.
+template <int U>
+__global__ void __launch_bounds__(256, U == 2 ? 3 : 4) append_norm_kernel(const Args a) {
+  __shared__ __align__(16) float s_w[128];
+  const int lane = threadIdx.x & 31, c = lane & 7;
+  if (threadIdx.x < 128) s_w[threadIdx.x] = normmath::weight_at(a.norm_w, a.norm_f32 != 0, threadIdx.x);
+  __syncthreads();
+  const unsigned unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);  // (the host keeps them within 32 bits)
+  const unsigned i = unit / a.units;
+  if (i >= a.nnz) return;
+  const int h0 = static_cast<int>(unit - i * a.units) * (4 * U) + (lane >> 3);
+  const int b = a.batch_indices[i];
+  const int pos = a.positions[i];
+  uint4 k0[U], k1[U], v0[U], v1[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long src = i * a.as_n + static_cast<long long>(min(h0 + 4 * u, a.H - 1)) * a.as_h;
+    k0[u] = *reinterpret_cast<const uint4*>(a.ak + src + 8 * c);
+    k1[u] = *reinterpret_cast<const uint4*>(a.ak + src + 64 + 8 * c);
+    v0[u] = *reinterpret_cast<const uint4*>(a.av + src + 8 * c);
+    v1[u] = *reinterpret_cast<const uint4*>(a.av + src + 64 + 8 * c);
+  }
+  long long rp = a.rope_pos != nullptr ? a.rope_pos[i] : pos;
+  rp = rp < 0 ? 0 : (rp >= a.n_pos ? a.n_pos - 1 : rp);
+  float cv[8], sv[8];
+  normmath::load8(a.cs + rp * a.cs_stride + 8 * c, cv);
+  normmath::load8(a.sn + rp * a.cs_stride + 8 * c, sv);
+  bool bad = b < 0 || b >= a.B || pos < 0;
+  long long page = -1;
+  if (!bad) {
+    const int pidx = a.kv_indptr[b] + pos / a.page_size;
+    bad = pidx >= a.kv_indptr[b + 1];
+    if (!bad) {
+      page = a.kv_indices[pidx];
+      bad = page < 0 || page >= a.num_pages;
+    }
+  }
+  if (bad) {
+    if (a.err != nullptr && lane == 0) atomicCAS(a.err, 0, kDevErrIndex);
+    return;
+  }
+  const int slot = pos % a.page_size;
+  const long long lstride = a.k_lm ? a.k_s_level : 16;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = h0 + 4 * u;
+    const bool on = h < a.H;
+    const long long dst = page * a.s_page + slot * a.s_tok + h * a.s_head;
+    if (on) {
+      *reinterpret_cast<uint4*>(a.vc + dst + 8 * c) = v0[u];
+      *reinterpret_cast<uint4*>(a.vc + dst + 64 + 8 * c) = v1[u];
+    }
+    float x1[8], x2[8], w1[8], w2[8];
+    normmath::unpack(k0[u], x1);
+    normmath::unpack(k1[u], x2);
+    normmath::load8(&s_w[8 * c], w1);
+    normmath::load8(&s_w[64 + 8 * c], w2);
+    normmath::normalise(x1, x2, w1, w2, a.eps, 0xffffffffu);
+    uint32_t o[8];
+    normmath::rotate(x1, x2, cv, sv, a.sorted != 0, o);
+    if (on)
+      normmath::store_pairs(a.kc + (a.k_lm ? page * a.k_s_page + h * a.k_s_head + slot * 16 : dst), c, a.sorted != 0,
+                            lstride, o);
+  }
 }
 
 }  // namespace append
@@ -186,15 +243,24 @@ int atf::append_bf16(const AtfAppendParams* p, const AtfKNorm* norm, atf_stream_
   a.k_s_head = p->k_stride_head;
   a.k_s_level = p->k_stride_level;
   const int threads = 256;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (norm != nullptr) {
+    a.norm_w = norm->weight;
+    a.norm_f32 = norm->weight_dtype == ATF_DTYPE_F32 ? 1 : 0;
+    a.eps = norm->eps;
+    const long long narrow = (a.H + 3) / 4, wide = (a.H + 7) / 8;
+    if (a.nnz > (1ll << 30) / narrow) return ATF_ERR_UNSUPPORTED;
+    const bool many = a.nnz * wide >= 2ll * 148 * 8;
+    a.units = static_cast<unsigned>(many ? wide : narrow);
+    const unsigned blocks = static_cast<unsigned>((a.nnz * a.units + 7) / 8);
+    if (many)
+      append::append_norm_kernel<2><<<blocks, threads, 0, st>>>(a);
+    else
+      append::append_norm_kernel<1><<<blocks, threads, 0, st>>>(a);
+    return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
+  }
   const long long blocks = (total + threads - 1) / threads;
   if (blocks > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
-  a.norm_w = norm != nullptr ? norm->weight : nullptr;
-  a.norm_f32 = norm != nullptr && norm->weight_dtype == ATF_DTYPE_F32 ? 1 : 0;
-  a.eps = norm != nullptr ? norm->eps : 0.f;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (a.norm_w != nullptr)
-    append::append_kernel<true><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
-  else
-    append::append_kernel<false><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
+  append::append_kernel<<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
 }

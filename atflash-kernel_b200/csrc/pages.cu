@@ -22,8 +22,11 @@
 // the free list is the rising list of what is free afterwards. Then the tables and the
 // counts follow. One launch.
 //
-// Copy: 16 KB pieces of (pair, tensor) over the grid, 16 bytes per lane and load, four
-// loads in flight. HBM-bound.
+// Copy: 16 KB pieces of (pair, tensor) over the grid, 16 bytes per lane and load, eight
+// loads in flight. HBM-bound: 2144 pairs x 4 tensors x 64 KB 174 us (floor 173); with four
+// loads and eight CTAs of 256 an SM, each going through its pieces, 209 (191 with eight
+// loads). Up to 128 CTAs an SM wait their turn; more bring nothing, and lists that are
+// mostly padding want few.
 //
 // What bounds the first three: the launch and a few dependent reads of the tables.
 #include <cooperative_groups.h>
@@ -441,8 +444,9 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) compa
 // ------------------------------------------------------------------ copy
 
 constexpr int MAX_TENSORS = ATF_COPY_MAX_TENSORS;
-constexpr int COPY_THREADS = 256;
-constexpr int PIECE = COPY_THREADS * 64;  // bytes: four 16-byte loads per thread
+constexpr int COPY_THREADS = 128;
+constexpr int COPY_LOADS = 8;
+constexpr int PIECE = COPY_THREADS * COPY_LOADS * 16;  // bytes
 
 struct CopyArgs {
   const int32_t* src;
@@ -458,7 +462,7 @@ struct CopyArgs {
 
 template <typename T>
 __device__ __forceinline__ void copy_piece(const uint8_t* from, uint8_t* to, int bytes) {
-  constexpr int U = 4;
+  constexpr int U = COPY_LOADS;
   const T* f = reinterpret_cast<const T*>(from);
   T* d = reinterpret_cast<T*>(to);
   const int n = bytes / static_cast<int>(sizeof(T));
@@ -625,7 +629,7 @@ extern "C" int atf_copy_pages(const AtfCopyPagesParams* p, atf_stream_t stream) 
     }
     a.first[a.tensors] = static_cast<int>(pieces);
     a.pieces = static_cast<int>(pieces);
-    const long long all = pieces * a.n, most = 148ll * 8;
+    const long long all = pieces * a.n, most = 148ll * 128;
     pages::copy_kernel<<<static_cast<unsigned>(all < most ? all : most), pages::COPY_THREADS, 0,
                          reinterpret_cast<cudaStream_t>(stream)>>>(a);
     if (cudaGetLastError() != cudaSuccess) return ATF_ERR_CUDA;

@@ -79,18 +79,28 @@ __device__ __forceinline__ void qk_rows_asm(uint32_t d_tmem, uint64_t qd, uint64
 
 constexpr int WARP_V = 10;  // the V producer (WARP_LOAD: Q and K)
 constexpr uint32_t QBOX_BYTES = QTILE_BYTES / 2;
+// Shared memory: seven slots of 32 KB. Two tiles of Q, two stages of K and three of V; or one
+// tile of Q and three stages each where the groups share out the keys, where a step takes
+// two of each.
+constexpr int V_STAGES = 3;
+template <bool SPLIT_KEYS>
+constexpr int K_STAGES = SPLIT_KEYS ? 3 : 2;
+constexpr uint32_t SLOT = 32 * 1024;
+static_assert(QTILE_BYTES == SLOT && KSTAGE_BYTES == SLOT && VSTAGE_BYTES == SLOT, "one size for all");
 constexpr uint32_t OFF_Q = 0;
-constexpr uint32_t OFF_K = OFF_Q + NQ * QTILE_BYTES;
-constexpr uint32_t OFF_V = OFF_K + KST * KSTAGE_BYTES;
-constexpr uint32_t OFF_BAR = OFF_V + VST * VSTAGE_BYTES;
+template <bool SPLIT_KEYS>
+constexpr uint32_t OFF_K = (SPLIT_KEYS ? 1 : 2) * SLOT;
+constexpr uint32_t OFF_V = 4 * SLOT;
+constexpr uint32_t OFF_STATE = 3 * SLOT;  // [t][128] of (max, sum), in K's place once all products are done
+constexpr uint32_t OFF_BAR = 7 * SLOT;
 
 enum {
   B_Q = 0,
   B_KFULL = 1,
-  B_KEMPTY = B_KFULL + KST,
-  B_VFULL = B_KEMPTY + KST,
-  B_VEMPTY = B_VFULL + VST,
-  B_SFULL = B_VEMPTY + VST,   // [t]
+  B_KEMPTY = B_KFULL + 3,
+  B_VFULL = B_KEMPTY + 3,
+  B_VEMPTY = B_VFULL + V_STAGES,
+  B_SFULL = B_VEMPTY + V_STAGES,  // [t]
   B_PFULL = B_SFULL + NQ,     // [t]
   B_ODONE = B_PFULL + NQ,     // [t], one phase per O += P V
   B_OFINAL = B_ODONE + NQ,    // [t], single phase: the group's last O += P V done
@@ -98,8 +108,7 @@ enum {
   B_FINAL = B_LOADED + NQ,
   NUM_BARS
 };
-constexpr uint32_t OFF_STATE = OFF_BAR + 8 * ((NUM_BARS + 1) / 2 * 2);  // [t][128] of (max, sum)
-constexpr uint32_t OFF_PLACE = OFF_STATE + NQ * BM * 8;                 // Place
+constexpr uint32_t OFF_PLACE = OFF_BAR + 8 * ((NUM_BARS + 1) / 2 * 2);  // Place
 constexpr uint32_t OFF_ABORT = OFF_PLACE + 48;
 constexpr uint32_t OFF_TMEM = OFF_ABORT + 16;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16 + 1024;  // slack for 1024-B alignment
@@ -201,8 +210,9 @@ __device__ __forceinline__ void load_slices(const Args& a, const Unit& u, const 
 template <bool SPLIT_KEYS>
 __device__ __forceinline__ void produce(const Args& a, const Unit& u, const CUtensorMap* map, bool is_k, int lane) {
   const int tiles = SPLIT_KEYS ? u.nk[0] + u.nk[1] : max(u.nk[0], u.nk[1]);
-  const int stages = is_k ? KST : VST, full = is_k ? B_KFULL : B_VFULL, empty = is_k ? B_KEMPTY : B_VEMPTY;
-  const uint32_t base = u.sb + (is_k ? OFF_K : OFF_V), bytes = is_k ? KSTAGE_BYTES : VSTAGE_BYTES;
+  const int stages = is_k ? K_STAGES<SPLIT_KEYS> : V_STAGES;
+  const int full = is_k ? B_KFULL : B_VFULL, empty = is_k ? B_KEMPTY : B_VEMPTY;
+  const uint32_t base = u.sb + (is_k ? OFF_K<SPLIT_KEYS> : OFF_V);
   int issued = 0;
   int id = tiles > 0 ? slice_page(a, u, u.kt0, lane) : -1;
   for (int g = 0; g < tiles; ++g) {
@@ -217,7 +227,7 @@ __device__ __forceinline__ void produce(const Args& a, const Unit& u, const CUte
         if (SPLIT_KEYS ? t == 0 : g < u.nk[t]) L = max(L, levels_for(u.lim[t], kt));
       halves = L > 4 ? 2 : 1;
     }
-    load_slices(a, u, map, base + s * bytes, u.bar(full + s), kt, id, halves, lane);
+    load_slices(a, u, map, base + s * SLOT, u.bar(full + s), kt, id, halves, lane);
     issued = g + 1;
     id = next;
   }
@@ -230,9 +240,10 @@ __device__ __forceinline__ void produce(const Args& a, const Unit& u, const CUte
 
 template <bool SPLIT_KEYS>
 __device__ __forceinline__ void issue_mmas(const Args& a, const Unit& u, int lane) {
+  constexpr int KS = K_STAGES<SPLIT_KEYS>, VS = V_STAGES;
   const uint32_t tm = __shfl_sync(FULL, u.tmem, 0);
   const uint64_t qdesc0 = make_sdesc(u.sb + OFF_Q, 16, 1024, kLayoutSw128);
-  const uint64_t kdesc0 = make_sdesc(u.sb + OFF_K, 16, 1024, kLayoutSw128);
+  const uint64_t kdesc0 = make_sdesc(u.sb + OFF_K<SPLIT_KEYS>, 16, 1024, kLayoutSw128);
   const uint64_t vdesc0 = make_sdesc(u.sb + OFF_V, VBOX_BYTES, 1024, kLayoutSw128);
   const int nk0 = u.nk[0], nk1 = u.nk[1], nk_max = max(nk0, nk1);
   // S_t(i) into group t's S columns
@@ -240,11 +251,11 @@ __device__ __forceinline__ void issue_mmas(const Args& a, const Unit& u, int lan
     const int g = nth<SPLIT_KEYS>(t, i);
     const int L = levels_for(u.lim[SPLIT_KEYS ? 0 : t], u.kt0 + g);
     qk_rows_asm(tm + static_cast<uint32_t>(t * 128), qdesc0 + (SPLIT_KEYS ? 0 : (t * QTILE_BYTES) >> 4),
-                kdesc0 + (((g % KST) * KSTAGE_BYTES) >> 4), IDESC_QK, L, u.bar(B_SFULL + t));
+                kdesc0 + (((g % KS) * SLOT) >> 4), IDESC_QK, L, u.bar(B_SFULL + t));
   };
   // O_t += P_t(i) V; P_t sits in columns 64..127 of the other group's S
   auto issue_PV = [&](int t, int i) {
-    const uint64_t vd = vdesc0 + (((nth<SPLIT_KEYS>(t, i) % VST) * VSTAGE_BYTES) >> 4);
+    const uint64_t vd = vdesc0 + (((nth<SPLIT_KEYS>(t, i) % VS) * SLOT) >> 4);
     pv_group_asm(tm + 256u + static_cast<uint32_t>(t * 128), tm + static_cast<uint32_t>((1 - t) * 128 + 64), vd, IDESC_PV,
                  i > 0 ? 1u : 0u, u.bar(B_ODONE + t));
   };
@@ -253,18 +264,18 @@ __device__ __forceinline__ void issue_mmas(const Args& a, const Unit& u, int lan
   auto kwait = [&](int g) -> bool {
     while (k_waited < g) {
       ++k_waited;
-      if (!__all_sync(FULL, mbar_wait_inl(u.bar(B_KFULL + k_waited % KST), (k_waited / KST) & 1, u.ab, kDevErrTimeout)))
+      if (!__all_sync(FULL, mbar_wait_inl(u.bar(B_KFULL + k_waited % KS), (k_waited / KS) & 1, u.ab, kDevErrTimeout)))
         return false;
       tc_fence_after();
     }
     return true;
   };
   auto vwait = [&](int g) -> bool {
-    if (!__all_sync(FULL, mbar_wait_inl(u.bar(B_VFULL + g % VST), (g / VST) & 1, u.ab, kDevErrTimeout))) return false;
+    if (!__all_sync(FULL, mbar_wait_inl(u.bar(B_VFULL + g % VS), (g / VS) & 1, u.ab, kDevErrTimeout))) return false;
     // V rows past the request's last key hold another time's bytes, or nothing
     const int live = u.sk - (u.kt0 + g) * BN;
     if (live < BN) {
-      uint8_t* v0 = u.sp + OFF_V + (g % VST) * VSTAGE_BYTES;
+      uint8_t* v0 = u.sp + OFF_V + (g % VS) * SLOT;
       for (int e = live * 8 + lane; e < BN * 8; e += 32) {
         *reinterpret_cast<uint4*>(v0 + 16 * e) = make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>(v0 + VBOX_BYTES + 16 * e) = make_uint4(0, 0, 0, 0);
@@ -293,7 +304,7 @@ __device__ __forceinline__ void issue_mmas(const Args& a, const Unit& u, int lan
   // S_0(1) once group 0 has read S_0(0)
   if (ok && nk0 > 1 && (ok = kwait(nth<SPLIT_KEYS>(0, 1)) && wait_for(B_LOADED, 0, 0))) {
     issue_S(0, 1);
-    if (SPLIT_KEYS || 1 >= nk1) tc_commit_elect(u.bar(B_KEMPTY + nth<SPLIT_KEYS>(0, 1) % KST));
+    if (SPLIT_KEYS || 1 >= nk1) tc_commit_elect(u.bar(B_KEMPTY + nth<SPLIT_KEYS>(0, 1) % KS));
   }
   for (int i = 0; ok && i < nk_max; ++i) {
     if (!SPLIT_KEYS && !(ok = vwait(i))) break;
@@ -302,30 +313,30 @@ __device__ __forceinline__ void issue_mmas(const Args& a, const Unit& u, int lan
       if (!(ok = wait_for(B_PFULL, 0, i))) break;
       issue_PV(0, i);
       if (i + 1 == nk0) tc_commit_elect(u.bar(B_OFINAL + 0));
-      if (SPLIT_KEYS) tc_commit_elect(u.bar(B_VEMPTY + (2 * i) % VST));
+      if (SPLIT_KEYS) tc_commit_elect(u.bar(B_VEMPTY + (2 * i) % VS));
     }
     // S_1(i+1) overwrites the columns P_0(i) occupies (O_0 += P_0(i) V was issued first;
     // tcgen05.mma ops of one thread run in order) and needs group 1 to have read S_1(i)
     if (i + 1 < nk1) {
       if (!(ok = kwait(nth<SPLIT_KEYS>(1, i + 1)) && wait_for(B_LOADED, 1, i))) break;
       issue_S(1, i + 1);
-      tc_commit_elect(u.bar(B_KEMPTY + nth<SPLIT_KEYS>(1, i + 1) % KST));
+      tc_commit_elect(u.bar(B_KEMPTY + nth<SPLIT_KEYS>(1, i + 1) % KS));
     }
     if (i < nk1) {
       if (SPLIT_KEYS && !(ok = vwait(2 * i + 1))) break;
       if (!(ok = wait_for(B_PFULL, 1, i))) break;
       issue_PV(1, i);
       if (i + 1 == nk1) tc_commit_elect(u.bar(B_OFINAL + 1));
-      if (SPLIT_KEYS) tc_commit_elect(u.bar(B_VEMPTY + (2 * i + 1) % VST));
+      if (SPLIT_KEYS) tc_commit_elect(u.bar(B_VEMPTY + (2 * i + 1) % VS));
     }
     // S_0(i+2): after O_1 += P_1(i) V (P_1(i) sits in S_0's columns) and group 0's read
     // of S_0(i+1)
     if (i + 2 < nk0) {
       if (!(ok = kwait(nth<SPLIT_KEYS>(0, i + 2)) && wait_for(B_LOADED, 0, i + 1))) break;
       issue_S(0, i + 2);
-      if (SPLIT_KEYS || i + 2 >= nk1) tc_commit_elect(u.bar(B_KEMPTY + nth<SPLIT_KEYS>(0, i + 2) % KST));
+      if (SPLIT_KEYS || i + 2 >= nk1) tc_commit_elect(u.bar(B_KEMPTY + nth<SPLIT_KEYS>(0, i + 2) % KS));
     }
-    if (!SPLIT_KEYS) tc_commit_elect(u.bar(B_VEMPTY + i % VST));
+    if (!SPLIT_KEYS) tc_commit_elect(u.bar(B_VEMPTY + i % VS));
   }
   // Every MMA issued by this CTA completes before TMEM is released.
   tc_commit_elect(u.bar(B_FINAL));
@@ -525,13 +536,13 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
     // both groups' states of the row: (max, sum) through shared memory, O from TMEM, where
     // the row has the same lane in both. Group t stores half t of the dims.
     float2* state = reinterpret_cast<float2*>(u.sp + OFF_STATE);
-    state[t * BM + r] = make_float2(m2, l);
 #pragma unroll
     for (int k = 0; k < NQ; ++k)
       if (ok && to.nk[k] > 0) ok = __all_sync(FULL, mbar_wait_inl(u.bar(B_OFINAL + k), 0, u.ab, kDevErrTimeout));
     // (without keys nothing has read Q, whose place the outputs take)
     if (ok && to.nk[0] == 0) ok = __all_sync(FULL, mbar_wait_inl(u.bar(B_Q), 0, u.ab, kDevErrTimeout));
     tc_fence_after();
+    if (ok) state[t * BM + r] = make_float2(m2, l);
     __syncwarp();
     asm volatile("bar.sync 1, 256;" ::: "memory");  // every softmax thread of the CTA comes here
     if (!ok) return;
@@ -629,11 +640,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   const bool stop0 = threadIdx.x == 0 && stops(a.err);
   if (threadIdx.x == 0) {
     mbar_init(u.bar(B_Q), 1);
-    for (int s = 0; s < KST; ++s) {
+    for (int s = 0; s < 3; ++s) {
       mbar_init(u.bar(B_KFULL + s), 1);
       mbar_init(u.bar(B_KEMPTY + s), 1);
     }
-    for (int s = 0; s < VST; ++s) {
+    for (int s = 0; s < V_STAGES; ++s) {
       mbar_init(u.bar(B_VFULL + s), 1);
       mbar_init(u.bar(B_VEMPTY + s), 1);
     }
@@ -833,10 +844,11 @@ struct Block {
   float cost() const { return tiles * step; }
 };
 
-// Measured on the device: 1.6 us for a step of two tiles of rows against a key tile, half of
-// that per key tile where the keys are shared out between the groups; 5 us of a CTA's start
-// and end, 3 more for writing states and merging them.
-constexpr float STEP_US = 1.6f, START_US = 5.f, STATES_US = 3.f;
+// Measured on the device, with K and V in L2 and all SMs at work: 2.2 us for a step of two
+// tiles of rows against a key tile; 1.4 us per key tile where the groups share out the keys
+// (1.6 with pages of 16, and HBM takes 1.5 for its 64 KB per SM); 5 us of a CTA's start and
+// end, 3 more for writing states and merging them.
+constexpr float STEP_US = 2.2f, SHARED_US = 1.5f, START_US = 5.f, STATES_US = 3.f;
 
 // when the last CTA ends if the blocks are cut into pieces of at most `most` us: the
 // hardware takes items in order, each for the first SM that is free
@@ -916,7 +928,7 @@ extern "C" int atf_prefill_paged_plan(const AtfPrefillPagedPlanParams* p, int32_
         kend = kend > nk ? nk : (kend < 0 ? 0 : kend);
         x.tiles = static_cast<int>((kend + BN - 1) / BN);
         x.units = pack ? p->num_kv_heads : p->num_qo_heads;
-        x.step = it.n1 == 0 ? STEP_US / 2 : STEP_US;
+        x.step = it.n1 == 0 ? SHARED_US : STEP_US;
         it.part = -1;
         it.n_parts = 1;
         blocks.push_back(x);

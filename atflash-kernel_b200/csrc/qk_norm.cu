@@ -13,7 +13,10 @@
 //
 // What bounds it: HBM for prompts, 512 bytes in and out per row; the launch and one
 // chain of loads (position -> angles -> row) for a step's tokens, where U = 1 spreads
-// them over more SMs.
+// them over more SMs. The loads in flight are what counts for prompts: 65521 tokens x 32
+// heads take 191 us (88% of HBM) with 16 heads a warp and four CTAs an SM (64 registers),
+// 196 with three, 202 with 32 heads and two, 216 with 8 heads and four; indexes in 64
+// bits cost 12 us, and streaming hints on loads or stores change nothing.
 #include "atf_internal.h"
 #include "norm_math.cuh"
 
@@ -31,8 +34,8 @@ struct Part {  // the query heads, or the key heads
 struct Args {
   Part p[2];
   int Hq, H;  // query heads, all heads
-  long long S, tokens;
-  int units;  // of 4 U heads per token
+  unsigned S, tokens;
+  unsigned units;  // of 4 U heads per token
   int w32, pos64, sorted;
   float eps;
   const float* cs;
@@ -43,7 +46,7 @@ struct Args {
 };
 
 template <int U>
-__global__ void __launch_bounds__(WARPS * 32) qk_norm_kernel(const Args a) {
+__global__ void __launch_bounds__(WARPS * 32, 4) qk_norm_kernel(const Args a) {
   __shared__ __align__(16) float s_w[2][128];
   const int tid = threadIdx.x, lane = tid & 31, c = lane & 7;
   {
@@ -51,11 +54,11 @@ __global__ void __launch_bounds__(WARPS * 32) qk_norm_kernel(const Args a) {
     s_w[tid >> 7][tid & 127] = w != nullptr ? normmath::weight_at(w, a.w32, tid & 127) : 0.f;
   }
   __syncthreads();
-  const long long unit = static_cast<long long>(blockIdx.x) * WARPS + (tid >> 5);
-  const long long t = unit / a.units;
+  const unsigned unit = blockIdx.x * WARPS + (tid >> 5);  // all units and a CTA more fit 32 bits
+  const unsigned t = unit / a.units;
   if (t >= a.tokens) return;
-  const int h0 = static_cast<int>(unit % a.units) * (4 * U) + (lane >> 3);
-  const long long b = t / a.S, s = t % a.S;
+  const int h0 = static_cast<int>(unit - t * a.units) * (4 * U) + (lane >> 3);
+  const long long b = t / a.S, s = t - static_cast<unsigned>(b) * a.S;
   long long pos = a.pos_offset + s;
   if (a.positions != nullptr) {
     const long long at = b * a.pos_b + s * a.pos_s;
@@ -132,9 +135,12 @@ extern "C" int atf_qk_norm_rope(const AtfQkNormParams* p, atf_stream_t stream) {
   qknorm::Args a = {};
   a.Hq = static_cast<int>(p->num_heads_q);
   a.H = static_cast<int>(p->num_heads_q + p->num_heads_k);
-  a.S = p->seqlen;
-  a.tokens = p->batch * p->seqlen;
-  if (a.tokens == 0 || a.H == 0) return ATF_OK;
+  if (p->batch == 0 || p->seqlen == 0 || a.H == 0) return ATF_OK;
+  const long long narrow = (a.H + 3) / 4;  // units of 4 heads a token
+  if (p->batch > (1ll << 30) || p->seqlen > (1ll << 30) || p->batch * p->seqlen > (1ll << 30) / narrow)
+    return ATF_ERR_UNSUPPORTED;
+  a.S = static_cast<unsigned>(p->seqlen);
+  a.tokens = static_cast<unsigned>(p->batch * p->seqlen);
   int dev = 0;
   int rc = check_device(&dev);
   if (rc != ATF_OK) return rc;
@@ -157,11 +163,10 @@ extern "C" int atf_qk_norm_rope(const AtfQkNormParams* p, atf_stream_t stream) {
   a.pos_s = p->pos_stride_s;
   a.pos_offset = p->pos_offset;
   // 16 heads per warp once that gives every SM two CTAs, else 4
-  const int wide = (a.H + 15) / 16, narrow = (a.H + 3) / 4;
+  const long long wide = (a.H + 15) / 16;
   const bool many = a.tokens * wide >= 2ll * 148 * qknorm::WARPS;
-  a.units = many ? wide : narrow;
-  const long long blocks = (a.tokens * a.units + qknorm::WARPS - 1) / qknorm::WARPS;
-  if (blocks > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
+  a.units = static_cast<unsigned>(many ? wide : narrow);
+  const long long blocks = (static_cast<long long>(a.tokens) * a.units + qknorm::WARPS - 1) / qknorm::WARPS;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (many)
     qknorm::qk_norm_kernel<4><<<static_cast<unsigned>(blocks), qknorm::WARPS * 32, 0, st>>>(a);
