@@ -54,12 +54,6 @@ def _output(out: torch.Tensor, x: torch.Tensor, name: str) -> Tuple[int, int, in
     return (0, st[0], st[1]) if len(shape) == 3 else st[:3]
 
 
-def _fresh(shape: torch.Size) -> Tuple[int, int, int]:
-    """The strides (batch, token, head) of a new tensor."""
-    row = shape[-2] * 128
-    return (0 if len(shape) == 3 else shape[1] * row), row, 128
-
-
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.Tensor, k_weight: Optional[torch.Tensor],
                  cos: torch.Tensor, sin: torch.Tensor, *, eps: float = 1e-6, pos_offset: int = 0,
                  positions: Optional[torch.Tensor] = None, out_layout: str = "rotate_half",
@@ -91,7 +85,9 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.Ten
             or csh[1] < 64 or cst != sin.stride() or cst[1] != 1):
         raise ValueError("cos/sin must be matching fp32 (n_pos, >=64) tables with a contiguous last axis")
     if q_out is None:
-        q_out, ost = torch.empty(shape, dtype=torch.bfloat16, device=dev), _fresh(shape)
+        q_out = torch.empty_like(q)
+        st = q_out.stride()
+        ost = (0, st[0], st[1]) if len(st) == 3 else st[:3]
     else:
         ost = _output(q_out, q, "q_out")
     k_ptr = k_out_ptr = k_w = hk = 0
@@ -105,7 +101,9 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.Ten
         if check_norm(k_weight, eps, dev, "k_weight") != wt:
             raise ValueError("q_weight and k_weight must have the same type")
         if k_out is None:
-            k_out, kost = torch.empty(kshape, dtype=torch.bfloat16, device=dev), _fresh(kshape)
+            k_out = torch.empty_like(k)
+            st = k_out.stride()
+            kost = (0, st[0], st[1]) if len(st) == 3 else st[:3]
         else:
             kost = _output(k_out, k, "k_out")
         k_ptr, k_out_ptr, k_w, hk = k.data_ptr(), k_out.data_ptr(), k_weight.data_ptr(), kshape[-2]

@@ -146,7 +146,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         if qst[2] != 1 or kst[3] != 1 or vst[3] != 1:
             raise ValueError("the head_dim axis must be contiguous")
         if out is None:
-            out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+            out = q.new_empty(shape)
         elif out.shape != shape or out.dtype != torch.bfloat16 or out.device != dev or out.stride(-1) != 1:
             raise ValueError(f"out must be a bf16 {shape} tensor on {dev} with a contiguous head_dim axis")
         if return_lse and lse is None:

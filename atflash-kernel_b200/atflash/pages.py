@@ -97,7 +97,7 @@ def fork_requests(parents: torch.Tensor, children: torch.Tensor, kv_lens: torch.
     kv_lens = _list(kv_lens, "kv_lens", dev, n)
     free_pages, free_head = _list(free_pages, "free_pages", dev), _list(free_head, "free_head", dev, 1)
     num_pages = _state(shared, "shared", dev)
-    out = torch.empty(2 * n + 1, dtype=torch.int32, device=dev)
+    out = parents.new_empty(2 * n + 1)
     src, head = out.data_ptr(), free_head.data_ptr()
     p = _ffi.AtfForkParams(
         parents.data_ptr(), children.data_ptr(), kv_lens.data_ptr(), n, int(page_size), *table, shared.data_ptr(), num_pages,
@@ -128,7 +128,7 @@ def free_requests(req_rows: Optional[torch.Tensor], kv_lens: torch.Tensor, req_p
     num_free = _state(free_pages, "free_pages", dev)
     free_head = _list(free_head, "free_head", dev, 1)
     num_pages = _state(shared, "shared", dev) if shared is not None else 0
-    out = torch.empty(1, dtype=torch.int32, device=dev)
+    out = kv_lens.new_empty(1)
     p = _ffi.AtfFreeParams(
         req_rows.data_ptr() if req_rows is not None else None, kv_lens.data_ptr(), n, int(page_size), *table,
         shared.data_ptr() if shared is not None else None, num_pages, free_pages.data_ptr(), free_head.data_ptr(),
@@ -162,7 +162,7 @@ def compact_pages(kv_lens: torch.Tensor, req_pages: torch.Tensor, page_size: int
     num_free = _state(free_pages, "free_pages", dev, num_pages)
     if shared is not None:
         _state(shared, "shared", dev, num_pages)
-    out = torch.empty(2 * max_moves + 1, dtype=torch.int32, device=dev)
+    out = kv_lens.new_empty(2 * max_moves + 1)
     src = out.data_ptr()
     p = _ffi.AtfCompactParams(
         req_rows.data_ptr() if req_rows is not None else None, kv_lens.data_ptr(), n, int(page_size), *table,

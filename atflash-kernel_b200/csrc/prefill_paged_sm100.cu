@@ -9,9 +9,9 @@
 // in fp32. The window is quantised per tile of 128 queries and 128 keys of the request.
 // Three things differ.
 //
-// Pages. A key tile is 128 / R slices of R = min(page, 128) rows; a lane of the K producer
-// warp, or of the V producer warp, fetches its slice's page id one tile ahead and issues
-// its boxes, {64 dims, R rows} with 128-byte swizzle, into the rows of the tile. So K lies
+// Pages. A key tile is 128 / R slices of R = min(page, 128) rows. The K producer warp, and the
+// V producer warp, read page ids 32 slices at a time, a batch ahead, and a lane per slice
+// and half issues its box, {64 dims, R rows} with 128-byte swizzle, into the rows of the tile. So K lies
 // as Q does: level i is 32 bytes into a row, and dims 64 and up are another 16 KB. Slices past the
 // request's last page are not loaded; their keys are masked and their V rows cleared.
 // K and V have a producer warp each: with one, K of the tile after next waited for a free
@@ -77,7 +77,7 @@ __device__ __forceinline__ void qk_rows_asm(uint32_t d_tmem, uint64_t qd, uint64
       : "memory");
 }
 
-constexpr int WARP_V = 10;  // the V producer (WARP_LOAD: Q and K)
+constexpr int WARP_V = 10;  // the producer of Q and V (WARP_LOAD: K)
 constexpr uint32_t QBOX_BYTES = QTILE_BYTES / 2;
 // Shared memory: seven slots of 32 KB. Two tiles of Q, two stages of K and three of V; or one
 // tile of Q and three stages each where the groups share out the keys, where a step takes
@@ -141,7 +141,8 @@ struct Args {
   int n_wide, n_items; // unpacked items come first
   long long total_q;
   const int* indices;
-  int num_indices, num_pages, page, rows;  // rows: R
+  int num_indices, num_pages, page_shift, row_shift;  // of the page size and of R
+  int merge;           // a merge of states follows
 };
 
 // key tile j reads level i when j >= lim[i]
@@ -160,7 +161,7 @@ struct Unit {
   uint8_t* sp;
   uint32_t tmem;
   AbortCtl ab;
-  int sk, q_offset, row0, n0, n1, kt0, page_beg, page_end;
+  int sk, q_offset, row0, n0, n1, kt0, page_beg;
   int nk[NQ];       // key tiles of each group
   int hk, P;        // heads side by side in a tile
   int lim[NQ][ATF_MAX_LEVELS];
@@ -181,44 +182,33 @@ __device__ __forceinline__ int nth(int t, int i) {
   return SPLIT_KEYS ? 2 * i + t : i;
 }
 
-// Page id of this lane's slice of key tile kt (-1: no such slice), and the slice's row in
-// its page
-__device__ __forceinline__ int slice_page(const Args& a, const Unit& u, int kt, int lane) {
-  const int slices = BN / a.rows;
-  const int key = kt * BN + lane % slices * a.rows;
-  if (lane >= 2 * slices || key >= u.sk) return -1;
-  const int at = u.page_beg + key / a.page;
-  return at < u.page_end ? __ldg(a.indices + at) : -1;
+// Page id of slice 32 batch + lane of the item's key tiles (-1: no such slice). A batch is 32
+// slices, so 4 (pages of 16) to 32 key tiles; one is read while another is used.
+__device__ __forceinline__ int slice_page(const Args& a, const Unit& u, int batch, int lane) {
+  const int key = u.kt0 * BN + ((32 * batch + lane) << a.row_shift);
+  const unsigned at = static_cast<unsigned>(u.page_beg + (key >> a.page_shift));
+  return key < u.sk && at < static_cast<unsigned>(a.num_indices) ? __ldg(a.indices + at) : -1;
 }
 
-// The boxes of a key tile of K or V: lane = half x slices + slice. An id outside the cache
-// is a coordinate outside the map, which reads zeros; it is reported.
-__device__ __forceinline__ void load_slices(const Args& a, const Unit& u, const CUtensorMap* map, uint32_t dst,
-                                            uint32_t bar, int kt, int id, int halves, int lane) {
-  const int slices = BN / a.rows, slice = lane % slices, half = lane / slices;
-  const int live = min(slices, (u.sk - kt * BN + a.rows - 1) / a.rows);
-  mbar_arrive_expect_tx_elect(bar, static_cast<uint32_t>(live * halves * a.rows) * 128u);
-  __syncwarp();
-  if (half < halves && slice < live) {
-    if ((id < 0 || id >= a.num_pages) && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
-    tma_load_4d(dst + half * (BN * 128) + slice * a.rows * 128, map, bar, 64 * half, (kt * BN + slice * a.rows) % a.page,
-                u.hk, id);
-  }
-  __syncwarp();
-}
-
+// The loads of K or V, tile by tile: lane = half x slices + slice issues the box of its
+// slice and half. An id outside the cache is a coordinate outside the map, which reads
+// zeros; it is reported.
 template <bool SPLIT_KEYS>
-__device__ __forceinline__ void produce(const Args& a, const Unit& u, const CUtensorMap* map, bool is_k, int lane) {
+__device__ __forceinline__ void produce(const Args& a, const Unit& u, const CUtensorMap* map, bool is_k, int ids, int lane) {
   const int tiles = SPLIT_KEYS ? u.nk[0] + u.nk[1] : max(u.nk[0], u.nk[1]);
   const int stages = is_k ? K_STAGES<SPLIT_KEYS> : V_STAGES;
   const int full = is_k ? B_KFULL : B_VFULL, empty = is_k ? B_KEMPTY : B_VEMPTY;
-  const uint32_t base = u.sb + (is_k ? OFF_K<SPLIT_KEYS> : OFF_V);
-  int issued = 0;
-  int id = tiles > 0 ? slice_page(a, u, u.kt0, lane) : -1;
+  const int slices_shift = 7 - a.row_shift, slices = 1 << slices_shift;
+  const int slice = lane & (slices - 1), half = lane >> slices_shift, first_row = slice << a.row_shift;
+  const uint32_t dst = u.sb + (is_k ? OFF_K<SPLIT_KEYS> : OFF_V) + half * (BN * 128) + first_row * 128;
+  int issued = 0, later = slice_page(a, u, 1, lane);
   for (int g = 0; g < tiles; ++g) {
-    const int s = g % stages, kt = u.kt0 + g;
-    const int next = g + 1 < tiles ? slice_page(a, u, kt + 1, lane) : -1;
-    if (!__all_sync(FULL, mbar_wait_inl(u.bar(empty + s), ((g / stages) & 1) ^ 1, u.ab, kDevErrTimeout))) break;
+    const int s = g % stages, kt = u.kt0 + g, at = g << slices_shift;
+    if (g > 0 && (at & 31) == 0) {  // the next batch of page ids
+      ids = later;
+      later = slice_page(a, u, (at >> 5) + 1, lane);
+    }
+    const int id = __shfl_sync(FULL, ids, (at + slice) & 31);
     int halves = 2;
     if (is_k && a.window) {  // the second 64 dims are levels 4 to 7
       int L = 0;
@@ -227,9 +217,18 @@ __device__ __forceinline__ void produce(const Args& a, const Unit& u, const CUte
         if (SPLIT_KEYS ? t == 0 : g < u.nk[t]) L = max(L, levels_for(u.lim[t], kt));
       halves = L > 4 ? 2 : 1;
     }
-    load_slices(a, u, map, base + s * SLOT, u.bar(full + s), kt, id, halves, lane);
+    // slices of the tile before the request's last key
+    const int live = min(slices, (u.sk - kt * BN + (1 << a.row_shift) - 1) >> a.row_shift);
+    if (!__all_sync(FULL, mbar_wait_inl(u.bar(empty + s), ((g / stages) & 1) ^ 1, u.ab, kDevErrTimeout))) break;
+    mbar_arrive_expect_tx_elect(u.bar(full + s), static_cast<uint32_t>(live * halves) << (a.row_shift + 7));
+    __syncwarp();
+    if (half < halves && slice < live) {
+      if ((id < 0 || id >= a.num_pages) && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
+      tma_load_4d(dst + s * SLOT, map, u.bar(full + s), 64 * half, (kt * BN + first_row) & ((1 << a.page_shift) - 1), u.hk,
+                  id);
+    }
+    __syncwarp();
     issued = g + 1;
-    id = next;
   }
   // Every copy this warp issued lands before shared memory is released (no wait on the
   // normal path, where the MMA warp consumed them).
@@ -345,62 +344,81 @@ __device__ __forceinline__ void issue_mmas(const Args& a, const Unit& u, int lan
   __syncwarp();
 }
 
-// A warp's 32 rows of 64 (bf16 outputs) or 2 x 32 (fp32 states) dims from `half` on, through
-// `stage` (4 KB): rows of 128 bytes, 16-byte chunks XORed with the row, then eight lanes
-// per row, so that whole 128-byte lines leave. get(c4, v): dims [32 c4, 32 c4 + 32) of
-// this lane's row.
-template <typename Get>
-__device__ __forceinline__ void store_half(const Args& a, const Place& to, int half, int tok0, int first_row, int n_rows,
-                                           uint8_t* stage, int lane, Get&& get) {
+// Where a lane stores: eight lanes a row of the warp's 32, rows lr, lr + 4, ... of them. In
+// elements (bf16 outputs, or fp32 states). One division, then steps: a division per
+// row made the end of a CTA 5 to 13 us long.
+struct Rows {
+  long long at, step, wrap;  // the first row; four rows on; and from a token's last head to the next's first
+  int head, head_step, P, left;  // the i-th row is one of the tile's if 4 i < left
+};
+__device__ __forceinline__ Rows find_rows(const Args& a, const Place& to, int tok0, int first_row, int n_rows, int lane) {
+  Rows w;
+  const int row = first_row + (lane >> 3);
+  w.P = to.P;
+  const int tok = row / w.P;
+  w.head = row - tok * w.P;
+  const int tok_step = 4 / w.P;
+  w.head_step = 4 - tok_step * w.P;
+  w.left = n_rows - row;
+  const bool out = to.part < 0;
+  const long long per_tok = out ? a.o_ss : static_cast<long long>(to.n_parts) * a.Hq * 128;
+  const long long per_head = out ? a.o_sh : 128;
+  w.at = (out ? to.q_tok * a.o_ss : static_cast<long long>(to.part) * a.Hq * 128 - to.row0 * per_tok) +
+         (tok0 + tok) * per_tok + (to.head0 + w.head) * per_head;
+  w.step = tok_step * per_tok + w.head_step * per_head;
+  w.wrap = per_tok - w.P * per_head;
+  return w;
+}
+
+// 64 dims of a warp's 32 rows (v: this lane's row) from dim 64 half on, through `stage`
+// (4 KB): rows of 128 bytes, 16-byte chunks XORed with the row, then eight lanes per row,
+// so that whole 128-byte lines leave.
+__device__ __forceinline__ void store_half(const Args& a, const Rows& w, bool out, int half, uint8_t* stage, int lane,
+                                           const float (&v)[64]) {
   const int lr = lane >> 3, c = lane & 7;
-  // (token, head) of a row of the tile
-  auto place = [&](int r, int* tok, int* head) {
-    *tok = tok0 + r / to.P;
-    *head = to.head0 + r % to.P;
-  };
-  float v[32];
-  if (to.part < 0) {
+  if (out) {
 #pragma unroll
-    for (int c4 = 0; c4 < 2; ++c4) {
-      get(2 * half + c4, v);
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint4*>(stage + lane * 128 + 16 * ((4 * c4 + q) ^ (lane & 7))) =
-            make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
-                       pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
-    }
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<uint4*>(stage + lane * 128 + 16 * (q ^ (lane & 7))) =
+          make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                     pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
     __syncwarp();
+    __nv_bfloat16* at = a.out + w.at + 64 * half + 8 * c;
+    int h = w.head;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = 4 * i + lr;
       const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + 16 * (c ^ (r & 7)));
-      if (first_row + r < n_rows) {
-        int tok, head;
-        place(first_row + r, &tok, &head);
-        *reinterpret_cast<uint4*>(a.out + static_cast<long long>(to.q_tok + tok) * a.o_ss +
-                                  static_cast<long long>(head) * a.o_sh + 64 * half + 8 * c) = x;
+      if (4 * i < w.left) *reinterpret_cast<uint4*>(at) = x;
+      at += w.step;
+      h += w.head_step;
+      if (h >= w.P) {
+        h -= w.P;
+        at += w.wrap;
       }
     }
     __syncwarp();
     return;
   }
 #pragma unroll
-  for (int c4 = 0; c4 < 2; ++c4) {
-    get(2 * half + c4, v);
+  for (int k = 0; k < 2; ++k) {
 #pragma unroll
     for (int q = 0; q < 8; ++q)
       *reinterpret_cast<float4*>(stage + lane * 128 + 16 * (q ^ (lane & 7))) =
-          make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          make_float4(v[32 * k + 4 * q], v[32 * k + 4 * q + 1], v[32 * k + 4 * q + 2], v[32 * k + 4 * q + 3]);
     __syncwarp();
+    float* at = a.part_o + w.at + 64 * half + 32 * k + 4 * c;
+    int h = w.head;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = 4 * i + lr;
       const float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + 16 * (c ^ (r & 7)));
-      if (first_row + r < n_rows) {
-        int tok, head;
-        place(first_row + r, &tok, &head);
-        const long long slot = to.part + static_cast<long long>(tok - to.row0) * to.n_parts;
-        *reinterpret_cast<float4*>(a.part_o + (slot * a.Hq + head) * 128 + 64 * half + 32 * c4 + 4 * c) = x;
+      if (4 * i < w.left) *reinterpret_cast<float4*>(at) = x;
+      at += w.step;
+      h += w.head_step;
+      if (h >= w.P) {
+        h -= w.P;
+        at += w.wrap;
       }
     }
     __syncwarp();
@@ -528,10 +546,12 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
   }
 
   float lse2;  // log2 of the row's sum
-  uint8_t* stage;
   const int r = wq * 32 + lane;
   const Place& to = *reinterpret_cast<const Place*>(u.sp + OFF_PLACE);
+  const bool out = to.part < 0;
   const int out0 = to.row0 + (!SPLIT_KEYS && t ? to.n0 : 0), n_rows = (!SPLIT_KEYS && t ? to.n1 : to.n0) * to.P;
+  const Rows w = find_rows(a, to, out0, wq * 32, n_rows, lane);
+  float v[64];
   if (SPLIT_KEYS) {
     // both groups' states of the row: (max, sum) through shared memory, O from TMEM, where
     // the row has the same lane in both. Group t stores half t of the dims.
@@ -554,55 +574,49 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
     const bool keyless = m == -INFINITY;  // 0, whatever V holds
     const float inv = l > 0.f ? 1.0f / l : 0.f;
     const float f0 = w0 * inv, f1 = w1 * inv;
-    const uint32_t tO0 = tO - static_cast<uint32_t>(t * 128);
-    stage = u.sp + OFF_Q + warp * 4096;
-    store_half(a, to, t, out0, wq * 32, n_rows, stage, lane, [&](int c4, float (&v)[32]) {
-      uint32_t rr[32];
-      if (to.nk[0] > 0) {  // (the same for every thread of the CTA)
-        tmem_ld32(tO0 + static_cast<uint32_t>(32 * c4), rr);
+    const uint32_t tO0 = tO + static_cast<uint32_t>(64 * t - 128 * t);
+    uint32_t rr[64];
+    if (to.nk[0] > 0) {  // (the same for every thread of the CTA)
+      tmem_ld64(tO0, rr);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = keyless ? 0.f : __uint_as_float(rr[e]) * f0;
-      } else {
+      for (int e = 0; e < 64; ++e) v[e] = keyless ? 0.f : __uint_as_float(rr[e]) * f0;
+    } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = 0.f;
-      }
-      if (to.nk[1] > 0) {
-        tmem_ld32(tO0 + static_cast<uint32_t>(128 + 32 * c4), rr);
+      for (int e = 0; e < 64; ++e) v[e] = 0.f;
+    }
+    if (to.nk[1] > 0) {
+      tmem_ld64(tO0 + 128u, rr);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = keyless ? 0.f : fmaf(__uint_as_float(rr[e]), f1, v[e]);
-      }
-    });
+      for (int e = 0; e < 64; ++e) v[e] = keyless ? 0.f : fmaf(__uint_as_float(rr[e]), f1, v[e]);
+    }
+    store_half(a, w, out, t, u.sp + OFF_Q + warp * 4096, lane, v);
     if (t != 0) return;
   } else {
     if (!ok || n_rows == 0) return;
-    if (my_nk > 0) {
-      if (!__all_sync(FULL, mbar_wait_inl(u.bar(B_OFINAL + t), 0, u.ab, kDevErrTimeout))) return;
-      tc_fence_after();
-    }
+    // through the tile's own Q in shared memory (its last product has read it; a tile without
+    // keys has no products)
+    if (!__all_sync(FULL, mbar_wait_inl(u.bar(my_nk > 0 ? B_OFINAL + t : B_Q), 0, u.ab, kDevErrTimeout))) return;
+    tc_fence_after();
     const bool keyless = m2 == -INFINITY;  // 0, whatever V holds
     const float inv = l > 0.f ? 1.0f / l : 0.f;
     lse2 = m2 + log2f(l);
-    // through the tile's own Q in shared memory (its last product has read it; a tile without
-    // keys has no products)
-    stage = u.sp + OFF_Q + t * QTILE_BYTES + wq * 4096;
-    if (my_nk == 0 && !__all_sync(FULL, mbar_wait_inl(u.bar(B_Q), 0, u.ab, kDevErrTimeout))) return;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      if (my_nk > 0) {
+        uint32_t rr[64];
+        tmem_ld64(tO + static_cast<uint32_t>(64 * half), rr);
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
-      store_half(a, to, half, out0, wq * 32, n_rows, stage, lane, [&](int c4, float (&v)[32]) {
-        if (my_nk > 0) {
-          uint32_t rr[32];
-          tmem_ld32(tO + static_cast<uint32_t>(32 * c4), rr);
+        for (int e = 0; e < 64; ++e) v[e] = keyless ? 0.f : __uint_as_float(rr[e]) * inv;
+      } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = keyless ? 0.f : __uint_as_float(rr[e]) * inv;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0.f;
-        }
-      });
+        for (int e = 0; e < 64; ++e) v[e] = 0.f;
+      }
+      store_half(a, w, out, half, u.sp + OFF_Q + t * QTILE_BYTES + wq * 4096, lane, v);
+    }
   }
   if (r < n_rows) {
     const int tok = out0 + r / to.P, head = to.head0 + r % to.P;
-    if (to.part >= 0)
+    if (!out)
       a.part_lse[(to.part + static_cast<long long>(tok - to.row0) * to.n_parts) * a.Hq + head] = lse2;
     else if (a.lse != nullptr)
       a.lse[static_cast<long long>(to.q_tok + tok) * a.Hq + head] = lse2 * 0.69314718055994531f;
@@ -658,17 +672,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     mbar_init(u.bar(B_FINAL), 1);
     fence_mbar_init();
   }
-  if (warp == WARP_LOAD && lane == 0) {
+  if (warp == WARP_LOAD && lane == 0) tma_prefetch_desc(&tmK);
+  if (warp == WARP_V && lane == 0) {
     tma_prefetch_desc(bid < wide ? &tmQ : &tmQP);
-    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
   }
-  if (warp == WARP_V && lane == 0) tma_prefetch_desc(&tmV);
   if (warp == WARP_MMA) {
     tmem_alloc(smem_u32(s_tmem), 512);
     tmem_relinquish();
   }
   // the merge of the states may be launched: it waits for this grid before it reads them
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (a.merge) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   u.sk = it0.z;
   u.q_offset = it0.z - it0.y;  // position of the request's query 0 among its keys (negative: rows without keys)
   u.page_beg = it0.w;
@@ -687,10 +701,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                    it1.y > tile_tokens || it1.z > tile_tokens || (split && it1.z != 0) || last_tok > it0.y ||
                    it0.x + static_cast<long long>(it0.y) > a.total_q || it2.x < 0 || it2.y < it2.x ||
                    packed != (bid >= wide) ||
-                   it0.w + (static_cast<long long>(it0.z) + a.page - 1) / a.page > a.num_indices ||
+                   it0.w + ((static_cast<long long>(it0.z) + (1 << a.page_shift) - 1) >> a.page_shift) > a.num_indices ||
                    (it2.z >= 0 && (it2.w < 1 || it2.z + (static_cast<long long>(it1.y) + it1.z - 1) * it2.w >= a.parts));
   if (bad) u.n0 = u.n1 = 0;
-  u.page_end = a.num_indices;
   if (threadIdx.x == 0) {
     *s_abort = stop0 ? 1 : 0;
     if (bad && a.err != nullptr) atomicCAS(a.err, 0, kDevErrIndex);
@@ -712,6 +725,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     *reinterpret_cast<Place*>(u.sp + OFF_PLACE) =
         Place{it0.x, u.row0, it2.z, it2.w, h, u.P, u.n0, u.n1, {u.nk[0], u.nk[1]}, {0, 0}};
 
+  // the producers' first page ids: on their way over the barrier
+  const int first_id = warp == WARP_LOAD || warp == WARP_V ? slice_page(a, u, 0, lane) : -1;
+
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -721,7 +737,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp >= 8) {
     reg_dealloc<REG_SMALL>();
     if (start_ok && warp == WARP_LOAD) {
-      // Q: rows of 128 bytes, two boxes of 64 dims a tile
+      if (split)
+        produce<true>(a, u, &tmK, true, first_id, lane);
+      else
+        produce<false>(a, u, &tmK, true, first_id, lane);
+    } else if (start_ok && warp == WARP_V) {
+      // Q (rows of 128 bytes, two boxes of 64 dims a tile), which the first S needs, then V
       const uint32_t qbytes = static_cast<uint32_t>(tile_tokens * u.P) * 256u;
       const int n_q = (u.n0 > 0 ? 1 : 0) + (u.n1 > 0 ? 1 : 0);
       mbar_arrive_expect_tx_elect(u.bar(B_Q), n_q * qbytes);
@@ -732,16 +753,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                             64 * half, h, it0.x + u.row0 + (t ? u.n0 : 0), 0);
       __syncwarp();
       if (split)
-        produce<true>(a, u, &tmK, true, lane);
+        produce<true>(a, u, &tmV, false, first_id, lane);
       else
-        produce<false>(a, u, &tmK, true, lane);
+        produce<false>(a, u, &tmV, false, first_id, lane);
       drain_wait(u.bar(B_Q), 0);
       __syncwarp();
-    } else if (start_ok && warp == WARP_V) {
-      if (split)
-        produce<true>(a, u, &tmV, false, lane);
-      else
-        produce<false>(a, u, &tmV, false, lane);
     } else if (start_ok && warp == WARP_MMA) {
       if (split)
         issue_mmas<true>(a, u, lane);
@@ -1047,7 +1063,9 @@ extern "C" int atf_prefill_paged_fwd(const AtfPrefillPagedParams* p, atf_stream_
   a.G = a.Hq / a.Hkv;
   a.T = BM / a.G;
   if (p->num_wide < p->num_items && a.T < 1) return ATF_ERR_INVALID_ARG;  // packed items of such a group
-  a.rows = p->page_size < BN ? p->page_size : BN;
+  for (a.page_shift = 4; (1 << a.page_shift) < p->page_size;) ++a.page_shift;
+  a.row_shift = a.page_shift < 7 ? a.page_shift : 7;
+  a.merge = p->num_rows > 0 ? 1 : 0;
   auto sane = [](int64_t stride, int64_t size) -> uint64_t {
     return static_cast<uint64_t>(size == 1 ? 16 : stride * 2);
   };
@@ -1067,7 +1085,7 @@ extern "C" int atf_prefill_paged_fwd(const AtfPrefillPagedParams* p, atf_stream_
     const uint64_t dims[4] = {128, static_cast<uint64_t>(p->page_size), static_cast<uint64_t>(p->num_heads_kv),
                               static_cast<uint64_t>(p->num_pages)};
     const uint64_t str[3] = {sane(stok, p->page_size), sane(sh, p->num_heads_kv), sane(sp, p->num_pages)};
-    const uint32_t box[4] = {64, static_cast<uint32_t>(a.rows), 1, 1};
+    const uint32_t box[4] = {64, 1u << a.row_shift, 1, 1};
     return encode_tiled_bf16(map, base, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   if ((rc = pages(&tk, p->k_cache, p->k_stride_page, p->k_stride_token, p->k_stride_head)) != ATF_OK) return rc;
@@ -1093,7 +1111,6 @@ extern "C" int atf_prefill_paged_fwd(const AtfPrefillPagedParams* p, atf_stream_
   a.indices = p->indices;
   a.num_indices = p->num_indices;
   a.num_pages = static_cast<int>(p->num_pages);
-  a.page = p->page_size;
   const long long units =
       static_cast<long long>(a.n_wide) * a.Hq + static_cast<long long>(a.n_items - a.n_wide) * a.Hkv;
   if (units > 0x7fffffffLL) return ATF_ERR_UNSUPPORTED;
