@@ -109,7 +109,8 @@ enum {
   NUM_BARS
 };
 constexpr uint32_t OFF_PLACE = OFF_BAR + 8 * ((NUM_BARS + 1) / 2 * 2);  // Place
-constexpr uint32_t OFF_ABORT = OFF_PLACE + 48;
+constexpr uint32_t OFF_ROWS = OFF_PLACE + 48;  // [t][128] of where a row goes
+constexpr uint32_t OFF_ABORT = OFF_ROWS + NQ * BM * 4;
 constexpr uint32_t OFF_TMEM = OFF_ABORT + 16;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16 + 1024;  // slack for 1024-B alignment
 
@@ -344,36 +345,22 @@ __device__ __forceinline__ void issue_mmas(const Args& a, const Unit& u, int lan
   __syncwarp();
 }
 
-// Where a lane stores: eight lanes a row of the warp's 32, rows lr, lr + 4, ... of them. In
-// elements (bf16 outputs, or fp32 states). One division, then steps: a division per
-// row made the end of a CTA 5 to 13 us long.
-struct Rows {
-  long long at, step, wrap;  // the first row; four rows on; and from a token's last head to the next's first
-  int head, head_step, P, left;  // the i-th row is one of the tile's if 4 i < left
-};
-__device__ __forceinline__ Rows find_rows(const Args& a, const Place& to, int tok0, int first_row, int n_rows, int lane) {
-  Rows w;
-  const int row = first_row + (lane >> 3);
-  w.P = to.P;
-  const int tok = row / w.P;
-  w.head = row - tok * w.P;
-  const int tok_step = 4 / w.P;
-  w.head_step = 4 - tok_step * w.P;
-  w.left = n_rows - row;
-  const bool out = to.part < 0;
-  const long long per_tok = out ? a.o_ss : static_cast<long long>(to.n_parts) * a.Hq * 128;
-  const long long per_head = out ? a.o_sh : 128;
-  w.at = (out ? to.q_tok * a.o_ss : static_cast<long long>(to.part) * a.Hq * 128 - to.row0 * per_tok) +
-         (tok0 + tok) * per_tok + (to.head0 + w.head) * per_head;
-  w.step = tok_step * per_tok + w.head_step * per_head;
-  w.wrap = per_tok - w.P * per_head;
-  return w;
+// Where row r of a tile goes, in steps of 16 bytes from the outputs' or the states' first
+// (NO_ROW: it is not one of the tile's). Found by the softmax threads while the CTA is set
+// up: divisions at its end cost 1 to 10 us.
+constexpr uint32_t NO_ROW = 0xffffffffu;
+__device__ __forceinline__ uint32_t row_place(const Args& a, const Place& to, int t, int r) {
+  if (r >= (t ? to.n1 : to.n0) * to.P) return NO_ROW;
+  const int k = r / to.P, tok = to.row0 + (t ? to.n0 : 0) + k, head = to.head0 + r - k * to.P;
+  if (to.part < 0)
+    return static_cast<uint32_t>(((to.q_tok + tok) * a.o_ss + head * a.o_sh) >> 3);
+  return static_cast<uint32_t>(((to.part + static_cast<long long>(tok - to.row0) * to.n_parts) * a.Hq + head) * 32);
 }
 
 // 64 dims of a warp's 32 rows (v: this lane's row) from dim 64 half on, through `stage`
 // (4 KB): rows of 128 bytes, 16-byte chunks XORed with the row, then eight lanes per row,
-// so that whole 128-byte lines leave.
-__device__ __forceinline__ void store_half(const Args& a, const Rows& w, bool out, int half, uint8_t* stage, int lane,
+// so that whole 128-byte lines leave. place: of the warp's rows.
+__device__ __forceinline__ void store_half(const Args& a, const uint32_t* place, bool out, int half, uint8_t* stage, int lane,
                                            const float (&v)[64]) {
   const int lr = lane >> 3, c = lane & 7;
   if (out) {
@@ -383,19 +370,13 @@ __device__ __forceinline__ void store_half(const Args& a, const Rows& w, bool ou
           make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
                      pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
     __syncwarp();
-    __nv_bfloat16* at = a.out + w.at + 64 * half + 8 * c;
-    int h = w.head;
+    uint4* to = reinterpret_cast<uint4*>(a.out) + 8 * half + c;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = 4 * i + lr;
       const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + 16 * (c ^ (r & 7)));
-      if (4 * i < w.left) *reinterpret_cast<uint4*>(at) = x;
-      at += w.step;
-      h += w.head_step;
-      if (h >= w.P) {
-        h -= w.P;
-        at += w.wrap;
-      }
+      const uint32_t at = place[r];
+      if (at != NO_ROW) to[at] = x;
     }
     __syncwarp();
     return;
@@ -407,19 +388,13 @@ __device__ __forceinline__ void store_half(const Args& a, const Rows& w, bool ou
       *reinterpret_cast<float4*>(stage + lane * 128 + 16 * (q ^ (lane & 7))) =
           make_float4(v[32 * k + 4 * q], v[32 * k + 4 * q + 1], v[32 * k + 4 * q + 2], v[32 * k + 4 * q + 3]);
     __syncwarp();
-    float* at = a.part_o + w.at + 64 * half + 32 * k + 4 * c;
-    int h = w.head;
+    float4* to = reinterpret_cast<float4*>(a.part_o) + 16 * half + 8 * k + c;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = 4 * i + lr;
       const float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + 16 * (c ^ (r & 7)));
-      if (4 * i < w.left) *reinterpret_cast<float4*>(at) = x;
-      at += w.step;
-      h += w.head_step;
-      if (h >= w.P) {
-        h -= w.P;
-        at += w.wrap;
-      }
+      const uint32_t at = place[r];
+      if (at != NO_ROW) to[at] = x;
     }
     __syncwarp();
   }
@@ -549,8 +524,8 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
   const int r = wq * 32 + lane;
   const Place& to = *reinterpret_cast<const Place*>(u.sp + OFF_PLACE);
   const bool out = to.part < 0;
-  const int out0 = to.row0 + (!SPLIT_KEYS && t ? to.n0 : 0), n_rows = (!SPLIT_KEYS && t ? to.n1 : to.n0) * to.P;
-  const Rows w = find_rows(a, to, out0, wq * 32, n_rows, lane);
+  const int tile = SPLIT_KEYS ? 0 : t;
+  const uint32_t* place = reinterpret_cast<const uint32_t*>(u.sp + OFF_ROWS) + tile * BM + wq * 32;
   float v[64];
   if (SPLIT_KEYS) {
     // both groups' states of the row: (max, sum) through shared memory, O from TMEM, where
@@ -589,10 +564,10 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
 #pragma unroll
       for (int e = 0; e < 64; ++e) v[e] = keyless ? 0.f : fmaf(__uint_as_float(rr[e]), f1, v[e]);
     }
-    store_half(a, w, out, t, u.sp + OFF_Q + warp * 4096, lane, v);
+    store_half(a, place, out, t, u.sp + OFF_Q + warp * 4096, lane, v);
     if (t != 0) return;
   } else {
-    if (!ok || n_rows == 0) return;
+    if (!ok || (t ? to.n1 : to.n0) == 0) return;
     // through the tile's own Q in shared memory (its last product has read it; a tile without
     // keys has no products)
     if (!__all_sync(FULL, mbar_wait_inl(u.bar(my_nk > 0 ? B_OFINAL + t : B_Q), 0, u.ab, kDevErrTimeout))) return;
@@ -611,14 +586,14 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
 #pragma unroll
         for (int e = 0; e < 64; ++e) v[e] = 0.f;
       }
-      store_half(a, w, out, half, u.sp + OFF_Q + t * QTILE_BYTES + wq * 4096, lane, v);
+      store_half(a, place, out, half, u.sp + OFF_Q + t * QTILE_BYTES + wq * 4096, lane, v);
     }
   }
-  if (r < n_rows) {
-    const int tok = out0 + r / to.P, head = to.head0 + r % to.P;
+  if (place[lane] != NO_ROW && (!out || a.lse != nullptr)) {
+    const int k = r / to.P, tok = to.row0 + (tile ? to.n0 : 0) + k, head = to.head0 + r - k * to.P;
     if (!out)
       a.part_lse[(to.part + static_cast<long long>(tok - to.row0) * to.n_parts) * a.Hq + head] = lse2;
-    else if (a.lse != nullptr)
+    else
       a.lse[static_cast<long long>(to.q_tok + tok) * a.Hq + head] = lse2 * 0.69314718055994531f;
   }
 }
@@ -721,9 +696,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     u.nk[1] = u.nk[0] / 2;
     u.nk[0] -= u.nk[1];
   }
-  if (threadIdx.x == 0)
-    *reinterpret_cast<Place*>(u.sp + OFF_PLACE) =
-        Place{it0.x, u.row0, it2.z, it2.w, h, u.P, u.n0, u.n1, {u.nk[0], u.nk[1]}, {0, 0}};
+  if (warp < 8) {
+    const Place to = {it0.x, u.row0, it2.z, it2.w, h, u.P, u.n0, u.n1, {u.nk[0], u.nk[1]}, {0, 0}};
+    reinterpret_cast<uint32_t*>(u.sp + OFF_ROWS)[threadIdx.x] = row_place(a, to, warp >> 2, threadIdx.x & (BM - 1));
+    if (threadIdx.x == 0) *reinterpret_cast<Place*>(u.sp + OFF_PLACE) = to;
+  }
 
   // the producers' first page ids: on their way over the barrier
   const int first_id = warp == WARP_LOAD || warp == WARP_V ? slice_page(a, u, 0, lane) : -1;
@@ -1034,6 +1011,9 @@ extern "C" int atf_prefill_paged_fwd(const AtfPrefillPagedParams* p, atf_stream_
       p->num_heads_q % p->num_heads_kv != 0 || p->num_items < 0 || p->num_wide < 0 || p->num_wide > p->num_items ||
       p->num_rows < 0 || p->num_parts < 0)
     return ATF_ERR_INVALID_ARG;
+  // (a row's place is counted in 32 bits, in steps of 16 bytes)
+  if (p->num_parts > 0 && static_cast<long long>(p->num_parts) * p->num_heads_q * 32 >= 0xffffffffLL)
+    return ATF_ERR_UNSUPPORTED;
   if (p->num_parts > 0 && (p->partial_o == nullptr || p->partial_lse == nullptr)) return ATF_ERR_INVALID_ARG;
   if (p->num_rows > 0 && p->rows == nullptr) return ATF_ERR_INVALID_ARG;
   if (p->total_q > 0x7fffffffLL - BM * NQ || p->num_pages > 0x7fffffffLL || p->num_heads_q > (1 << 20))
@@ -1049,6 +1029,9 @@ extern "C" int atf_prefill_paged_fwd(const AtfPrefillPagedParams* p, atf_stream_
                                p->v_stride_page,  p->v_stride_token, p->v_stride_head, p->o_stride_s,    p->o_stride_h};
   for (int i = 0; i < 10; ++i)
     if (strides[i] < 0 || (strides[i] & 7) != 0) return ATF_ERR_ALIGNMENT;
+  if (p->o_stride_s > (1ll << 40) || p->o_stride_h > (1ll << 40) ||
+      (((p->total_q - 1) * p->o_stride_s + (p->num_heads_q - 1) * p->o_stride_h) >> 3) >= 0xffffffffLL)
+    return ATF_ERR_UNSUPPORTED;
   if (p->window == ATF_WINDOW_SNAP16)
     for (int i = 0; i < ATF_MAX_LEVELS; ++i)
       if (p->zhi[i] < 0 || (i > 0 && p->zhi[i] > p->zhi[i - 1])) return ATF_ERR_INVALID_ARG;
