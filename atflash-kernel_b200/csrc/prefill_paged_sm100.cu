@@ -837,11 +837,11 @@ struct Block {
   float cost() const { return tiles * step; }
 };
 
-// Measured on the device, with K and V in L2 and all SMs at work: 2.2 us for a step of two
-// tiles of rows against a key tile; 1.4 us per key tile where the groups share out the keys
-// (1.6 with pages of 16, and HBM takes 1.5 for its 64 KB per SM); 5 us of a CTA's start and
-// end, 3 more for writing states and merging them.
-constexpr float STEP_US = 2.2f, SHARED_US = 1.5f, START_US = 5.f, STATES_US = 3.f;
+// Measured on the device: 1.8 us for a step of two tiles of rows against a key tile; 1.1 us
+// per key tile where the groups share out the keys, with K and V in L2, and 1.5 with all
+// SMs reading them from HBM; 6 us of a CTA's start and end; 4 more for writing states and
+// merging them.
+constexpr float STEP_US = 1.8f, SHARED_US = 1.3f, START_US = 6.f, STATES_US = 4.f;
 
 // when the last CTA ends if the blocks are cut into pieces of at most `most` us: the
 // hardware takes items in order, each for the first SM that is free
