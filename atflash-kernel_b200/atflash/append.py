@@ -194,6 +194,8 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
     ip, ix = _dev_i32(kv_indptr, dev, kv_indices.numel()), _dev_i32(kv_indices, dev)
     if bi.numel() != nnz or ps.numel() != nnz:
         raise ValueError("batch_indices and positions need one entry per appended token")
+    if nnz == 0:
+        return
     p = _ffi.AtfAppendParams(append_key.data_ptr(), append_value.data_ptr(), nnz, st[0], st[1], bi.data_ptr(),
                              ps.data_ptr(), kc.data_ptr(), vc.data_ptr(), npages, s_page, s_tok, s_head, hkv, 128, page,
                              ip.numel() - 1, ip.data_ptr(), ix.data_ptr())
