@@ -3,9 +3,11 @@ pages, over the tables of ``build_page_tables`` (req_pages, free_pages, free_hea
 
 ``shared`` (int32, one entry per page, zeros to begin with) counts the holders of a page
 beyond the first. It is 0 for a free page and for a page of one request, so pages that
-``build_page_tables`` takes from the free list need no entry. A request writes into its
-last page only, and a fork gives the child a copy of a last page that is partly filled,
-so a page with several holders is never written.
+``build_page_tables`` takes from the free list need no entry. A request that only grows
+writes into its last page and new ones, and a fork gives the child a copy of a last page
+that is partly filled, so a page with several holders is never written. (A request whose
+length is cut back into pages that it shares would write into them: fork it at that length
+instead, and free the old row.)
 
 Index reports of these calls go to ``atflash.check_device_errors()`` (code 2). The
 reference serves one request and has no counterpart."""

@@ -546,7 +546,7 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
     const float w0 = s0.x == -INFINITY ? 0.f : ex2_approx(s0.x - m), w1 = s1.x == -INFINITY ? 0.f : ex2_approx(s1.x - m);
     l = s0.y * w0 + s1.y * w1;
     lse2 = m + log2f(l);
-    const bool keyless = m == -INFINITY;  // 0, whatever V holds
+    const bool keyless = l == 0.f;  // no key, or none with weight: 0, whatever V holds
     const float inv = l > 0.f ? 1.0f / l : 0.f;
     const float f0 = w0 * inv, f1 = w1 * inv;
     const uint32_t tO0 = tO + static_cast<uint32_t>(64 * t - 128 * t);
@@ -572,7 +572,7 @@ __device__ __forceinline__ void softmax(const Args& a, const Unit& u, int warp, 
     // keys has no products)
     if (!__all_sync(FULL, mbar_wait_inl(u.bar(my_nk > 0 ? B_OFINAL + t : B_Q), 0, u.ab, kDevErrTimeout))) return;
     tc_fence_after();
-    const bool keyless = m2 == -INFINITY;  // 0, whatever V holds
+    const bool keyless = l == 0.f;  // no key, or none with weight: 0, whatever V holds
     const float inv = l > 0.f ? 1.0f / l : 0.f;
     lse2 = m2 + log2f(l);
 #pragma unroll 1
@@ -791,6 +791,16 @@ __global__ void __launch_bounds__(256) merge_states_kernel(const MergeArgs a) {
   const float* pl = a.part_lse + static_cast<long long>(row.y) * a.Hq + h;
   const float* po = a.part_o + (static_cast<long long>(row.y) * a.Hq + h) * 128 + 4 * lane;
   const long long step = static_cast<long long>(a.Hq) * 128;
+  // the first states on their way while the largest LSE is found
+  constexpr int AHEAD = 4;
+  float x0[AHEAD];
+  float4 v0[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (i < row.z) {
+      x0[i] = pl[static_cast<long long>(i) * a.Hq];
+      v0[i] = *reinterpret_cast<const float4*>(po + i * step);
+    }
   float m = -INFINITY;
   bool nan = false;  // (a maximum passes a NaN over)
   for (int i = lane; i < row.z; i += 32) {
@@ -804,10 +814,7 @@ __global__ void __launch_bounds__(256) merge_states_kernel(const MergeArgs a) {
   const float base = m == -INFINITY ? 0.f : m;
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < row.z; ++i) {
-    const float x = pl[static_cast<long long>(i) * a.Hq];
-    const float4 v = *reinterpret_cast<const float4*>(po + i * step);
+  auto add = [&](float x, const float4& v) {
     const float wgt = x == -INFINITY ? 0.f : exp2f(x - base);
     sum += wgt;
     if (wgt != 0.f) {  // a state without weight may hold anything
@@ -816,7 +823,13 @@ __global__ void __launch_bounds__(256) merge_states_kernel(const MergeArgs a) {
       acc.z = fmaf(wgt, v.z, acc.z);
       acc.w = fmaf(wgt, v.w, acc.w);
     }
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (i < row.z) add(x0[i], v0[i]);
+#pragma unroll 4
+  for (int i = AHEAD; i < row.z; ++i)
+    add(pl[static_cast<long long>(i) * a.Hq], *reinterpret_cast<const float4*>(po + i * step));
   const float inv = sum > 0.f || nan ? 1.0f / sum : 0.f;
   uint2 pk;
   pk.x = pack_bf16x2(acc.x * inv, acc.y * inv);

@@ -192,7 +192,8 @@ int atf_prefill_ragged_fwd(const AtfPrefillRaggedParams* p, atf_stream_t stream)
  * token i sees the keys up to nk - nq + i), which are already in the pages. A row that
  * sees no key gets 0 and an LSE of -inf. The window is quantised per tile of 128 tokens and
  * 128 keys of a request, as in atf_prefill_ragged_fwd. Pages past the last key and rows past it in
- * its page are not used, whatever they hold. No counterpart in the reference, whose
+ * its page are not used, whatever they hold; a NaN or an infinity in V of a key reaches the
+ * rows of every tile that loads its key tile, as in atf_prefill_fwd. No counterpart in the reference, whose
  * prefill reads contiguous K and V. */
 typedef struct {
   int32_t batch_size, num_qo_heads, num_kv_heads, page_size; /* pages of 16, 32, 64, 128 or 256 */

@@ -204,6 +204,17 @@ def test_nan_and_infinity_of_a_key_stay_with_the_rows_that_see_it():
     assert torch.isfinite(lse).all() and not torch.isfinite(out[c.cq[2] - 1]).any()
 
 
+@pytest.mark.parametrize("reqs", [[(1, 1)], [(2, 2), (1, 129)], [(128, 128)], [(256, 256)]])
+def test_a_nan_key_reaches_every_row_that_sees_it(reqs):
+    """Each request's first key is NaN: no row may pass it over, the one that sees nothing
+    else included."""
+    c = Case(16, "NHD", 2, 1, reqs, seed=8)
+    for b in range(len(reqs)):
+        c.k[c.indices[c.starts[b]].long(), 0] = float("nan")
+    out, lse = c.run(c.plan())
+    assert out.isnan().all() and lse.isnan().all()
+
+
 def test_plans_kept_dropped_and_small_workspaces():
     import atflash
     c = Case(16, "NHD", 28, 4, [(5, 16001)], seed=1)
