@@ -217,31 +217,35 @@ struct FreeArgs {
 // the reads of the counts between the phases come from L2, where the atomics are
 __device__ __forceinline__ int fresh(const int* p) { return __ldcg(p); }
 
+constexpr int KEPT = 4;  // entries of a lane whose pages stay in registers over the phases
+
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) free_kernel(const FreeArgs a) {
   extern __shared__ int sm[];
   int* s_owner = sm;            // [R] first entry of a row
   int* s_n = s_owner + a.R;     // [N] pages to free, 0 for a request that is left out
+  int* s_row = s_n + a.N;       // [N]
   __shared__ int s_warp[33];
   __shared__ int s_count;       // pages that this CTA frees
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, rank = static_cast<int>(cluster.block_rank());
   for (int r = tid; r < a.R; r += THREADS) s_owner[r] = 0x7fffffff;
   __syncthreads();
-  auto row_of = [&](int i) { return a.req_rows != nullptr ? a.req_rows[i] : i; };
   for (int i = tid; i < a.N; i += THREADS) {
-    const int r = row_of(i);
+    const int r = a.req_rows != nullptr ? a.req_rows[i] : i;
+    s_row[i] = r;
+    s_n[i] = a.lens[i];
     if (r >= 0 && r < a.R) atomicMin(&s_owner[r], i);
   }
+  const int head = *a.free_head;
   __syncthreads();
   bool bad = false;
   for (int i = tid; i < a.N; i += THREADS) {
-    const int r = row_of(i), len = a.lens[i];
+    const int r = s_row[i], len = s_n[i];
     const bool ok = r >= 0 && r < a.R && s_owner[r] == i && len >= 0 && pages_of(max(len, 0), a.page) <= a.M;
     bad |= !ok;
     s_n[i] = ok ? pages_of(len, a.page) : 0;
   }
   __syncthreads();
-  const int head = *a.free_head;
   // this thread's entries: CTA, warp and lane in the order of e, in steps of 32
   const int all = a.N * a.M;  // under 2^30
   const int warps = CLUSTER * THREADS / 32;
@@ -249,44 +253,54 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) free_
   const int gw = rank * (THREADS / 32) + (tid >> 5), lane = tid & 31;
   const int e0 = static_cast<int>(min(static_cast<long long>(gw) * per_warp, static_cast<long long>(all)));
   const int e1 = static_cast<int>(min(static_cast<long long>(e0) + per_warp, static_cast<long long>(all)));
-  // page of entry e, -1 where there is none
-  auto page_at = [&](int e, long long* at) -> int {
-    if (e >= e1) return -1;
+  // where entry e's page id stands, null where there is no entry
+  auto place_of = [&](int e) -> int32_t* {
+    if (e >= e1) return nullptr;
     const int i = static_cast<int>(static_cast<unsigned>(e) / static_cast<unsigned>(a.M)), j = e - i * a.M;
-    if (j >= s_n[i]) return -1;
-    *at = row_of(i) * a.stride + j;
-    const int id = a.rows[*at];
+    return j < s_n[i] ? a.rows + s_row[i] * a.stride + j : nullptr;
+  };
+  // page of entry e, -1 where there is none
+  auto page_at = [&](int e) -> int {
+    const int32_t* at = place_of(e);
+    if (at == nullptr) return -1;
+    const int id = *at;
     if (id < 0 || id >= a.P) {
       bad = true;
       return -1;
     }
     return id;
   };
+  int kept[KEPT];  // pages of the lane's first entries, read side by side
+#pragma unroll
+  for (int k = 0; k < KEPT; ++k) kept[k] = page_at(e0 + lane + 32 * k);
+  // f(e, page) for the lane's entries in order, every lane of the warp together
+  auto entries = [&](auto&& f) {
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k)
+      if (e0 + 32 * k < e1) f(e0 + lane + 32 * k, kept[k]);
+    for (int e = e0 + lane + 32 * KEPT; e - lane < e1; e += 32) f(e, page_at(e));
+  };
   auto mark_of = [&](int e) { return static_cast<int>(0x80000000u) + (all - 1 - e); };
-  long long at = 0;
   if (a.shared != nullptr) {
-    for (int e = e0 + lane; e < e1; e += 32) {
-      const int id = page_at(e, &at);
+    entries([&](int, int id) {
       if (id >= 0) atomicSub(a.shared + id, 1);
-    }
+    });
     cluster.sync();
-    for (int e = e0 + lane; e < e1; e += 32) {
-      const int id = page_at(e, &at);
-      if (id < 0) continue;
+    entries([&](int e, int id) {
+      if (id < 0) return;
       const int left = fresh(a.shared + id);
-      if (left >= 0) continue;
+      if (left >= 0) return;
       // (marks are far below any count) more requests gave the page up than held it
       if (left < -1 && left > -(1 << 30)) bad = true;
       atomicMin(a.shared + id, mark_of(e));
-    }
+    });
     cluster.sync();
   }
-  auto freed = [&](int e, long long* where) -> int {
-    const int id = page_at(e, where);
-    return id >= 0 && (a.shared == nullptr || fresh(a.shared + id) == mark_of(e)) ? id : -1;
+  auto freed = [&](int e, int id) {
+    return id >= 0 && (a.shared == nullptr || fresh(a.shared + id) == mark_of(e));
   };
   int mine = 0;  // of this warp
-  for (int e = e0 + lane; e - lane < e1; e += 32) mine += __popc(__ballot_sync(0xffffffffu, freed(e, &at) >= 0));
+  entries([&](int e, int id) { mine += __popc(__ballot_sync(0xffffffffu, freed(e, id))); });
   int in_cta = 0;
   int before = cta_exclusive(lane == 0 ? mine : 0, s_warp, &in_cta);
   before = __shfl_sync(0xffffffffu, before, 0);
@@ -299,10 +313,10 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) free_
     total += n;
   }
   const long long start = static_cast<long long>(head) - total;
-  for (int e = e0 + lane; e - lane < e1; e += 32) {
-    const int id = freed(e, &at);
-    const unsigned who = __ballot_sync(0xffffffffu, id >= 0);
-    if (id >= 0) {
+  entries([&](int e, int id) {
+    const bool is = freed(e, id);
+    const unsigned who = __ballot_sync(0xffffffffu, is);
+    if (is) {
       const long long to = start + before + __popc(who & ((1u << lane) - 1u));
       if (to >= 0 && to < a.F)
         a.free_pages[to] = id;
@@ -311,12 +325,8 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) free_
       if (a.shared != nullptr) a.shared[id] = 0;
     }
     before += __popc(who);
-    __syncwarp();
-    if (e < e1 && e >= 0) {
-      const int i = static_cast<int>(static_cast<unsigned>(e) / static_cast<unsigned>(a.M)), j = e - i * a.M;
-      if (j < s_n[i]) a.rows[row_of(i) * a.stride + j] = -1;
-    }
-  }
+    if (int32_t* at = place_of(e)) *at = -1;
+  });
   if (rank == 0 && tid == 0) *a.free_head_out = static_cast<int>(start < 0 ? 0 : start);
   if (bad) report(a.err);
   cluster.sync();  // no CTA leaves while another reads its count
@@ -567,7 +577,7 @@ extern "C" int atf_free_requests(const AtfFreeParams* p, atf_stream_t stream) {
                              p->req_stride,    p->num_rows,  p->max_req_pages, p->shared,
                              p->shared != nullptr ? p->num_pages : 0x7fffffff, p->free_pages, p->free_head,
                              p->free_head_out, p->num_free,  p->error_flag};
-  const size_t smem = (static_cast<size_t>(a.R) + static_cast<size_t>(a.N)) * sizeof(int);
+  const size_t smem = (static_cast<size_t>(a.R) + 2 * static_cast<size_t>(a.N)) * sizeof(int);
   if ((rc = allow_smem(pages::free_kernel, smem)) != ATF_OK) return rc;
   pages::free_kernel<<<pages::CLUSTER, pages::THREADS, smem, reinterpret_cast<cudaStream_t>(stream)>>>(a);
   return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
