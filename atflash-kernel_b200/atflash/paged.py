@@ -21,7 +21,7 @@ _LAYOUTS = ("sorted_pair", "rotate_half")
 
 class BatchPrefillWithPagedKVCacheWrapper:
     """plan() once per step, run() for each layer, on any stream (runs share the workspace, so
-    those of one wrapper follow one another). Request b's new tokens are the rows
+    those of one wrapper, and its captured graphs, follow one another). Request b's new tokens are the rows
     [qo_indptr[b], qo_indptr[b+1]) of q; they are the last of its tokens, whose K and V are
     all in its pages (append them first)."""
 

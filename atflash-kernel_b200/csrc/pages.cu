@@ -28,7 +28,9 @@
 // loads). Up to 128 CTAs an SM wait their turn; more bring nothing, and lists that are
 // mostly padding want few.
 //
-// What bounds the first three: the launch and a few dependent reads of the tables.
+// What bounds the first three: the launch and a few dependent reads of the tables. 96
+// children of up to 128 pages: fork 7 us, free 7.4 (10.7 with the page ids read again in
+// each phase); compaction of a pool of 8703 pages 8.5.
 #include <cooperative_groups.h>
 
 #include "atf_internal.h"

@@ -11,11 +11,12 @@
 //
 // Pages. A key tile is 128 / R slices of R = min(page, 128) rows. The K producer warp, and the
 // V producer warp, read page ids 32 slices at a time, a batch ahead, and a lane per slice
-// and half issues its box, {64 dims, R rows} with 128-byte swizzle, into the rows of the tile. So K lies
-// as Q does: level i is 32 bytes into a row, and dims 64 and up are another 16 KB. Slices past the
-// request's last page are not loaded; their keys are masked and their V rows cleared.
-// K and V have a producer warp each: with one, K of the tile after next waited for a free
-// V stage.
+// and half issues its box, {64 dims, R rows} with 128-byte swizzle, into the rows of the
+// tile. So K lies as Q does: level i is 32 bytes into a row, and dims 64 and up are another
+// 16 KB. Slices past the request's last page are not loaded; their keys are masked and their
+// V rows cleared. (With ids read tile by tile the producers were what a step waited for: 2.2
+// us for two tiles of rows against a key tile instead of 1.8, and long chunks 5.45 ms
+// instead of 4.8.)
 //
 // Rows. A tile's 128 rows are 128 tokens of a query head, or, where that takes fewer
 // tiles, 128 / G tokens with the G heads of a kv head side by side (row = token x G + head;
@@ -28,7 +29,13 @@
 // the even key tiles with one group and on the odd ones with the other, and the groups'
 // states are joined in TMEM at the end (a row's lane is the same for both). Where
 // there are fewer blocks than SMs, the plan also cuts the keys of a block over
-// CTAs; their states go to a workspace (fp32) and merge_kernel joins them.
+// CTAs; their states go to a workspace (fp32) and merge_states_kernel joins them.
+//
+// What bounds it: HBM where rows are few (24 requests x 5 tokens over up to 16001 keys, 28 /
+// 4 heads, pages of 16: 127 us with L2 warm, 142 cold; the floor is 113. A key tile takes
+// 1.1 us from L2 and 1.5 with all SMs reading HBM, and a CTA's start and end 6 more); else
+// the step of two tiles, as in the packed prefill (2 chunks of 8192 behind 24K keys, the
+// window on: 4.3 to 5.0 ms by the clock, 61 to 71% of the burst rate).
 #include <math.h>
 
 #include <algorithm>
@@ -113,6 +120,7 @@ constexpr uint32_t OFF_ROWS = OFF_PLACE + 48;  // [t][128] of where a row goes
 constexpr uint32_t OFF_ABORT = OFF_ROWS + NQ * BM * 4;
 constexpr uint32_t OFF_TMEM = OFF_ABORT + 16;
 constexpr uint32_t SMEM_BYTES = OFF_TMEM + 16 + 1024;  // slack for 1024-B alignment
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of a CTA");
 
 enum { PACKED = 1, SPLIT = 2 };
 // One work item: the rows of one or two tiles of a request against the key tiles [kt0,
