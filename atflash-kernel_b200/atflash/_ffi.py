@@ -10,6 +10,7 @@ import threading
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libatflash_b200.so")
 _lib = None
+_bind = None
 _lock = threading.Lock()
 
 ATF_OK = 0
@@ -287,6 +288,28 @@ def load() -> ctypes.CDLL:
             lib.atf_exchange_region_bytes.restype = _i64
             _lib = lib
     return _lib
+
+
+def binding():
+    """The compiled binding of the calls with short kernels (csrc/binding.cpp), over load()'s
+    library. Raises if it has not been built, or for another version of torch."""
+    global _bind
+    if _bind is None:
+        lib = load()
+        import torch
+
+        from . import _runtime
+        how = "build it again with `python atflash-kernel_b200/build.py`"
+        try:
+            from . import _binding
+        except ImportError as e:
+            raise ImportError(f"the compiled binding cannot be loaded ({e}): {how}") from e
+        if torch.__version__.split("+")[0] != _binding.torch_version.split("+")[0] or _binding.version != ATF_VERSION:
+            raise ImportError(f"the compiled binding is for torch {_binding.torch_version} and version {_binding.version} of "
+                              f"the C interface: {how}")
+        _binding.init({name: ctypes.cast(getattr(lib, name), _vp).value for name in EXPORTED}, check, _runtime)
+        _bind = _binding
+    return _bind
 
 
 def status_string(status: int) -> str:

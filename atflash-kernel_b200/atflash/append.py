@@ -5,15 +5,11 @@ it into the kernels' pair order on the way.
 The reference's decode reads the KV cache that FlashInfer's append fills
 (e2e_pipeline/atflash_e2e_fafi.py:219-223); this is that write side on the
 library's own kernel (``atf_paged_kv_append``)."""
-import ctypes
 from typing import Optional, Tuple
 
 import torch
 
-from . import _ffi, _runtime
-from .norm import check_norm, refuse_gradients
-
-_LAYOUTS = {"sorted_pair": _ffi.ATF_LAYOUT_SORTED_PAIR, "rotate_half": _ffi.ATF_LAYOUT_ROTATE_HALF}
+from . import _ffi
 
 
 def get_batch_indices_positions(append_indptr: torch.Tensor, seq_lens: torch.Tensor,
@@ -31,7 +27,8 @@ def get_batch_indices_positions(append_indptr: torch.Tensor, seq_lens: torch.Ten
 
 
 def check_e4m3_cache(kc: torch.Tensor, vc: torch.Tensor, kv_scales, kv_layout: str) -> Tuple[tuple, tuple, _ffi.AtfKvScales]:
-    """Pages and scales of an e4m3 cache, the append's and the decode's checks. Returns
+    """Pages and scales of an e4m3 cache, the decode's checks (the append's are in the compiled
+    binding). Returns
     (pages, page size, kv heads), the byte strides (page, token, head) and the scales
     for the C call. (Sizes and strides are read once: on a short step the checks'
     host time is the call's.)"""
@@ -58,67 +55,6 @@ def check_e4m3_cache(kc: torch.Tensor, vc: torch.Tensor, kv_scales, kv_layout: s
     if ss != vs.stride():
         raise ValueError("k_scales and v_scales must have the same strides")
     return size, strides, _ffi.AtfKvScales(ks.data_ptr(), vs.data_ptr(), ss[0], ss[1])
-
-
-def _dev_i32(t: torch.Tensor, dev: torch.device, top: int = 0x7fffffff) -> torch.Tensor:
-    if t.dtype == torch.int32 and t.device == dev and t.is_contiguous():
-        return t
-    return _runtime.narrow_i32(t, dev, top)
-
-
-def _k_norm(k_norm, rope, key: torch.Tensor, dev: torch.device) -> _ffi.AtfKNorm:
-    if not isinstance(k_norm, (tuple, list)) or len(k_norm) != 2:
-        raise ValueError("k_norm is (weight, eps)")
-    weight, eps = k_norm
-    if rope is None:
-        raise ValueError("k_norm needs rope: the norm stands before the rotation")
-    refuse_gradients(weight, key)
-    return _ffi.AtfKNorm(weight.data_ptr(), check_norm(weight, eps, dev, "k_norm's weight"), eps)
-
-
-def _append_e4m3(k: torch.Tensor, v: torch.Tensor, batch_indices, positions, kc, vc, kv_indices, kv_indptr, kv_layout,
-                 rope, rope_positions, out_layout, kv_scales, k_norm) -> None:
-    dev = _runtime.require_cuda(k, v, kc, vc)
-    (npages, page, hkv), (s_page, s_tok, s_head), scales = check_e4m3_cache(kc, vc, kv_scales, kv_layout)
-    shape, st = k.shape, k.stride()
-    if (len(shape) != 3 or shape[2] != 128 or st[2] != 1 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16):
-        raise ValueError("keys and values must be (tokens, kv heads, 128) bf16 with a contiguous head_dim")
-    if v.shape != shape or v.stride() != st:
-        raise ValueError("append_key and append_value must have the same shape and strides")
-    nnz = shape[0]
-    if shape[1] != hkv:
-        raise ValueError("append_key heads do not match the cache")
-    layout = _LAYOUTS[out_layout]
-    norm = _k_norm(k_norm, rope, k, dev) if k_norm is not None else None
-    bi, ps = _dev_i32(batch_indices, dev), _dev_i32(positions, dev)
-    ip, ix = _dev_i32(kv_indptr, dev, kv_indices.numel()), _dev_i32(kv_indices, dev)
-    if bi.numel() != nnz or ps.numel() != nnz:
-        raise ValueError("batch_indices and positions need one entry per appended token")
-    if nnz == 0:
-        return
-    p = _ffi.AtfAppendParams(k.data_ptr(), v.data_ptr(), nnz, st[0], st[1], bi.data_ptr(), ps.data_ptr(), kc.data_ptr(),
-                             vc.data_ptr(), npages, s_page, s_tok, s_head, hkv, 128, page, ip.numel() - 1,
-                             ip.data_ptr(), ix.data_ptr())
-    p.out_layout = layout
-    p.error_flag = _runtime.error_flag_ptr(dev)
-    if rope is not None:
-        cos, sin = rope
-        cst, csh = cos.stride(), cos.shape
-        if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(csh) != 2 or csh != sin.shape
-                or csh[1] < 64 or cst != sin.stride() or cst[1] != 1 or cos.device != dev or sin.device != dev):
-            raise ValueError("cos/sin must be matching fp32 (n_pos, >=64) tables")
-        p.cos, p.sin, p.cs_stride_pos, p.n_pos = cos.data_ptr(), sin.data_ptr(), cst[0], csh[0]
-        if rope_positions is not None:
-            rp = rope_positions.to(device=dev, dtype=torch.int64).contiguous()
-            if rp.numel() != nnz:
-                raise ValueError("rope_positions needs one entry per appended token")
-            p.rope_positions = rp.data_ptr()
-    if norm is not None:
-        _runtime.launch("atf_paged_kv_append_norm", _ffi.load().atf_paged_kv_append_norm, dev, ctypes.byref(p),
-                        ctypes.byref(scales), ctypes.byref(norm))
-        return
-    _runtime.launch("atf_paged_kv_append_e4m3", _ffi.load().atf_paged_kv_append_e4m3, dev, ctypes.byref(p),
-                    ctypes.byref(scales))
 
 
 def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, batch_indices: torch.Tensor,
@@ -151,75 +87,8 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
         kc, vc = paged_kv_cache
     else:
         kc, vc = paged_kv_cache[:, 0], paged_kv_cache[:, 1]
-    if kv_scales is not None:
-        _append_e4m3(append_key, append_value, batch_indices, positions, kc, vc, kv_indices, kv_indptr, kv_layout, rope,
-                     rope_positions, out_layout, kv_scales, k_norm)
-        return
-    dev = _runtime.require_cuda(append_key, append_value, kc, vc)
-    if torch.float8_e4m3fn in (kc.dtype, vc.dtype):
-        raise ValueError("float8_e4m3fn pages need kv_scales")
-    # (sizes and strides are read once: on a short step the checks' host time is the call's)
-    kcs, vcs, kct, vct = kc.shape, vc.shape, kc.stride(), vc.stride()
-    shape, st = append_key.shape, append_key.stride()
-    k_level_major = len(kcs) == 5
-    bf16 = torch.bfloat16
-    if (append_key.dtype != bf16 or append_value.dtype != bf16 or vc.dtype != bf16 or kc.dtype != bf16
-            or shape[-1] != 128 or vcs[-1] != 128 or st[-1] != 1 or vct[-1] != 1
-            or (not k_level_major and (kcs[-1] != 128 or kct[-1] != 1))):
-        raise ValueError("keys, values and cache pages must be bf16 with a contiguous head_dim of 128")
-    if shape != append_value.shape or st != append_value.stride():
-        raise ValueError("append_key and append_value must have the same shape and strides")
-    if k_level_major:
-        # (P, Hkv, 8 levels, page, 16) sorted-pair K pages (see BatchDecodeWithPagedKVCacheWrapper.run)
-        if (kcs[2] != 8 or kcs[4] != 16 or kct[4] != 1 or kct[3] != 16 or len(vcs) != 4 or kcs[0] != vcs[0]):
-            raise ValueError("level-major k pages must be (P, Hkv, 8, page, 16) bf16 with 16-element rows")
-        if rope is not None and out_layout != "sorted_pair":
-            raise ValueError("level-major k pages hold sorted-pair K")
-    elif kcs != vcs or kct != vct or len(kcs) != 4:
-        raise ValueError("k and v pages must have the same 4-d shape and strides")
-    nnz, hkv, _ = shape
-    if kv_layout == "NHD":
-        npages, page, hk2, _ = vcs
-        s_page, s_tok, s_head, _ = vct
-    elif kv_layout == "HND":
-        npages, hk2, page, _ = vcs
-        s_page, s_head, s_tok, _ = vct
-    else:
-        raise ValueError("kv_layout must be NHD or HND")
-    if hk2 != hkv:
-        raise ValueError("append_key heads do not match the cache")
-    layout = _LAYOUTS[out_layout]
-    norm = _k_norm(k_norm, rope, append_key, dev) if k_norm is not None else None
-    bi, ps = _dev_i32(batch_indices, dev), _dev_i32(positions, dev)
-    ip, ix = _dev_i32(kv_indptr, dev, kv_indices.numel()), _dev_i32(kv_indices, dev)
-    if bi.numel() != nnz or ps.numel() != nnz:
-        raise ValueError("batch_indices and positions need one entry per appended token")
-    if nnz == 0:
-        return
-    p = _ffi.AtfAppendParams(append_key.data_ptr(), append_value.data_ptr(), nnz, st[0], st[1], bi.data_ptr(),
-                             ps.data_ptr(), kc.data_ptr(), vc.data_ptr(), npages, s_page, s_tok, s_head, hkv, 128, page,
-                             ip.numel() - 1, ip.data_ptr(), ix.data_ptr())
+    cos = sin = None
     if rope is not None:
         cos, sin = rope
-        cst, csh = cos.stride(), cos.shape
-        if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or csh != sin.shape or len(csh) != 2
-                or csh[1] < 64 or cst != sin.stride() or cst[1] != 1 or cos.device != dev or sin.device != dev):
-            raise ValueError("cos/sin must be matching fp32 (n_pos, >=64) tables")
-        p.cos, p.sin, p.cs_stride_pos, p.n_pos = cos.data_ptr(), sin.data_ptr(), cst[0], csh[0]
-        if rope_positions is not None:
-            rp = rope_positions.to(device=dev, dtype=torch.int64).contiguous()
-            if rp.numel() != nnz:
-                raise ValueError("rope_positions needs one entry per appended token")
-            p.rope_positions = rp.data_ptr()
-    p.out_layout = layout
-    p.error_flag = _runtime.error_flag_ptr(dev)
-    if k_level_major:
-        if kcs[1] != hkv or kcs[3] != page:
-            raise ValueError("level-major k pages do not match the v pages")
-        p.k_level_major = 1
-        p.k_stride_page, p.k_stride_head, p.k_stride_level = kct[0], kct[1], kct[2]
-    if norm is not None:
-        _runtime.launch("atf_paged_kv_append_norm", _ffi.load().atf_paged_kv_append_norm, dev, ctypes.byref(p), None,
-                        ctypes.byref(norm))
-    else:
-        _runtime.launch("atf_paged_kv_append", _ffi.load().atf_paged_kv_append, dev, ctypes.byref(p))
+    _ffi.binding().append(append_key, append_value, batch_indices, positions, kc, vc, kv_indices, kv_indptr, kv_layout,
+                          cos, sin, rope_positions, out_layout, kv_scales, k_norm)

@@ -112,7 +112,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         for i, z in enumerate(zhi or ()):
             t.zhi[i] = z
         t.error_flag = _runtime.error_flag(self._dev).data_ptr()
-        self._plan = t
+        self._plan, self._plan_ptr = t, ctypes.addressof(t)
 
     begin_forward = plan
 
@@ -125,47 +125,12 @@ class BatchPrefillWithPagedKVCacheWrapper:
         ``atflash.check_device_errors()`` (code 2); its request's outputs are not valid then."""
         if self._plan is None:
             raise RuntimeError("plan() must be called before run()")
-        t = self._plan
-        nq, hq, hkv, page = t.total_q, t.num_heads_q, t.num_heads_kv, t.page_size
         if isinstance(paged_kv_cache, (tuple, list)):
             kc, vc = paged_kv_cache
         else:
             kc, vc = paged_kv_cache[:, 0], paged_kv_cache[:, 1]
-        dev = _runtime.require_cuda(q, kc, vc)
-        if dev != self._dev:
-            raise ValueError(f"the plan is on {self._dev}, the tensors are on {dev}")
-        if q.dtype != torch.bfloat16 or kc.dtype != torch.bfloat16 or vc.dtype != torch.bfloat16:
-            raise TypeError("q and the KV cache must be bfloat16")
-        nhd, size = self._kv_layout == "NHD", vc.shape
-        want = (page, hkv, 128) if nhd else (hkv, page, 128)
-        if kc.shape != size or len(size) != 4 or size[1:] != want or size[0] < 1:
-            raise ValueError(f"planned for k and v pages of {want}")
-        shape, qst, kst, vst = (nq, hq, 128), q.stride(), kc.stride(), vc.stride()
-        if q.shape != shape:
-            raise ValueError(f"planned for q {shape}")
-        if qst[2] != 1 or kst[3] != 1 or vst[3] != 1:
-            raise ValueError("the head_dim axis must be contiguous")
-        if out is None:
-            out = q.new_empty(shape)
-        elif out.shape != shape or out.dtype != torch.bfloat16 or out.device != dev or out.stride(-1) != 1:
-            raise ValueError(f"out must be a bf16 {shape} tensor on {dev} with a contiguous head_dim axis")
-        if return_lse and lse is None:
-            lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
-        if lse is not None and (lse.shape != shape[:2] or lse.dtype != torch.float32 or lse.device != dev
-                                or not lse.is_contiguous()):
-            raise ValueError(f"lse must be a contiguous float32 {shape[:2]} tensor on {dev}")
-        if nq > 0:
-            p = _ffi.AtfPrefillPagedParams.from_buffer_copy(t)
-            p.q, p.k_cache, p.v_cache, p.out, p.num_pages = q.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr(), size[0]
-            if lse is not None:
-                p.lse = lse.data_ptr()
-            p.q_stride_s, p.q_stride_h, _ = qst
-            p.o_stride_s, p.o_stride_h, _ = out.stride()
-            tok, head = (1, 2) if nhd else (2, 1)
-            p.k_stride_page, p.k_stride_token, p.k_stride_head = kst[0], kst[tok], kst[head]
-            p.v_stride_page, p.v_stride_token, p.v_stride_head = vst[0], vst[tok], vst[head]
-            self._held.use()
-            _runtime.launch("atf_prefill_paged_fwd", _ffi.load().atf_prefill_paged_fwd, dev, ctypes.byref(p))
-        return (out, lse) if return_lse else out
+        self._held.use()
+        return _ffi.binding().paged_run(self._plan_ptr, self._dev.index, self._kv_layout == "NHD", q, kc, vc, out, lse,
+                                        return_lse)
 
     forward = run

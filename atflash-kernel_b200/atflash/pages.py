@@ -13,7 +13,7 @@ Index reports of these calls go to ``atflash.check_device_errors()`` (code 2). T
 reference serves one request and has no counterpart."""
 import ctypes
 from dataclasses import dataclass
-from typing import Optional, Sequence, Tuple
+from typing import Optional, Sequence
 
 import torch
 
@@ -27,55 +27,6 @@ class PageMoves:
     src: torch.Tensor
     dst: torch.Tensor
     free_head: torch.Tensor
-
-
-def _list(t: torch.Tensor, name: str, dev: torch.device, n: Optional[int] = None) -> torch.Tensor:
-    """An index list that a call reads, as contiguous int32."""
-    shape = t.shape
-    if len(shape) != 1 or (n is not None and shape[0] != n) or t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{name} must be a 1-d integer tensor" + (f" of {n} entries" if n is not None else ""))
-    if t.device != dev:
-        raise ValueError("all tensors must be on the same device")
-    return t if t.dtype == torch.int32 and t.is_contiguous() else _runtime.narrow_i32(t, dev)
-
-
-def _state(t: torch.Tensor, name: str, dev: torch.device, least: int = 1) -> int:
-    """A tensor that a call changes in place, taken as it is; returns its number of entries."""
-    shape = t.shape
-    if len(shape) != 1 or shape[0] < least or t.dtype != torch.int32 or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous 1-d int32 tensor" + (f" of {least} entries or more" if least > 1 else ""))
-    if t.device != dev:
-        raise ValueError("all tensors must be on the same device")
-    return shape[0]
-
-
-def _table(req_pages: torch.Tensor, batch: int, page_size: int) -> Tuple[torch.device, Tuple[int, int, int, int]]:
-    """Checks the request table; returns its device, and its address, row stride, rows and
-    pages per row."""
-    dev = _runtime.require_cuda(req_pages)
-    shape, st = req_pages.shape, req_pages.stride()
-    if len(shape) != 2 or req_pages.dtype != torch.int32 or (shape[1] > 1 and st[1] != 1):
-        raise ValueError("req_pages must be an int32 (rows, pages) tensor with contiguous rows")
-    rows, width = shape
-    if rows < 1 or width < 1 or rows > _ffi.ATF_PAGES_MAX_ROWS:
-        raise ValueError(f"req_pages must have between 1 and {_ffi.ATF_PAGES_MAX_ROWS} rows, of one page or more")
-    if rows > 1 and st[0] < width:
-        raise ValueError("the rows of req_pages must not overlap")
-    if batch < 1 or batch > _ffi.ATF_TABLES_MAX_BATCH:
-        raise ValueError(f"between 1 and {_ffi.ATF_TABLES_MAX_BATCH} requests")
-    if batch * width >= 1 << 30:
-        raise ValueError("requests x pages must be under 2^30")
-    if page_size < 1:
-        raise ValueError("page_size must be positive")
-    return dev, (req_pages.data_ptr(), st[0] if rows > 1 else width, rows, width)
-
-
-def _rows(req_rows: Optional[torch.Tensor], rows: int, batch: int, dev: torch.device) -> Optional[torch.Tensor]:
-    if req_rows is not None:
-        return _list(req_rows, "req_rows", dev, batch)
-    if rows < batch:
-        raise ValueError("req_pages needs a row for each request")
-    return None
 
 
 def fork_requests(parents: torch.Tensor, children: torch.Tensor, kv_lens: torch.Tensor, req_pages: torch.Tensor,
@@ -93,21 +44,8 @@ def fork_requests(parents: torch.Tensor, children: torch.Tensor, kv_lens: torch.
     lengths out of range are left out. A page that the free list cannot give is -1 in the
     row, and its pair is -1. Each is reported (code 2). src and dst have one entry per
     child, -1 where there is nothing to copy; free_head itself stays."""
-    n = parents.numel()
-    dev, table = _table(req_pages, n, page_size)
-    parents, children = _list(parents, "parents", dev), _list(children, "children", dev, n)
-    kv_lens = _list(kv_lens, "kv_lens", dev, n)
-    free_pages, free_head = _list(free_pages, "free_pages", dev), _list(free_head, "free_head", dev, 1)
-    num_pages = _state(shared, "shared", dev)
-    out = parents.new_empty(2 * n + 1)
-    src, head = out.data_ptr(), free_head.data_ptr()
-    p = _ffi.AtfForkParams(
-        parents.data_ptr(), children.data_ptr(), kv_lens.data_ptr(), n, int(page_size), *table, shared.data_ptr(), num_pages,
-        # an empty list still has a head: any valid address will do for its pages
-        free_pages.data_ptr() or head, head, src + 8 * n, free_pages.shape[0], src, src + 4 * n,
-        _runtime.error_flag_ptr(dev))
-    _runtime.launch("atf_fork_requests", _ffi.load().atf_fork_requests, dev, ctypes.byref(p))
-    return PageMoves(*out.split_with_sizes((n, n, 1)))
+    return PageMoves(*_ffi.binding().fork_requests(parents, children, kv_lens, req_pages, page_size, free_pages, free_head,
+                                                   shared))
 
 
 def free_requests(req_rows: Optional[torch.Tensor], kv_lens: torch.Tensor, req_pages: torch.Tensor, page_size: int, *,
@@ -123,20 +61,7 @@ def free_requests(req_rows: Optional[torch.Tensor], kv_lens: torch.Tensor, req_p
     A row that is named twice (its first entry counts), rows and lengths out of range,
     page ids outside the cache, a page given up more often than it was held and a list
     without room are reported (code 2) and left out."""
-    n = kv_lens.numel()
-    dev, table = _table(req_pages, n, page_size)
-    kv_lens = _list(kv_lens, "kv_lens", dev)
-    req_rows = _rows(req_rows, table[2], n, dev)
-    num_free = _state(free_pages, "free_pages", dev)
-    free_head = _list(free_head, "free_head", dev, 1)
-    num_pages = _state(shared, "shared", dev) if shared is not None else 0
-    out = kv_lens.new_empty(1)
-    p = _ffi.AtfFreeParams(
-        req_rows.data_ptr() if req_rows is not None else None, kv_lens.data_ptr(), n, int(page_size), *table,
-        shared.data_ptr() if shared is not None else None, num_pages, free_pages.data_ptr(), free_head.data_ptr(),
-        out.data_ptr(), num_free, _runtime.error_flag_ptr(dev))
-    _runtime.launch("atf_free_requests", _ffi.load().atf_free_requests, dev, ctypes.byref(p))
-    return out
+    return _ffi.binding().free_requests(req_rows, kv_lens, req_pages, page_size, free_pages, free_head, shared)
 
 
 def compact_pages(kv_lens: torch.Tensor, req_pages: torch.Tensor, page_size: int, num_pages: int, *, max_moves: int,
@@ -153,25 +78,8 @@ def compact_pages(kv_lens: torch.Tensor, req_pages: torch.Tensor, page_size: int
 
     Pages that no named request holds count as free. Rows, lengths and page ids out of
     range are reported (code 2) and left out. At most 2^20 pages."""
-    n, num_pages, max_moves = kv_lens.numel(), int(num_pages), int(max_moves)
-    dev, table = _table(req_pages, n, page_size)
-    if num_pages < 1 or num_pages > _ffi.ATF_COMPACT_MAX_PAGES:
-        raise ValueError(f"between 1 and {_ffi.ATF_COMPACT_MAX_PAGES} pages")
-    if max_moves < 0 or max_moves > num_pages:
-        raise ValueError("max_moves must be between 0 and num_pages")
-    kv_lens = _list(kv_lens, "kv_lens", dev)
-    req_rows = _rows(req_rows, table[2], n, dev)
-    num_free = _state(free_pages, "free_pages", dev, num_pages)
-    if shared is not None:
-        _state(shared, "shared", dev, num_pages)
-    out = kv_lens.new_empty(2 * max_moves + 1)
-    src = out.data_ptr()
-    p = _ffi.AtfCompactParams(
-        req_rows.data_ptr() if req_rows is not None else None, kv_lens.data_ptr(), n, int(page_size), *table,
-        shared.data_ptr() if shared is not None else None, num_pages, max_moves, free_pages.data_ptr(),
-        src + 8 * max_moves, num_free, src, src + 4 * max_moves, _runtime.error_flag_ptr(dev))
-    _runtime.launch("atf_compact_pages", _ffi.load().atf_compact_pages, dev, ctypes.byref(p))
-    return PageMoves(*out.split_with_sizes((max_moves, max_moves, 1)))
+    return PageMoves(*_ffi.binding().compact_pages(kv_lens, req_pages, page_size, num_pages, max_moves, free_pages, req_rows,
+                                                   shared))
 
 
 class PageCopier:
@@ -206,14 +114,7 @@ class PageCopier:
         other ids outside the cache are reported by ``atflash.check_device_errors()`` (code 2)
         and left out. The pages of dst differ from one another and are none of src's, as in
         the lists of ``fork_requests`` and ``compact_pages``; src may name a page twice."""
-        src = _list(src, "src", self._dev)
-        n = src.shape[0]
-        dst = _list(dst, "dst", self._dev, n)
-        if n == 0:
-            return
-        p = _ffi.AtfCopyPagesParams(self._desc_ptr, len(self._desc), self._pages, src.data_ptr(), dst.data_ptr(), n,
-                                    _runtime.error_flag_ptr(self._dev))
-        _runtime.launch("atf_copy_pages", _ffi.load().atf_copy_pages, self._dev, ctypes.byref(p))
+        _ffi.binding().copy_pages(self._desc_ptr, len(self._desc), self._pages, self._dev.index, src, dst)
 
 
 def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:

@@ -1,22 +1,27 @@
 #!/usr/bin/env python
-"""Build libatflash_b200.so (sm_100a) in-tree with nvcc.
+"""Build libatflash_b200.so (sm_100a) in-tree with nvcc, and the Python binding of its
+short calls with g++ (against the installed torch's headers).
 
     python atflash-kernel_b200/build.py [--verbose-ptxas]
 
-The library is written to atflash-kernel_b200/atflash/_lib/ so that it travels
-with the source tree; nothing is installed.
+The library is written to atflash-kernel_b200/atflash/_lib/, the binding to
+atflash-kernel_b200/atflash/_binding.so, so that they travel with the source tree;
+nothing is installed.
 """
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "atflash", "_lib")
 LIB = os.path.join(OUT_DIR, "libatflash_b200.so")
+BINDING = os.path.join(HERE, "atflash", "_binding.so")
 SOURCES = ["api.cu", "prefill_sm100.cu", "prefill_ragged_sm100.cu", "prefill_paged_sm100.cu", "decode.cu",
            "decode_e4m3.cu", "decode_noalloc.cu", "exchange.cu", "rope.cu", "append.cu", "append_e4m3.cu", "tables.cu", "pages.cu", "qk_norm.cu",
            "selftest.cu"]
@@ -30,7 +35,7 @@ def nvcc_path():
     raise RuntimeError("nvcc not found")
 
 
-def build(verbose_ptxas=False, force=False):
+def build_library(verbose_ptxas=False, force=False):
     os.makedirs(OUT_DIR, exist_ok=True)
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
     deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
@@ -46,6 +51,32 @@ def build(verbose_ptxas=False, force=False):
     subprocess.run(cmd, check=True)
     os.replace(LIB + ".tmp", LIB)
     return LIB
+
+
+def build_binding(force=False):
+    src = os.path.join(CSRC, "binding.cpp")
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    deps = [src, os.path.join(ROOT, "include", "atflash_b200.h"),
+            os.path.join(torch_dir, "include", "torch", "headeronly", "version.h")]
+    if not force and os.path.exists(BINDING):
+        t = os.path.getmtime(BINDING)
+        if all(os.path.getmtime(d) <= t for d in deps):
+            return BINDING
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path())))
+    inc = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{i}" for i in inc), "-o",
+           BINDING + ".tmp", src, f"-L{os.path.join(torch_dir, 'lib')}",
+           *(f"-l{lib}" for lib in ("c10", "c10_cuda", "torch_cpu", "torch", "torch_python"))]
+    subprocess.run(cmd, check=True)
+    os.replace(BINDING + ".tmp", BINDING)
+    return BINDING
+
+
+def build(verbose_ptxas=False, force=False):
+    lib = build_library(verbose_ptxas, force)
+    build_binding(force)
+    return lib
 
 
 if __name__ == "__main__":
