@@ -62,15 +62,7 @@ const Tensor* tensor_or_none(PyObject* o, const char* name) { return o == Py_Non
 
 int64_t integer(PyObject* o) {
   const int64_t v = PyLong_AsLongLong(o);
-  if (v == -1 && PyErr_Occurred()) {
-    PyErr_Clear();
-    PyObject* i = PyNumber_Index(o);
-    if (i == nullptr) throw python_error();
-    const int64_t w = PyLong_AsLongLong(i);
-    Py_DECREF(i);
-    if (w == -1 && PyErr_Occurred()) throw python_error();
-    return w;
-  }
+  if (v == -1 && PyErr_Occurred()) throw python_error();
   return v;
 }
 
