@@ -1,6 +1,5 @@
-"""Attention of new tokens over a paged cache: a plan()/run() wrapper with the names and
-the plan's arguments of FlashInfer's ``BatchPrefillWithPagedKVCacheWrapper``, with ATFlash
-windows. One batch may hold decodes (one token), drafted tokens to verify (a few)
+"""Attention of new tokens over a paged cache: a plan()/run() wrapper whose plan takes the
+arguments of the decode's and the packed prefill's together, with ATFlash windows. One batch may hold decodes (one token), drafted tokens to verify (a few)
 and chunks of prompts behind what their requests, or the requests they were forked
 from, have in the cache.
 

@@ -30,7 +30,7 @@
 //
 // What bounds the first three: the launch and a few dependent reads of the tables. 96
 // children of up to 128 pages: fork 7 us, free 7.4 (10.7 with the page ids read again in
-// each phase); compaction of a pool of 8703 pages 8.5.
+// each phase, 7.7 with the marks read twice); compaction of a pool of 8703 pages 8.5.
 #include <cooperative_groups.h>
 
 #include "atf_internal.h"
@@ -279,16 +279,16 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) free_
   auto entries = [&](auto&& f) {
 #pragma unroll
     for (int k = 0; k < KEPT; ++k)
-      if (e0 + 32 * k < e1) f(e0 + lane + 32 * k, kept[k]);
-    for (int e = e0 + lane + 32 * KEPT; e - lane < e1; e += 32) f(e, page_at(e));
+      if (e0 + 32 * k < e1) f(e0 + lane + 32 * k, kept[k], k);
+    for (int e = e0 + lane + 32 * KEPT; e - lane < e1; e += 32) f(e, page_at(e), KEPT);
   };
   auto mark_of = [&](int e) { return static_cast<int>(0x80000000u) + (all - 1 - e); };
   if (a.shared != nullptr) {
-    entries([&](int, int id) {
+    entries([&](int, int id, int) {
       if (id >= 0) atomicSub(a.shared + id, 1);
     });
     cluster.sync();
-    entries([&](int e, int id) {
+    entries([&](int e, int id, int) {
       if (id < 0) return;
       const int left = fresh(a.shared + id);
       if (left >= 0) return;
@@ -301,8 +301,13 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) free_
   auto freed = [&](int e, int id) {
     return id >= 0 && (a.shared == nullptr || fresh(a.shared + id) == mark_of(e));
   };
-  int mine = 0;  // of this warp
-  entries([&](int e, int id) { mine += __popc(__ballot_sync(0xffffffffu, freed(e, id))); });
+  int mine = 0;        // of this warp
+  unsigned known = 0;  // whether the kept entries are freed
+  entries([&](int e, int id, int k) {
+    const bool is = freed(e, id);
+    if (k < KEPT) known |= is ? 1u << k : 0u;
+    mine += __popc(__ballot_sync(0xffffffffu, is));
+  });
   int in_cta = 0;
   int before = cta_exclusive(lane == 0 ? mine : 0, s_warp, &in_cta);
   before = __shfl_sync(0xffffffffu, before, 0);
@@ -315,8 +320,8 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) free_
     total += n;
   }
   const long long start = static_cast<long long>(head) - total;
-  entries([&](int e, int id) {
-    const bool is = freed(e, id);
+  entries([&](int e, int id, int k) {
+    const bool is = k < KEPT ? ((known >> k) & 1u) != 0 : freed(e, id);
     const unsigned who = __ballot_sync(0xffffffffu, is);
     if (is) {
       const long long to = start + before + __popc(who & ((1u << lane) - 1u));

@@ -109,6 +109,21 @@ def test_one_parent_of_many_and_pages_freed_together():
     assert x.m.shared == [0] * 64 and sorted(x.m.free) == list(range(64)) and x.m.head == 0
 
 
+@pytest.mark.parametrize("rows,kids", [(10900, 50), (10200, 700), (11900, 60)])
+def test_tables_whose_lists_fill_48_kb_of_shared_memory(rows, kids):
+    # R + 2 N words, of which 48 KB need no leave
+    x = Mirror(kids + 200, rows, 3, 8, 6)
+    for r in range(40):
+        x.m.take(r, 3)
+    x.upload()
+    children = list(range(rows - kids, rows))
+    take = [24 - i % 25 for i in range(kids)]
+    x.fork([i % 40 for i in range(kids)], children, take)
+    x.same()
+    x.give_back(children, take)
+    x.same()
+
+
 def test_the_largest_tables():
     rows, width = 8192, 20
     x = Mirror(rows * width // 2, rows, width, 16, 5)
