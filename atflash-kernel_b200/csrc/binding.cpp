@@ -610,6 +610,8 @@ PyObject* paged_run(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   if (out != nullptr && (out->sizes() != q.sizes() || out->scalar_type() != at::kBFloat16 || out->device() != dev ||
                          out->stride(2) != 1))
     throw ValueError("out must be a bf16 " + shape + " tensor" + on(dev) + " with a contiguous head_dim axis");
+  for (int i = 0; out != nullptr && i < 2; ++i)
+    if (out->size(i) > 1 && out->stride(i) == 0) throw ValueError("out must not be expanded: its rows are written");
   if (lse != nullptr && (lse->dim() != 2 || lse->size(0) != nq || lse->size(1) != hq || lse->scalar_type() != at::kFloat ||
                          lse->device() != dev || !lse->is_contiguous()))
     throw ValueError("lse must be a contiguous float32 (" + std::to_string(nq) + ", " + std::to_string(hq) + ") tensor" + on(dev));

@@ -304,3 +304,14 @@ def test_refusals():
     with pytest.raises(atflash.AtfError, match="aligned"):
         w.run(odd, (c, c))
     w.run(q, (c, c))
+
+
+def test_an_expanded_output_is_refused():
+    import atflash
+    w = atflash.BatchPrefillWithPagedKVCacheWrapper(torch.empty(1 << 20, dtype=torch.uint8, device=DEV))
+    w.plan([0, 2], [0, 1], [0], [5], 4, 2, 128, 16)
+    q = torch.zeros((2, 4, 128), dtype=torch.bfloat16, device=DEV)
+    c = torch.zeros((1, 16, 2, 128), dtype=torch.bfloat16, device=DEV)
+    for out in (q[:1].expand(2, 4, 128), q[:, :1].expand(2, 4, 128)):
+        with pytest.raises(ValueError, match="expanded"):
+            w.run(q, (c, c), out=out)
