@@ -41,7 +41,7 @@ struct Args {
   const void* norm_w;
   int norm_f32;
   float eps;
-  unsigned units;  // of 4 U heads per token
+  unsigned units;  // of heads, per token or per four tokens
 };
 
 __global__ void append_kernel(const Args a) {
@@ -92,31 +92,38 @@ __global__ void append_kernel(const Args a) {
                          a.sorted != 0, lstride);
 }
 
-// With a norm of K in front of the rotation (norm_math.cuh). A warp takes 4 U heads of a
-// token, 8 lanes a row as above, so that the token's page is looked up and its angles are
-// read once for them, while their rows are on the way.
+// With a norm of K in front of the rotation (norm_math.cuh). 8 lanes hold a row, as above,
+// and a warp 8 rows, whose loads are on the way while the pages are looked up: two heads
+// of four tokens, so that no lane is idle for few heads and the pieces that level-major K
+// leaves in (32 bytes a row and level) make up whole lines. A step's tokens (too few for two
+// CTAs an SM) go by 4 heads of one token.
 //
-// HBM-bound for prompts: 64K tokens x 8 heads take 96 us into pages of 16 (91% of HBM), 107
-// into level-major ones, whose K leaves in pieces of 32 bytes. A thread per (row, 8 pairs)
-// as above took 129 / 120 us (115 / 104 with the loads in front of the lookup), 4 heads a
-// warp 119 / 107, 8 heads with more registers and fewer CTAs 123 / 111. A step's tokens (too
-// few for two CTAs an SM) go by 4 heads.
-template <int U>
-__global__ void __launch_bounds__(256, U == 2 ? 3 : 4) append_norm_kernel(const Args a) {
+// HBM-bound for prompts: 64K tokens x 8 heads take 96 us into pages of 16 (91% of HBM), 102
+// into level-major ones; x 4 heads 53 and 57, x 1 head 25 and 27. With 8 heads of a token per
+// warp 96 and 107, 73 and 77, 64 and 65. A thread per (row, 8 pairs) as above took 129 / 120
+// us (115 / 104 with the loads in front of the lookup), 4 heads a warp 119 / 107, 8 heads with
+// more registers and fewer CTAs 123 / 111.
+template <bool MANY>
+__global__ void __launch_bounds__(256, MANY ? 3 : 4) append_norm_kernel(const Args a) {
+  constexpr int U = MANY ? 2 : 1, HSTEP = MANY ? 1 : 4;
   __shared__ __align__(16) float s_w[128];
   const int lane = threadIdx.x & 31, c = lane & 7;
   if (threadIdx.x < 128) s_w[threadIdx.x] = normmath::weight_at(a.norm_w, a.norm_f32 != 0, threadIdx.x);
   __syncthreads();
   const unsigned unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);  // (the host keeps them within 32 bits)
-  const unsigned i = unit / a.units;
-  if (i >= a.nnz) return;
-  const int h0 = static_cast<int>(unit - i * a.units) * (4 * U) + (lane >> 3);
+  const unsigned first = unit / a.units;  // token, or four of them
+  if (first * (MANY ? 4u : 1u) >= a.nnz) return;
+  const int hu = static_cast<int>(unit - first * a.units);
+  const int h0 = MANY ? hu * U : hu * 4 + (lane >> 3);
+  // (lanes behind the last token repeat it and write nothing)
+  const bool in = !MANY || first * 4u + (lane >> 3) < a.nnz;
+  const unsigned i = MANY ? min(first * 4u + (lane >> 3), static_cast<unsigned>(a.nnz - 1)) : first;
   const int b = a.batch_indices[i];
   const int pos = a.positions[i];
   uint4 k0[U], k1[U], v0[U], v1[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const long long src = i * a.as_n + static_cast<long long>(min(h0 + 4 * u, a.H - 1)) * a.as_h;
+    const long long src = i * a.as_n + static_cast<long long>(min(h0 + HSTEP * u, a.H - 1)) * a.as_h;
     k0[u] = *reinterpret_cast<const uint4*>(a.ak + src + 8 * c);
     k1[u] = *reinterpret_cast<const uint4*>(a.ak + src + 64 + 8 * c);
     v0[u] = *reinterpret_cast<const uint4*>(a.av + src + 8 * c);
@@ -138,15 +145,15 @@ __global__ void __launch_bounds__(256, U == 2 ? 3 : 4) append_norm_kernel(const 
     }
   }
   if (bad) {
-    if (a.err != nullptr && lane == 0) atomicCAS(a.err, 0, kDevErrIndex);
-    return;
+    if (a.err != nullptr && c == 0) atomicCAS(a.err, 0, kDevErrIndex);
+    if (!MANY) return;  // (the shuffles below need all lanes of a warp with several tokens)
   }
   const int slot = pos % a.page_size;
   const long long lstride = a.k_lm ? a.k_s_level : 16;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int h = h0 + 4 * u;
-    const bool on = h < a.H;
+    const int h = h0 + HSTEP * u;
+    const bool on = in && !bad && h < a.H;
     const long long dst = page * a.s_page + slot * a.s_tok + h * a.s_head;
     if (on) {
       *reinterpret_cast<uint4*>(a.vc + dst + 8 * c) = v0[u];
@@ -248,15 +255,17 @@ int atf::append_bf16(const AtfAppendParams* p, const AtfKNorm* norm, atf_stream_
     a.norm_w = norm->weight;
     a.norm_f32 = norm->weight_dtype == ATF_DTYPE_F32 ? 1 : 0;
     a.eps = norm->eps;
-    const long long narrow = (a.H + 3) / 4, wide = (a.H + 7) / 8;
+    const long long narrow = (a.H + 3) / 4;  // units of 4 heads a token
     if (a.nnz > (1ll << 30) / narrow) return ATF_ERR_UNSUPPORTED;
-    const bool many = a.nnz * wide >= 2ll * 148 * 8;
-    a.units = static_cast<unsigned>(many ? wide : narrow);
-    const unsigned blocks = static_cast<unsigned>((a.nnz * a.units + 7) / 8);
+    // 8 rows per warp once that gives every SM two CTAs
+    const bool many = a.nnz * ((a.H + 7) / 8) >= 2ll * 148 * 8;
+    a.units = static_cast<unsigned>(many ? (a.H + 1) / 2 : narrow);
+    const long long items = many ? (a.nnz + 3) / 4 : a.nnz;
+    const unsigned blocks = static_cast<unsigned>((items * a.units + 7) / 8);
     if (many)
-      append::append_norm_kernel<2><<<blocks, threads, 0, st>>>(a);
+      append::append_norm_kernel<true><<<blocks, threads, 0, st>>>(a);
     else
-      append::append_norm_kernel<1><<<blocks, threads, 0, st>>>(a);
+      append::append_norm_kernel<false><<<blocks, threads, 0, st>>>(a);
     return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
   }
   const long long blocks = (total + threads - 1) / threads;

@@ -7,8 +7,8 @@
 // 8 lanes hold a row: 8 pairs each, two 16-byte loads, so that the sum of squares is 16
 // products and three shuffles, both elements of a pair are in one lane, and each lane's
 // 8 angles are those of its column. They are loaded once for all heads of the token that
-// the warp covers: a warp takes 4 U heads of a token, 4 at a time, with the loads of all
-// of them issued before the first is used. A row is read whole before any of it is
+// the warp covers: a warp takes 4 U heads of a token, 4 at a time, or U heads of four tokens,
+// with the loads of all of them issued before the first is used. A row is read whole before any of it is
 // written (the shuffles wait for all 8 lanes), so the outputs may be the inputs.
 //
 // What bounds it: HBM for prompts, 512 bytes in and out per row; the launch and one
@@ -35,7 +35,7 @@ struct Args {
   Part p[2];
   int Hq, H;  // query heads, all heads
   unsigned S, tokens;
-  unsigned units;  // of 4 U heads per token
+  unsigned units;  // of 4 U heads per token, or of U heads per four tokens
   int w32, pos64, sorted;
   float eps;
   const float* cs;
@@ -45,7 +45,7 @@ struct Args {
   long long pos_b, pos_s, pos_offset;
 };
 
-template <int U>
+template <int U, bool TOKENS>
 __global__ void __launch_bounds__(WARPS * 32, 4) qk_norm_kernel(const Args a) {
   __shared__ __align__(16) float s_w[2][128];
   const int tid = threadIdx.x, lane = tid & 31, c = lane & 7;
@@ -55,9 +55,13 @@ __global__ void __launch_bounds__(WARPS * 32, 4) qk_norm_kernel(const Args a) {
   }
   __syncthreads();
   const unsigned unit = blockIdx.x * WARPS + (tid >> 5);  // all units and a CTA more fit 32 bits
-  const unsigned t = unit / a.units;
-  if (t >= a.tokens) return;
-  const int h0 = static_cast<int>(unit - t * a.units) * (4 * U) + (lane >> 3);
+  const unsigned first = unit / a.units;  // token, or four of them
+  if ((TOKENS ? 4 * first : first) >= a.tokens) return;
+  const int hu = static_cast<int>(unit - first * a.units);
+  const int h0 = TOKENS ? hu * U : hu * (4 * U) + (lane >> 3);
+  constexpr int STEP = TOKENS ? 1 : 4;
+  const bool in = !TOKENS || 4 * first + (lane >> 3) < a.tokens;
+  const unsigned t = TOKENS ? min(4 * first + (lane >> 3), a.tokens - 1) : first;
   const long long b = t / a.S, s = t - static_cast<unsigned>(b) * a.S;
   long long pos = a.pos_offset + s;
   if (a.positions != nullptr) {
@@ -68,7 +72,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) qk_norm_kernel(const Args a) {
   uint4 lo[U], hi[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int h = min(h0 + 4 * u, a.H - 1);  // (rows past the last head are not written)
+    const int h = min(h0 + STEP * u, a.H - 1);  // (rows past the last head are not written)
     const Part& p = a.p[h < a.Hq ? 0 : 1];
     const __nv_bfloat16* row = p.x + b * p.x_b + s * p.x_s + (h < a.Hq ? h : h - a.Hq) * p.x_h;
     lo[u] = *reinterpret_cast<const uint4*>(row + 8 * c);
@@ -79,7 +83,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) qk_norm_kernel(const Args a) {
   normmath::load8(a.sn + pos * a.cs_stride + 8 * c, sv);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int h = h0 + 4 * u;
+    const int h = h0 + STEP * u;
     const bool q = h < a.Hq;
     float x1[8], x2[8], w1[8], w2[8];
     normmath::unpack(lo[u], x1);
@@ -89,7 +93,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) qk_norm_kernel(const Args a) {
     normmath::normalise(x1, x2, w1, w2, a.eps, 0xffffffffu);
     uint32_t o[8];
     normmath::rotate(x1, x2, cv, sv, a.sorted != 0, o);
-    if (h < a.H) {
+    if (in && h < a.H) {
       const Part& p = a.p[q ? 0 : 1];
       __nv_bfloat16* row = p.out + b * p.o_b + s * p.o_s + (q ? h : h - a.Hq) * p.o_h;
       normmath::store_pairs(row, c, a.sorted != 0, 16, o);
@@ -162,15 +166,22 @@ extern "C" int atf_qk_norm_rope(const AtfQkNormParams* p, atf_stream_t stream) {
   a.pos_b = p->pos_stride_b;
   a.pos_s = p->pos_stride_s;
   a.pos_offset = p->pos_offset;
-  // 16 heads per warp once that gives every SM two CTAs, else 4
+  // 16 rows per warp once that gives every SM two CTAs, else 4: 16 heads of a token, or 4 of
+  // four tokens where that leaves fewer lanes idle (65521 tokens x 5 heads 84 and 54 us, x 8
+  // 88 and 62, x 20 170 and 133, x 40 263 and 250; but x 16 104 and 109, x 32 194 and 203)
   const long long wide = (a.H + 15) / 16;
   const bool many = a.tokens * wide >= 2ll * 148 * qknorm::WARPS;
-  a.units = static_cast<unsigned>(many ? wide : narrow);
-  const long long blocks = (static_cast<long long>(a.tokens) * a.units + qknorm::WARPS - 1) / qknorm::WARPS;
+  const bool tokens = many && narrow < 4 * wide;
+  a.units = static_cast<unsigned>(many && !tokens ? wide : narrow);
+  const long long items = tokens ? (a.tokens + 3ll) / 4 : a.tokens;
+  const unsigned blocks = static_cast<unsigned>((items * a.units + qknorm::WARPS - 1) / qknorm::WARPS);
+  constexpr int threads = qknorm::WARPS * 32;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (many)
-    qknorm::qk_norm_kernel<4><<<static_cast<unsigned>(blocks), qknorm::WARPS * 32, 0, st>>>(a);
+  if (tokens)
+    qknorm::qk_norm_kernel<4, true><<<blocks, threads, 0, st>>>(a);
+  else if (many)
+    qknorm::qk_norm_kernel<4, false><<<blocks, threads, 0, st>>>(a);
   else
-    qknorm::qk_norm_kernel<1><<<static_cast<unsigned>(blocks), qknorm::WARPS * 32, 0, st>>>(a);
+    qknorm::qk_norm_kernel<1, false><<<blocks, threads, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? ATF_OK : ATF_ERR_CUDA;
 }
