@@ -864,6 +864,11 @@ struct Block {
 // merging them.
 constexpr float STEP_US = 1.8f, SHARED_US = 1.3f, START_US = 6.f, STATES_US = 4.f;
 
+// pieces of at most `most` us (or of one key tile)
+inline int parts(const Block& b, float most) {
+  return std::max(1, std::min(b.tiles, static_cast<int>(ceilf(b.cost() / most))));
+}
+
 // when the last CTA ends if the blocks are cut into pieces of at most `most` us: the
 // hardware takes items in order, each for the first SM that is free
 inline float makespan(const std::vector<Block>& blocks, float most, int sms) {
@@ -871,7 +876,7 @@ inline float makespan(const std::vector<Block>& blocks, float most, int sms) {
   float last = 0.f;
   bool cut = false;
   for (const Block& b : blocks) {
-    const int n = std::max(1, std::min(b.tiles, static_cast<int>(ceilf(b.cost() / most))));
+    const int n = parts(b, most);
     cut |= n > 1;
     const float c = (b.tiles + n - 1) / n * b.step + START_US;
     for (int k = 0; k < n * b.units; ++k) {
@@ -974,10 +979,27 @@ extern "C" int atf_prefill_paged_plan(const AtfPrefillPagedPlanParams* p, int32_
           most = m;
         }
       }
+      // and, where an SM takes few pieces, between that length and its neighbours (chunks of 9
+      // requests, 1 to 72 tokens, up to 5003 keys: 37.7 us instead of 41.2, from cold memory 49
+      // instead of 52; 36 random batches from cold memory 2.30 ms instead of 2.335; with many
+      // pieces nothing is gained)
+      const float found = most < longest ? most : longest;
+      long long pieces = 0;
+      for (const Block& x : blocks) pieces += x.units * parts(x, found);
+      for (float f : {1.25f, 1.12f, 0.93f, 0.86f, 0.8f, 0.74f, 0.68f}) {
+        const float m = found * f;
+        if (pieces > 2ll * sms || best <= 1.02f * (share + START_US)) break;
+        if (m >= longest || m < START_US / 2 || m < share / 4) continue;
+        const float end = makespan(blocks, m, sms);
+        if (end < 0.98f * best) {
+          best = end;
+          most = m;
+        }
+      }
     }
     long long items = 0, wide = 0, rows = 0, slots = 0;
     for (Block& x : blocks) {
-      const int n = most < 1e30f ? std::max(1, std::min(x.tiles, static_cast<int>(ceilf(x.cost() / most)))) : 1;
+      const int n = most < 1e30f ? parts(x, most) : 1;
       const int tok = x.it.n0 + x.it.n1;
       const int each = (x.tiles + n - 1) / n;
       const int pieces = each > 0 ? std::max(1, (x.tiles + each - 1) / each) : 1;
