@@ -98,10 +98,9 @@ def draw(rng):
                     kind=rng.choice(["level", "nhd", "hnd", "e4m3_nhd", "e4m3_hnd"]), mix=mix)
     if op == "fork":
         parents, each = _log_int(rng, 1, 12), _log_int(rng, 1, 8)
-        kind = rng.choice(["bf16", "e4m3"])  # (e4m3 layers come back as four tensors each, with their scales)
-        layers = _log_int(rng, 1, max(1, min(28 if kind == "bf16" else 14, 900000 // (parents * each * page * hkv))))
+        layers = _log_int(rng, 1, max(1, min(28, 900000 // (parents * each * page * hkv))))
         return dict(op=op, parents=parents, each=each, max_len=_log_int(rng, 1, 8192 // parents + 500), page=page,
-                    hkv=hkv, layers=layers, kind=kind, mix=mix)
+                    hkv=hkv, layers=layers, kind=rng.choice(["bf16", "e4m3"]), mix=mix)
     if op == "compact":
         batch = _log_int(rng, 1, 200)
         return dict(op=op, batch=batch, max_len=_log_int(rng, 1, min(4000, 100000 // batch)), page=page,
