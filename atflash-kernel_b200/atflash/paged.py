@@ -93,10 +93,12 @@ class BatchPrefillWithPagedKVCacheWrapper:
         need = 4 * (P.partial_o_floats + P.partial_lse_floats) + 256
         if P.num_parts > 0 and self._ws.numel() * self._ws.element_size() < need:
             raise ValueError(f"workspace too small: need {need} bytes")
-        items = torch.from_numpy(buf).to(self._dev)
+        # the indices first: what converts them on this stream is done when the copy of the
+        # items, which waits for the stream, returns, so that runs on any stream may read them
         indices = _runtime.narrow_i32(idx, self._dev)
         if indices.numel() == 0:
             indices = torch.full((1,), -1, dtype=torch.int32, device=self._dev)
+        items = torch.from_numpy(buf).to(self._dev)
         self._held = _runtime.PlanTensors(self._dev, items, indices)
         t = _ffi.AtfPrefillPagedParams()
         t.total_q, t.num_heads_q, t.num_heads_kv, t.head_dim = int(cq[-1]), num_qo_heads, num_kv_heads, head_dim
