@@ -34,7 +34,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         self._ws = float_workspace_buffer
         self._dev = float_workspace_buffer.device
         self._kv_layout = kv_layout
-        self._plan = None
+        self._plan = self._planned = None
 
     def plan(self, qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, num_qo_heads: int,
              num_kv_heads: int, head_dim: int, page_size: int, *, causal: bool = True, sm_scale: Optional[float] = None,
@@ -99,7 +99,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         if indices.numel() == 0:
             indices = torch.full((1,), -1, dtype=torch.int32, device=self._dev)
         items = torch.from_numpy(buf).to(self._dev)
-        self._held = _runtime.PlanTensors(self._dev, items, indices)
+        held = _runtime.PlanTensors(self._dev, items, indices)
         t = _ffi.AtfPrefillPagedParams()
         t.total_q, t.num_heads_q, t.num_heads_kv, t.head_dim = int(cq[-1]), num_qo_heads, num_kv_heads, head_dim
         t.page_size, t.num_indices, t.indices = page_size, int(ck[-1]), indices.data_ptr()
@@ -113,7 +113,9 @@ class BatchPrefillWithPagedKVCacheWrapper:
         for i, z in enumerate(zhi or ()):
             t.zhi[i] = z
         t.error_flag = _runtime.error_flag(self._dev).data_ptr()
-        self._plan, self._plan_ptr = t, ctypes.addressof(t)
+        # in one piece: a run of another thread takes all of the old plan or all of this one
+        self._planned = t, ctypes.addressof(t), held
+        self._plan = t
 
     begin_forward = plan
 
@@ -124,14 +126,15 @@ class BatchPrefillWithPagedKVCacheWrapper:
         Returns out (total_q, Hq, 128) [, lse (total_q, Hq), natural log]; a row that sees no key
         is 0 with an lse of -inf. A page id outside the cache is reported by
         ``atflash.check_device_errors()`` (code 2); its request's outputs are not valid then."""
-        if self._plan is None:
+        if self._planned is None:
             raise RuntimeError("plan() must be called before run()")
+        params, address, held = self._planned  # (held on to until the call has returned)
         if isinstance(paged_kv_cache, (tuple, list)):
             kc, vc = paged_kv_cache
         else:
             kc, vc = paged_kv_cache[:, 0], paged_kv_cache[:, 1]
-        self._held.use()
-        return _ffi.binding().paged_run(self._plan_ptr, self._dev.index, self._kv_layout == "NHD", q, kc, vc, out, lse,
+        held.use()
+        return _ffi.binding().paged_run(address, self._dev.index, self._kv_layout == "NHD", q, kc, vc, out, lse,
                                         return_lse)
 
     forward = run
