@@ -76,7 +76,9 @@ def compact_pages(kv_lens: torch.Tensor, req_pages: torch.Tensor, page_size: int
     more) becomes the list of all other pages, rising, at its end, and free_head in the
     result points to its first.
 
-    Pages that no named request holds count as free. Rows, lengths and page ids out of
+    Pages that no named request holds count as free, and their entries of `shared` become 0.
+    A page that named and other requests held together keeps its count of holders: free a
+    request, rather than leave it out, when others share its pages. Rows, lengths and page ids out of
     range are reported (code 2) and left out. At most 2^20 pages."""
     return PageMoves(*_ffi.binding().compact_pages(kv_lens, req_pages, page_size, num_pages, max_moves, free_pages, req_rows,
                                                    shared))

@@ -439,6 +439,9 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) compa
       const int live_before = r + min(moves, z) - max(0, r - (live - moves));
       a.free_pages[a.F - n_free + (p - live_before)] = p;
     }
+    // Holders that were not named are gone: a free page has none. (A hole that a page moves
+    // into takes that page's count below, and the page that leaves is 0 from then on.)
+    if (!is_live && z >= moves && a.shared != nullptr) a.shared[p] = 0;
   }
   for (int i = gt; i < a.max_moves; i += all_threads)
     if (i >= moves) a.src[i] = a.dst[i] = -1;

@@ -669,7 +669,9 @@ typedef struct {
 /* Move the L pages that the requests hold towards the first L of the cache: the
  * highest one at or above L to the lowest free one, and so on, at most max_moves. The
  * tables and counts are changed, the pairs to copy are in src and dst (-1 past the last),
- * and the free list becomes the pages that no request holds, rising, at its end. */
+ * and the free list becomes the pages that no request holds, rising, at its end; their
+ * counts are 0. (The count of a page that is still held stays what it was: it is not
+ * counted anew for holders that were not named.) */
 int atf_compact_pages(const AtfCompactParams* p, atf_stream_t stream);
 
 typedef struct {
