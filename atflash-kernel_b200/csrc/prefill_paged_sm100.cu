@@ -892,6 +892,25 @@ inline float makespan(const std::vector<Block>& blocks, float most, int sms) {
   return last + (cut ? STATES_US : 0.f);
 }
 
+// The same for more pieces than are worth going through one by one: the SMs are full until
+// the work runs out, or until the longest piece ends. Unpacked blocks come first, so the
+// longest packed one begins when these are under way everywhere.
+inline float estimate(const std::vector<Block>& blocks, float most, int sms) {
+  float load[2] = {0.f, 0.f}, longest[2] = {0.f, 0.f};  // unpacked, packed
+  long long wide = 0;
+  bool cut = false;
+  for (const Block& b : blocks) {
+    const int n = parts(b, most), packed = b.it.flags & PACKED ? 1 : 0;
+    const float c = (b.tiles + n - 1) / n * b.step + START_US;
+    cut |= n > 1;
+    if (!packed) wide += static_cast<long long>(n) * b.units;
+    load[packed] += c * static_cast<float>(n) * static_cast<float>(b.units) / static_cast<float>(sms);
+    longest[packed] = std::max(longest[packed], c);
+  }
+  const float begins = wide < sms ? 0.f : load[0];
+  return std::max({load[0] + load[1], longest[0], begins + longest[1]}) + (cut ? STATES_US : 0.f);
+}
+
 }  // namespace paged
 }  // namespace atf
 
@@ -967,13 +986,19 @@ extern "C" int atf_prefill_paged_plan(const AtfPrefillPagedPlanParams* p, int32_
       share += x.units * x.cost() / sms;
     }
     float most = 1e30f;
-    if (units > 0 && units <= 4ll * sms) {
-      float best = makespan(blocks, most, sms);
-      for (int k = 2; k <= 2 * sms && best > 1.05f * (share + START_US); k += k < 4 ? 1 : k / 2) {
+    if (units > 0) {
+      // Few blocks are gone through one by one. For many an estimate will do (each step of
+      // the search is a pass over the blocks): they are only cut where the longest goes on
+      // after the others.
+      const bool few = units <= 4ll * sms;
+      auto end_with = [&](float m) { return few ? makespan(blocks, m, sms) : estimate(blocks, m, sms); };
+      const float full = share + (few ? START_US : START_US * static_cast<float>(units) / static_cast<float>(sms));
+      float best = end_with(most);
+      for (int k = 2; k <= 2 * sms && best > 1.05f * full; k += k < 4 ? 1 : k / 2) {
         const float m = longest / k;
         // shorter pieces cost more than they bring
         if (m < START_US / 2 || m < share / 4) break;
-        const float end = makespan(blocks, m, sms);
+        const float end = end_with(m);
         if (end < 0.97f * best) {
           best = end;
           most = m;
@@ -988,9 +1013,9 @@ extern "C" int atf_prefill_paged_plan(const AtfPrefillPagedPlanParams* p, int32_
       for (const Block& x : blocks) pieces += x.units * parts(x, found);
       for (float f : {1.25f, 1.12f, 0.93f, 0.86f, 0.8f, 0.74f, 0.68f}) {
         const float m = found * f;
-        if (pieces > 2ll * sms || best <= 1.02f * (share + START_US)) break;
+        if (pieces > 2ll * sms || best <= 1.02f * full) break;
         if (m >= longest || m < START_US / 2 || m < share / 4) continue;
-        const float end = makespan(blocks, m, sms);
+        const float end = end_with(m);
         if (end < 0.98f * best) {
           best = end;
           most = m;
