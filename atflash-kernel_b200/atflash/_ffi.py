@@ -6,9 +6,12 @@ without it raises immediately (there is no CPU fallback).
 """
 import ctypes
 import os
+import sysconfig
 import threading
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libatflash_b200.so")
+_BINDING_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)),
+                             "_binding" + sysconfig.get_config_var("EXT_SUFFIX"))
 _lib = None
 _bind = None
 _lock = threading.Lock()
@@ -300,6 +303,9 @@ def binding():
 
         from . import _runtime
         how = "build it again with `python atflash-kernel_b200/build.py`"
+        # (a file without the suffix of this Python may be another's)
+        if not os.path.exists(_BINDING_PATH):
+            raise ImportError(f"the compiled binding {_BINDING_PATH} has not been built for this Python: {how}")
         try:
             from . import _binding
         except ImportError as e:
