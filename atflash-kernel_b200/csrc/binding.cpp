@@ -100,6 +100,13 @@ int pair_order(PyObject* o) {  // -1: neither
 
 // ------------------------------------------------------------------ calls
 
+// Lets other Python threads run: over a launch, which waits where the queue of launches
+// is full (perhaps for a host callback that needs Python), and over allocations.
+struct NoGil {
+  PyThreadState* state = PyEval_SaveThread();
+  ~NoGil() { PyEval_RestoreThread(state); }
+};
+
 PyObject* device_object(c10::Device dev) {
   PyObject* r = THPDevice_New(dev);
   if (r == nullptr) throw python_error();
@@ -127,10 +134,14 @@ int* error_flag(c10::Device dev) {
 // fn(params ..., current stream) with the tensors' device current; raises on a non-zero status
 template <typename F, typename... P>
 void launch(const char* name, F fn, c10::Device dev, P... params) {
-  const c10::DeviceIndex idx = dev.index();
-  c10::cuda::OptionalCUDAGuard guard;
-  if (c10::cuda::current_device() != idx) guard.set_index(idx);
-  const int rc = fn(params..., c10::cuda::getCurrentCUDAStream(idx).stream());
+  int rc;
+  {
+    const NoGil no_gil;
+    const c10::DeviceIndex idx = dev.index();
+    c10::cuda::OptionalCUDAGuard guard;
+    if (c10::cuda::current_device() != idx) guard.set_index(idx);
+    rc = fn(params..., c10::cuda::getCurrentCUDAStream(idx).stream());
+  }
   if (rc != ATF_OK) {
     PyObject* r = PyObject_CallFunction(g_check, "si", name, rc);
     Py_XDECREF(r);
@@ -195,7 +206,10 @@ Heads heads(const Tensor& x, const std::string& name) {
 }
 
 Tensor output(const Tensor* out, const Tensor& x, const std::string& name) {
-  if (out == nullptr) return at::empty_like(x);
+  if (out == nullptr) {
+    const NoGil no_gil;
+    return at::empty_like(x);
+  }
   if (out->sizes() != x.sizes() || out->scalar_type() != at::kBFloat16 || out->device() != x.device() || out->stride(-1) != 1)
     throw ValueError(name + " must be a bf16 tensor of its input's shape and device with a contiguous last axis");
   for (int64_t i = 0; i < out->dim(); ++i)
@@ -411,7 +425,10 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Angles t = angles(*cos, *sin, dev, "cos/sin must be matching fp32 (n_pos, >=64) tables");
     p.cos = t.cos, p.sin = t.sin, p.cs_stride_pos = t.stride, p.n_pos = t.n_pos;
     if (const Tensor* given = tensor_or_none(a[11], "rope_positions")) {
-      rp = given->to(dev, at::kLong).contiguous();
+      {
+        const NoGil no_gil;
+        rp = given->to(dev, at::kLong).contiguous();
+      }
       if (rp.numel() != nnz) throw ValueError("rope_positions needs one entry per appended token");
       p.rope_positions = data<int64_t>(rp);
     }
@@ -460,7 +477,11 @@ Tensor request_rows(const Tensor* rows, int64_t table_rows, int64_t batch, c10::
   if (table_rows < batch) throw ValueError("req_pages needs a row for each request");
   return {};
 }
-Tensor new_i32(int64_t n, c10::Device dev) { return at::empty({n}, at::TensorOptions().dtype(at::kInt).device(dev)); }
+Tensor empty(at::IntArrayRef sizes, at::ScalarType type, c10::Device dev) {
+  const NoGil no_gil;
+  return at::empty(sizes, at::TensorOptions().dtype(type).device(dev));
+}
+Tensor new_i32(int64_t n, c10::Device dev) { return empty({n}, at::kInt, dev); }
 
 // (src, dst, head) of one buffer
 PyObject* moves(const Tensor& buf, int64_t n) {
@@ -615,12 +636,12 @@ PyObject* paged_run(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   if (lse != nullptr && (lse->dim() != 2 || lse->size(0) != nq || lse->size(1) != hq || lse->scalar_type() != at::kFloat ||
                          lse->device() != dev || !lse->is_contiguous()))
     throw ValueError("lse must be a contiguous float32 (" + std::to_string(nq) + ", " + std::to_string(hq) + ") tensor" + on(dev));
-  const Tensor o = out != nullptr ? *out : at::empty({nq, hq, 128}, q.options());
+  const Tensor o = out != nullptr ? *out : empty({nq, hq, 128}, at::kBFloat16, dev);
   Tensor l;
   if (lse != nullptr)
     l = *lse;
   else if (return_lse)
-    l = at::empty({nq, hq}, q.options().dtype(at::kFloat));
+    l = empty({nq, hq}, at::kFloat, dev);
   if (nq > 0) {
     p.q = q.data_ptr();
     p.k_cache = kc.data_ptr();
