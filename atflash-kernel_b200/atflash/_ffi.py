@@ -15,6 +15,7 @@ _BINDING_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)),
 _lib = None
 _bind = None
 _lock = threading.Lock()
+_bind_lock = threading.Lock()
 
 ATF_OK = 0
 ATF_LAYOUT_SORTED_PAIR, ATF_LAYOUT_ROTATE_HALF = 0, 1
@@ -306,15 +307,19 @@ def binding():
         # (a file without the suffix of this Python may be another's)
         if not os.path.exists(_BINDING_PATH):
             raise ImportError(f"the compiled binding {_BINDING_PATH} has not been built for this Python: {how}")
-        try:
-            from . import _binding
-        except ImportError as e:
-            raise ImportError(f"the compiled binding cannot be loaded ({e}): {how}") from e
-        if torch.__version__.split("+")[0] != _binding.torch_version.split("+")[0] or _binding.version != ATF_VERSION:
-            raise ImportError(f"the compiled binding is for torch {_binding.torch_version} and version {_binding.version} of "
-                              f"the C interface: {how}")
-        _binding.init({name: ctypes.cast(getattr(lib, name), _vp).value for name in EXPORTED}, check, _runtime)
-        _bind = _binding
+        with _bind_lock:
+            if _bind is not None:
+                return _bind
+            try:
+                from . import _binding
+            except ImportError as e:
+                raise ImportError(f"the compiled binding cannot be loaded ({e}): {how}") from e
+            if (torch.__version__.split("+")[0] != _binding.torch_version.split("+")[0]
+                    or _binding.version != ATF_VERSION):
+                raise ImportError(f"the compiled binding is for torch {_binding.torch_version} and version "
+                                  f"{_binding.version} of the C interface: {how}")
+            _binding.init({name: ctypes.cast(getattr(lib, name), _vp).value for name in EXPORTED}, check, _runtime)
+            _bind = _binding
     return _bind
 
 
