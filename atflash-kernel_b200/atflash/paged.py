@@ -124,7 +124,10 @@ class BatchPrefillWithPagedKVCacheWrapper:
         """q (total_q, Hq, 128) bf16; paged_kv_cache = (k_pages, v_pages) or one tensor with a
         k/v axis at dim 1, bf16 pages in the wrapper's kv_layout (K neither level-major nor e4m3).
         Returns out (total_q, Hq, 128) [, lse (total_q, Hq), natural log]; a row that sees no key
-        is 0 with an lse of -inf. A page id outside the cache is reported by
+        is 0 with an lse of -inf. A NaN key makes the rows that see it NaN and no others. A NaN
+        or an infinity in V of a key reaches all rows of every tile (up to 128 rows of a
+        request) that loads the key's tile of 128 keys, those that do not see it too: there
+        it meets a probability of 0, whose product with it is NaN. A page id outside the cache is reported by
         ``atflash.check_device_errors()`` (code 2); its request's outputs are not valid then."""
         if self._planned is None:
             raise RuntimeError("plan() must be called before run()")
