@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "../../include/atflash_b200.h"
@@ -36,7 +37,7 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // read 16 bytes at a time.
 inline int norm_args_ok(const AtfAppendParams* p, const AtfKNorm* n) {
   if (n == nullptr) return ATF_OK;
-  if (n->weight == nullptr || p->cos == nullptr || !(n->eps > 0.f) ||
+  if (n->weight == nullptr || p->cos == nullptr || !(n->eps > 0.f && n->eps <= FLT_MAX) ||
       (n->weight_dtype != ATF_DTYPE_BF16 && n->weight_dtype != ATF_DTYPE_F32))
     return ATF_ERR_INVALID_ARG;
   if (!aligned16(n->weight) || !aligned16(p->cos) || !aligned16(p->sin) || (p->cs_stride_pos & 3) != 0)

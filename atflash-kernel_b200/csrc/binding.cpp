@@ -190,7 +190,8 @@ int check_norm(const Tensor& w, double eps, c10::Device dev, const char* name) {
   const at::ScalarType t = w.scalar_type();
   if ((t != at::kBFloat16 && t != at::kFloat) || w.dim() != 1 || w.size(0) != 128 || w.stride(0) != 1 || w.device() != dev)
     throw ValueError(std::string(name) + " must be 128 contiguous bf16 or fp32 weights" + on(dev));
-  if (!(eps >= 1e-38 && eps < INFINITY)) throw ValueError("the norm's eps must be a positive number");  // (a normal fp32 number)
+  // as the kernels take it: far enough from 0 for a root, and finite
+  if (!(eps >= 1e-38 && static_cast<float>(eps) < INFINITY)) throw ValueError("the norm's eps must be a positive fp32 number");
   return t == at::kFloat ? ATF_DTYPE_F32 : ATF_DTYPE_BF16;
 }
 

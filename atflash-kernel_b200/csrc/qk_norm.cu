@@ -110,7 +110,7 @@ extern "C" int atf_qk_norm_rope(const AtfQkNormParams* p, atf_stream_t stream) {
   if (p == nullptr || p->cos == nullptr || p->sin == nullptr) return ATF_ERR_INVALID_ARG;
   if (p->head_dim != ATF_HEAD_DIM) return ATF_ERR_UNSUPPORTED;
   if (p->batch < 0 || p->seqlen < 0 || p->num_heads_q < 0 || p->num_heads_k < 0 || p->n_pos < 1 ||
-      p->cs_stride_pos < 64 || !(p->eps > 0.f))
+      p->cs_stride_pos < 64 || !(p->eps > 0.f && p->eps <= FLT_MAX))
     return ATF_ERR_INVALID_ARG;
   if ((p->num_heads_q > 0 && (p->q == nullptr || p->q_out == nullptr || p->q_weight == nullptr)) ||
       (p->num_heads_k > 0 && (p->k == nullptr || p->k_out == nullptr || p->k_weight == nullptr)))

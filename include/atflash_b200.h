@@ -491,7 +491,7 @@ typedef struct {
   const void* q_weight; /* [128] */
   const void* k_weight;
   int weight_dtype;     /* ATF_DTYPE_* of both */
-  float eps;            /* positive */
+  float eps;            /* positive, finite */
   const float* cos;     /* fp32 [n_pos, >= 64], rows 16-byte aligned */
   const float* sin;
   int64_t cs_stride_pos, n_pos;
@@ -732,7 +732,7 @@ int atf_decode_run_e4m3(const AtfDecodeParams* p, const AtfKvScales* s, atf_stre
 typedef struct {
   const void* weight; /* [128], 16-byte aligned */
   int weight_dtype;   /* ATF_DTYPE_* */
-  float eps;          /* positive */
+  float eps;          /* positive, finite */
 } AtfKNorm;
 
 /* atf_paged_kv_append (s NULL) or atf_paged_kv_append_e4m3 of a K that is normed first:
