@@ -24,6 +24,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.Ten
     None. Weights: 128 bf16 or fp32, both of one type. positions: integers (S,) or (B, S), or
     (T,); default pos_offset + s; positions outside the tables are clamped into them, as
     by ``rope_pack``. q_out may be q and k_out may be k (in place); otherwise outputs overlap
-    no input. There is no backward pass."""
+    no input. A row whose squares overflow fp32 (elements over 1e18) gives 0. There is no
+    backward pass."""
     return _ffi.binding().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps, pos_offset, positions, out_layout, q_out,
                                        k_out)

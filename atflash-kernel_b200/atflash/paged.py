@@ -22,7 +22,14 @@ class BatchPrefillWithPagedKVCacheWrapper:
     """plan() once per step, run() for each layer, on any stream (runs share the workspace, so
     those of one wrapper, and its captured graphs, follow one another). Request b's new tokens are the rows
     [qo_indptr[b], qo_indptr[b+1]) of q; they are the last of its tokens, whose K and V are
-    all in its pages (append them first)."""
+    all in its pages (append them first).
+
+    A window is quantised as in the packed prefill, per tile of 128 queries, counted from the
+    request's first new token, and 128 keys: a level counts where any pair of the tile is within
+    its reach. So the scores of a token depend on where its chunk begins, and a request of one
+    token keeps levels of some keys that ``BatchDecodeWithPagedKVCacheWrapper``, which goes by each
+    key's own distance, drops (never the other way round). Chunks that begin on multiples of 128
+    tokens keep what the whole prompt in one chunk keeps."""
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD"):
         if kv_layout not in ("NHD", "HND"):

@@ -60,7 +60,9 @@ def free_requests(req_rows: Optional[torch.Tensor], kv_lens: torch.Tensor, req_p
 
     A row that is named twice (its first entry counts), rows and lengths out of range,
     page ids outside the cache, a page given up more often than it was held and a list
-    without room are reported (code 2) and left out."""
+    without room are reported (code 2) and left out. (Without `shared` the call knows
+    neither the cache's size nor the holders: it reports negative ids, and lists any other id
+    as often as the rows hold it.)"""
     return _ffi.binding().free_requests(req_rows, kv_lens, req_pages, page_size, free_pages, free_head, shared)
 
 

@@ -989,7 +989,8 @@ extern "C" int atf_prefill_paged_plan(const AtfPrefillPagedPlanParams* p, int32_
     if (units > 0) {
       // Few blocks are gone through one by one. For many an estimate will do (each step of
       // the search is a pass over the blocks): they are only cut where the longest goes on
-      // after the others.
+      // after the others. One token over 128K keys beside 74 over 1000 (32 / 8 heads, from cold
+      // memory) takes 168 us, 1044 uncut; behind 4 chunks of 2048 over 8192 keys 910, 1720 uncut.
       const bool few = units <= 4ll * sms;
       auto end_with = [&](float m) { return few ? makespan(blocks, m, sms) : estimate(blocks, m, sms); };
       const float full = share + (few ? START_US : START_US * static_cast<float>(units) / static_cast<float>(sms));

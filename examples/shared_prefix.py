@@ -6,6 +6,9 @@ it for layers with norms of their q and k heads.
 
     python examples/shared_prefix.py [--each 4] [--steps 4] [--window]
 
+With --window the scores depend a little on where chunks begin, as
+BatchPrefillWithPagedKVCacheWrapper says.
+
 The layers' projections are random matrices; what the loop shows is which call feeds
 which. `Engine` keeps what each request's tokens were projected to, so that a test can
 compare every output with a plain implementation."""

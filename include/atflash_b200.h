@@ -645,7 +645,9 @@ typedef struct {
  * page loses a holder per entry, and one that has none left goes back to the free
  * list: n such pages to free_pages[*free_head - n .. *free_head), by their last entry in the
  * call, and *free_head_out = *free_head - n. The entries become -1. A page given up more often
- * than it was held is freed once and reported. */
+ * than it was held is freed once and reported. (With shared NULL the cache's size and the
+ * holders are not known: negative ids are reported, any other is listed as often as the
+ * rows hold it.) */
 int atf_free_requests(const AtfFreeParams* p, atf_stream_t stream);
 
 typedef struct {
