@@ -6,7 +6,8 @@
 // softmax in the log2 domain over 128-key tiles, S = Q K^T over the window's 16-dim levels
 // and O += P V on the tensor cores with both accumulators in TMEM, P in bf16 (the tensor
 // core's f16 kind has one type for both operands, and V is bf16), sums and statistics
-// in fp32. The window is quantised per tile of 128 queries and 128 keys of the request.
+// in fp32: off by 0.0021 to 0.0024 of the outputs' size from 64 bits, where the rounding of the
+// bf16 outputs alone makes 0.0017. The window is quantised per tile of 128 queries and 128 keys of the request.
 // Three things differ.
 //
 // Pages. A key tile is 128 / R slices of R = min(page, 128) rows. The K producer warp, and the
@@ -32,10 +33,11 @@
 // CTAs; their states go to a workspace (fp32) and merge_states_kernel joins them.
 //
 // What bounds it: HBM where rows are few (24 requests x 5 tokens over up to 16001 keys, 28 /
-// 4 heads, pages of 16: 127 us with L2 warm, 142 cold; the floor is 113. A key tile takes
+// 4 heads, pages of 16: 127 to 131 us replayed from a graph, 142 to 154 a call from cold memory;
+// the floor is 113. A key tile takes
 // 1.1 us from L2 and 1.5 with all SMs reading HBM, and a CTA's start and end 6 more); else
 // the step of two tiles, as in the packed prefill (2 chunks of 8192 behind 24K keys, the
-// window on: 4.3 to 5.0 ms by the clock, 61 to 71% of the burst rate).
+// window on: 4.9 to 5.0 ms, 61% of the burst rate; 4.3 in a few launches at a higher clock).
 #include <math.h>
 
 #include <algorithm>
@@ -986,14 +988,15 @@ extern "C" int atf_prefill_paged_plan(const AtfPrefillPagedPlanParams* p, int32_
       share += x.units * x.cost() / sms;
     }
     float most = 1e30f;
-    if (units > 0) {
+    const bool few = units <= 4ll * sms;
+    const float full = share + (few ? START_US : START_US * static_cast<float>(units) / static_cast<float>(sms));
+    // (no end is later than a full machine's by more than the longest block)
+    if (units > 0 && (few || longest > 0.05f * full)) {
       // Few blocks are gone through one by one. For many an estimate will do (each step of
       // the search is a pass over the blocks): they are only cut where the longest goes on
       // after the others. One token over 128K keys beside 74 over 1000 (32 / 8 heads, from cold
       // memory) takes 168 us, 1044 uncut; behind 4 chunks of 2048 over 8192 keys 910, 1720 uncut.
-      const bool few = units <= 4ll * sms;
       auto end_with = [&](float m) { return few ? makespan(blocks, m, sms) : estimate(blocks, m, sms); };
-      const float full = share + (few ? START_US : START_US * static_cast<float>(units) / static_cast<float>(sms));
       float best = end_with(most);
       for (int k = 2; k <= 2 * sms && best > 1.05f * full; k += k < 4 ? 1 : k / 2) {
         const float m = longest / k;
@@ -1011,17 +1014,19 @@ extern "C" int atf_prefill_paged_plan(const AtfPrefillPagedPlanParams* p, int32_
       // pieces nothing is gained)
       const float found = most < longest ? most : longest;
       long long pieces = 0;
-      for (const Block& x : blocks) pieces += x.units * parts(x, found);
-      for (float f : {1.25f, 1.12f, 0.93f, 0.86f, 0.8f, 0.74f, 0.68f}) {
-        const float m = found * f;
-        if (pieces > 2ll * sms || best <= 1.02f * full) break;
-        if (m >= longest || m < START_US / 2 || m < share / 4) continue;
-        const float end = end_with(m);
-        if (end < 0.98f * best) {
-          best = end;
-          most = m;
+      if (few)
+        for (const Block& x : blocks) pieces += x.units * parts(x, found);
+      if (few && pieces <= 2ll * sms)
+        for (float f : {1.25f, 1.12f, 0.93f, 0.86f, 0.8f, 0.74f, 0.68f}) {
+          const float m = found * f;
+          if (best <= 1.02f * full) break;
+          if (m >= longest || m < START_US / 2 || m < share / 4) continue;
+          const float end = end_with(m);
+          if (end < 0.98f * best) {
+            best = end;
+            most = m;
+          }
         }
-      }
     }
     long long items = 0, wide = 0, rows = 0, slots = 0;
     for (Block& x : blocks) {
