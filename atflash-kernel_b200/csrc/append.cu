@@ -98,9 +98,10 @@ __global__ void append_kernel(const Args a) {
 // leaves in (32 bytes a row and level) make up whole lines. A step's tokens (too few for two
 // CTAs an SM) go by 4 heads of one token.
 //
-// HBM-bound for prompts: 64K tokens x 8 heads take 96 us into pages of 16 (91% of HBM), 102
-// into level-major ones; x 4 heads 53 and 57, x 1 head 25 and 27. With 8 heads of a token per
-// warp 96 and 107, 73 and 77, 64 and 65. A thread per (row, 8 pairs) as above took 129 / 120
+// HBM-bound for prompts, from cold memory: 64K tokens x 8 heads take 96 us into pages of 16 (90%
+// of HBM), 102 into level-major ones; x 4 heads 55 and 57, x 1 head 27 and 29. (Replayed from a
+// graph 91 and 96, 49 and 53, 20 and 21: a part comes from L2.) With 8 heads of a token per warp,
+// cold, 96 and 107, 73 and 77, 64 and 65. A thread per (row, 8 pairs) as above took 129 / 120
 // us (115 / 104 with the loads in front of the lookup), 4 heads a warp 119 / 107, 8 heads with
 // more registers and fewer CTAs 123 / 111.
 template <bool MANY>

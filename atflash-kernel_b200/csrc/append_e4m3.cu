@@ -33,8 +33,9 @@
 // (130). CTAs of 4 warps: 96-102 us, but 18-19 instead of 13 for pages of 64. From cold
 // memory, with as many warps to every run as the page has rows and with them by the run:
 // 512 single tokens x 8 heads in pages of 64 51 and 10 us (pages of 16: 16.4 and 10), 200
-// single tokens beside 2 prompts of 3000 x 4 heads 107 and 21; 64K tokens in pages of 64
-// 141 and 144.
+// single tokens beside 2 prompts of 3000 x 4 heads 107 and 21. Prompts alone pay for that where a
+// CTA has little to do (64K tokens x 8 heads with RoPE in pages of 64 145 and 149, 63486 x 1 head
+// in pages of 32, replayed from a graph, 18 and 20) and gain 4 to 6% in pages of 128 and 256.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -364,8 +365,8 @@ __device__ __forceinline__ void stage_angles(const Args& a, long long i0, int po
 }
 
 // The norm's weights stay in registers, with two CTAs an SM instead of three: 64K tokens x 8
-// heads in pages of 16 127 us (102 with the rotation alone); from shared memory 135, and
-// 157 with three CTAs (spills).
+// heads in pages of 16 125 us (98 with the rotation alone; in pages of 64 165 and 141); from
+// shared memory 135, and 157 with three CTAs (spills).
 template <bool ROPE, bool NORM>
 __global__ void __launch_bounds__(THREADS, NORM ? 2 : 3) append_e4m3_kernel(const Args a) {
   __shared__ Run s_run[MAX_WINDOW];

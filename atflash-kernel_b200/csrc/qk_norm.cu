@@ -14,9 +14,10 @@
 // What bounds it: HBM for prompts, 512 bytes in and out per row; the launch and one
 // chain of loads (position -> angles -> row) for a step's tokens, where U = 1 spreads
 // them over more SMs. The loads in flight are what counts for prompts: 65521 tokens x 32
-// heads take 191 us (88% of HBM) with 16 heads a warp and four CTAs an SM (64 registers),
-// 196 with three, 202 with 32 heads and two, 216 with 8 heads and four; indexes in 64
-// bits cost 12 us, and streaming hints on loads or stores change nothing.
+// heads take 183 to 191 us on the device (replayed from a graph; 88 to 92% of HBM) with 16 heads
+// a warp and four CTAs an SM (64 registers), and beside the 191 196 with three, 202 with 32 heads
+// and two, 216 with 8 heads and four; indexes in 64 bits cost 12 us, and streaming hints on loads
+// or stores change nothing.
 #include "atf_internal.h"
 #include "norm_math.cuh"
 
