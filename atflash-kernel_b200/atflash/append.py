@@ -179,6 +179,7 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor, 
     try:
         binding = _ffi.binding()
     except ImportError as e:
+        _ffi.load()  # (raises where it is the library that is missing)
         if k_norm is not None:
             raise
         warnings.warn(f"append_paged_kv_cache goes through ctypes, which takes longer: {e}", RuntimeWarning, stacklevel=2)
